@@ -495,6 +495,107 @@ NMOE_API nmoe_status nmoe_route_tokens_noalloc(
     int32_t experts, int32_t top_k, int32_t n_group, int32_t topk_group,
     int32_t norm_topk_prob, float routed_scaling, int32_t* top_index, float* top_weight);
 
+/* --- attention and its paged 8-bit cache -----------------------------------------
+ * The attention layers that stand between the expert layers in the model's loop
+ * (single_token_forward_model.cpp:603-636) are the caller's own code; these are
+ * the operators it runs between its projections.  The reference attends in
+ * bf16 over bf16 pages (cudnn_paged_attention.cpp); here the pages hold 8-bit
+ * codes.  Queries, keys, values and results are bf16 rows of heads x 128
+ * elements, one head's beside the next's; `*_stride` is the number of elements
+ * from one token's row to the next's (a multiple of 8; rows of a fused
+ * projection are taken as they lie), rows begin on 16-byte boundaries.  Query
+ * head h attends key head h / (heads / kv_heads).
+ *
+ * Everything is enqueued on the caller's stream, nothing allocates or
+ * synchronises (nmoe_kv_sync_status and nmoe_attention_sync_status do), and all
+ * lists and lengths are read on the device: a step can be recorded in a CUDA
+ * graph and replayed while they change.
+ *
+ * Batches.  `sequences` [count] names sequences (rows of the block table, each
+ * at most once in a list), `offsets` [count + 1] the rows that belong to each:
+ * entry i has the rows [offsets[i], offsets[i+1]) of `rows`, possibly none.
+ *
+ * What only the device can see is wrong (a list entry out of range or named
+ * twice, too few pages) leaves a status in the workspace: nmoe_kv_sync_status
+ * returns and clears it.  Until then nmoe_kv_extend, _append, _fork, _free and
+ * _compact do nothing, so that rows without a place are not written over others.
+ */
+typedef struct nmoe_kv_cache {
+  int32_t layers;
+  int32_t pages;                   /* of every layer */
+  int32_t kv_heads;
+  int32_t page_tokens;             /* 16, 32, 64 or 128 */
+  int32_t max_sequences;           /* rows of the block table */
+  int32_t max_pages_per_sequence;  /* its columns */
+  /* Device memory, the caller's.  codes: E4M3 [layers][pages][2][kv_heads]
+   * [page_tokens][128], keys then values, 128-byte aligned; exponents:
+   * [layers][pages][2][kv_heads]; a code stands for its value x 2^exponent. */
+  uint8_t* codes;
+  int8_t* exponents;
+  int32_t* block_table;  /* [max_sequences][max_pages_per_sequence] pages in order */
+  int32_t* lengths;      /* [max_sequences] tokens */
+  int32_t* references;   /* [pages] sequences that hold the page; 0 = free */
+  void* workspace;       /* nmoe_kv_workspace_bytes() bytes, 256-byte aligned, zero at
+                            first; one call at a time uses it */
+  size_t workspace_bytes;
+} nmoe_kv_cache;
+
+/* Reads the sizes only; 0 for sizes that are none. */
+NMOE_API size_t nmoe_kv_workspace_bytes(const nmoe_kv_cache* cache);
+/* Makes room for new tokens: lengths grow by each entry's rows, the pages this
+ * takes are the lowest free ones, in list order.  Too few pages or columns:
+ * NMOE_ERR_CAPACITY, and nothing changes. */
+NMOE_API nmoe_status nmoe_kv_extend(const nmoe_kv_cache* cache, void* stream,
+                                    const int32_t* sequences, const int32_t* offsets,
+                                    int32_t count, int64_t rows);
+/* Quantises rows of keys and values into their places, the LAST tokens of each
+ * sequence.  A page and head's exponent is the least e in [-32, 32] with
+ * |x| <= 448 * 2^e for its finite values; codes are rounded to nearest even and
+ * saturate, NaN and infinities become NaN.  A page that held tokens before keeps
+ * the larger of both exponents, and its older codes are rounded to that. */
+NMOE_API nmoe_status nmoe_kv_append(const nmoe_kv_cache* cache, void* stream, int32_t layer,
+                                    const void* k, int64_t k_stride, const void* v,
+                                    int64_t v_stride, const int32_t* sequences,
+                                    const int32_t* offsets, int32_t count, int64_t rows);
+/* children[i] becomes a copy of parents[i]: what it held is given up, full
+ * pages are shared (references), a partly filled last page is copied in every
+ * layer to the lowest free one.  Children are distinct and no parents.
+ * NMOE_ERR_CAPACITY leaves everything as it was. */
+NMOE_API nmoe_status nmoe_kv_fork(const nmoe_kv_cache* cache, void* stream, const int32_t* parents,
+                                  const int32_t* children, int32_t count);
+/* Gives up the sequences' pages: lengths and table entries become 0, a page
+ * that nobody holds any more is free. */
+NMOE_API nmoe_status nmoe_kv_free(const nmoe_kv_cache* cache, void* stream,
+                                  const int32_t* sequences, int32_t count);
+/* With L pages in use, moves those at or above L, in order, to the free ones
+ * below L, in order; block table and references follow. */
+NMOE_API nmoe_status nmoe_kv_compact(const nmoe_kv_cache* cache, void* stream);
+/* Copies pages in every layer; no target is a source or another's target. */
+NMOE_API nmoe_status nmoe_kv_copy_pages(const nmoe_kv_cache* cache, void* stream,
+                                        const int32_t* sources, const int32_t* targets,
+                                        int32_t count);
+NMOE_API nmoe_status nmoe_kv_sync_status(const nmoe_kv_cache* cache, void* stream);
+
+/* Attention of new rows over the cache: row j of an entry with c rows stands at
+ * position length - c + j of its sequence and sees every token up to itself
+ * (which nmoe_kv_append has written).  out [rows][heads][128]:
+ * softmax(scale * q k^T) v, sums in FP32. */
+NMOE_API nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* stream, int32_t layer,
+                                           const void* q, int64_t q_stride, int32_t heads,
+                                           const int32_t* sequences, const int32_t* offsets,
+                                           int32_t count, int64_t rows, float scale, void* out);
+/* Causal attention over `count` whole prompts packed one behind the other, prompt
+ * i in rows [offsets[i], offsets[i+1]) (device, rising from 0 to `tokens`).
+ * out [tokens][heads][128]; lse [tokens][heads], nullable: the logarithms of
+ * the rows' sums of exponentials; error, nullable: a device word (zero at
+ * first) for nmoe_attention_sync_status. */
+NMOE_API nmoe_status nmoe_attention_prefill(void* stream, const void* q, int64_t q_stride,
+                                            const void* k, int64_t k_stride, const void* v,
+                                            int64_t v_stride, int64_t tokens, int32_t heads,
+                                            int32_t kv_heads, const int32_t* offsets, int32_t count,
+                                            float scale, void* out, float* lse, int32_t* error);
+NMOE_API nmoe_status nmoe_attention_sync_status(int32_t* error, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -45,6 +45,9 @@ EXPORTED_SYMBOLS = (
     "nmoe_ep_window_experts", "nmoe_ep_window_combine", "nmoe_ep_window_fork_shared",
     "nmoe_layer_set_wait_limit_ms", "nmoe_layer_wait_flag", "nmoe_layer_reserve_tokens",
     "nmoe_layer_set_unfused_activation", "nmoe_layer_export_unfused", "nmoe_layer_keep_trace",
+    "nmoe_kv_workspace_bytes", "nmoe_kv_extend", "nmoe_kv_append", "nmoe_kv_fork", "nmoe_kv_free",
+    "nmoe_kv_compact", "nmoe_kv_copy_pages", "nmoe_kv_sync_status", "nmoe_attention_cached",
+    "nmoe_attention_prefill", "nmoe_attention_sync_status",
 )
 
 

@@ -1,0 +1,287 @@
+"""Attention over prompts and over a paged 8-bit cache of keys and values.
+
+The attention layers between the expert layers of a model are the caller's own code
+(runtime/src/api/single_token_forward_model.cpp:603-636); these are the operators such a
+layer runs between its projections, over the C ABI of include/nmoe.h:
+
+    cache = KvCache.allocate(layers, pages, kv_heads, max_sequences, max_pages_per_sequence)
+    cache.extend(sequences, offsets)                  # once a step: room for the new tokens
+    for every attention layer:
+        cache.append(layer, k, v, sequences, offsets)     # the new rows, as 8-bit codes
+        out = attention_prefill(q, k, v, offsets)         # whole prompts, or
+        out = cache.attend(layer, q, sequences, offsets)  # new rows over all tokens so far
+    cache.fork(parents, children)                     # several continuations of a prompt
+    cache.free(sequences)                             # finished
+    cache.compact()                                   # the pages in use, without holes
+
+q is [rows, heads, 128] bf16, k and v [rows, kv_heads, 128]; slices of a fused projection's
+rows are taken as they lie.  `sequences` [n] (rows of the block table, each at most once) and
+`offsets` [n + 1] (rows of each) are int32 tensors on the device; the host reads neither, so
+a step can be recorded in a CUDA graph.  Calls run on the current stream; a cache is used by
+one stream at a time.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Dict, Optional
+
+import torch
+
+from . import NMOE_OK, NmoeError, _check, _stream, load_library
+
+HEAD_DIM = 128
+
+
+class _KvCache(ctypes.Structure):
+    _fields_ = [("layers", ctypes.c_int32), ("pages", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("page_tokens", ctypes.c_int32),
+                ("max_sequences", ctypes.c_int32), ("max_pages_per_sequence", ctypes.c_int32),
+                ("codes", ctypes.c_void_p), ("exponents", ctypes.c_void_p),
+                ("block_table", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("references", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
+_library = None
+
+
+def _lib() -> ctypes.CDLL:
+    global _library
+    if _library is None:
+        lib = load_library()
+        vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+        cache = ctypes.POINTER(_KvCache)
+        lib.nmoe_kv_workspace_bytes.restype = ctypes.c_size_t
+        lib.nmoe_kv_workspace_bytes.argtypes = [cache]
+        lib.nmoe_kv_extend.argtypes = [cache, vp, vp, vp, i32, i64]
+        lib.nmoe_kv_append.argtypes = [cache, vp, i32, vp, i64, vp, i64, vp, vp, i32, i64]
+        lib.nmoe_kv_fork.argtypes = [cache, vp, vp, vp, i32]
+        lib.nmoe_kv_free.argtypes = [cache, vp, vp, i32]
+        lib.nmoe_kv_compact.argtypes = [cache, vp]
+        lib.nmoe_kv_copy_pages.argtypes = [cache, vp, vp, vp, i32]
+        lib.nmoe_kv_sync_status.argtypes = [cache, vp]
+        lib.nmoe_attention_cached.argtypes = [cache, vp, i32, vp, i64, i32, vp, vp, i32, i64, f32, vp]
+        lib.nmoe_attention_prefill.argtypes = [vp, vp, i64, vp, i64, vp, i64, i64, i32, i32, vp, i32,
+                                               f32, vp, vp, vp]
+        lib.nmoe_attention_sync_status.argtypes = [vp, vp]
+        _library = lib
+    return _library
+
+
+def _require_rows(t: torch.Tensor, name: str, device: torch.device) -> None:
+    """[rows, heads, 128] bf16, a row's heads side by side; rows may lie further apart."""
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}: this library has no CPU path")
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be bfloat16, not {t.dtype}")
+    if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.shape[1] == 0:
+        raise ValueError(f"{name} must be [rows, heads, {HEAD_DIM}], not {list(t.shape)}")
+    if t.shape[0] and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != HEAD_DIM)):
+        raise ValueError(f"{name}: the heads of a row must lie side by side")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * HEAD_DIM
+
+
+def _require_list(t: torch.Tensor, name: str, device: torch.device) -> None:
+    if t.device != device or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 vector on {device}")
+
+
+def _require_current(device: torch.device, what: str) -> None:
+    if device.type != "cuda":
+        raise ValueError(f"{what} must be a CUDA tensor: this library has no CPU path")
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"{what} is on {device}, which is not the current device")
+
+
+def _output(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    if out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device or \
+            not out.is_contiguous():
+        raise ValueError(f"out must be contiguous bfloat16 {list(q.shape)} on {q.device}")
+    return out
+
+
+_error_words: Dict[torch.device, torch.Tensor] = {}
+
+
+def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
+                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                      return_lse: bool = False):
+    """Causal attention over whole prompts packed one behind the other: prompt i is the rows
+    [offsets[i], offsets[i + 1]), and each of its rows sees those up to itself.  Query head h
+    attends key head h // (heads // kv_heads).  Returns [rows, heads, 128] bf16 and, if asked
+    for, the FP32 logarithms [rows, heads] of the rows' sums of exponentials.  `scale` is
+    1 / sqrt(128) unless given."""
+    device = q.device
+    _require_current(device, "q")
+    _require_rows(q, "q", device)
+    _require_rows(k, "k", device)
+    _require_rows(v, "v", device)
+    _require_list(offsets, "offsets", device)
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or q.shape[1] % k.shape[1] or \
+            offsets.numel() == 0:
+        raise NmoeError(1, "attention_prefill", "k and v need q's rows and a divisor of its heads, "
+                                                "offsets one entry more than there are prompts")
+    out = _output(out, q)
+    lse = None
+    if return_lse:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device)
+    error = _error_words.get(device)
+    if error is None:
+        error = _error_words[device] = torch.zeros(1, dtype=torch.int32, device=device)
+    _check(_lib().nmoe_attention_prefill(
+        _stream(), q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(),
+        _row_stride(v), q.shape[0], q.shape[1], k.shape[1], offsets.data_ptr(), offsets.numel() - 1,
+        HEAD_DIM ** -0.5 if scale is None else scale, out.data_ptr(),
+        lse.data_ptr() if lse is not None else None, error.data_ptr()), "nmoe_attention_prefill")
+    return (out, lse) if return_lse else out
+
+
+def prefill_sync_status() -> int:
+    """Waits for the current stream; the status of `attention_prefill` on this device."""
+    device = torch.device("cuda", torch.cuda.current_device())
+    error = _error_words.get(device)
+    return NMOE_OK if error is None else _lib().nmoe_attention_sync_status(error.data_ptr(), _stream())
+
+
+class KvCache:
+    """Keys and values of `layers` attention layers in pages of `page_tokens` tokens: E4M3 codes
+    with an exponent for each page, head, and keys or values (`nmoe_kv_cache`, include/nmoe.h).
+    The tensors are the caller's and may be read or set between calls."""
+
+    def __init__(self, codes: torch.Tensor, exponents: torch.Tensor, block_table: torch.Tensor,
+                 lengths: torch.Tensor, references: torch.Tensor):
+        """codes [layers, pages, 2, kv_heads, page_tokens, 128] float8_e4m3fn, exponents
+        [layers, pages, 2, kv_heads] int8, block_table [max_sequences, max_pages] int32, lengths
+        [max_sequences] int32, references [pages] int32."""
+        device = codes.device
+        _require_current(device, "codes")
+        if codes.dtype != torch.float8_e4m3fn or codes.dim() != 6 or codes.shape[2] != 2 or \
+                codes.shape[5] != HEAD_DIM:
+            raise ValueError("codes must be float8_e4m3fn [layers, pages, 2, kv_heads, page_tokens, "
+                             f"{HEAD_DIM}]")
+        if codes.shape[4] not in (16, 32, 64, 128):
+            raise ValueError("page_tokens must be 16, 32, 64 or 128")
+        for t, name, dtype, shape in (
+                (exponents, "exponents", torch.int8, codes.shape[:4]),
+                (block_table, "block_table", torch.int32, block_table.shape),
+                (lengths, "lengths", torch.int32, block_table.shape[:1]),
+                (references, "references", torch.int32, codes.shape[1:2])):
+            if t.dtype != dtype or t.shape != shape or t.device != device:
+                raise ValueError(f"{name} must be {dtype} {list(shape)} on {device}")
+        if block_table.dim() != 2:
+            raise ValueError("block_table must be [max_sequences, max_pages]")
+        for t in (codes, exponents, block_table, lengths, references):
+            if not t.is_contiguous():
+                raise ValueError("the cache's tensors must be contiguous")
+        self.codes, self.exponents = codes, exponents
+        self.block_table, self.lengths, self.references = block_table, lengths, references
+        self.device, self.kv_heads = device, codes.shape[3]
+        self._c = _KvCache(codes.shape[0], codes.shape[1], codes.shape[3], codes.shape[4],
+                           block_table.shape[0], block_table.shape[1], codes.data_ptr(),
+                           exponents.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
+                           references.data_ptr(), None, 0)
+        needed = _lib().nmoe_kv_workspace_bytes(ctypes.byref(self._c))
+        if needed == 0:
+            raise NmoeError(1, "KvCache", "a size is zero or too large")
+        self._workspace = torch.zeros(needed, dtype=torch.uint8, device=device)
+        self._c.workspace, self._c.workspace_bytes = self._workspace.data_ptr(), needed
+        self._ref = ctypes.byref(self._c)
+
+    @staticmethod
+    def allocate(layers: int, pages: int, kv_heads: int, max_sequences: int,
+                 max_pages_per_sequence: int, page_tokens: int = 64, device=None) -> "KvCache":
+        """An empty cache on the current device."""
+        if not torch.cuda.is_available():
+            raise RuntimeError("KvCache needs a CUDA device: there is no CPU path")
+        device = device or torch.device("cuda", torch.cuda.current_device())
+        int32 = dict(dtype=torch.int32, device=device)
+        codes = torch.zeros((layers, pages, 2, kv_heads, page_tokens, HEAD_DIM), dtype=torch.uint8,
+                            device=device).view(torch.float8_e4m3fn)
+        exponents = torch.zeros((layers, pages, 2, kv_heads), dtype=torch.int8, device=device)
+        return KvCache(codes, exponents, torch.zeros((max_sequences, max_pages_per_sequence), **int32),
+                       torch.zeros((max_sequences,), **int32), torch.zeros((pages,), **int32))
+
+    def _batch(self, sequences: torch.Tensor, offsets: torch.Tensor) -> None:
+        _require_current(self.device, "the cache")
+        _require_list(sequences, "sequences", self.device)
+        _require_list(offsets, "offsets", self.device)
+        if offsets.numel() != sequences.numel() + 1:
+            raise ValueError("offsets must have one entry more than sequences")
+
+    def extend(self, sequences: torch.Tensor, offsets: torch.Tensor, rows: int) -> None:
+        """Makes room for `rows` new tokens, entry i's offsets[i + 1] - offsets[i] of them: the
+        lowest free pages, in list order.  Too few: NMOE_ERR_CAPACITY from `sync_status`, and
+        nothing has changed."""
+        self._batch(sequences, offsets)
+        _check(_lib().nmoe_kv_extend(self._ref, _stream(), sequences.data_ptr(), offsets.data_ptr(),
+                                     sequences.numel(), rows), "nmoe_kv_extend")
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, sequences: torch.Tensor,
+               offsets: torch.Tensor) -> None:
+        """Quantises the rows into their places, the last tokens of each sequence."""
+        self._batch(sequences, offsets)
+        _require_rows(k, "k", self.device)
+        _require_rows(v, "v", self.device)
+        if k.shape != v.shape or k.shape[1] != self.kv_heads:
+            raise NmoeError(1, "KvCache.append", "k and v must be [rows, kv_heads, 128]")
+        _check(_lib().nmoe_kv_append(self._ref, _stream(), layer, k.data_ptr(), _row_stride(k),
+                                     v.data_ptr(), _row_stride(v), sequences.data_ptr(),
+                                     offsets.data_ptr(), sequences.numel(), k.shape[0]),
+               "nmoe_kv_append")
+
+    def attend(self, layer: int, q: torch.Tensor, sequences: torch.Tensor, offsets: torch.Tensor,
+               scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of new rows, the last tokens of their sequences: row j of c sees every token
+        up to position length - c + j.  Returns [rows, heads, 128] bf16."""
+        self._batch(sequences, offsets)
+        _require_rows(q, "q", self.device)
+        if q.shape[1] % self.kv_heads:
+            raise NmoeError(1, "KvCache.attend", "heads must be a multiple of kv_heads")
+        out = _output(out, q)
+        _check(_lib().nmoe_attention_cached(
+            self._ref, _stream(), layer, q.data_ptr(), _row_stride(q), q.shape[1],
+            sequences.data_ptr(), offsets.data_ptr(), sequences.numel(), q.shape[0],
+            HEAD_DIM ** -0.5 if scale is None else scale, out.data_ptr()), "nmoe_attention_cached")
+        return out
+
+    def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
+        """children[i] becomes a copy of parents[i]: full pages are shared, a partly filled last
+        one is copied.  What a child held is given up first."""
+        _require_current(self.device, "the cache")
+        _require_list(parents, "parents", self.device)
+        _require_list(children, "children", self.device)
+        if parents.numel() != children.numel():
+            raise ValueError("every child needs one parent")
+        _check(_lib().nmoe_kv_fork(self._ref, _stream(), parents.data_ptr(), children.data_ptr(),
+                                   parents.numel()), "nmoe_kv_fork")
+
+    def free(self, sequences: torch.Tensor) -> None:
+        """Gives up the sequences' pages; what nobody holds any more is free."""
+        _require_current(self.device, "the cache")
+        _require_list(sequences, "sequences", self.device)
+        _check(_lib().nmoe_kv_free(self._ref, _stream(), sequences.data_ptr(), sequences.numel()),
+               "nmoe_kv_free")
+
+    def compact(self) -> None:
+        """Moves the pages in use to the front of the pool, into the free ones there."""
+        _require_current(self.device, "the cache")
+        _check(_lib().nmoe_kv_compact(self._ref, _stream()), "nmoe_kv_compact")
+
+    def copy_pages(self, sources: torch.Tensor, targets: torch.Tensor) -> None:
+        """Copies pages in every layer; no target is a source or another's target."""
+        _require_current(self.device, "the cache")
+        _require_list(sources, "sources", self.device)
+        _require_list(targets, "targets", self.device)
+        if sources.numel() != targets.numel():
+            raise ValueError("every source needs one target")
+        _check(_lib().nmoe_kv_copy_pages(self._ref, _stream(), sources.data_ptr(),
+                                         targets.data_ptr(), sources.numel()), "nmoe_kv_copy_pages")
+
+    def sync_status(self) -> int:
+        """Waits for the current stream; what its calls on this cache could not do, and clears it."""
+        return _lib().nmoe_kv_sync_status(self._ref, _stream())

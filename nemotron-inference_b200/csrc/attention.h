@@ -1,0 +1,163 @@
+// Internal declarations of the attention operators: the paged 8-bit cache as kernels see it, and the
+// launchers behind the C ABI of attention_api.cu.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace nmoe {
+
+constexpr int kHeadDim = 128;
+constexpr int kMinExponent = -32, kMaxExponent = 32;  // of a page and head's scale, 2^exponent
+
+// What a kernel can leave in a cache's error word, beside kDevWaitTimeout.
+enum CacheError : int {
+  kCacheNoPages = 16,      // fewer free pages, or places in the block table, than asked for
+  kCacheBadSequence = 17,  // a sequence out of range or twice in a list, a page out of range
+};
+
+// Codes [layers][pages][2: keys, values][kv_heads][page_tokens][128], exponents without the last two.
+struct PagedCache {
+  int layers, pages, kv_heads, page_tokens, page_shift, max_sequences, max_pages;
+  uint8_t* codes;
+  int8_t* exponents;
+  int* table;       // [max_sequences][max_pages]
+  int* lengths;     // [max_sequences]
+  int* references;  // [pages]; 0: free
+  int* error;
+  int* move_count;   // pages for the copy kernel: the first *move_count of the two lists
+  int* move_source;  // [pages]
+  int* move_target;  // [pages]
+  int* remap;        // [max(pages, max_sequences)]: where a page went, a child's copy
+  int* claims;       // [max_sequences], zero between calls
+  char* attend_workspace;
+};
+
+// Rows of a batch: sequence i has the rows [offsets[i], offsets[i + 1]) of `rows`.
+struct Batch {
+  const int* sequences;
+  const int* offsets;
+  int count;
+  int rows;
+};
+
+struct BatchEntry {
+  int sequence, first, rows, length;  // length: tokens in the cache, these rows among them
+  bool valid;
+};
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ void report_cache_error(int* error, int code) {
+  if (error != nullptr) atomicCAS(error, 0, code);
+}
+
+// Entry i of a batch, brought into range: whatever the arrays hold, its rows lie within the batch's
+// and its tokens within the block table.
+__device__ __forceinline__ BatchEntry batch_entry(const PagedCache& c, const Batch& b, int i) {
+  BatchEntry e;
+  e.sequence = b.sequences[i];
+  const int from = b.offsets[i], to = b.offsets[i + 1];
+  e.first = min(max(from, 0), b.rows);
+  e.rows = min(max(to, e.first), b.rows) - e.first;
+  e.valid = static_cast<unsigned>(e.sequence) < static_cast<unsigned>(c.max_sequences) &&
+            from == e.first && to == e.first + e.rows;
+  e.length = 0;
+  if (e.valid) {
+    const int held = c.lengths[e.sequence];
+    const int64_t room = static_cast<int64_t>(c.max_pages) << c.page_shift;
+    e.valid = held >= e.rows && held <= room;
+    e.length = e.valid ? held : 0;
+  }
+  if (!e.valid) e.rows = 0;
+  return e;
+}
+
+__device__ __forceinline__ int pages_of(const PagedCache& c, int tokens) {
+  return (tokens >> c.page_shift) + ((tokens & (c.page_tokens - 1)) != 0);
+}
+
+// The page that holds tokens [page_tokens * place, ...) of a sequence, -1 for an entry out of range.
+__device__ __forceinline__ int page_at(const PagedCache& c, int sequence, int place) {
+  const int page = c.table[static_cast<size_t>(sequence) * c.max_pages + place];
+  return static_cast<unsigned>(page) < static_cast<unsigned>(c.pages) ? page : -1;
+}
+
+// Index of the (half, head) block of a page; its codes begin at this times page_tokens * 128.
+__device__ __forceinline__ size_t block_of_page(const PagedCache& c, int layer, int page, int half,
+                                                int head) {
+  return ((static_cast<size_t>(layer) * c.pages + page) * 2 + half) * c.kv_heads + head;
+}
+
+// Unit `u` of the units that entries 0..n-1 have (units(i) of them, in order): its entry and its place
+// in it, entry -1 behind the last.  Called by whole warps with the same u.
+template <typename Units>
+__device__ __forceinline__ int2 locate_unit(int n, int64_t u, Units units) {
+  const int lane = threadIdx.x & 31;
+  int64_t before = 0;
+  for (int start = 0; start < n; start += 32) {
+    const int i = start + lane;
+    const int mine = i < n ? units(i) : 0;
+    int64_t upto = mine;
+#pragma unroll
+    for (int step = 1; step < 32; step *= 2) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, upto, step);
+      if (lane >= step) upto += other;
+    }
+    const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
+    if (u < before + total) {
+      const int owner = __ffs(__ballot_sync(0xffffffffu, u < before + upto)) - 1;
+      const int place = static_cast<int>(u - (before + upto - mine));
+      return make_int2(start + owner, __shfl_sync(0xffffffffu, place, owner));
+    }
+    before += total;
+  }
+  return make_int2(-1, 0);
+}
+
+#endif  // __CUDACC__
+
+struct PrefillArgs {
+  const __nv_bfloat16* q;
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  int64_t q_stride, k_stride, v_stride;  // elements from one token's row to the next
+  int tokens, heads, kv_heads;
+  const int* offsets;
+  int sequences;
+  float scale;
+  __nv_bfloat16* out;  // [tokens][heads][128]
+  float* lse;          // [tokens][heads], may be null
+  int* error;          // may be null
+};
+
+struct CachedArgs {
+  PagedCache cache;
+  Batch batch;
+  int layer;
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  int heads;
+  float scale;
+  __nv_bfloat16* out;
+};
+
+cudaError_t launch_attention_prefill(const PrefillArgs& args, cudaStream_t stream);
+size_t attention_cached_workspace_bytes();
+cudaError_t launch_attention_cached(const CachedArgs& args, cudaStream_t stream);
+cudaError_t launch_kv_append(const PagedCache& cache, const Batch& batch, int layer,
+                             const __nv_bfloat16* k, int64_t k_stride, const __nv_bfloat16* v,
+                             int64_t v_stride, cudaStream_t stream);
+cudaError_t launch_kv_extend(const PagedCache& cache, const Batch& batch, cudaStream_t stream);
+cudaError_t launch_kv_fork(const PagedCache& cache, const int* parents, const int* children, int count,
+                           cudaStream_t stream);
+cudaError_t launch_kv_free(const PagedCache& cache, const int* sequences, int count,
+                           cudaStream_t stream);
+cudaError_t launch_kv_compact(const PagedCache& cache, cudaStream_t stream);
+cudaError_t launch_kv_copy_pages(const PagedCache& cache, const int* sources, const int* targets,
+                                 int count, cudaStream_t stream);
+
+}  // namespace nmoe

@@ -1,0 +1,531 @@
+// The paged 8-bit cache of keys and values: new rows are quantised into it, its pages are handed out,
+// shared, copied, moved and given back.  Everything is decided on the device: a step launches these
+// kernels without reading a length or a free page on the host, and can be recorded once and replayed.
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "attention.h"
+#include "common.cuh"
+#include "kernels.h"
+
+namespace nmoe {
+namespace {
+
+// ---------------------------------------------------------------------------
+// New rows
+// ---------------------------------------------------------------------------
+
+// The least e with amax <= 448 * 2^e (448 = 1.75 * 2^8).
+__device__ __forceinline__ int exponent_for(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  const int power = static_cast<int>(bits >> 23) - 127;
+  const int e = power - 8 + ((bits & 0x7fffffu) > 0x600000u);
+  return min(max(e, kMinExponent), kMaxExponent);
+}
+
+__device__ __forceinline__ float power_of_two(int e) {
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+// Two values to two codes; values beyond the range saturate, NaN becomes NaN.
+__device__ __forceinline__ uint32_t encode_two(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+__device__ __forceinline__ float2 decode_two(uint32_t codes) {
+  const __half2_raw h =
+      __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes & 0xffffu), __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+constexpr int kAppendThreads = 256;
+constexpr int kAppendChunks = 128 * kHeadDim / 8 / kAppendThreads;  // of 8 values, the largest page
+
+// A block per page that gets new rows, head, and keys or values.  The page's new values stay in
+// registers between the maximum that gives the exponent and their rounding, so they are read once.
+// A page that held tokens may get a larger exponent: its older codes are rounded again then, which
+// is exact but for values that fall among the subnormal codes.
+__global__ void __launch_bounds__(kAppendThreads)
+    kv_append_kernel(PagedCache c, Batch b, int layer, const __nv_bfloat16* k, int64_t k_stride,
+                     const __nv_bfloat16* v, int64_t v_stride) {
+  __shared__ float warp_max[kAppendThreads / 32];
+  if (*c.error != 0) return;  // a reservation failed: these rows have no place of their own
+  const int half = blockIdx.y & 1, head = blockIdx.y >> 1;
+  const int2 unit = locate_unit(b.count, blockIdx.x, [&](int i) {
+    const BatchEntry e = batch_entry(c, b, i);
+    if (!e.valid) report_cache_error(c.error, kCacheBadSequence);
+    if (e.rows == 0) return 0;
+    return ((e.length - 1) >> c.page_shift) - ((e.length - e.rows) >> c.page_shift) + 1;
+  });
+  if (unit.x < 0) return;
+  const BatchEntry e = batch_entry(c, b, unit.x);
+  const int place = ((e.length - e.rows) >> c.page_shift) + unit.y;
+  const int begin = max(e.length - e.rows, place << c.page_shift);  // positions in the sequence
+  const int end = min(e.length, (place + 1) << c.page_shift);
+  const int held = begin & (c.page_tokens - 1);
+  const int page = page_at(c, e.sequence, place);
+  if (page < 0) {
+    report_cache_error(c.error, kCacheBadSequence);
+    return;
+  }
+  const size_t block = block_of_page(c, layer, page, half, head);
+  uint8_t* codes = c.codes + block * c.page_tokens * kHeadDim;
+  const int before = c.exponents[block];
+  const int64_t stride = half ? v_stride : k_stride;
+  const __nv_bfloat16* from = (half ? v : k) + head * kHeadDim +
+                              (e.first + begin - (e.length - e.rows)) * stride;
+  const int chunks = (end - begin) * (kHeadDim / 8);
+  uint4 raw[kAppendChunks];
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kAppendChunks; ++i) {
+    const int chunk = i * kAppendThreads + threadIdx.x;
+    if (chunk < chunks) {
+      raw[i] = *reinterpret_cast<const uint4*>(from + (chunk / 16) * stride + (chunk % 16) * 8);
+      const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float lo = fabsf(__uint_as_float(words[w] << 16));
+        const float hi = fabsf(__uint_as_float(words[w] & 0xffff0000u));
+        if (lo < INFINITY) amax = fmaxf(amax, lo);
+        if (hi < INFINITY) amax = fmaxf(amax, hi);
+      }
+    }
+  }
+#pragma unroll
+  for (int step = 16; step > 0; step /= 2) {
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, step));
+  }
+  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, warp_max[w]);
+  int after = exponent_for(amax);
+  if (held > 0) after = max(after, before);
+  if (threadIdx.x == 0) c.exponents[block] = static_cast<int8_t>(after);
+  if (held > 0 && after > before) {
+    const float lower = power_of_two(before - after);
+    uint4* older = reinterpret_cast<uint4*>(codes);
+    for (int i = threadIdx.x; i < held * (kHeadDim / 16); i += kAppendThreads) {
+      uint4 x = older[i];
+      uint32_t* words = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float2 a = decode_two(words[w]), z = decode_two(words[w] >> 16);
+        words[w] = encode_two(a.x * lower, a.y * lower) | (encode_two(z.x * lower, z.y * lower) << 16);
+      }
+      older[i] = x;
+    }
+  }
+  const float factor = power_of_two(-after);
+#pragma unroll
+  for (int i = 0; i < kAppendChunks; ++i) {
+    const int chunk = i * kAppendThreads + threadIdx.x;
+    if (chunk < chunks) {
+      const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      uint32_t two[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float lo = __uint_as_float(words[w] << 16), hi = __uint_as_float(words[w] & 0xffff0000u);
+        // an infinity is not hidden behind the largest code
+        lo = fabsf(lo) < INFINITY ? lo * factor : NAN;
+        hi = fabsf(hi) < INFINITY ? hi * factor : NAN;
+        two[w] = encode_two(lo, hi);
+      }
+      *reinterpret_cast<uint2*>(codes + held * kHeadDim + chunk * 8) =
+          make_uint2(two[0] | (two[1] << 16), two[2] | (two[3] << 16));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Pages.  One block keeps the books: lists are short, and every decision (which free page goes to
+// whom) follows from a sum over those before.
+// ---------------------------------------------------------------------------
+
+constexpr int kBookThreads = 1024;
+
+struct BookShared {
+  int warp_sums[kBookThreads / 32];
+  int flag;
+  int released;
+};
+
+// Exclusive sum of `mine` over the block; `total` is the whole sum.
+__device__ int block_prefix(int mine, BookShared& s, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int upto = mine;
+#pragma unroll
+  for (int step = 1; step < 32; step *= 2) {
+    const int other = __shfl_up_sync(0xffffffffu, upto, step);
+    if (lane >= step) upto += other;
+  }
+  __syncthreads();  // (the sums of the call before are read)
+  if (lane == 31) s.warp_sums[warp] = upto;
+  __syncthreads();
+  int below = 0;
+  total = 0;
+  const int other = s.warp_sums[lane];
+#pragma unroll
+  for (int w = 0; w < kBookThreads / 32; ++w) {
+    const int sum = __shfl_sync(0xffffffffu, other, w);
+    if (w < warp) below += sum;
+    total += sum;
+  }
+  return below + upto - mine;
+}
+
+// The `need` lowest free pages into `list`; false when there are fewer.
+__device__ bool list_free_pages(const PagedCache& c, int need, int* list, BookShared& s) {
+  int found = 0;
+  for (int start = 0; start < c.pages && found < need; start += kBookThreads) {
+    const int page = start + threadIdx.x;
+    const bool is_free = page < c.pages && c.references[page] == 0;
+    int total;
+    const int rank = found + block_prefix(is_free, s, total);
+    if (is_free && rank < need) list[rank] = page;
+    found += total;
+  }
+  __syncthreads();
+  return found >= need;
+}
+
+// Marks the sequences of a list as taken; a second mark, or one out of range, raises s.flag.
+__device__ void claim(const PagedCache& c, int sequence, BookShared& s) {
+  if (static_cast<unsigned>(sequence) >= static_cast<unsigned>(c.max_sequences) ||
+      atomicAdd(&c.claims[sequence], 1) != 0) {
+    s.flag = kCacheBadSequence;
+  }
+}
+
+__device__ void unclaim(const PagedCache& c, int sequence) {
+  if (static_cast<unsigned>(sequence) < static_cast<unsigned>(c.max_sequences)) {
+    c.claims[sequence] = 0;
+  }
+}
+
+__device__ __forceinline__ int held_tokens(const PagedCache& c, int sequence) {
+  const int64_t room = static_cast<int64_t>(c.max_pages) << c.page_shift;
+  const int held = c.lengths[sequence];
+  return held < 0 ? 0 : held > room ? static_cast<int>(room) : held;
+}
+
+// The rows that sequence i of the list is to get; s.flag where the books do not allow it.
+__device__ int extension(const PagedCache& c, const Batch& b, int i, int& old_length, BookShared& s) {
+  const int rows = b.offsets[i + 1] - b.offsets[i];
+  old_length = held_tokens(c, b.sequences[i]);
+  if (rows < 0 || b.offsets[i] < 0 || b.offsets[i + 1] > b.rows) {
+    s.flag = kCacheBadSequence;
+    return 0;
+  }
+  if (static_cast<int64_t>(old_length) + rows > (static_cast<int64_t>(c.max_pages) << c.page_shift)) {
+    s.flag = kCacheNoPages;
+    return 0;
+  }
+  return rows;
+}
+
+__global__ void __launch_bounds__(kBookThreads) kv_extend_kernel(PagedCache c, Batch b) {
+  __shared__ BookShared s;
+  if (*c.error != 0) return;
+  if (threadIdx.x == 0) s.flag = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < b.count; i += kBookThreads) claim(c, b.sequences[i], s);
+  __syncthreads();
+  int need = 0;
+  if (s.flag == 0) {
+    __syncthreads();
+    for (int start = 0; start < b.count; start += kBookThreads) {
+      const int i = start + threadIdx.x;
+      int mine = 0, held;
+      if (i < b.count) {
+        const int rows = extension(c, b, i, held, s);
+        mine = pages_of(c, held + rows) - pages_of(c, held);
+      }
+      int total;
+      block_prefix(mine, s, total);
+      need = min(need + total, c.pages + 1);
+    }
+    __syncthreads();
+    if (s.flag == 0) {
+      __syncthreads();
+      if (!list_free_pages(c, need, c.move_target, s) && threadIdx.x == 0) s.flag = kCacheNoPages;
+    }
+  }
+  __syncthreads();
+  if (s.flag == 0) {
+    int before = 0;
+    for (int start = 0; start < b.count; start += kBookThreads) {
+      const int i = start + threadIdx.x;
+      int mine = 0, held = 0, rows = 0;
+      if (i < b.count) {
+        rows = extension(c, b, i, held, s);
+        mine = pages_of(c, held + rows) - pages_of(c, held);
+      }
+      int total;
+      const int at = before + block_prefix(mine, s, total);
+      if (i < b.count) {
+        const int sequence = b.sequences[i];
+        int* row = c.table + static_cast<size_t>(sequence) * c.max_pages + pages_of(c, held);
+        for (int j = 0; j < mine; ++j) {
+          const int page = c.move_target[at + j];
+          row[j] = page;
+          c.references[page] = 1;
+        }
+        c.lengths[sequence] = held + rows;
+      }
+      before += total;
+    }
+  } else if (threadIdx.x == 0) {
+    report_cache_error(c.error, s.flag);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < b.count; i += kBookThreads) unclaim(c, b.sequences[i]);
+}
+
+// Adds `change` to the references of the pages that a list's sequences hold; a warp per sequence.
+__device__ void count_pages(const PagedCache& c, const int* sequences, int count, int change) {
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < count; i += kBookThreads / 32) {
+    const int sequence = sequences[i], held = pages_of(c, held_tokens(c, sequence));
+    for (int place = lane; place < held; place += 32) {
+      const int page = page_at(c, sequence, place);
+      if (page >= 0) atomicAdd(&c.references[page], change);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kBookThreads)
+    kv_free_kernel(PagedCache c, const int* sequences, int count) {
+  __shared__ BookShared s;
+  if (*c.error != 0) return;
+  if (threadIdx.x == 0) s.flag = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < count; i += kBookThreads) claim(c, sequences[i], s);
+  __syncthreads();
+  if (s.flag == 0) {
+    count_pages(c, sequences, count, -1);
+    __syncthreads();
+    for (int i = threadIdx.x >> 5; i < count; i += kBookThreads / 32) {
+      const int sequence = sequences[i], held = pages_of(c, held_tokens(c, sequence));
+      int* row = c.table + static_cast<size_t>(sequence) * c.max_pages;
+      for (int place = threadIdx.x & 31; place < held; place += 32) row[place] = 0;
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) c.lengths[sequence] = 0;
+    }
+  } else if (threadIdx.x == 0) {
+    report_cache_error(c.error, s.flag);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < count; i += kBookThreads) unclaim(c, sequences[i]);
+}
+
+// The books of a fork.  The children's own pages are given up first, so that they can serve as the
+// copies; where the free ones do not suffice all the same, they are taken back.
+__global__ void __launch_bounds__(kBookThreads)
+    kv_fork_kernel(PagedCache c, const int* parents, const int* children, int count) {
+  __shared__ BookShared s;
+  if (threadIdx.x == 0) {
+    s.flag = 0;
+    *c.move_count = 0;
+  }
+  if (*c.error != 0) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < count; i += kBookThreads) claim(c, children[i], s);
+  __syncthreads();
+  for (int i = threadIdx.x; i < count; i += kBookThreads) {
+    const int parent = parents[i];  // in range, and no child
+    if (static_cast<unsigned>(parent) >= static_cast<unsigned>(c.max_sequences) ||
+        c.claims[parent] != 0) {
+      s.flag = kCacheBadSequence;
+    }
+  }
+  __syncthreads();
+  if (s.flag == 0) {
+    count_pages(c, children, count, -1);
+    int need = 0;
+    for (int start = 0; start < count; start += kBookThreads) {
+      const int i = start + threadIdx.x;
+      const int mine = i < count && (held_tokens(c, parents[i]) & (c.page_tokens - 1)) != 0;
+      int total;
+      const int at = need + block_prefix(mine, s, total);
+      if (mine && at < c.pages) {
+        const int sequence = parents[i];
+        c.move_source[at] = page_at(c, sequence, pages_of(c, held_tokens(c, sequence)) - 1);
+        if (c.move_source[at] < 0) s.flag = kCacheBadSequence;
+      }
+      need += total;
+    }
+    __syncthreads();
+    const bool enough = need <= c.pages && list_free_pages(c, need, c.move_target, s);
+    if (!enough && threadIdx.x == 0) s.flag = kCacheNoPages;
+    __syncthreads();
+    if (s.flag != 0) {
+      count_pages(c, children, count, 1);
+    } else {
+      int before = 0;
+      for (int start = 0; start < count; start += kBookThreads) {
+        const int i = start + threadIdx.x;
+        const int mine = i < count && (held_tokens(c, parents[i]) & (c.page_tokens - 1)) != 0;
+        int total;
+        const int at = before + block_prefix(mine, s, total);
+        if (mine) c.remap[i] = c.move_target[at];  // (count <= pages where every parent has one)
+        before += total;
+      }
+      __syncthreads();
+      for (int i = threadIdx.x >> 5; i < count; i += kBookThreads / 32) {
+        const int tokens = held_tokens(c, parents[i]), full = tokens >> c.page_shift;
+        const bool partial = (tokens & (c.page_tokens - 1)) != 0;
+        int* row = c.table + static_cast<size_t>(children[i]) * c.max_pages;
+        for (int place = threadIdx.x & 31; place < c.max_pages; place += 32) {
+          int page = 0;
+          if (place < full) {
+            page = max(page_at(c, parents[i], place), 0);
+            atomicAdd(&c.references[page], 1);
+          } else if (place == full && partial) {
+            page = c.remap[i];
+            c.references[page] = 1;
+          }
+          row[place] = page;
+        }
+        if ((threadIdx.x & 31) == 0) c.lengths[children[i]] = tokens;
+      }
+      if (threadIdx.x == 0) *c.move_count = need;
+    }
+  }
+  __syncthreads();
+  if (s.flag != 0 && threadIdx.x == 0) report_cache_error(c.error, s.flag);
+  for (int i = threadIdx.x; i < count; i += kBookThreads) unclaim(c, children[i]);
+}
+
+// The books of a compaction: with L pages in use, the i-th of them at or above L goes to the i-th free
+// one below L.  The block table follows in the copy kernel, which has the threads for it.
+__global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) {
+  __shared__ BookShared s;
+  if (threadIdx.x == 0) *c.move_count = 0;
+  if (*c.error != 0) return;
+  int live = 0;
+  for (int page = threadIdx.x; page < c.pages; page += kBookThreads) {
+    live += c.references[page] > 0;
+    c.remap[page] = page;
+  }
+  int total;
+  block_prefix(live, s, total);
+  live = total;
+  int sources = 0, targets = 0;
+  for (int start = 0; start < c.pages; start += kBookThreads) {
+    const int page = start + threadIdx.x;
+    const bool used = page < c.pages && c.references[page] > 0;
+    const bool source = used && page >= live, target = page < live && !used;
+    const int s_at = sources + block_prefix(source, s, total);
+    sources += total;
+    const int t_at = targets + block_prefix(target, s, total);
+    targets += total;
+    if (source) c.move_source[s_at] = page;
+    if (target) c.move_target[t_at] = page;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < sources; i += kBookThreads) {
+    const int from = c.move_source[i], to = c.move_target[i];
+    c.remap[from] = to;
+    c.references[to] = c.references[from];
+    c.references[from] = 0;
+  }
+  if (threadIdx.x == 0) *c.move_count = sources;
+}
+
+// ---------------------------------------------------------------------------
+// Contents of pages, all layers
+// ---------------------------------------------------------------------------
+
+constexpr int kCopyThreads = 256;
+
+__global__ void __launch_bounds__(kCopyThreads)
+    kv_copy_kernel(PagedCache c, const int* sources, const int* targets, const int* count_at,
+                   int count, bool rewrite_table) {
+  if (count_at != nullptr) {
+    if (*c.error != 0) return;
+    count = *count_at;
+  }
+  const int heads2 = 2 * c.kv_heads;
+  const size_t page_bytes = static_cast<size_t>(heads2) * c.page_tokens * kHeadDim;
+  for (int64_t u = blockIdx.x; u < static_cast<int64_t>(count) * c.layers; u += gridDim.x) {
+    const int from = sources[u / c.layers], to = targets[u / c.layers];
+    const size_t layer = u % c.layers;
+    if (static_cast<unsigned>(from) >= static_cast<unsigned>(c.pages) ||
+        static_cast<unsigned>(to) >= static_cast<unsigned>(c.pages)) {
+      report_cache_error(c.error, kCacheBadSequence);
+      continue;
+    }
+    const uint4* read = reinterpret_cast<const uint4*>(c.codes + (layer * c.pages + from) * page_bytes);
+    uint4* write = reinterpret_cast<uint4*>(c.codes + (layer * c.pages + to) * page_bytes);
+    for (size_t i = threadIdx.x; i < page_bytes / 16; i += kCopyThreads) write[i] = read[i];
+    for (int i = threadIdx.x; i < heads2; i += kCopyThreads) {
+      c.exponents[(layer * c.pages + to) * heads2 + i] = c.exponents[(layer * c.pages + from) * heads2 + i];
+    }
+  }
+  if (!rewrite_table) return;
+  const int warps = gridDim.x * (kCopyThreads / 32);
+  for (int i = (blockIdx.x * kCopyThreads + threadIdx.x) >> 5; i < c.max_sequences; i += warps) {
+    const int held = pages_of(c, held_tokens(c, i));
+    int* row = c.table + static_cast<size_t>(i) * c.max_pages;
+    for (int place = threadIdx.x & 31; place < held; place += 32) {
+      const int page = page_at(c, i, place);
+      if (page >= 0) row[place] = c.remap[page];
+    }
+  }
+}
+
+cudaError_t launch_copy(const PagedCache& cache, const int* sources, const int* targets,
+                        const int* count_at, int count, bool rewrite_table, cudaStream_t stream) {
+  kv_copy_kernel<<<device_sms() * 8, kCopyThreads, 0, stream>>>(cache, sources, targets, count_at,
+                                                                count, rewrite_table);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_kv_append(const PagedCache& cache, const Batch& batch, int layer,
+                             const __nv_bfloat16* k, int64_t k_stride, const __nv_bfloat16* v,
+                             int64_t v_stride, cudaStream_t stream) {
+  // c rows of a sequence touch at most c / page_tokens + 2 pages, and no more than c
+  const int64_t units = std::min<int64_t>(
+      batch.rows, (batch.rows >> cache.page_shift) + 2 * static_cast<int64_t>(batch.count));
+  kv_append_kernel<<<dim3(static_cast<unsigned>(units), 2 * cache.kv_heads), kAppendThreads, 0,
+                     stream>>>(cache, batch, layer, k, k_stride, v, v_stride);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv_extend(const PagedCache& cache, const Batch& batch, cudaStream_t stream) {
+  kv_extend_kernel<<<1, kBookThreads, 0, stream>>>(cache, batch);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv_fork(const PagedCache& cache, const int* parents, const int* children, int count,
+                           cudaStream_t stream) {
+  kv_fork_kernel<<<1, kBookThreads, 0, stream>>>(cache, parents, children, count);
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  return launch_copy(cache, cache.move_source, cache.move_target, cache.move_count, 0, false, stream);
+}
+
+cudaError_t launch_kv_free(const PagedCache& cache, const int* sequences, int count,
+                           cudaStream_t stream) {
+  kv_free_kernel<<<1, kBookThreads, 0, stream>>>(cache, sequences, count);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv_compact(const PagedCache& cache, cudaStream_t stream) {
+  kv_compact_kernel<<<1, kBookThreads, 0, stream>>>(cache);
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  return launch_copy(cache, cache.move_source, cache.move_target, cache.move_count, 0, true, stream);
+}
+
+cudaError_t launch_kv_copy_pages(const PagedCache& cache, const int* sources, const int* targets,
+                                 int count, cudaStream_t stream) {
+  return launch_copy(cache, sources, targets, nullptr, count, false, stream);
+}
+
+}  // namespace nmoe
