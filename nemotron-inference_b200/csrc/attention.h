@@ -2,6 +2,7 @@
 // launchers behind the C ABI of attention_api.cu.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -131,7 +132,7 @@ struct PrefillArgs {
   float scale;
   __nv_bfloat16* out;  // [tokens][heads][128]
   float* lse;          // [tokens][heads], may be null
-  int* error;          // may be null
+  int* error;
 };
 
 struct CachedArgs {
@@ -144,6 +145,10 @@ struct CachedArgs {
   float scale;
   __nv_bfloat16* out;
 };
+
+// bf16 rows of heads x 128 as [rows][heads * 128], boxes of 64 columns x box_rows, 128-byte swizzle.
+bool rows_tensor_map(const void* base, int64_t rows, int64_t heads, int64_t stride, int box_rows,
+                     CUtensorMap* map);
 
 cudaError_t launch_attention_prefill(const PrefillArgs& args, cudaStream_t stream);
 size_t attention_cached_workspace_bytes();

@@ -121,6 +121,43 @@ bool scale_valid(float scale) { return std::isfinite(scale) && scale > 0.0f; }
 
 }  // namespace
 
+namespace nmoe {
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                 CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+  static const EncodeTiled found = [] {
+    void* symbol = nullptr;
+    cudaDriverEntryPointQueryResult query;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &symbol, cudaEnableDefault, &query) !=
+            cudaSuccess ||
+        query != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      symbol = nullptr;
+    }
+    return reinterpret_cast<EncodeTiled>(symbol);
+  }();
+  return found;
+}
+
+bool rows_tensor_map(const void* base, int64_t rows, int64_t heads, int64_t stride, int box_rows,
+                     CUtensorMap* map) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(heads) * kHeadDim, static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+  const cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t steps[2] = {1u, 1u};
+  const EncodeTiled encode = encode_tiled();
+  return encode != nullptr &&
+         encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+                steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace nmoe
+
 extern "C" {
 
 size_t nmoe_kv_workspace_bytes(const nmoe_kv_cache* cache) {
@@ -242,7 +279,7 @@ nmoe_status nmoe_attention_prefill(void* stream, const void* q, int64_t q_stride
   if (tokens == 0 || count == 0) return NMOE_OK;
   if (!rows_valid(q, q_stride, heads) || !rows_valid(k, k_stride, kv_heads) ||
       !rows_valid(v, v_stride, kv_heads) || offsets == nullptr || out == nullptr ||
-      misaligned(out, 16)) {
+      misaligned(out, 16) || error == nullptr) {
     return NMOE_ERR_INVALID_ARGUMENT;
   }
   nmoe::PrefillArgs args;

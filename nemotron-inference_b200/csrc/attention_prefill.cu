@@ -1,36 +1,520 @@
 // Causal attention over whole prompts packed one behind the other.
-#include "attention_simple.cuh"
+//
+//   s_tj = scale q_t . k_j for j <= t,  m_t = max_j s_tj,  o_t = sum_j e^(s_tj - m_t) v_j / sum_j e^(s_tj - m_t)
+//
+// in one pass over the keys: 128 rows against 128 keys at a time, the running maximum and sum of a row
+// in the registers of one thread, scores and results in TMEM.
+//
+// A block works on two tiles of 128 query rows of one key head, so that each key and value tile that it
+// brings in serves both, and one tile's exponentials run while the tensor cores work on the other.  The
+// tiles are the same rows of two heads where a key head has an even number of them (the two then
+// have as many key tiles each), else consecutive rows of one head.  Per key tile and query tile:
+//   S = Q K^T      8 MMAs of 128 x 128 x 16, shared memory x shared memory -> TMEM
+//   softmax warps  S -> registers, P = 2^(c S - c m) as bf16 back into TMEM, over S
+//   O += P V       8 MMAs, TMEM x shared memory -> TMEM
+// The reference m of a row is the maximum that it began with; only when a maximum has risen by more
+// than 2^8 are O and the sum scaled anew, which keeps P within bf16's precision and the exponentials
+// far from overflow, and which hardly ever happens after a row's first tile.
+//
+// Blocks ask for further blocks of the grid as they finish (no counter in memory, nothing to clear), so
+// loads of the next tiles go on during the last exponentials of the current ones.
+#include <algorithm>
+
+#include "attention.h"
+#include "attention_mma.cuh"
+#include "kernels.h"
 
 namespace nmoe {
 namespace {
 
-__global__ void __launch_bounds__(kHeadDim) prefill_row_kernel(PrefillArgs args) {
-  const int row = blockIdx.x, head = blockIdx.y;
-  int sequence = -1, first = 0;
-  for (int i = 0; i < args.sequences; ++i) {
-    const int from = max(args.offsets[i], 0), to = min(args.offsets[i + 1], args.tokens);
-    if (row >= from && row < to) {
-      sequence = i;
-      first = from;
+constexpr int kTile = 128;                    // query rows, and keys, of a tile
+constexpr int kTileBytes = kTile * kHeadDim * 2;
+constexpr int kPanelBytes = kTileBytes / 2;   // 64 of the 128 dimensions: rows of 128 bytes
+constexpr int kSlots = 5;                     // key and value tiles in flight, in turn
+constexpr int kSoftmaxWarps = 8;              // four per query tile, a thread per row
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kThreads = 384;                 // two warps have nothing to do: registers go by four warps
+constexpr int kSoftmaxRegisters = 216, kOtherRegisters = 72;  // 2 * 216 + 72 = 3 * 168, as launched
+constexpr int kTmemColumns = 512;             // S of both tiles, O of both tiles, 128 columns each
+constexpr float kRescale = 8.0f;              // binary orders by which a maximum may outgrow its reference
+
+struct Work {
+  int first, length;   // the prompt's first row, its rows
+  int head[2], row[2]; // of each tile; row: first query row in the prompt
+  int tiles[2];        // key tiles of each, 0: no such tile
+  int kv_head;
+};
+
+struct Control {
+  uint64_t q_full[2], q_empty[2], kv_full[kSlots], kv_empty[kSlots];
+  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t work_full[2], work_empty[2], next_full, drained;
+  alignas(16) uint32_t next[4];
+  Work work[2];
+  int has_work[2];
+  uint32_t tmem;
+  int bad_values;  // a value in a masked tile is no number
+};
+
+constexpr size_t kSharedBytes = 1024 + (2 + kSlots) * kTileBytes + sizeof(Control);
+static_assert(kSharedBytes <= kMaxSharedBytes);
+
+__device__ __forceinline__ bool is_no_number(uint32_t two_bf16) {
+  return (two_bf16 & 0x7f80u) == 0x7f80u || (two_bf16 & 0x7f800000u) == 0x7f800000u;
+}
+
+// What block `index` of the grid works on; a warp together.  Prompts in order, their last rows (which
+// have the most keys) first, the heads that share keys next to one another.
+__device__ __forceinline__ bool find_work(const PrefillArgs& args, bool two_heads, int index, Work& w) {
+  const int rows = two_heads ? kTile : 2 * kTile;
+  const int columns = two_heads ? args.heads / 2 : args.heads;
+  const int column = index % columns;
+  auto bounds = [&](int i, int& from, int& length) {
+    from = min(max(args.offsets[i], 0), args.tokens);
+    length = min(max(args.offsets[i + 1], from), args.tokens) - from;
+  };
+  const int2 unit = locate_unit(args.sequences, index / columns, [&](int i) {
+    int from, length;
+    bounds(i, from, length);
+    return (length + rows - 1) / rows;
+  });
+  if (unit.x < 0) return false;
+  bounds(unit.x, w.first, w.length);
+  const int row = ((w.length + rows - 1) / rows - 1 - unit.y) * rows;
+  const int head = two_heads ? 2 * column : column;
+  w.kv_head = head / (args.heads / args.kv_heads);
+  w.head[0] = head;
+  w.head[1] = two_heads ? head + 1 : head;
+  w.row[0] = row;
+  w.row[1] = two_heads ? row : row + kTile;
+  w.tiles[0] = row / kTile + 1;
+  w.tiles[1] = w.row[1] < w.length ? w.row[1] / kTile + 1 : 0;
+  return true;
+}
+
+// Brings queries, keys and values in.  The whole warp runs it, one lane issues.
+__device__ void load_role(const PrefillArgs& args, bool two_heads, const CUtensorMap* q_map,
+                          const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t q_at,
+                          uint32_t slots_at, Control* c) {
+  uint32_t loads = 0, q_loads[2] = {0, 0}, items = 0;
+  int index = blockIdx.x;
+  bool ok = true;
+  for (;; ++items) {
+    Work w;
+    const bool some = index >= 0 && find_work(args, two_heads, index, w);
+    const uint32_t place = items & 1;
+    if (!(ok = wait_warp(smem_u32(&c->work_empty[place]), ((items >> 1) & 1) ^ 1))) break;
+    if (elect_one()) {
+      c->work[place] = w;
+      c->has_work[place] = some;
+      mbar_arrive(&c->work_full[place]);
+      if (some) {
+        fence_proxy_async_smem();  // (the answer before this one has been read)
+        mbar_arrive_expect_tx(&c->next_full, 16);
+        request_next_block(smem_u32(c->next), smem_u32(&c->next_full));
+      }
+    }
+    __syncwarp();
+    if (!some) break;
+    const int most = max(w.tiles[0], w.tiles[1]);
+    for (int load = 0; load < 2 * most && ok; ++load) {
+      if (load == 0) {  // (the queries go with the first keys)
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (w.tiles[t] == 0) continue;
+          if (!(ok = wait_warp(smem_u32(&c->q_empty[t]), (q_loads[t] & 1) ^ 1))) break;
+          ++q_loads[t];
+          if (elect_one()) {
+            const uint32_t bar = smem_u32(&c->q_full[t]);
+            mbar_arrive_expect_tx_at(bar, kTileBytes);
+            for (int panel = 0; panel < 2; ++panel) {
+              tma_load_2d_at(q_at + t * kTileBytes + panel * kPanelBytes, q_map,
+                             w.head[t] * kHeadDim + panel * 64, w.first + w.row[t], bar);
+            }
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+      }
+      const uint32_t slot = loads % kSlots;
+      if (!(ok = wait_warp(smem_u32(&c->kv_empty[slot]), ((loads / kSlots) & 1) ^ 1))) break;
+      if (elect_one()) {
+        const uint32_t bar = smem_u32(&c->kv_full[slot]);
+        mbar_arrive_expect_tx_at(bar, kTileBytes);
+        for (int panel = 0; panel < 2; ++panel) {
+          tma_load_2d_at(slots_at + slot * kTileBytes + panel * kPanelBytes, load & 1 ? v_map : k_map,
+                         w.kv_head * kHeadDim + panel * 64, w.first + (load >> 1) * kTile, bar);
+        }
+      }
+      __syncwarp();
+      ++loads;
+    }
+    if (!ok) break;
+    if (!(ok = wait_warp(smem_u32(&c->next_full), items & 1))) break;
+    index = next_block(smem_u32(c->next));
+  }
+  if (ok) return;
+  if (elect_one()) report_cache_error(args.error, kDevWaitTimeout);
+  // what is in flight arrives before the block's shared memory is given up
+  for (uint32_t back = 1; back <= min(loads, static_cast<uint32_t>(kSlots)); ++back) {
+    const uint32_t load = loads - back;
+    wait_warp(smem_u32(&c->kv_full[load % kSlots]), (load / kSlots) & 1);
+  }
+  for (int t = 0; t < 2; ++t) {
+    if (q_loads[t]) wait_warp(smem_u32(&c->q_full[t]), (q_loads[t] - 1) & 1);
+  }
+}
+
+struct MmaRole {
+  Control* c;
+  uint32_t q_at, slots_at, tmem;
+  uint32_t loads = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0}, o_uses[2] = {0, 0};
+
+  // S of tile t against the keys in `slot`.
+  __device__ void scores(int t, uint32_t slot) {
+    constexpr uint32_t idesc = make_idesc_bf16(kTile, false);
+    const uint64_t a = make_smem_desc(q_at + t * kTileBytes, 16, 1024, 2);
+    const uint64_t b = make_smem_desc(slots_at + slot * kTileBytes, 16, 1024, 2);
+    if (elect_one()) {
+#pragma unroll
+      for (int k = 0; k < kHeadDim / 16; ++k) {
+        const uint32_t at = (k / 4) * kPanelBytes + (k % 4) * 32;
+        mma_f16_ss(tmem + t * kTile, advance_smem_desc(a, at), advance_smem_desc(b, at), idesc, k > 0);
+      }
+      tcgen05_commit(&c->s_full[t]);
+    }
+    __syncwarp();
+  }
+
+  // O of tile t, with the values in `slot`: a token's row is 128 consecutive n, 64 to a panel; eight
+  // tokens are 1024 bytes.
+  __device__ void values(int t, uint32_t slot, bool first, bool last) {
+    constexpr uint32_t idesc = make_idesc_bf16(kHeadDim, true);
+    const uint64_t b = make_smem_desc(slots_at + slot * kTileBytes, kPanelBytes, 1024, 2);
+    if (elect_one()) {
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k) {
+        mma_f16_ts(tmem + 2 * kTile + t * kHeadDim, tmem + t * kTile + k * 8,
+                   advance_smem_desc(b, k * 2048), idesc, !first || k > 0);
+      }
+      if (last) tcgen05_commit(&c->o_full[t]);
+    }
+    __syncwarp();
+  }
+
+  __device__ bool wait(uint64_t* bar, uint32_t parity) {
+    const bool ok = wait_warp(smem_u32(bar), parity);
+    tcgen05_fence_after();
+    return ok;
+  }
+  __device__ bool wait_load(uint32_t load) {
+    return wait(&c->kv_full[load % kSlots], (load / kSlots) & 1);
+  }
+  __device__ void release(uint64_t* bar) {
+    if (elect_one()) tcgen05_commit(bar);
+    __syncwarp();
+  }
+
+  __device__ bool item(const int (&tiles)[2]) {
+    const int most = max(tiles[0], tiles[1]);
+    if (!wait_load(loads)) return false;
+    for (int t = 0; t < 2; ++t) {
+      if (tiles[t] == 0) continue;
+      if (!wait(&c->q_full[t], q_uses[t] & 1)) return false;
+      ++q_uses[t];
+      scores(t, loads % kSlots);
+      if (tiles[t] == 1) release(&c->q_empty[t]);
+    }
+    release(&c->kv_empty[loads % kSlots]);
+    for (int j = 0; j < most; ++j) {
+      const uint32_t v_load = loads + 2 * j + 1, k_load = v_load + 1;
+      if (!wait_load(v_load)) return false;
+      if (j + 1 < most && !wait_load(k_load)) return false;
+      for (int t = 0; t < 2; ++t) {
+        if (j >= tiles[t]) continue;
+        if (j == 0) {
+          if (!wait(&c->o_empty[t], (o_uses[t] & 1) ^ 1)) return false;
+          ++o_uses[t];
+        }
+        if (!wait(&c->p_full[t], p_uses[t] & 1)) return false;
+        ++p_uses[t];
+        values(t, v_load % kSlots, j == 0, j + 1 == tiles[t]);
+        if (j + 1 < tiles[t]) {
+          scores(t, k_load % kSlots);
+          if (j + 2 == tiles[t]) release(&c->q_empty[t]);
+        }
+      }
+      release(&c->kv_empty[v_load % kSlots]);
+      if (j + 1 < most) release(&c->kv_empty[k_load % kSlots]);
+    }
+    loads += 2 * most;
+    return true;
+  }
+};
+
+// The values of a masked tile, seen by the 128 threads of a query tile before they let the tensor cores
+// have it: a weight of 0 times a value that is no number would be none either.  Such values become 0
+// here and are added by add_bad_values().
+__device__ __forceinline__ void clear_bad_values(uint8_t* tile, Control* c, int thread) {
+#pragma unroll 4
+  for (int i = thread; i < kTileBytes / 16; i += kTile) {
+    uint4* at = reinterpret_cast<uint4*>(tile) + i;
+    const uint4 x = *at;
+    if (is_no_number(x.x) || is_no_number(x.y) || is_no_number(x.z) || is_no_number(x.w)) {
+      atomicExch(&c->bad_values, 1);
+      __threadfence_block();
+      uint16_t* each = reinterpret_cast<uint16_t*>(at);
+      for (int k = 0; k < 8; ++k) {
+        if ((each[k] & 0x7f80u) == 0x7f80u) each[k] = 0;
+      }
     }
   }
-  if (sequence < 0) return;
-  const int kv_head = head / (args.heads / args.kv_heads);
-  auto load = [&](int token, int half, int dim, float(&x)[4]) {
-    const __nv_bfloat16* from = (half ? args.v + (first + token) * args.v_stride
-                                      : args.k + (first + token) * args.k_stride) +
-                                kv_head * kHeadDim + dim;
-    for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(from[i]);
-  };
-  const size_t at = static_cast<size_t>(row) * args.heads + head;
-  attend_row(args.q + row * args.q_stride + head * kHeadDim, row - first + 1, args.scale, load,
-             args.out + at * kHeadDim, args.lse ? args.lse + at : nullptr);
+  fence_proxy_async_smem();
+}
+
+// Adds what clear_bad_values() took out of the block's tiles to 32 columns of a row's result.
+__device__ __forceinline__ void add_bad_values(const PrefillArgs& args, const Work& w, int t, int row,
+                                            int column, float* o) {
+  for (int other = 0; other <= t; ++other) {
+    if (w.tiles[other] == 0) continue;
+    const int begin = (w.tiles[other] - 1) * kTile, end = min(begin + kTile, row + 1);
+    for (int j = begin; j < end; ++j) {
+      const __nv_bfloat16* v = args.v + (w.first + j) * args.v_stride + w.kv_head * kHeadDim + column;
+      for (int i = 0; i < 32; ++i) {
+        const float x = __bfloat162float(v[i]);
+        if (!(fabsf(x) < INFINITY)) o[i] += x;
+      }
+    }
+    if (w.row[0] == w.row[1]) break;  // (both tiles have the same last one)
+  }
+}
+
+// Four warps per query tile, a thread per row.
+__device__ void softmax_role(const PrefillArgs& args, uint8_t* slots, uint32_t tmem, Control* c) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = warp >> 2, thread = threadIdx.x & (kTile - 1);
+  const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp, from bit 16
+  const uint32_t s_at = tmem + lanes + t * kTile, o_at = tmem + lanes + 2 * kTile + t * kHeadDim;
+  const float factor = args.scale * kLog2e;
+  const uint64_t factor2 = pack2(factor, factor);
+  uint32_t s_uses = 0, o_uses = 0, loads = 0;
+  for (uint32_t items = 0;; ++items) {
+    const uint32_t place = items & 1;
+    if (!wait_warp(smem_u32(&c->work_full[place]), (items >> 1) & 1)) break;
+    if (!c->has_work[place]) return;
+    const Work w = c->work[place];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&c->work_empty[place]);
+    const int tiles = w.tiles[t], most = max(w.tiles[0], w.tiles[1]);
+    const uint32_t first_load = loads;
+    loads += 2 * most;
+    float top = 0.0f;
+    uint64_t sum2 = 0;
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      if (!(ok = wait_warp(smem_u32(&c->s_full[t]), s_uses & 1))) break;
+      ++s_uses;
+      tcgen05_fence_after();
+      if (j + 1 == tiles || j + 1 == w.tiles[0]) {  // a tile on a diagonal, one's own or the other's
+        const uint32_t load = first_load + 2 * j + 1;
+        if (!(ok = wait_warp(smem_u32(&c->kv_full[load % kSlots]), (load / kSlots) & 1))) break;
+        clear_bad_values(slots + (load % kSlots) * kTileBytes, c, thread);
+      }
+      uint32_t s[kTile];
+#pragma unroll
+      for (int part = 0; part < 4; ++part) tmem_ld_x32_async(s_at + part * 32, s + part * 32);
+      tmem_ld_wait();
+      registers_loaded<kTile>(s);
+      if (j + 1 == tiles) {
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) {
+          if (i > thread) s[i] = 0xff800000u;
+        }
+      }
+      float high[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) high[i] = __uint_as_float(s[i]);
+#pragma unroll
+      for (int i = 4; i < kTile; ++i) high[i & 3] = fmaxf(high[i & 3], __uint_as_float(s[i]));
+      const float highest = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
+      if (j == 0) {
+        top = highest;
+      } else if (__any_sync(0xffffffffu, (highest - top) * factor > kRescale)) {
+        // (S of this tile is complete, so O of those before it is)
+        const float higher = fmaxf(highest, top);
+        const float keep = exp2_approx((top - higher) * factor);
+        top = higher;
+        const uint64_t keep2 = pack2(keep, keep);
+        sum2 = mul2(sum2, keep2);
+#pragma unroll 1
+        for (int part = 0; part < 4; ++part) {
+          uint32_t o[32];
+          tmem_ld_x32_async(o_at + part * 32, o);
+          tmem_ld_wait();
+          registers_loaded<32>(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+          tmem_st_x32(o_at + part * 32, o);
+        }
+      }
+      const float shift = top == -INFINITY ? 0.0f : -top * factor;
+      const uint64_t shift2 = pack2(shift, shift);
+      uint64_t part2[2] = {0, 0};
+#pragma unroll
+      for (int part = 0; part < 4; ++part) {
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int at = part * 32 + 2 * i;
+          const uint64_t x = fma2(pack2(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), factor2, shift2);
+          float a, b;
+          unpack2(x, a, b);
+          a = exp2_approx(a);
+          b = exp2_approx(b);
+          part2[i & 1] = add2(part2[i & 1], pack2(a, b));
+          p[i] = pack_bf16(a, b);
+        }
+        tmem_st_x16(s_at + part * 16, p);
+      }
+      sum2 = add2(sum2, add2(part2[0], part2[1]));
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c->p_full[t]);
+    }
+    if (!ok) break;
+    if (tiles == 0) continue;
+    if (!wait_warp(smem_u32(&c->o_full[t]), o_uses & 1)) break;
+    ++o_uses;
+    tcgen05_fence_after();
+    float sum, other;
+    unpack2(sum2, sum, other);
+    sum += other;
+    const int row = w.row[t] + thread;
+    const bool valid = row < w.length;
+    const bool bad = *reinterpret_cast<volatile int*>(&c->bad_values) != 0;
+    const float inverse = 1.0f / sum;
+    const size_t at = static_cast<size_t>(w.first + row) * args.heads + w.head[t];
+#pragma unroll
+    for (int part = 0; part < 4; ++part) {
+      uint32_t o[32];
+      tmem_ld_x32_async(o_at + part * 32, o);
+      tmem_ld_wait();
+      registers_loaded<32>(o);
+      if (part == 3) {
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c->o_empty[t]);
+      }
+      if (!valid) continue;
+      if (bad) {
+        float copy[32];
+        for (int i = 0; i < 32; ++i) copy[i] = __uint_as_float(o[i]);
+        add_bad_values(args, w, t, row, part * 32, copy);
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(copy[i]);
+      }
+      uint32_t two[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        two[i] = pack_bf16(__uint_as_float(o[2 * i]) * inverse, __uint_as_float(o[2 * i + 1]) * inverse);
+      }
+      uint4* to = reinterpret_cast<uint4*>(args.out + at * kHeadDim + part * 32);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[i] = make_uint4(two[4 * i], two[4 * i + 1], two[4 * i + 2], two[4 * i + 3]);
+    }
+    if (valid && args.lse != nullptr) args.lse[at] = kLn2 * (top * factor + log2f(sum));
+  }
+  if (lane == 0) report_cache_error(args.error, kDevWaitTimeout);
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                   const __grid_constant__ CUtensorMap v_map, const PrefillArgs args, bool two_heads) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* shared = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  uint8_t* slots = shared + 2 * kTileBytes;
+  Control* c = reinterpret_cast<Control*>(slots + kSlots * kTileBytes);
+  const int warp = threadIdx.x >> 5;
+  if (*args.error != 0) return;  // a wait of an earlier call ran out
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&c->q_full[t], 1);
+      mbar_init(&c->q_empty[t], 1);
+      mbar_init(&c->s_full[t], 1);
+      mbar_init(&c->p_full[t], 4);
+      mbar_init(&c->o_full[t], 1);
+      mbar_init(&c->o_empty[t], 4);
+      mbar_init(&c->work_full[t], 1);
+      mbar_init(&c->work_empty[t], kSoftmaxWarps + 1);
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&c->kv_full[i], 1);
+      mbar_init(&c->kv_empty[i], 1);
+    }
+    mbar_init(&c->next_full, 1);
+    mbar_init(&c->drained, 1);
+    c->bad_values = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&c->tmem, kTmemColumns);
+    tmem_relinquish();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = c->tmem;
+  if (warp < kSoftmaxWarps) {
+    more_registers<kSoftmaxRegisters>();
+    softmax_role(args, slots, tmem, c);
+  } else if (warp == kMmaWarp) {
+    fewer_registers<kOtherRegisters>();
+    MmaRole role{c, smem_u32(shared), smem_u32(slots), tmem};
+    bool ok = true;
+    for (uint32_t items = 0;; ++items) {
+      const uint32_t place = items & 1;
+      if (!(ok = wait_warp(smem_u32(&c->work_full[place]), (items >> 1) & 1))) break;
+      if (!c->has_work[place]) break;
+      const int tiles[2] = {warp_uniform(c->work[place].tiles[0]), warp_uniform(c->work[place].tiles[1])};
+      __syncwarp();
+      if (elect_one()) mbar_arrive(&c->work_empty[place]);
+      __syncwarp();
+      if (!(ok = role.item(tiles))) break;
+    }
+    if (!ok && elect_one()) report_cache_error(args.error, kDevWaitTimeout);
+    role.release(&c->drained);
+    wait_warp(smem_u32(&c->drained), 0);
+  } else {
+    fewer_registers<kOtherRegisters>();
+    if (warp == kLoadWarp) {
+      load_role(args, two_heads, &q_map, &k_map, &v_map, smem_u32(shared), smem_u32(slots), c);
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem, kTmemColumns);
+  }
 }
 
 }  // namespace
 
 cudaError_t launch_attention_prefill(const PrefillArgs& args, cudaStream_t stream) {
-  prefill_row_kernel<<<dim3(args.tokens, args.heads), kHeadDim, 0, stream>>>(args);
+  CUtensorMap q, k, v;
+  if (!rows_tensor_map(args.q, args.tokens, args.heads, args.q_stride, kTile, &q) ||
+      !rows_tensor_map(args.k, args.tokens, args.kv_heads, args.k_stride, kTile, &k) ||
+      !rows_tensor_map(args.v, args.tokens, args.kv_heads, args.v_stride, kTile, &v)) {
+    return cudaErrorInvalidValue;
+  }
+  const bool two_heads = args.heads / args.kv_heads % 2 == 0;
+  const int64_t rows = two_heads ? kTile : 2 * kTile;
+  const int64_t columns = two_heads ? args.heads / 2 : args.heads;
+  const int64_t blocks = std::min<int64_t>(args.tokens, args.tokens / rows + args.sequences) * columns;
+  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  cudaError_t err = allow_shared_memory(prefill_kernel);
+  if (err != cudaSuccess) return err;
+  prefill_kernel<<<static_cast<unsigned>(blocks), kThreads, kSharedBytes, stream>>>(q, k, v, args,
+                                                                                    two_heads);
   return cudaGetLastError();
 }
 
