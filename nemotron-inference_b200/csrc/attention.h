@@ -150,6 +150,9 @@ struct CachedArgs {
 bool rows_tensor_map(const void* base, int64_t rows, int64_t heads, int64_t stride, int box_rows,
                      CUtensorMap* map);
 
+// A cache's codes as rows of 128 bytes, boxes of a page and head, 128-byte swizzle.
+bool pages_tensor_map(const PagedCache& cache, CUtensorMap* map);
+
 cudaError_t launch_attention_prefill(const PrefillArgs& args, cudaStream_t stream);
 size_t attention_cached_workspace_bytes();
 cudaError_t launch_attention_cached(const CachedArgs& args, cudaStream_t stream);

@@ -156,6 +156,20 @@ bool rows_tensor_map(const void* base, int64_t rows, int64_t heads, int64_t stri
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool pages_tensor_map(const PagedCache& cache, CUtensorMap* map) {
+  const uint64_t rows = static_cast<uint64_t>(cache.layers) * cache.pages * 2 * cache.kv_heads * cache.page_tokens;
+  if (rows > INT32_MAX) return false;  // a coordinate has 31 bits: 256 GB of codes
+  const cuuint64_t dims[2] = {kHeadDim, rows};
+  const cuuint64_t strides[1] = {kHeadDim};
+  const cuuint32_t box[2] = {kHeadDim, static_cast<cuuint32_t>(cache.page_tokens)};
+  const cuuint32_t steps[2] = {1u, 1u};
+  const EncodeTiled encode = encode_tiled();
+  return encode != nullptr &&
+         encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, cache.codes, dims, strides, box, steps,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace nmoe
 
 extern "C" {
