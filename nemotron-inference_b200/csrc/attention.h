@@ -154,6 +154,8 @@ bool rows_tensor_map(const void* base, int64_t rows, int64_t heads, int64_t stri
 bool pages_tensor_map(const PagedCache& cache, CUtensorMap* map);
 
 cudaError_t launch_attention_prefill(const PrefillArgs& args, cudaStream_t stream);
+// The workspace begins with counters, zero between calls.
+constexpr size_t kAttendCounterBytes = 4096;
 size_t attention_cached_workspace_bytes();
 cudaError_t launch_attention_cached(const CachedArgs& args, cudaStream_t stream);
 cudaError_t launch_kv_append(const PagedCache& cache, const Batch& batch, int layer,

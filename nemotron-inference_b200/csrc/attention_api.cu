@@ -105,13 +105,16 @@ nmoe_status device_status(int code) {
   }
 }
 
-// Waits for the stream, reads an error word and clears it.
-nmoe_status sync_error_word(int* word, cudaStream_t stream) {
+// Waits for the stream, reads an error word and clears it, with what a call that gave up may have left.
+nmoe_status sync_error_word(int* word, cudaStream_t stream, void* counters = nullptr) {
   int code = 0;
   cudaError_t err = cudaMemcpyAsync(&code, word, sizeof(code), cudaMemcpyDeviceToHost, stream);
   if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
   if (err == cudaSuccess && code != 0) {
     err = cudaMemsetAsync(word, 0, sizeof(code), stream);
+    if (err == cudaSuccess && counters != nullptr) {
+      err = cudaMemsetAsync(counters, 0, nmoe::kAttendCounterBytes, stream);
+    }
     if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
   }
   return err == cudaSuccess ? device_status(code) : status_of(err);
@@ -254,7 +257,7 @@ nmoe_status nmoe_kv_copy_pages(const nmoe_kv_cache* cache, void* stream, const i
 nmoe_status nmoe_kv_sync_status(const nmoe_kv_cache* cache, void* stream) {
   PagedCache view;
   if (!view_of(cache, view)) return NMOE_ERR_INVALID_ARGUMENT;
-  return sync_error_word(view.error, static_cast<cudaStream_t>(stream));
+  return sync_error_word(view.error, static_cast<cudaStream_t>(stream), view.attend_workspace);
 }
 
 nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* stream, int32_t layer,

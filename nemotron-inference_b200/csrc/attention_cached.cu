@@ -37,8 +37,8 @@ constexpr int kTile = 128;  // tokens
 constexpr int kTileBytes = kTile * kHeadDim;
 constexpr int kMaxPagesPerTile = kTile / 16;
 constexpr int kMaxRows = 128;
-constexpr float kWeightBits = 8.0f;  // the largest weight is 2^8 or less ...
-constexpr float kSlack = 0.8f;       // ... until its maximum has risen by this: 2^8.8 < 448
+constexpr float kWeightBits = 7.0f;    // a row's largest weight is 2^7 when its reference is set ...
+constexpr float kLargestBits = 8.8f;   // ... and less than 2^8.8 < 448 before it is set anew
 
 // R query rows, `Groups` times four warps that take R / Groups of them each.
 template <int R, int Groups>
@@ -47,8 +47,14 @@ struct Shape {
   static constexpr int kN = 2 * R;
   static constexpr int kBlocks = R == kMaxRows ? 1 : 2;                // on an SM
   static constexpr int kScores = R >= 64 ? 1 : 2;                      // buffers of S
-  static constexpr int kStages = R == kMaxRows ? 4 : R == 64 ? 2 : 3;  // tiles of keys and values in flight
+  // Columns of S, O and weights, rows of the two terms of the queries: group by group, first terms, second
+  // terms; so fewer groups are fewer columns.
+  __device__ static int column(int row, int term) {
+    return row / kGroupRows * 2 * kGroupRows + term * kGroupRows + row % kGroupRows;
+  }
+  static constexpr int kStages = R == kMaxRows ? 4 : R >= 32 ? 2 : 3;  // tiles of keys and values in flight
   static constexpr int kSoftmaxWarps = 4 * Groups;
+  static constexpr int kRowsPerWarp = R / kSoftmaxWarps;  // of queries
   static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
   static constexpr int kPanel = kN < 128 ? kN : 128;  // bytes of a token's row of weights in a panel
   static constexpr int kColumnsUsed = (kScores + 1) * kN;
@@ -60,6 +66,7 @@ struct Segment {
   int first, rows, length;  // of the batch entry
   int kv_head, row0;        // first of the query rows
   int tile, tiles;
+  int groups;               // of the shape's groups of rows, those that have any
   int part;                 // -1: all of them; else where its sums go
   int lead, parts;          // the first block with a part, and how many have one
 };
@@ -74,17 +81,20 @@ struct Control {
   int powers[S::kStages][2][kMaxPagesPerTile];  // of a tile's pages, keys and values
   alignas(16) float factor[S::kRows];           // what a row's product of codes is multiplied by
   alignas(16) float shift[S::kRows];            // kWeightBits - the row's reference
-  float top[S::kRows], fade[S::kRows];
-  float warp_top[S::kSoftmaxWarps][S::kGroupRows];
+  alignas(16) float rise[S::kRows], fade[S::kRows];  // of a reference, and what that leaves of its sums
+  int highest[S::kRows];                        // largest exponents of a tile, as ordered()
+  uint32_t risen[S::kGroups][(S::kGroupRows + 31) / 32];                         // by group: the rows whose references have changed
   float warp_sum[S::kSoftmaxWarps][S::kGroupRows];
-  float sum[S::kRows];
+  float sum[S::kRows], inverse[S::kRows];
+  int out_row[S::kRows];                        // of the result, -1: none
   int limit[S::kRows];                          // a row's position: the last token it sees
   int first_bad[kHeadDim];                      // position of the first masked value that is no number
-  int failed[2];
-  int last;
+  int failed[S::kGroups];
+  int joined;
   uint32_t tmem;
   int64_t before[S::kThreads / 32];
   int64_t total, found_before;
+  BatchEntry entry;
   int found, blocks;  // the entry in which this block's tiles begin; blocks that have any
 };
 
@@ -93,11 +103,17 @@ constexpr size_t shared_bytes() {
   return 1024 + S::kStages * 2 * kTileBytes + 2 * S::kN * kTile + sizeof(Control<S>);
 }
 
+// All blocks of a launch run at once.
+template <typename S>
+constexpr bool fits_on_sm() {
+  return S::kBlocks * (shared_bytes<S>() + 1024) <= 228 * 1024 && S::kBlocks * S::kColumns <= 512;
+}
+
 // What a block leaves for the join: a row's 128 sums, then the references and the sums of weights.
 __host__ __device__ constexpr size_t part_floats(int rows) { return static_cast<size_t>(rows) * (kHeadDim + 2); }
 
 struct Split {
-  int* counters;  // a block's part of the sequence that begins in it: pieces that are done
+  int* counters;  // by the block in which a (sequence, key head) begins: pieces that are done, twice
   float* parts;
 };
 
@@ -115,11 +131,17 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
       : "memory");
 }
 
+// Floats as integers of the same order (no NaN), and back.
+__device__ __forceinline__ int ordered(float x) {
+  const int bits = __float_as_int(x);
+  return bits ^ ((bits >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float from_ordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+constexpr int kLowest = static_cast<int>(0x807fffffu);  // of -infinity
+
 // The largest over the warp, in all lanes.
 __device__ __forceinline__ float warp_max(float x) {
-  float y;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
-  return y;
+  return from_ordered(__reduce_max_sync(0xffffffffu, ordered(x)));
 }
 
 __device__ __forceinline__ void group_sync(int group) {
@@ -139,7 +161,42 @@ __device__ __forceinline__ bool group_any(int group, bool mine) {
 }
 template <typename S>
 __device__ __forceinline__ void softmax_sync() {
-  asm volatile("bar.sync 3, %0;" ::"n"(S::kSoftmaxWarps * 32) : "memory");
+  asm volatile("bar.sync 5, %0;" ::"n"(S::kSoftmaxWarps * 32) : "memory");
+}
+
+// Sums N values over the warp: lane L holds in v[0..] the totals of the rows sum_row<N>(L, 0..).  Half of
+// the values change hands in each step.
+template <int N>
+__device__ __forceinline__ void warp_sums(float (&v)[N], int lane) {
+  int count = N;
+#pragma unroll
+  for (int stride = 16; stride > 0; stride /= 2) {
+    if (count > 1) {
+      count /= 2;
+      const bool upper = (lane & stride) != 0;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        if (i < count) {
+          const float send = upper ? v[i] : v[i + count], keep = upper ? v[i + count] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, stride);
+        }
+      }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], stride);
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ int sum_row(int lane, int i) {
+  int row = 0, count = N;
+#pragma unroll
+  for (int stride = 16; stride > 0; stride /= 2) {
+    if (count > 1) {
+      count /= 2;
+      if (lane & stride) row += count;
+    }
+  }
+  return row + i;
 }
 
 // Two E4M3 codes, `lo` in the low byte, of two binary16 values, and back.
@@ -176,6 +233,7 @@ __device__ void find_begin(const CachedArgs& args, Control<S>* c) {
   const int begin = min(n, static_cast<int>(threadIdx.x) * each), end = min(n, begin + each);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t mine = 0;
+#pragma unroll 1
   for (int i = begin; i < end; ++i) {
     const BatchEntry e = batch_entry(args.cache, args.batch, i);
     if (!e.valid && blockIdx.x == 0) report_cache_error(args.cache.error, kCacheBadSequence);
@@ -203,11 +261,14 @@ __device__ void find_begin(const CachedArgs& args, Control<S>* c) {
   if (static_cast<int>(blockIdx.x) >= blocks) return;
   const int64_t start = total * blockIdx.x / blocks;
   if (start >= below && start < below + mine) {  // one thread's
+#pragma unroll 1
     for (int i = begin; i < end; ++i) {
-      const int64_t tiles = entry_tiles<S>(args, batch_entry(args.cache, args.batch, i));
+      const BatchEntry e = batch_entry(args.cache, args.batch, i);
+      const int64_t tiles = entry_tiles<S>(args, e);
       if (start < below + tiles) {
         c->found = i;
         c->found_before = below;
+        c->entry = e;
         break;
       }
       below += tiles;
@@ -230,7 +291,7 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
   int64_t entry_at = c->found_before;
   bool ok = true;
   while (at < stop && ok) {
-    const BatchEntry e = batch_entry(cache, args.batch, i);
+    const BatchEntry e = entry_at == c->found_before ? c->entry : batch_entry(cache, args.batch, i);
     const int tiles = (e.length + kTile - 1) / kTile, rows = row_tiles<S>(args, e);
     const int64_t entry_end = entry_at + entry_tiles<S>(args, e);
     const int last_page = pages_of(cache, e.length);
@@ -243,13 +304,15 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
       s.length = e.length;
       s.kv_head = unit / rows;
       s.row0 = (unit % rows) * S::kRows;
+      const int left = e.rows * (args.heads / cache.kv_heads) - s.row0;
+      s.groups = min(S::kGroups, (left + S::kGroupRows - 1) / S::kGroupRows);
       s.tile = static_cast<int>(at - unit_at);
       s.tiles = static_cast<int>(min(stop, unit_at + tiles) - at);
       s.lead = static_cast<int>(((unit_at + 1) * G - 1) / total);
       s.parts = static_cast<int>(((unit_at + tiles) * G - 1) / total) - s.lead + 1;
       s.part = s.parts == 1 ? -1 : 2 * g + (g == s.lead);
       const uint32_t place = segments & 1;
-      if (!(ok = wait_warp(smem_u32(&c->segment_empty[place]), ((segments >> 1) & 1) ^ 1))) break;
+      if (!(ok = mbar_wait_warp(smem_u32(&c->segment_empty[place]), ((segments >> 1) & 1) ^ 1))) break;
       if (lane == 0) {
         c->segment[place] = s;
         c->has_segment[place] = 1;
@@ -260,7 +323,8 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
       int first_page = -1, page = 0, k_power = 0, v_power = 0;  // a lane per page, 32 at a time
       for (int tile = s.tile; tile < s.tile + s.tiles; ++tile) {
         const int wanted = tile * pages_per_tile;
-        if (first_page < 0 || wanted >= first_page + 32) {
+        const bool new_pages = first_page < 0 || wanted >= first_page + 32;
+        if (new_pages) {
           first_page = wanted;
           if (wanted + lane < last_page) {
             page = page_at(cache, e.sequence, wanted + lane);
@@ -268,35 +332,45 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
               report_cache_error(cache.error, kCacheBadSequence);
               page = 0;
             }
-            k_power = cache.exponents[block_of_page(cache, args.layer, page, 0, s.kv_head)];
-            v_power = cache.exponents[block_of_page(cache, args.layer, page, 1, s.kv_head)];
           }
         }
         const int count = min(pages_per_tile, last_page - wanted), from = wanted - first_page;
+        // the copies are asked for first: a tile is there once its powers are as well
+        bool keys_asked = false;
+#pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           uint64_t* empty = half ? &c->v_empty[stage] : &c->k_empty[stage];
-          if (!(ok = wait_warp(smem_u32(empty), phase ^ 1))) break;
-          if (half == 0) {  // (read by the softmax warps before they let the values' place go)
-            if (!(ok = wait_warp(smem_u32(&c->v_empty[stage]), phase ^ 1))) break;
-            const int p = __shfl_sync(0xffffffffu, k_power, (from + lane) & 31);
-            const int z = __shfl_sync(0xffffffffu, v_power, (from + lane) & 31);
-            if (lane < count) {
-              c->powers[stage][0][lane] = p;
-              c->powers[stage][1][lane] = z;
-            }
-            __syncwarp();
-          }
+          if (!(ok = mbar_wait_warp(smem_u32(empty), phase ^ 1))) break;
           const uint32_t bar = smem_u32(half ? &c->v_full[stage] : &c->k_full[stage]);
           const uint32_t to = stages_at + (2 * stage + half) * kTileBytes;
-          if (elect_one()) mbar_arrive_expect_tx_at(bar, count * page_bytes);
-          __syncwarp();
+#pragma unroll 1
           for (int j = 0; j < count; ++j) {
             const int id = __shfl_sync(0xffffffffu, page, from + j);
             const int row = static_cast<int>(block_of_page(cache, args.layer, id, half, s.kv_head) << cache.page_shift);
             if (elect_one()) tma_load_2d_at(to + j * page_bytes, map, 0, row, bar);
             __syncwarp();
           }
+          if (half && elect_one()) mbar_arrive_expect_tx_at(bar, count * page_bytes);
+          __syncwarp();
+          keys_asked = true;
           ++loads;
+        }
+        if (new_pages && wanted + lane < last_page) {
+          k_power = cache.exponents[block_of_page(cache, args.layer, page, 0, s.kv_head)];
+          v_power = cache.exponents[block_of_page(cache, args.layer, page, 1, s.kv_head)];
+        }
+        if (ok) {  // (the softmax warps have read the powers before these when they let the values go)
+          const int p = __shfl_sync(0xffffffffu, k_power, (from + lane) & 31);
+          const int z = __shfl_sync(0xffffffffu, v_power, (from + lane) & 31);
+          if (lane < count) {
+            c->powers[stage][0][lane] = p;
+            c->powers[stage][1][lane] = z;
+          }
+        }
+        __syncwarp();
+        if (keys_asked) {
+          if (elect_one()) mbar_arrive_expect_tx_at(smem_u32(&c->k_full[stage]), count * page_bytes);
+          __syncwarp();
         }
         if (!ok) break;
         if (++stage == S::kStages) {
@@ -311,7 +385,7 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
   }
   if (ok) {
     const uint32_t place = segments & 1;
-    ok = wait_warp(smem_u32(&c->segment_empty[place]), ((segments >> 1) & 1) ^ 1);
+    ok = mbar_wait_warp(smem_u32(&c->segment_empty[place]), ((segments >> 1) & 1) ^ 1);
     if (ok && lane == 0) {
       c->has_segment[place] = 0;
       mbar_arrive(&c->segment_full[place]);
@@ -320,15 +394,15 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
   if (ok) return;
   if (lane == 0) report_cache_error(cache.error, kDevWaitTimeout);
   // what is in flight arrives before the block's shared memory is given up
+#pragma unroll 1
   for (uint32_t back = 1; back <= min(loads, 2u * S::kStages); ++back) {
     const uint32_t load = loads - back, of = (load >> 1) % S::kStages;
-    wait_warp(smem_u32(load & 1 ? &c->v_full[of] : &c->k_full[of]), ((load >> 1) / S::kStages) & 1);
+    mbar_wait_warp(smem_u32(load & 1 ? &c->v_full[of] : &c->k_full[of]), ((load >> 1) / S::kStages) & 1);
   }
 }
 
 template <typename S>
 __device__ bool mma_role(uint32_t stages_at, uint32_t q_at, uint32_t p_at, uint32_t tmem, Control<S>* c) {
-  constexpr uint32_t kScoresDesc = make_idesc_e4m3(S::kN, false), kValuesDesc = make_idesc_e4m3(S::kN, true);
   // rows of weights are 16, 32, 64 or 128 bytes, swizzled in as many
   constexpr uint32_t kSwizzle = S::kPanel == 128 ? 2 : S::kPanel == 64 ? 4 : S::kPanel == 32 ? 6 : 0;
   const uint64_t q_desc = make_smem_desc(q_at, 16, 1024, 2);
@@ -338,28 +412,31 @@ __device__ bool mma_role(uint32_t stages_at, uint32_t q_at, uint32_t p_at, uint3
   uint32_t tile_no = 0;  // of all segments
   for (uint32_t segments = 0;; ++segments) {
     const uint32_t place = segments & 1;
-    if (!wait_warp(smem_u32(&c->segment_full[place]), (segments >> 1) & 1)) return false;
+    if (!mbar_wait_warp(smem_u32(&c->segment_full[place]), (segments >> 1) & 1)) return false;
     const int some = c->has_segment[place];
-    const int tiles = c->segment[place].tiles;
+    const int tiles = warp_uniform(c->segment[place].tiles);
+    const uint32_t n = warp_uniform(c->segment[place].groups) * 2 * S::kGroupRows;
+    const uint32_t scores_desc = make_idesc_e4m3(n, false), values_desc = make_idesc_e4m3(n, true);
     __syncwarp();
     if (!some) return true;
     if (elect_one()) mbar_arrive(&c->segment_empty[place]);
     __syncwarp();
-    if (!wait_warp(smem_u32(&c->q_full), segments & 1)) return false;
+    if (!mbar_wait_warp(smem_u32(&c->q_full), segments & 1)) return false;
     tcgen05_fence_after();
     // scores one tile ahead of the values
+#pragma unroll 1
     for (int j = 0; j <= tiles; ++j) {
       if (j < tiles) {
         const uint32_t no = tile_no + j, stage = no % S::kStages, buffer = no % S::kScores;
-        if (!wait_warp(smem_u32(&c->k_full[stage]), (no / S::kStages) & 1)) return false;
-        if (!wait_warp(smem_u32(&c->s_empty[buffer]), ((no / S::kScores) & 1) ^ 1)) return false;
+        if (!mbar_wait_warp(smem_u32(&c->k_full[stage]), (no / S::kStages) & 1)) return false;
+        if (!mbar_wait_warp(smem_u32(&c->s_empty[buffer]), ((no / S::kScores) & 1) ^ 1)) return false;
         tcgen05_fence_after();
         if (elect_one()) {
           const uint64_t k_desc = make_smem_desc(stages_at + 2 * stage * kTileBytes, 16, 1024, 2);
 #pragma unroll
           for (int k = 0; k < kHeadDim / 32; ++k) {
             mma_e4m3(tmem + buffer * S::kN, advance_smem_desc(k_desc, k * 32), advance_smem_desc(q_desc, k * 32),
-                     kScoresDesc, k > 0);
+                     scores_desc, k > 0);
           }
           tcgen05_commit(&c->s_full[buffer]);
           tcgen05_commit(&c->k_empty[stage]);
@@ -368,8 +445,8 @@ __device__ bool mma_role(uint32_t stages_at, uint32_t q_at, uint32_t p_at, uint3
       }
       if (j > 0) {
         const uint32_t no = tile_no + j - 1, stage = no % S::kStages;
-        if (!wait_warp(smem_u32(&c->v_full[stage]), (no / S::kStages) & 1)) return false;
-        if (!wait_warp(smem_u32(&c->p_full), no & 1)) return false;
+        if (!mbar_wait_warp(smem_u32(&c->v_full[stage]), (no / S::kStages) & 1)) return false;
+        if (!mbar_wait_warp(smem_u32(&c->p_full), no & 1)) return false;
         tcgen05_fence_after();
         if (elect_one()) {
           // eight tokens are 1024 bytes of values
@@ -377,7 +454,7 @@ __device__ bool mma_role(uint32_t stages_at, uint32_t q_at, uint32_t p_at, uint3
 #pragma unroll
           for (int k = 0; k < kTile / 32; ++k) {
             mma_e4m3(o, advance_smem_desc(v_desc, k * 4096), advance_smem_desc(p_desc, k * 32 * S::kPanel),
-                     kValuesDesc, j > 1 || k > 0);
+                     values_desc, j > 1 || k > 0);
           }
           tcgen05_commit(&c->p_empty);
           tcgen05_commit(&c->v_empty[stage]);
@@ -402,41 +479,66 @@ __device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t* r) {
                : "memory");
 }
 
-// The queries of a segment as two terms, each row scaled by a power of two; a warp per row.
+__device__ __forceinline__ float power_of_two(int e) {  // -126 <= e <= 127
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+// The queries of a segment, a warp per row: read ...
 template <typename S>
-__device__ __forceinline__ void prepare_queries(const CachedArgs& args, const Segment& s, uint8_t* q, Control<S>* c) {
+__device__ __forceinline__ void load_queries(const CachedArgs& args, const Segment& s, uint2 (&raw)[S::kRowsPerWarp]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = args.heads / args.cache.kv_heads;
-  for (int r = warp; r < S::kRows; r += S::kSoftmaxWarps) {
-    const int row = s.row0 + r, token = row / group;
-    const bool valid = row < s.rows * group;
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (valid) {
-      const uint2 raw = *reinterpret_cast<const uint2*>(args.q + static_cast<int64_t>(s.first + token) * args.q_stride +
-                                                        (s.kv_head * group + row % group) * kHeadDim + lane * 4);
-      x[0] = __uint_as_float(raw.x << 16);
-      x[1] = __uint_as_float(raw.x & 0xffff0000u);
-      x[2] = __uint_as_float(raw.y << 16);
-      x[3] = __uint_as_float(raw.y & 0xffff0000u);
+#pragma unroll
+  for (int k = 0; k < S::kRowsPerWarp; ++k) {
+    const int row = s.row0 + k * S::kSoftmaxWarps + warp, token = row / group;
+    raw[k] = make_uint2(0, 0);
+    if (token < s.rows) {
+      raw[k] = *reinterpret_cast<const uint2*>(args.q + static_cast<int64_t>(s.first + token) * args.q_stride +
+                                               (s.kv_head * group + row % group) * kHeadDim + lane * 4);
     }
-    const float largest = warp_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-    const bool finite = __all_sync(0xffffffffu, fabsf(x[0]) < INFINITY && fabsf(x[1]) < INFINITY &&
-                                                    fabsf(x[2]) < INFINITY && fabsf(x[3]) < INFINITY);
+  }
+}
+
+// ... and put into shared memory as two terms, each row scaled by a power of two.
+template <typename S>
+__device__ __forceinline__ void store_queries(const CachedArgs& args, const Segment& s,
+                                              const uint2 (&raw)[S::kRowsPerWarp], uint8_t* q, Control<S>* c) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = args.heads / args.cache.kv_heads;
+#pragma unroll
+  for (int k = 0; k < S::kRowsPerWarp; ++k) {
+    const int r = k * S::kSoftmaxWarps + warp;
+    if (r >= s.groups * S::kGroupRows) break;
+    float x[4];
+    x[0] = __uint_as_float(raw[k].x << 16);
+    x[1] = __uint_as_float(raw[k].x & 0xffff0000u);
+    x[2] = __uint_as_float(raw[k].y << 16);
+    x[3] = __uint_as_float(raw[k].y & 0xffff0000u);
+    // (magnitudes as whole numbers: what is no number is beyond them all)
+    const uint32_t m = max(max(raw[k].x & 0x7fffu, (raw[k].x >> 16) & 0x7fffu),
+                           max(raw[k].y & 0x7fffu, (raw[k].y >> 16) & 0x7fffu));
+    const int largest = static_cast<int>(__reduce_max_sync(0xffffffffu, m));
     // the largest element's exponent becomes 7: below 256
-    const int power = largest > 0.0f && finite ? ilogbf(largest) - 7 : 0;
+    const int power = max(largest >> 7, 1) - 134;
+    const int some = max(power, -100), rest = power - some;  // (2^-power may be beyond FP32)
+    const float down = power_of_two(-some), downer = power_of_two(-rest);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = x[i] * down * downer;
     uint32_t a[2], b[2];
-    two_terms(scalbnf(x[0], -power), scalbnf(x[1], -power), a[0], b[0]);
-    two_terms(scalbnf(x[2], -power), scalbnf(x[3], -power), a[1], b[1]);
-    const int chunk = lane >> 2, inside = (lane & 3) * 4;
-    *reinterpret_cast<uint32_t*>(q + r * 128 + ((chunk ^ (r & 7)) << 4) + inside) = a[0] | (a[1] << 16);
-    const int r2 = S::kRows + r;
+    two_terms(x[0], x[1], a[0], b[0]);
+    two_terms(x[2], x[3], a[1], b[1]);
+    const int chunk = lane >> 2, inside = (lane & 3) * 4, r1 = S::column(r, 0), r2 = S::column(r, 1);
+    *reinterpret_cast<uint32_t*>(q + r1 * 128 + ((chunk ^ (r1 & 7)) << 4) + inside) = a[0] | (a[1] << 16);
     *reinterpret_cast<uint32_t*>(q + r2 * 128 + ((chunk ^ (r2 & 7)) << 4) + inside) = b[0] | (b[1] << 16);
     if (lane == 0) {
       // (a row that is no number: its scores are none)
-      c->factor[r] = finite ? scalbnf(args.scale * kLog2e, power) : NAN;
-      c->limit[r] = s.length - s.rows + (valid ? token : 0);
-      c->top[r] = -INFINITY;
+      c->factor[r] = largest < 0x7f80 ? args.scale * kLog2e * power_of_two(some) * power_of_two(rest) : NAN;
       c->shift[r] = 0.0f;
+      c->highest[r] = kLowest;
+      const int token = (s.row0 + r) / group;
+      const bool valid = token < s.rows;
+      c->limit[r] = s.length - s.rows + (valid ? token : 0);
+      c->out_row[r] = valid ? (s.first + token) * args.heads + s.kv_head * group + (s.row0 + r) % group : -1;
     }
   }
 }
@@ -448,18 +550,19 @@ template <typename S>
 __device__ __forceinline__ void clean_values(uint8_t* values, int token, int position, const Segment& s, Control<S>* c) {
   uint4* row = reinterpret_cast<uint4*>(values + token * kHeadDim);
   if (position >= s.length) {
+#pragma unroll
     for (int i = 0; i < 8; ++i) row[i] = make_uint4(0, 0, 0, 0);
   } else if (position > s.length - s.rows) {
-    for (int i = 0; i < 8; ++i) {
-      const uint4 x = row[i];
-      const uint32_t words[4] = {x.x, x.y, x.z, x.w};
-      for (int w = 0; w < 4; ++w) {
-        if ((((words[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0) continue;
-        for (int k = 0; k < 4; ++k) {
-          if (((words[w] >> (8 * k)) & 0x7fu) != 0x7fu) continue;
-          atomicMin(&c->first_bad[((i ^ (token & 7)) << 4) + 4 * w + k], position);
-          reinterpret_cast<uint8_t*>(row + i)[4 * w + k] = 0;
-        }
+    uint32_t* words = reinterpret_cast<uint32_t*>(row);
+#pragma unroll 1
+    for (int i = 0; i < kHeadDim / 4; ++i) {
+      const uint32_t x = words[i];
+      if ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0) continue;
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) {
+        if (((x >> (8 * k)) & 0x7fu) != 0x7fu) continue;
+        atomicMin(&c->first_bad[(((i >> 2) ^ (token & 7)) << 4) + 4 * (i & 3) + k], position);
+        reinterpret_cast<uint8_t*>(words + i)[k] = 0;
       }
     }
   }
@@ -475,37 +578,59 @@ __device__ __forceinline__ uint32_t weight_offset(int token, int column) {
   return at ^ ((at >> 3) & mask);
 }
 
+// Joins the pieces of a segment's (sequence, key head), this block its share of the rows; a warp per row.
 template <typename S>
 __device__ void join(const CachedArgs& args, const Split& split, const Segment& s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = args.heads / args.cache.kv_heads;
-  const int rows = min(S::kRows, s.rows * group - s.row0);
+  const int rows = min(S::kRows, s.rows * group - s.row0), piece = static_cast<int>(blockIdx.x) - s.lead;
   auto part_of = [&](int p) {
     return split.parts + part_floats(S::kRows) * (p == 0 ? 2 * s.lead + 1 : 2 * (s.lead + p));
   };
-  for (int r = warp; r < rows; r += S::kSoftmaxWarps) {
-    float top = -INFINITY;
-    for (int p = lane; p < s.parts; p += 32) top = fmaxf(top, __ldcg(part_of(p) + S::kRows * kHeadDim + r));
-    top = warp_max(top);
-    if (top == -INFINITY) top = 0.0f;
-    float sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int end = rows * (piece + 1) / s.parts;
+#pragma unroll 1
+  for (int r = rows * piece / s.parts + warp; r < end; r += S::kSoftmaxWarps) {
+    // references and sums of weights, a lane per piece; the maximum so far is raised where there are over 32
+    float top = -INFINITY, sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
     for (int start = 0; start < s.parts; start += 32) {
-      float scale = 0.0f, weight = 0.0f;
-      if (start + lane < s.parts) {
-        const float* part = part_of(start + lane) + S::kRows * kHeadDim;
-        scale = exp2_approx(__ldcg(part + r) - top);
-        weight = __ldcg(part + S::kRows + r) * scale;
-      }
       const int count = min(32, s.parts - start);
-#pragma unroll 8
-      for (int p = 0; p < count; ++p) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(part_of(start + p) + r * kHeadDim) + lane);
-        const float f = __shfl_sync(0xffffffffu, scale, p);
-        sum += __shfl_sync(0xffffffffu, weight, p);
-        o[0] += x.x * f;
-        o[1] += x.y * f;
-        o[2] += x.z * f;
-        o[3] += x.w * f;
+      float reference = -INFINITY, weight = 0.0f;
+      if (lane < count) {
+        const float* part = part_of(start + lane) + S::kRows * kHeadDim + r;
+        reference = __ldcg(part);
+        weight = __ldcg(part + S::kRows);
+      }
+      float scale = 0.0f;
+#pragma unroll 1
+      for (int first = 0; first < count; first += 8) {
+        // (pieces from the second on lie evenly; what is behind the last is read again, with no weight)
+        float4 x[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          x[p] = __ldcg(reinterpret_cast<const float4*>(part_of(min(start + first + p, s.parts - 1)) + r * kHeadDim) + lane);
+        }
+        if (first == 0) {
+          const float higher = fmaxf(top, warp_max(reference));
+          const float keep = top > -INFINITY ? exp2_approx(top - higher) : 0.0f;
+          top = higher;
+          sum *= keep;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] *= keep;
+          if (reference > -INFINITY) scale = exp2_approx(reference - top);
+          // (a lane's own product: a sum that is no number stays none)
+          weight = scale != 0.0f || weight != weight ? weight * scale : 0.0f;
+        }
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const float f = __shfl_sync(0xffffffffu, scale, first + p);
+          if (first + p >= count || f == 0.0f) continue;
+          sum += __shfl_sync(0xffffffffu, weight, first + p);
+          o[0] = fmaf(x[p].x, f, o[0]);
+          o[1] = fmaf(x[p].y, f, o[1]);
+          o[2] = fmaf(x[p].z, f, o[2]);
+          o[3] = fmaf(x[p].w, f, o[3]);
+        }
       }
     }
     const float inverse = 1.0f / sum;
@@ -516,65 +641,111 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
   }
 }
 
+// Waits until every piece of a segment's (sequence, key head) has left its sums, then joins.  All blocks
+// with tiles run at once (as many as the SMs hold, and none waits before its own tiles are done).  The
+// counter is 0 again when the last of them has joined.
+template <typename S>
+__device__ bool wait_and_join(const CachedArgs& args, const Split& split, const Segment& s, Control<S>* c) {
+  if (threadIdx.x == 0) {
+    volatile int* done = split.counters + s.lead;
+    const long long start = clock64();
+    bool there = *done >= s.parts;
+    while (!there && clock64() - start < (1ll << 31)) there = *done >= s.parts;
+    __threadfence();
+    c->joined = there;
+  }
+  softmax_sync<S>();
+  if (!c->joined) return false;
+  join<S>(args, split, s);
+  softmax_sync<S>();
+  if (threadIdx.x == 0 && atomicAdd(&split.counters[s.lead], 1) == 2 * s.parts - 1) split.counters[s.lead] = 0;
+  return true;
+}
+
 template <typename S>
 __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t* stages, uint8_t* q, uint8_t* weights,
                              uint32_t tmem, Control<S>* c) {
-  constexpr int RG = S::kGroupRows;
+  constexpr int RG = S::kGroupRows, kChunk = RG < 16 ? RG : 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = warp >> 2;
   const int token = threadIdx.x & (kTile - 1), r0 = group * RG;
   const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
-  const uint32_t o_at = lanes + S::kScores * S::kN + r0;
+  const uint32_t o_at = lanes + S::kScores * S::kN + 2 * r0;
   const int page_shift = args.cache.page_shift;
+  const uint64_t* factors = reinterpret_cast<const uint64_t*>(c->factor + r0);
+  const uint64_t* shifts = reinterpret_cast<const uint64_t*>(c->shift + r0);
+  const uint64_t* rises = reinterpret_cast<const uint64_t*>(c->rise + r0);
+  const uint64_t* fades = reinterpret_cast<const uint64_t*>(c->fade + r0);
   volatile int* failed = &c->failed[group];
+  Segment to_join[2];  // the (at most two) that other blocks have pieces of
+  int joins = 0;
   uint32_t tile_no = 0;
+  bool ok = mbar_wait_warp(smem_u32(&c->segment_full[0]), 0);
+  int some = ok && c->has_segment[0];
+  Segment next = c->segment[0];
+  uint2 queries[S::kRowsPerWarp];
+  if (some) load_queries<S>(args, next, queries);
+#pragma unroll 1
   for (uint32_t segments = 0;; ++segments) {
-    const uint32_t place = segments & 1;
-    bool ok = wait_warp(smem_u32(&c->segment_full[place]), (segments >> 1) & 1);
-    const int some = ok && c->has_segment[place];
-    const Segment s = c->segment[place];
+    const Segment s = next;
     if (!ok) *failed = 1;
     softmax_sync<S>();
-    if (c->failed[0] || c->failed[S::kGroups - 1]) return false;
-    if (!some) return true;
-    if (lane == 0) mbar_arrive(&c->segment_empty[place]);
+    for (int i = 0; i < S::kGroups; ++i) ok = ok && c->failed[i] == 0;
+    if (!ok) return false;
+    if (!some) break;
+    if (lane == 0) mbar_arrive(&c->segment_empty[segments & 1]);
     if (threadIdx.x < kHeadDim) c->first_bad[threadIdx.x] = INT32_MAX;
-    prepare_queries<S>(args, s, q, c);
+    store_queries<S>(args, s, queries, q, c);
     fence_proxy_async_smem();
     softmax_sync<S>();
     if (lane == 0) mbar_arrive(&c->q_full);
-    float sum[RG];
+    uint64_t sum[RG / 2];
 #pragma unroll
-    for (int r = 0; r < RG; ++r) sum[r] = 0.0f;
+    for (int r = 0; r < RG / 2; ++r) sum[r] = 0;
     const int clear = s.length - s.rows;  // the last token that every row sees
+#pragma unroll 1
     for (int j = 0; j < s.tiles; ++j, ++tile_no) {
       const uint32_t stage = tile_no % S::kStages, buffer = tile_no % S::kScores;
       const int first = (s.tile + j) * kTile, position = first + token;
       const bool at_end = first + kTile - 1 > clear;
-      ok = wait_warp(smem_u32(&c->k_full[stage]), (tile_no / S::kStages) & 1);
-      ok = wait_warp(smem_u32(&c->s_full[buffer]), (tile_no / S::kScores) & 1) && ok;
+      if (group >= s.groups) {  // no rows: only the steps that others count on
+        ok = mbar_wait_warp(smem_u32(&c->s_full[buffer]), (tile_no / S::kScores) & 1);
+        if (lane == 0) mbar_arrive(&c->s_empty[buffer]);
+        ok = mbar_wait_warp(smem_u32(&c->p_empty), (tile_no & 1) ^ 1) && ok;
+        if (!ok) return false;
+        if (lane == 0) mbar_arrive(&c->p_full);
+        continue;
+      }
+      ok = mbar_wait_warp(smem_u32(&c->k_full[stage]), (tile_no / S::kStages) & 1);
+      ok = mbar_wait_warp(smem_u32(&c->s_full[buffer]), (tile_no / S::kScores) & 1) && ok;
       tcgen05_fence_after();
-      if (at_end) ok = wait_warp(smem_u32(&c->v_full[stage]), (tile_no / S::kStages) & 1) && ok;
+      if (at_end) ok = mbar_wait_warp(smem_u32(&c->v_full[stage]), (tile_no / S::kStages) & 1) && ok;
       // (places behind the sequence may lie in pages that it does not have)
       const int page = token >> page_shift;
       const float k_scale = exp2_approx(static_cast<float>(position < s.length ? c->powers[stage][0][page] : 0));
       const float v_power = static_cast<float>(position < s.length ? c->powers[stage][1][page] : 0);
-      float y[RG];
+      const uint64_t k2 = pack2(k_scale, k_scale), k2_16 = pack2(k_scale * 0.0625f, k_scale * 0.0625f);
+      const uint64_t v2 = pack2(v_power, v_power);
+      // exponents of the weights, rows in pairs: score + power of the values - reference + kWeightBits
+      uint64_t y[RG / 2];
+      float high = -INFINITY;
 #pragma unroll
-      for (int part = 0; part < RG; part += 32) {
-        constexpr int kChunk = RG < 32 ? RG : 32;
+      for (int part = 0; part < RG; part += kChunk) {
         uint32_t a[kChunk], b[kChunk];
 #pragma unroll
         for (int i = 0; i < kChunk; i += 8) {
-          tmem_ld_x8_async(lanes + buffer * S::kN + r0 + part + i, a + i);
-          tmem_ld_x8_async(lanes + buffer * S::kN + S::kRows + r0 + part + i, b + i);
+          tmem_ld_x8_async(lanes + buffer * S::kN + 2 * r0 + part + i, a + i);
+          tmem_ld_x8_async(lanes + buffer * S::kN + 2 * r0 + RG + part + i, b + i);
         }
         tmem_ld_wait();
         registers_loaded<kChunk>(a);
         registers_loaded<kChunk>(b);
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) {
-          const float product = fmaf(__uint_as_float(b[i]), 0.0625f, __uint_as_float(a[i]));
-          y[part + i] = fmaf(product, c->factor[r0 + part + i] * k_scale, v_power);
+        for (int i = 0; i < kChunk / 2; ++i) {
+          const int r = part / 2 + i;
+          const uint64_t product =
+              fma2(pack2(__uint_as_float(b[2 * i]), __uint_as_float(b[2 * i + 1])), k2_16,
+                   mul2(pack2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), k2));
+          y[r] = fma2(product, factors[r], add2(shifts[r], v2));
         }
       }
       tcgen05_fence_before();
@@ -582,79 +753,107 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       if (lane == 0) mbar_arrive(&c->s_empty[buffer]);
       if (at_end) {
 #pragma unroll
-        for (int r = 0; r < RG; ++r) {
-          if (position > c->limit[r0 + r]) y[r] = -INFINITY;
+        for (int r = 0; r < RG; r += 2) {
+          float y0, y1;
+          unpack2(y[r / 2], y0, y1);
+          if (position > c->limit[r0 + r]) y0 = -INFINITY;
+          if (position > c->limit[r0 + r + 1]) y1 = -INFINITY;
+          y[r / 2] = pack2(y0, y1);
         }
         if (group == 0) clean_values<S>(stages + (2 * stage + 1) * kTileBytes, token, position, s, c);
       }
-      // the largest of each row, row r in lane r
-      bool higher = false;
-      float mine[(RG + 31) / 32];
 #pragma unroll
-      for (int r = 0; r < RG; ++r) {
-        const float largest = warp_max(y[r]);
-        if (lane == (r & 31)) mine[r / 32] = largest;
-      }
-#pragma unroll
-      for (int r = lane, i = 0; i < (RG + 31) / 32; r += 32, ++i) {
-        if (r < RG) {
-          c->warp_top[warp][r] = mine[i];
-          higher = higher || mine[i] > c->top[r0 + r] + kSlack;
-        }
+      for (int r = 0; r < RG / 2; ++r) {
+        float y0, y1;
+        unpack2(y[r], y0, y1);
+        high = fmaxf(high, fmaxf(y0, y1));
       }
       // the weights of the tile before have been read, and O holds it
-      ok = wait_warp(smem_u32(&c->p_empty), (tile_no & 1) ^ 1) && ok;
+      ok = mbar_wait_warp(smem_u32(&c->p_empty), (tile_no & 1) ^ 1) && ok;
       tcgen05_fence_after();
       if (!ok) *failed = 1;
-      const bool rise = group_any(group, higher);
+      const bool rise = group_any(group, j == 0 || high > kLargestBits);
       if (*failed) return false;
       if (rise) {
-        if (token < RG) {
-          const int r = r0 + token;
-          float top = c->top[r];
-          const float was = top;
+        // the largest of each row that it may be, eight rows at a time
 #pragma unroll
-          for (int w = 0; w < 4; ++w) top = fmaxf(top, c->warp_top[group * 4 + w][token]);
-          c->fade[r] = was == -INFINITY ? 0.0f : exp2_approx(was - top);
-          c->top[r] = top;
-          c->shift[r] = top == -INFINITY ? 0.0f : kWeightBits - top;
+        for (int i = 0; i < RG; i += 8) {
+          float z[8];
+#pragma unroll
+          for (int k = 0; k < 8; k += 2) unpack2(y[(i + k) / 2], z[k], z[k + 1]);
+          const float of_eight = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])),
+                                       fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
+          if (!__any_sync(0xffffffffu, j == 0 || of_eight > kLargestBits)) continue;
+          int mine = kLowest;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int largest = __reduce_max_sync(0xffffffffu, ordered(z[k]));
+            if (lane == k) mine = largest;
+          }
+          if (lane < 8 && (j == 0 || mine > ordered(kLargestBits))) atomicMax(&c->highest[r0 + i + lane], mine);
         }
         group_sync(group);
+        if (token < (RG + 31) / 32 * 32) {
+          bool risen = false;
+          if (token < RG) {
+            const int r = r0 + token;
+            const float top = from_ordered(c->highest[r]);
+            c->highest[r] = kLowest;
+            risen = top > -INFINITY;
+            if (risen) {  // (in a row's first tile the reference may fall, too)
+              const float by = top - kWeightBits;
+              c->rise[r] = -by;
+              c->fade[r] = j > 0 ? exp2_approx(-by) : 1.0f;
+              c->shift[r] -= by;
+            } else {
+              c->rise[r] = 0.0f;
+              c->fade[r] = 1.0f;
+            }
+          }
+          const uint32_t rows = __ballot_sync(0xffffffffu, risen);
+          if (lane == 0) c->risen[group][token / 32] = rows;
+        }
+        group_sync(group);
+#pragma unroll
+        for (int r = 0; r < RG / 2; ++r) {
+          y[r] = add2(y[r], rises[r]);
+          sum[r] = mul2(sum[r], fades[r]);
+        }
         if (j > 0) {
 #pragma unroll 1
           for (int i = 0; i < RG; i += 8) {
+            if ((c->risen[group][i / 32] >> (i & 31) & 0xffu) == 0) continue;
+            uint32_t o[16];
+            tmem_ld_x8_async(o_at + i, o);
+            tmem_ld_x8_async(o_at + RG + i, o + 8);
+            tmem_ld_wait();
+            registers_loaded<16>(o);
 #pragma unroll
-            for (int term = 0; term < 2; ++term) {
-              uint32_t o[8];
-              tmem_ld_x8_async(o_at + term * S::kRows + i, o);
-              tmem_ld_wait();
-              registers_loaded<8>(o);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * c->fade[r0 + i + k]);
-              tmem_st_x8(o_at + term * S::kRows + i, o);
-            }
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * c->fade[r0 + i + (k & 7)]);
+            tmem_st_x8(o_at + i, o);
+            tmem_st_x8(o_at + RG + i, o + 8);
           }
           tmem_st_wait();
-#pragma unroll
-          for (int r = 0; r < RG; ++r) sum[r] *= c->fade[r0 + r];
         }
       }
       const float v_inverse = exp2_approx(-v_power);
+      const uint64_t v2_inverse = pack2(v_inverse, v_inverse);
 #pragma unroll
       for (int i = 0; i < RG; i += 8) {
         uint32_t a[4], b[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int r = i + 2 * k;
-          const float p0 = exp2_approx(y[r] + c->shift[r0 + r]);
-          const float p1 = exp2_approx(y[r + 1] + c->shift[r0 + r + 1]);
-          sum[r] = fmaf(p0, v_inverse, sum[r]);
-          sum[r + 1] = fmaf(p1, v_inverse, sum[r + 1]);
+          const int r = i / 2 + k;
+          float p0, p1;
+          unpack2(y[r], p0, p1);
+          p0 = exp2_approx(p0);
+          p1 = exp2_approx(p1);
+          sum[r] = fma2(pack2(p0, p1), v2_inverse, sum[r]);
           two_terms(p0, p1, a[k], b[k]);
         }
-        *reinterpret_cast<uint2*>(weights + weight_offset<S>(token, r0 + i)) =
+        *reinterpret_cast<uint2*>(weights + weight_offset<S>(token, 2 * r0 + i)) =
             make_uint2(a[0] | (a[1] << 16), a[2] | (a[3] << 16));
-        *reinterpret_cast<uint2*>(weights + weight_offset<S>(token, S::kRows + r0 + i)) =
+        *reinterpret_cast<uint2*>(weights + weight_offset<S>(token, 2 * r0 + RG + i)) =
             make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
       }
       fence_proxy_async_smem();
@@ -662,15 +861,20 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       __syncwarp();
       if (lane == 0) mbar_arrive(&c->p_full);
     }
+    // the next segment's queries are on their way during the end of this one
+    const uint32_t following = segments + 1;
+    const bool known = mbar_wait_warp(smem_u32(&c->segment_full[following & 1]), (following >> 1) & 1);
+    some = known && c->has_segment[following & 1];
+    next = c->segment[following & 1];
+    if (some) load_queries<S>(args, next, queries);
     // the rows' sums of weights over the 128 threads, in a fixed order
+    float each[RG];
 #pragma unroll
-    for (int r = 0; r < RG; ++r) {
-      float x = sum[r];
+    for (int r = 0; r < RG; r += 2) unpack2(sum[r / 2], each[r], each[r + 1]);
+    warp_sums<RG>(each, lane);
 #pragma unroll
-      for (int step = 16; step > 0; step /= 2) x += __shfl_xor_sync(0xffffffffu, x, step);
-      if (lane == 0) c->warp_sum[warp][r] = x;
-    }
-    ok = wait_warp(smem_u32(&c->p_empty), (tile_no & 1) ^ 1);
+    for (int i = 0; i < (RG + 31) / 32; ++i) c->warp_sum[warp][sum_row<RG>(lane, i)] = each[i];
+    ok = mbar_wait_warp(smem_u32(&c->p_empty), (tile_no & 1) ^ 1) && known;
     tcgen05_fence_after();
     if (!ok) *failed = 1;
     group_sync(group);
@@ -680,57 +884,60 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
 #pragma unroll
       for (int w = 0; w < 4; ++w) x += c->warp_sum[group * 4 + w][token];
       c->sum[r0 + token] = x;
+      c->inverse[r0 + token] = 1.0f / x;
     }
     group_sync(group);
     // a thread per dimension now
-    const int heads_per = args.heads / args.cache.kv_heads;
-    const int rows = min(RG, s.rows * heads_per - s.row0 - r0);
     float* part = s.part < 0 ? nullptr : split.parts + part_floats(S::kRows) * s.part;
     const int bad = c->first_bad[token];
 #pragma unroll 1
-    for (int i = 0; i < RG; i += 8) {
-      uint32_t a[8], b[8];
+    for (int i = 0; i < RG && group < s.groups && c->out_row[r0 + i] >= 0; i += 8) {
+      uint32_t a[16];
       tmem_ld_x8_async(o_at + i, a);
-      tmem_ld_x8_async(o_at + S::kRows + i, b);
+      tmem_ld_x8_async(o_at + RG + i, a + 8);
       tmem_ld_wait();
-      registers_loaded<8>(a);
-      registers_loaded<8>(b);
+      registers_loaded<16>(a);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (i + k >= rows) break;
-        const int r = r0 + i + k, row = s.row0 + r;
-        float o = fmaf(__uint_as_float(b[k]), 0.0625f, __uint_as_float(a[k]));
+        const int r = r0 + i + k, to = c->out_row[r];
+        float o = fmaf(__uint_as_float(a[k + 8]), 0.0625f, __uint_as_float(a[k]));
         if (c->limit[r] >= bad) o = NAN;
+        if (to < 0) continue;
         if (part != nullptr) {
           __stcg(part + r * kHeadDim + token, o);
         } else {
-          const size_t at = static_cast<size_t>(s.first + row / heads_per) * args.heads + s.kv_head * heads_per + row % heads_per;
-          args.out[at * kHeadDim + token] = __float2bfloat16(o / c->sum[r]);
+          args.out[static_cast<size_t>(to) * kHeadDim + token] = __float2bfloat16(o * c->inverse[r]);
         }
       }
     }
     tcgen05_fence_before();
     if (part != nullptr) {
-      if (token < RG) {
-        __stcg(part + S::kRows * kHeadDim + r0 + token, c->top[r0 + token]);
-        __stcg(part + S::kRows * (kHeadDim + 1) + r0 + token, c->sum[r0 + token]);
+      if (token < RG && group < s.groups) {
+        const int r = r0 + token;
+        __stcg(part + S::kRows * kHeadDim + r, c->sum[r] == 0.0f ? -INFINITY : -c->shift[r]);
+        __stcg(part + S::kRows * (kHeadDim + 1) + r, c->sum[r]);
       }
-      __threadfence();
-      softmax_sync<S>();
-      if (threadIdx.x == 0) c->last = atomicAdd(&split.counters[s.lead], 1) == s.parts - 1;
-      softmax_sync<S>();
-      if (c->last) {
-        __threadfence();
-        if (threadIdx.x == 0) split.counters[s.lead] = 0;
-        join<S>(args, split, s);
-      }
+      to_join[joins++] = s;
     }
   }
+  if (joins == 0) return true;
+  // (all threads' sums are behind the barrier at the top of the loop, so one thread speaks for them)
+  if (threadIdx.x == 0) {
+    __threadfence();
+#pragma unroll 1
+    for (int i = 0; i < joins; ++i) atomicAdd(&split.counters[to_join[i].lead], 1);
+  }
+#pragma unroll 1
+  for (int i = 0; i < joins; ++i) {
+    if (!wait_and_join<S>(args, split, to_join[i], c)) return false;
+  }
+  return true;
 }
 
 template <typename S>
 __global__ void __launch_bounds__(S::kThreads, S::kBlocks)
     cached_kernel(const __grid_constant__ CUtensorMap map, const CachedArgs args, const Split split) {
+  static_assert(fits_on_sm<S>());
   extern __shared__ uint8_t raw[];
   uint8_t* stages = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   uint8_t* q = stages + S::kStages * 2 * kTileBytes;
@@ -755,8 +962,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c->segment_full[i], 1);
       mbar_init(&c->segment_empty[i], S::kSoftmaxWarps + 1);
-      c->failed[i] = 0;
     }
+    for (int i = 0; i < S::kGroups; ++i) c->failed[i] = 0;
     c->found = 0;
     c->found_before = 0;
     fence_barrier_init();
@@ -781,7 +988,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks)
       tcgen05_commit(&c->drained);
     }
     __syncwarp();
-    wait_warp(smem_u32(&c->drained), 0);
+    mbar_wait_warp(smem_u32(&c->drained), 0);
   } else {
     load_role<S>(args, &map, smem_u32(stages), c);
   }
@@ -793,7 +1000,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks)
   }
 }
 
-constexpr size_t kCounterBytes = 4096;
+constexpr size_t kCounterBytes = kAttendCounterBytes;
 
 template <typename S>
 cudaError_t launch(const CUtensorMap& map, const CachedArgs& args, const Split& split, int sms, cudaStream_t stream) {
@@ -817,15 +1024,17 @@ cudaError_t launch_attention_cached(const CachedArgs& args, cudaStream_t stream)
   if (!pages_tensor_map(args.cache, &map)) return cudaErrorInvalidValue;
   const Split split{reinterpret_cast<int*>(args.cache.attend_workspace),
                     reinterpret_cast<float*>(args.cache.attend_workspace + kCounterBytes)};
-  // as many query rows at a time as the entries have on average, up to 128: further rows of an entry
-  // read its keys and values again
+  // As many query rows at a time as the entries have on average, up to 128: further rows of an entry
+  // read its keys and values again.  Entries that differ get 128 sooner.
   const int64_t rows = (args.batch.rows + args.batch.count - 1) / args.batch.count *
                        static_cast<int64_t>(args.heads / args.cache.kv_heads);
   if (rows <= 8) return launch<Shape<8, 1>>(map, args, split, sms, stream);
   if (rows <= 16) return launch<Shape<16, 1>>(map, args, split, sms, stream);
   if (rows <= 32) return launch<Shape<32, 1>>(map, args, split, sms, stream);
-  if (rows <= 64) return launch<Shape<64, 1>>(map, args, split, sms, stream);
-  return launch<Shape<128, 2>>(map, args, split, sms, stream);
+  if (rows <= 64 && args.batch.rows % args.batch.count == 0) {
+    return launch<Shape<64, 2>>(map, args, split, sms, stream);
+  }
+  return launch<Shape<128, 4>>(map, args, split, sms, stream);
 }
 
 }  // namespace nmoe
