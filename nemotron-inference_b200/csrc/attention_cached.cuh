@@ -491,48 +491,65 @@ __device__ __forceinline__ void clean_values(uint8_t* values, int token, int pos
   fence_proxy_async_smem();
 }
 
-// Joins the pieces of a (sequence, key head): this block its share of the rows, a warp per row.
+// Joins the pieces of a (sequence, key head): this block its share of the rows, a warp per row.  With few pieces
+// the next row's are on their way meanwhile.
 template <typename S>
 __device__ void join(const CachedArgs& args, const Split& split, const Segment& s) {
+  constexpr int kAtOnce = 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = args.heads / args.cache.kv_heads, pieces = s.parts, piece = static_cast<int>(blockIdx.x) - s.lead;
-  const int rows = min(S::kRows, s.rows * group - s.row0);
+  const int pieces = s.parts, piece = static_cast<int>(blockIdx.x) - s.lead;
+  const int rows = min(S::kRows, s.rows * (args.heads / args.cache.kv_heads) - s.row0);
   auto sums_of = [&](int p) { return split.slots + slot_floats(S::kRows) * (kSlotsPerBlock * (s.lead + p) + (p == 0)); };
   const int end = rows * (piece + 1) / pieces;
+  struct Read {
+    float reference, weight;  // a lane per piece
+    float4 x[kAtOnce];        // the sums of pieces `first` on
+  };
+  auto read_x = [&](Read& read, int r, int first) {
+#pragma unroll
+    for (int p = 0; p < kAtOnce; ++p) {
+      if (first + p < pieces) read.x[p] = __ldcg(reinterpret_cast<const float4*>(sums_of(first + p) + r * kHeadDim) + lane);
+    }
+  };
+  auto read_start = [&](Read& read, int r, int start) {
+    read.reference = -INFINITY;
+    read.weight = 0.0f;
+    if (start + lane < pieces) {
+      const float* at = sums_of(start + lane) + S::kRows * kHeadDim + r;
+      read.reference = __ldcg(at);
+      read.weight = __ldcg(at + S::kRows);
+    }
+    read_x(read, r, start);
+  };
+  Read read;
+  int r = rows * piece / pieces + warp;
+  if (r < end) read_start(read, r, 0);
 #pragma unroll 1
-  for (int r = rows * piece / pieces + warp; r < end; r += S::kSoftmaxWarps) {
-    // references and sums of weights, a lane per piece; the maximum so far is raised where there are over 32
+  for (; r < end; r += S::kSoftmaxWarps) {
+    const int next = r + S::kSoftmaxWarps, row = s.row0 + r;
+    // the maximum so far is raised where there are over 32 pieces
     float top = -INFINITY, sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
     for (int start = 0; start < pieces; start += 32) {
+      if (start > 0) read_start(read, r, start);
       const int count = min(32, pieces - start);
-      float reference = -INFINITY, weight = 0.0f;
-      if (lane < count) {
-        const float* at = sums_of(start + lane) + S::kRows * kHeadDim + r;
-        reference = __ldcg(at);
-        weight = __ldcg(at + S::kRows);
-      }
-      float scale = 0.0f;
+      const float higher = fmaxf(top, warp_max(read.reference));
+      const float keep = top > -INFINITY ? exp2_approx(top - higher) : 0.0f;
+      const float scale = read.reference > -INFINITY ? exp2_approx(read.reference - higher) : 0.0f;
+      const float weight = scale != 0.0f ? read.weight * scale : 0.0f;
+      top = higher;
+      sum *= keep;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] *= keep;
 #pragma unroll 1
-      for (int first = 0; first < count; first += 8) {
-        float4 x[8];  // (what is behind the last is read again, with no weight)
+      for (int first = 0; first < count; first += kAtOnce) {
+        if (first > 0) read_x(read, r, start + first);
+        float4 x[kAtOnce];
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
-          const int of = min(start + first + p, pieces - 1);
-          x[p] = __ldcg(reinterpret_cast<const float4*>(sums_of(of) + r * kHeadDim) + lane);
-        }
-        if (first == 0) {
-          const float higher = fmaxf(top, warp_max(reference));
-          const float keep = top > -INFINITY ? exp2_approx(top - higher) : 0.0f;
-          top = higher;
-          sum *= keep;
+        for (int p = 0; p < kAtOnce; ++p) x[p] = read.x[p];
+        if (start + first + kAtOnce >= pieces && next < end) read_start(read, next, 0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] *= keep;
-          if (reference > -INFINITY) scale = exp2_approx(reference - top);
-          weight = scale != 0.0f ? weight * scale : 0.0f;
-        }
-#pragma unroll
-        for (int p = 0; p < 8; ++p) {
+        for (int p = 0; p < kAtOnce; ++p) {
           const float f = __shfl_sync(0xffffffffu, scale, first + p);
           if (first + p >= count || f == 0.0f) continue;
           sum += __shfl_sync(0xffffffffu, weight, first + p);
@@ -544,7 +561,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
       }
     }
     const float inverse = 1.0f / sum;
-    const int row = s.row0 + r;
+    const int group = args.heads / args.cache.kv_heads;
     const size_t at = static_cast<size_t>(s.first + row / group) * args.heads + s.kv_head * group + row % group;
     *reinterpret_cast<uint2*>(args.out + at * kHeadDim + lane * 4) =
         make_uint2(pack_bf16(o[0] * inverse, o[1] * inverse), pack_bf16(o[2] * inverse, o[3] * inverse));

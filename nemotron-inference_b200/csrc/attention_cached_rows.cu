@@ -214,8 +214,14 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
 #pragma unroll
           for (int i = p * kPart; i < (p + 1) * kPart; i += 4) {
             float w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = exp2_approx(__uint_as_float(y[i + k]));
+            w[0] = exp2_approx(__uint_as_float(y[i]));
+            w[1] = exp2_approx(__uint_as_float(y[i + 1]));
+            if (i % 8 == 0) {
+              unpack2(exp2_polynomial2<3>(pack2(__uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]))), w[2], w[3]);
+            } else {
+              w[2] = exp2_approx(__uint_as_float(y[i + 2]));
+              w[3] = exp2_approx(__uint_as_float(y[i + 3]));
+            }
             of_part = add2(of_part, add2(pack2(w[0], w[1]), pack2(w[2], w[3])));
             weight_codes(w, a[i / 4], b[i / 4]);
           }

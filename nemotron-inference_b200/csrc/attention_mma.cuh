@@ -97,6 +97,36 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// 2^x for two x <= 120 without the unit for special functions, which takes sixteen a cycle on an SM: x is split
+// into the nearest whole number and a rest f, 2^f is a polynomial 1 + f (c1 + f (c2 + ...)) whose largest
+// relative error over |f| <= 1/2 is as small as the leading 1 allows (1.0e-4 of degree 3, 2.9e-6 of degree 4),
+// and the whole number is added to its exponent.  0 for x <= -127.
+template <int Degree>
+__device__ __forceinline__ uint64_t exp2_polynomial2(uint64_t x) {
+  static_assert(Degree == 3 || Degree == 4);
+  constexpr float kToWhole = 12582912.0f;  // 1.5 * 2^23: the sum's last bits are the nearest whole number
+  float x0, x1;
+  unpack2(x, x0, x1);
+  x = pack2(fmaxf(x0, -127.0f), fmaxf(x1, -127.0f));
+  const uint64_t whole = add2(x, pack2(kToWhole, kToWhole));
+  const uint64_t f = fma2(add2(whole, pack2(-kToWhole, -kToWhole)), pack2(-1.0f, -1.0f), x);
+  uint64_t p;
+  if constexpr (Degree == 3) {
+    p = fma2(pack2(0.055009060f, 0.055009060f), f, pack2(0.24221097f, 0.24221097f));
+    p = fma2(p, f, pack2(0.69328290f, 0.69328290f));
+  } else {
+    p = fma2(pack2(0.0095825763f, 0.0095825763f), f, pack2(0.055906828f, 0.055906828f));
+    p = fma2(p, f, pack2(0.24024107f, 0.24024107f));
+    p = fma2(p, f, pack2(0.69312412f, 0.69312412f));
+  }
+  p = fma2(p, f, pack2(1.0f, 1.0f));
+  float p0, p1, w0, w1;
+  unpack2(p, p0, p1);
+  unpack2(whole, w0, w1);
+  return pack2(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(w0) << 23)),
+               __uint_as_float(__float_as_uint(p1) + (__float_as_uint(w1) << 23)));
+}
+
 // Two values as bf16, `lo` in the low half.
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t w;
