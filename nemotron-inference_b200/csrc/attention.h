@@ -131,6 +131,7 @@ struct PrefillArgs {
   int sequences;
   float scale;
   __nv_bfloat16* out;  // [tokens][heads][128]
+  bool out_aligned;    // to 32 bytes
   float* lse;          // [tokens][heads], may be null
   int* error;
 };

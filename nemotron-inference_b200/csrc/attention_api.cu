@@ -313,6 +313,7 @@ nmoe_status nmoe_attention_prefill(void* stream, const void* q, int64_t q_stride
   args.sequences = count;
   args.scale = scale;
   args.out = static_cast<__nv_bfloat16*>(out);
+  args.out_aligned = !misaligned(out, 32);
   args.lse = lse;
   args.error = error;
   return status_of(nmoe::launch_attention_prefill(args, static_cast<cudaStream_t>(stream)));

@@ -100,14 +100,16 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // 2^x for two x <= 120 without the unit for special functions, which takes sixteen a cycle on an SM: x is split
 // into the nearest whole number and a rest f, 2^f is a polynomial 1 + f (c1 + f (c2 + ...)) whose largest
 // relative error over |f| <= 1/2 is as small as the leading 1 allows (1.0e-4 of degree 3, 2.9e-6 of degree 4),
-// and the whole number is added to its exponent.  0 for x <= -127.
+// and the power of two of the whole number multiplies it.  0 for x <= -127, NaN for NaN.
 template <int Degree>
 __device__ __forceinline__ uint64_t exp2_polynomial2(uint64_t x) {
   static_assert(Degree == 3 || Degree == 4);
   constexpr float kToWhole = 12582912.0f;  // 1.5 * 2^23: the sum's last bits are the nearest whole number
   float x0, x1;
   unpack2(x, x0, x1);
-  x = pack2(fmaxf(x0, -127.0f), fmaxf(x1, -127.0f));
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x0));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x1));
+  x = pack2(x0, x1);
   const uint64_t whole = add2(x, pack2(kToWhole, kToWhole));
   const uint64_t f = fma2(add2(whole, pack2(-kToWhole, -kToWhole)), pack2(-1.0f, -1.0f), x);
   uint64_t p;
@@ -120,11 +122,10 @@ __device__ __forceinline__ uint64_t exp2_polynomial2(uint64_t x) {
     p = fma2(p, f, pack2(0.69312412f, 0.69312412f));
   }
   p = fma2(p, f, pack2(1.0f, 1.0f));
-  float p0, p1, w0, w1;
-  unpack2(p, p0, p1);
+  float w0, w1;
   unpack2(whole, w0, w1);
-  return pack2(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(w0) << 23)),
-               __uint_as_float(__float_as_uint(p1) + (__float_as_uint(w1) << 23)));
+  return mul2(p, pack2(__uint_as_float((__float_as_uint(w0) << 23) + 0x3f800000u),
+                       __uint_as_float((__float_as_uint(w1) << 23) + 0x3f800000u)));
 }
 
 // Two values as bf16, `lo` in the low half.
@@ -132,6 +133,18 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t w;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
   return w;
+}
+
+// A sector of a row, from a 16-byte boundary; in one piece where that is one of 32.
+__device__ __forceinline__ void store_32_bytes(void* to, const uint32_t (&w)[8], bool aligned) {
+  if (aligned) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
 }
 
 // Registers of four warps, all of which call it: what some give up others take, out of those that the

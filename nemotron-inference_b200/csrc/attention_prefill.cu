@@ -32,8 +32,8 @@ constexpr int kTileBytes = kTile * kHeadDim * 2;
 constexpr int kPanelBytes = kTileBytes / 2;   // 64 of the 128 dimensions: rows of 128 bytes
 constexpr int kSlots = 5;                     // key and value tiles in flight, in turn
 constexpr int kSoftmaxWarps = 8;              // four per query tile, a thread per row
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
-constexpr int kThreads = 384;                 // two warps have nothing to do: registers go by four warps
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kCheckWarps = 10;  // and 11
+constexpr int kThreads = 384;
 constexpr int kSoftmaxRegisters = 216, kOtherRegisters = 72;  // 2 * 216 + 72 = 3 * 168, as launched
 constexpr int kTmemColumns = 512;             // S of both tiles, O of both tiles, 128 columns each
 constexpr float kRescale = 8.0f;              // binary orders by which a maximum may outgrow its reference
@@ -49,6 +49,7 @@ struct Control {
   uint64_t q_full[2], q_empty[2], kv_full[kSlots], kv_empty[kSlots];
   uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
   uint64_t work_full[2], work_empty[2], next_full, drained;
+  uint64_t unchecked_full[kSlots];  // values of a masked tile that the check warps have yet to see
   alignas(16) uint32_t next[4];
   Work work[2];
   int has_work[2];
@@ -138,8 +139,11 @@ __device__ void load_role(const PrefillArgs& args, bool two_heads, const CUtenso
       const uint32_t slot = loads % kSlots;
       if (!(ok = wait_warp(smem_u32(&c->kv_empty[slot]), ((loads / kSlots) & 1) ^ 1))) break;
       if (elect_one()) {
-        const uint32_t bar = smem_u32(&c->kv_full[slot]);
+        const int tile = (load >> 1) + 1;
+        const bool masked = (load & 1) && (tile == w.tiles[0] || tile == w.tiles[1]);
+        const uint32_t bar = smem_u32(masked ? &c->unchecked_full[slot] : &c->kv_full[slot]);
         mbar_arrive_expect_tx_at(bar, kTileBytes);
+        if (!masked) mbar_arrive_at(bar);  // (as many arrivals as the two check warps')
         for (int panel = 0; panel < 2; ++panel) {
           tma_load_2d_at(slots_at + slot * kTileBytes + panel * kPanelBytes, load & 1 ? v_map : k_map,
                          w.kv_head * kHeadDim + panel * 64, w.first + (load >> 1) * kTile, bar);
@@ -157,7 +161,7 @@ __device__ void load_role(const PrefillArgs& args, bool two_heads, const CUtenso
   // what is in flight arrives before the block's shared memory is given up
   for (uint32_t back = 1; back <= min(loads, static_cast<uint32_t>(kSlots)); ++back) {
     const uint32_t load = loads - back;
-    wait_warp(smem_u32(&c->kv_full[load % kSlots]), (load / kSlots) & 1);
+    wait_warp(smem_u32(&c->kv_full[load % kSlots]), (load / kSlots) & 1);  // (the check warps' arrivals, too)
   }
   for (int t = 0; t < 2; ++t) {
     if (q_loads[t]) wait_warp(smem_u32(&c->q_full[t]), (q_loads[t] - 1) & 1);
@@ -251,37 +255,67 @@ struct MmaRole {
   }
 };
 
-// The values of a masked tile, seen by the 128 threads of a query tile before they let the tensor cores
-// have it: a weight of 0 times a value that is no number would be none either.  Such values become 0
-// here and are added by add_bad_values().
-__device__ __forceinline__ void clear_bad_values(uint8_t* tile, Control* c, int thread) {
-#pragma unroll 4
-  for (int i = thread; i < kTileBytes / 16; i += kTile) {
-    uint4* at = reinterpret_cast<uint4*>(tile) + i;
-    const uint4 x = *at;
-    if (is_no_number(x.x) || is_no_number(x.y) || is_no_number(x.z) || is_no_number(x.w)) {
-      atomicExch(&c->bad_values, 1);
-      __threadfence_block();
-      uint16_t* each = reinterpret_cast<uint16_t*>(at);
-      for (int k = 0; k < 8; ++k) {
-        if ((each[k] & 0x7f80u) == 0x7f80u) each[k] = 0;
+// Two warps that see the values of masked tiles before the tensor cores do: a weight of 0 times a value that is
+// no number would be none either.  Such values become 0 here and are added by add_bad_values().  The masked tiles
+// of a block's work are the last one of each query tile.
+__device__ bool check_role(uint8_t* slots, Control* c) {
+  const int thread = threadIdx.x - kCheckWarps * 32;
+  uint32_t loads = 0, seen = 0;  // a bit per slot: the parity of what has been checked there
+#pragma unroll 1
+  for (uint32_t items = 0;; ++items) {
+    const uint32_t place = items & 1;
+    if (!wait_warp(smem_u32(&c->work_full[place]), (items >> 1) & 1)) return false;
+    const int some = c->has_work[place], tiles[2] = {c->work[place].tiles[0], c->work[place].tiles[1]};
+    __syncwarp();
+    if (!some) return true;
+    if ((thread & 31) == 0) mbar_arrive(&c->work_empty[place]);
+#pragma unroll 1
+    for (int t = 0; t < 2; ++t) {
+      if (tiles[t] == 0 || (t == 1 && tiles[1] == tiles[0])) continue;
+      const uint32_t slot = (loads + 2 * tiles[t] - 1) % kSlots;
+      if (!wait_warp(smem_u32(&c->unchecked_full[slot]), (seen >> slot) & 1)) return false;
+      seen ^= 1u << slot;
+      uint4* tile = reinterpret_cast<uint4*>(slots + slot * kTileBytes) + thread;
+#pragma unroll 1
+      for (int i = 0; i < kTileBytes / 16; i += 8 * 64) {
+        uint4 x[8];
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = tile[i + k * 64];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          bad = bad || is_no_number(x[k].x) || is_no_number(x[k].y) || is_no_number(x[k].z) || is_no_number(x[k].w);
+        }
+        if (!bad) continue;
+        c->bad_values = 1;
+#pragma unroll 1
+        for (int k = 0; k < 64; ++k) {
+          uint16_t* value = reinterpret_cast<uint16_t*>(tile + i + k / 8 * 64) + k % 8;
+          if ((*value & 0x7f80u) == 0x7f80u) *value = 0;
+        }
       }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if ((thread & 31) == 0) mbar_arrive(&c->kv_full[slot]);
     }
+    loads += 2 * max(tiles[0], tiles[1]);
   }
-  fence_proxy_async_smem();
 }
 
-// Adds what clear_bad_values() took out of the block's tiles to 32 columns of a row's result.
+// Adds what check_role() took out of the block's tiles to a row's result.
 __device__ __forceinline__ void add_bad_values(const PrefillArgs& args, const Work& w, int t, int row,
-                                            int column, float* o) {
+                                               uint32_t (&o)[kHeadDim]) {
+#pragma unroll 1
   for (int other = 0; other <= t; ++other) {
     if (w.tiles[other] == 0) continue;
     const int begin = (w.tiles[other] - 1) * kTile, end = min(begin + kTile, row + 1);
+#pragma unroll 1
     for (int j = begin; j < end; ++j) {
-      const __nv_bfloat16* v = args.v + (w.first + j) * args.v_stride + w.kv_head * kHeadDim + column;
-      for (int i = 0; i < 32; ++i) {
+      const __nv_bfloat16* v = args.v + (w.first + j) * args.v_stride + w.kv_head * kHeadDim;
+#pragma unroll
+      for (int i = 0; i < kHeadDim; ++i) {
         const float x = __bfloat162float(v[i]);
-        if (!(fabsf(x) < INFINITY)) o[i] += x;
+        if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
       }
     }
     if (w.row[0] == w.row[1]) break;  // (both tiles have the same last one)
@@ -289,14 +323,14 @@ __device__ __forceinline__ void add_bad_values(const PrefillArgs& args, const Wo
 }
 
 // Four warps per query tile, a thread per row.
-__device__ void softmax_role(const PrefillArgs& args, uint8_t* slots, uint32_t tmem, Control* c) {
+__device__ void softmax_role(const PrefillArgs& args, uint32_t tmem, Control* c) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = warp >> 2, thread = threadIdx.x & (kTile - 1);
   const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp, from bit 16
   const uint32_t s_at = tmem + lanes + t * kTile, o_at = tmem + lanes + 2 * kTile + t * kHeadDim;
   const float factor = args.scale * kLog2e;
   const uint64_t factor2 = pack2(factor, factor);
-  uint32_t s_uses = 0, o_uses = 0, loads = 0;
+  uint32_t s_uses = 0, o_uses = 0;
   for (uint32_t items = 0;; ++items) {
     const uint32_t place = items & 1;
     if (!wait_warp(smem_u32(&c->work_full[place]), (items >> 1) & 1)) break;
@@ -304,9 +338,7 @@ __device__ void softmax_role(const PrefillArgs& args, uint8_t* slots, uint32_t t
     const Work w = c->work[place];
     __syncwarp();
     if (lane == 0) mbar_arrive(&c->work_empty[place]);
-    const int tiles = w.tiles[t], most = max(w.tiles[0], w.tiles[1]);
-    const uint32_t first_load = loads;
-    loads += 2 * most;
+    const int tiles = w.tiles[t];
     float top = 0.0f;
     uint64_t sum2 = 0;
     bool ok = true;
@@ -314,11 +346,6 @@ __device__ void softmax_role(const PrefillArgs& args, uint8_t* slots, uint32_t t
       if (!(ok = wait_warp(smem_u32(&c->s_full[t]), s_uses & 1))) break;
       ++s_uses;
       tcgen05_fence_after();
-      if (j + 1 == tiles || j + 1 == w.tiles[0]) {  // a tile on a diagonal, one's own or the other's
-        const uint32_t load = first_load + 2 * j + 1;
-        if (!(ok = wait_warp(smem_u32(&c->kv_full[load % kSlots]), (load / kSlots) & 1))) break;
-        clear_bad_values(slots + (load % kSlots) * kTileBytes, c, thread);
-      }
       uint32_t s[kTile];
 #pragma unroll
       for (int part = 0; part < 4; ++part) tmem_ld_x32_async(s_at + part * 32, s + part * 32);
@@ -367,10 +394,17 @@ __device__ void softmax_role(const PrefillArgs& args, uint8_t* slots, uint32_t t
           const int at = part * 32 + 2 * i;
           const uint64_t x = fma2(pack2(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), factor2, shift2);
           float a, b;
-          unpack2(x, a, b);
-          a = exp2_approx(a);
-          b = exp2_approx(b);
-          part2[i & 1] = add2(part2[i & 1], pack2(a, b));
+          uint64_t e;
+          if (i % 4 == 3) {
+            e = exp2_polynomial2<4>(x);
+            unpack2(e, a, b);
+          } else {
+            unpack2(x, a, b);
+            a = exp2_approx(a);
+            b = exp2_approx(b);
+            e = pack2(a, b);
+          }
+          part2[i & 1] = add2(part2[i & 1], e);
           p[i] = pack_bf16(a, b);
         }
         tmem_st_x16(s_at + part * 16, p);
@@ -394,32 +428,26 @@ __device__ void softmax_role(const PrefillArgs& args, uint8_t* slots, uint32_t t
     const bool bad = *reinterpret_cast<volatile int*>(&c->bad_values) != 0;
     const float inverse = 1.0f / sum;
     const size_t at = static_cast<size_t>(w.first + row) * args.heads + w.head[t];
+    uint32_t o[kHeadDim];
 #pragma unroll
-    for (int part = 0; part < 4; ++part) {
-      uint32_t o[32];
-      tmem_ld_x32_async(o_at + part * 32, o);
-      tmem_ld_wait();
-      registers_loaded<32>(o);
-      if (part == 3) {
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&c->o_empty[t]);
-      }
-      if (!valid) continue;
-      if (bad) {
-        float copy[32];
-        for (int i = 0; i < 32; ++i) copy[i] = __uint_as_float(o[i]);
-        add_bad_values(args, w, t, row, part * 32, copy);
-        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(copy[i]);
-      }
-      uint32_t two[16];
+    for (int part = 0; part < 4; ++part) tmem_ld_x32_async(o_at + part * 32, o + part * 32);
+    tmem_ld_wait();
+    registers_loaded<kHeadDim>(o);
+    tcgen05_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&c->o_empty[t]);
+    if (valid) {
+      if (bad) add_bad_values(args, w, t, row, o);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        two[i] = pack_bf16(__uint_as_float(o[2 * i]) * inverse, __uint_as_float(o[2 * i + 1]) * inverse);
-      }
-      uint4* to = reinterpret_cast<uint4*>(args.out + at * kHeadDim + part * 32);
+      for (int part = 0; part < 8; ++part) {  // 32 bytes, whole sectors
+        uint32_t two[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) to[i] = make_uint4(two[4 * i], two[4 * i + 1], two[4 * i + 2], two[4 * i + 3]);
+        for (int i = 0; i < 8; ++i) {
+          const int column = part * 16 + 2 * i;
+          two[i] = pack_bf16(__uint_as_float(o[column]) * inverse, __uint_as_float(o[column + 1]) * inverse);
+        }
+        store_32_bytes(args.out + at * kHeadDim + part * 16, two, args.out_aligned);
+      }
     }
     if (valid && args.lse != nullptr) args.lse[at] = kLn2 * (top * factor + log2f(sum));
   }
@@ -444,10 +472,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&c->o_full[t], 1);
       mbar_init(&c->o_empty[t], 4);
       mbar_init(&c->work_full[t], 1);
-      mbar_init(&c->work_empty[t], kSoftmaxWarps + 1);
+      mbar_init(&c->work_empty[t], kSoftmaxWarps + 3);
     }
     for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&c->kv_full[i], 1);
+      mbar_init(&c->kv_full[i], 2);
+      mbar_init(&c->unchecked_full[i], 1);
       mbar_init(&c->kv_empty[i], 1);
     }
     mbar_init(&c->next_full, 1);
@@ -465,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = c->tmem;
   if (warp < kSoftmaxWarps) {
     more_registers<kSoftmaxRegisters>();
-    softmax_role(args, slots, tmem, c);
+    softmax_role(args, tmem, c);
   } else if (warp == kMmaWarp) {
     fewer_registers<kOtherRegisters>();
     MmaRole role{c, smem_u32(shared), smem_u32(slots), tmem};
@@ -487,6 +516,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     fewer_registers<kOtherRegisters>();
     if (warp == kLoadWarp) {
       load_role(args, two_heads, &q_map, &k_map, &v_map, smem_u32(shared), smem_u32(slots), c);
+    } else if (!check_role(slots, c) && elect_one()) {
+      report_cache_error(args.error, kDevWaitTimeout);
     }
   }
   tcgen05_fence_before();

@@ -82,6 +82,19 @@ def test_prefill_against_64_bits(attention, lengths, heads, kv_heads):
     assert torch.equal(again, got)  # the same bits every time, with or without the sums
 
 
+@pytest.mark.parametrize("lengths,heads,kv_heads", [
+    ([2100], 32, 2), ([700, 1300, 40, 0, 950], 16, 8), ([1500, 300], 15, 5), ([128] * 20, 40, 8)])
+def test_prefill_with_more_tiles_than_blocks(attention, lengths, heads, kv_heads):
+    t = sum(lengths)
+    q, k, v = (_normal(50 + i, t, h, D).to(torch.bfloat16) for i, h in enumerate((heads, kv_heads, kv_heads)))
+    got, lse = attention.attention_prefill(q, k, v, _offsets(lengths), return_lse=True)
+    assert attention.prefill_sync_status() == 0
+    _check_prefill(q, k, v, lengths, got, lse)
+    for _ in range(3):
+        assert torch.equal(attention.attention_prefill(q, k, v, _offsets(lengths)), got)
+    assert attention.prefill_sync_status() == 0
+
+
 def test_prefill_of_separate_tensors_and_a_scale_of_its_own(attention):
     n, heads, kv_heads = 321, 6, 2
     q = _normal(1, n, heads, D).to(torch.bfloat16)
@@ -103,6 +116,28 @@ def test_prefill_of_scores_far_from_zero(attention):
     v = _normal(7, n, 1, D).to(torch.bfloat16)
     got = attention.attention_prefill(q, k, v, _offsets([n]))
     _check_prefill(q, k, v, [n], got)
+
+
+@pytest.mark.parametrize("token", range(20, 29))
+def test_prefill_of_a_key_that_is_no_number(attention, token):
+    # wherever it stands in its tile: the rows that see it are no numbers, those before it are the same
+    q, k, v = (_normal(40 + i, 150, h, D).to(torch.bfloat16) for i, h in enumerate((2, 1, 1)))
+    clean = attention.attention_prefill(q, k, v, _offsets([150]))
+    k[token, 0, 7] = math.nan
+    got = attention.attention_prefill(q, k, v, _offsets([150]))
+    assert torch.equal(got[:token], clean[:token]) and bool(got[token:].float().isnan().all())
+
+
+@pytest.mark.parametrize("heads,token", [(2, t) for t in range(64, 74)] + [(32, t) for t in range(64, 74)])
+def test_attend_to_a_key_that_is_no_number(attention, heads, token):
+    cache = _filled(attention, [100, 100], 1, 64, seed=6, layers=1)
+    q = _normal(14, 2, heads, D).to(torch.bfloat16)
+    batch = (_int([0, 1]), _offsets([1, 1]))
+    clean = cache.attend(0, q, *batch)
+    page = int(cache.block_table[1, token // 64])
+    cache.codes.view(torch.uint8)[0, page, 0, 0, token % 64, 11] = 0x7F
+    got = cache.attend(0, q, *batch)
+    assert torch.equal(got[0], clean[0]) and bool(got[1].float().isnan().all())
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
