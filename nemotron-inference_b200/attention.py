@@ -30,6 +30,7 @@ import torch
 from . import NMOE_OK, NmoeError, _check, _stream, load_library
 
 HEAD_DIM = 128
+DEFAULT_SCALE = HEAD_DIM ** -0.5
 
 
 class _KvCache(ctypes.Structure):
@@ -68,44 +69,49 @@ def _lib() -> ctypes.CDLL:
     return _library
 
 
-def _require_rows(t: torch.Tensor, name: str, device: torch.device) -> None:
-    """[rows, heads, 128] bf16, a row's heads side by side; rows may lie further apart."""
+def _row_layout(t: torch.Tensor, name: str, device: torch.device):
+    """Rows, heads and the elements from row to row of a [rows, heads, 128] bf16 tensor whose rows have
+    their heads side by side (rows may lie further apart)."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is torch.bfloat16 and len(shape) == 3 and t.device == device:
+        rows, heads, dim = shape
+        if dim == HEAD_DIM and heads and (
+                not rows or (stride[2] == 1 and (heads == 1 or stride[1] == HEAD_DIM))):
+            return rows, heads, stride[0] if rows > 1 else heads * HEAD_DIM
     if t.device != device:
         raise ValueError(f"{name} must be on {device}: this library has no CPU path")
-    if t.dtype != torch.bfloat16:
+    if t.dtype is not torch.bfloat16:
         raise ValueError(f"{name} must be bfloat16, not {t.dtype}")
-    if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.shape[1] == 0:
-        raise ValueError(f"{name} must be [rows, heads, {HEAD_DIM}], not {list(t.shape)}")
-    if t.shape[0] and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != HEAD_DIM)):
-        raise ValueError(f"{name}: the heads of a row must lie side by side")
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * HEAD_DIM
+    if len(shape) != 3 or shape[2] != HEAD_DIM or shape[1] == 0:
+        raise ValueError(f"{name} must be [rows, heads, {HEAD_DIM}], not {list(shape)}")
+    raise ValueError(f"{name}: the heads of a row must lie side by side")
 
 
 def _require_list(t: torch.Tensor, name: str, device: torch.device) -> None:
-    if t.device != device or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{name} must be a contiguous int32 vector on {device}")
 
 
-def _require_current(device: torch.device, what: str) -> None:
+def _stream_of(device: torch.device, what: str) -> int:
+    """The current stream, if `device` is the current device."""
     if device.type != "cuda":
         raise ValueError(f"{what} must be a CUDA tensor: this library has no CPU path")
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch._C._cuda_getDevice():
         raise ValueError(f"{what} is on {device}, which is not the current device")
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _output(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device or \
             not out.is_contiguous():
         raise ValueError(f"out must be contiguous bfloat16 {list(q.shape)} on {q.device}")
     return out
 
 
-_error_words: Dict[torch.device, torch.Tensor] = {}
+_error_words: Dict[int, torch.Tensor] = {}
 
 
 def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
@@ -117,34 +123,31 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets
     for, the FP32 logarithms [rows, heads] of the rows' sums of exponentials.  `scale` is
     1 / sqrt(128) unless given."""
     device = q.device
-    _require_current(device, "q")
-    _require_rows(q, "q", device)
-    _require_rows(k, "k", device)
-    _require_rows(v, "v", device)
+    stream = _stream_of(device, "q")
+    rows, heads, q_stride = _row_layout(q, "q", device)
+    k_rows, kv_heads, k_stride = _row_layout(k, "k", device)
+    v_rows, v_heads, v_stride = _row_layout(v, "v", device)
     _require_list(offsets, "offsets", device)
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or q.shape[1] % k.shape[1] or \
-            offsets.numel() == 0:
+    prompts = offsets.shape[0] - 1
+    if k_rows != rows or v_rows != rows or v_heads != kv_heads or heads % kv_heads or prompts < 0:
         raise NmoeError(1, "attention_prefill", "k and v need q's rows and a divisor of its heads, "
                                                 "offsets one entry more than there are prompts")
     out = _output(out, q)
-    lse = None
-    if return_lse:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device)
-    error = _error_words.get(device)
+    lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
+    error = _error_words.get(device.index)
     if error is None:
-        error = _error_words[device] = torch.zeros(1, dtype=torch.int32, device=device)
-    _check(_lib().nmoe_attention_prefill(
-        _stream(), q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(),
-        _row_stride(v), q.shape[0], q.shape[1], k.shape[1], offsets.data_ptr(), offsets.numel() - 1,
-        HEAD_DIM ** -0.5 if scale is None else scale, out.data_ptr(),
-        lse.data_ptr() if lse is not None else None, error.data_ptr()), "nmoe_attention_prefill")
+        error = _error_words[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+    _check((_library or _lib()).nmoe_attention_prefill(
+        stream, q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, rows, heads,
+        kv_heads, offsets.data_ptr(), prompts, DEFAULT_SCALE if scale is None else scale,
+        out.data_ptr(), None if lse is None else lse.data_ptr(), error.data_ptr()),
+        "nmoe_attention_prefill")
     return (out, lse) if return_lse else out
 
 
 def prefill_sync_status() -> int:
     """Waits for the current stream; the status of `attention_prefill` on this device."""
-    device = torch.device("cuda", torch.cuda.current_device())
-    error = _error_words.get(device)
+    error = _error_words.get(torch.cuda.current_device())
     return NMOE_OK if error is None else _lib().nmoe_attention_sync_status(error.data_ptr(), _stream())
 
 
@@ -159,7 +162,7 @@ class KvCache:
         [layers, pages, 2, kv_heads] int8, block_table [max_sequences, max_pages] int32, lengths
         [max_sequences] int32, references [pages] int32."""
         device = codes.device
-        _require_current(device, "codes")
+        _stream_of(device, "codes")
         if codes.dtype != torch.float8_e4m3fn or codes.dim() != 6 or codes.shape[2] != 2 or \
                 codes.shape[5] != HEAD_DIM:
             raise ValueError("codes must be float8_e4m3fn [layers, pages, 2, kv_heads, page_tokens, "
@@ -206,80 +209,80 @@ class KvCache:
         return KvCache(codes, exponents, torch.zeros((max_sequences, max_pages_per_sequence), **int32),
                        torch.zeros((max_sequences,), **int32), torch.zeros((pages,), **int32))
 
-    def _batch(self, sequences: torch.Tensor, offsets: torch.Tensor) -> None:
-        _require_current(self.device, "the cache")
-        _require_list(sequences, "sequences", self.device)
-        _require_list(offsets, "offsets", self.device)
-        if offsets.numel() != sequences.numel() + 1:
+    def _batch(self, sequences: torch.Tensor, offsets: torch.Tensor) -> int:
+        """The current stream, if the lists are a batch's."""
+        device = self.device
+        _require_list(sequences, "sequences", device)
+        _require_list(offsets, "offsets", device)
+        if offsets.shape[0] != sequences.shape[0] + 1:
             raise ValueError("offsets must have one entry more than sequences")
+        return _stream_of(device, "the cache")
 
     def extend(self, sequences: torch.Tensor, offsets: torch.Tensor, rows: int) -> None:
         """Makes room for `rows` new tokens, entry i's offsets[i + 1] - offsets[i] of them: the
         lowest free pages, in list order.  Too few: NMOE_ERR_CAPACITY from `sync_status`, and
         nothing has changed."""
-        self._batch(sequences, offsets)
-        _check(_lib().nmoe_kv_extend(self._ref, _stream(), sequences.data_ptr(), offsets.data_ptr(),
+        stream = self._batch(sequences, offsets)
+        _check(_lib().nmoe_kv_extend(self._ref, stream, sequences.data_ptr(), offsets.data_ptr(),
                                      sequences.numel(), rows), "nmoe_kv_extend")
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, sequences: torch.Tensor,
                offsets: torch.Tensor) -> None:
         """Quantises the rows into their places, the last tokens of each sequence."""
-        self._batch(sequences, offsets)
-        _require_rows(k, "k", self.device)
-        _require_rows(v, "v", self.device)
-        if k.shape != v.shape or k.shape[1] != self.kv_heads:
+        stream = self._batch(sequences, offsets)
+        rows, heads, k_stride = _row_layout(k, "k", self.device)
+        v_rows, v_heads, v_stride = _row_layout(v, "v", self.device)
+        if v_rows != rows or heads != self.kv_heads or v_heads != heads:
             raise NmoeError(1, "KvCache.append", "k and v must be [rows, kv_heads, 128]")
-        _check(_lib().nmoe_kv_append(self._ref, _stream(), layer, k.data_ptr(), _row_stride(k),
-                                     v.data_ptr(), _row_stride(v), sequences.data_ptr(),
-                                     offsets.data_ptr(), sequences.numel(), k.shape[0]),
-               "nmoe_kv_append")
+        _check(_lib().nmoe_kv_append(self._ref, stream, layer, k.data_ptr(), k_stride, v.data_ptr(),
+                                     v_stride, sequences.data_ptr(), offsets.data_ptr(),
+                                     sequences.shape[0], rows), "nmoe_kv_append")
 
     def attend(self, layer: int, q: torch.Tensor, sequences: torch.Tensor, offsets: torch.Tensor,
                scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of new rows, the last tokens of their sequences: row j of c sees every token
         up to position length - c + j.  Returns [rows, heads, 128] bf16."""
-        self._batch(sequences, offsets)
-        _require_rows(q, "q", self.device)
-        if q.shape[1] % self.kv_heads:
+        stream = self._batch(sequences, offsets)
+        rows, heads, q_stride = _row_layout(q, "q", self.device)
+        if heads % self.kv_heads:
             raise NmoeError(1, "KvCache.attend", "heads must be a multiple of kv_heads")
         out = _output(out, q)
         _check(_lib().nmoe_attention_cached(
-            self._ref, _stream(), layer, q.data_ptr(), _row_stride(q), q.shape[1],
-            sequences.data_ptr(), offsets.data_ptr(), sequences.numel(), q.shape[0],
-            HEAD_DIM ** -0.5 if scale is None else scale, out.data_ptr()), "nmoe_attention_cached")
+            self._ref, stream, layer, q.data_ptr(), q_stride, heads, sequences.data_ptr(),
+            offsets.data_ptr(), sequences.shape[0], rows, DEFAULT_SCALE if scale is None else scale,
+            out.data_ptr()), "nmoe_attention_cached")
         return out
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
         """children[i] becomes a copy of parents[i]: full pages are shared, a partly filled last
         one is copied.  What a child held is given up first."""
-        _require_current(self.device, "the cache")
+        stream = _stream_of(self.device, "the cache")
         _require_list(parents, "parents", self.device)
         _require_list(children, "children", self.device)
         if parents.numel() != children.numel():
             raise ValueError("every child needs one parent")
-        _check(_lib().nmoe_kv_fork(self._ref, _stream(), parents.data_ptr(), children.data_ptr(),
+        _check(_lib().nmoe_kv_fork(self._ref, stream, parents.data_ptr(), children.data_ptr(),
                                    parents.numel()), "nmoe_kv_fork")
 
     def free(self, sequences: torch.Tensor) -> None:
         """Gives up the sequences' pages; what nobody holds any more is free."""
-        _require_current(self.device, "the cache")
+        stream = _stream_of(self.device, "the cache")
         _require_list(sequences, "sequences", self.device)
-        _check(_lib().nmoe_kv_free(self._ref, _stream(), sequences.data_ptr(), sequences.numel()),
+        _check(_lib().nmoe_kv_free(self._ref, stream, sequences.data_ptr(), sequences.numel()),
                "nmoe_kv_free")
 
     def compact(self) -> None:
         """Moves the pages in use to the front of the pool, into the free ones there."""
-        _require_current(self.device, "the cache")
-        _check(_lib().nmoe_kv_compact(self._ref, _stream()), "nmoe_kv_compact")
+        _check(_lib().nmoe_kv_compact(self._ref, _stream_of(self.device, "the cache")), "nmoe_kv_compact")
 
     def copy_pages(self, sources: torch.Tensor, targets: torch.Tensor) -> None:
         """Copies pages in every layer; no target is a source or another's target."""
-        _require_current(self.device, "the cache")
+        stream = _stream_of(self.device, "the cache")
         _require_list(sources, "sources", self.device)
         _require_list(targets, "targets", self.device)
         if sources.numel() != targets.numel():
             raise ValueError("every source needs one target")
-        _check(_lib().nmoe_kv_copy_pages(self._ref, _stream(), sources.data_ptr(),
+        _check(_lib().nmoe_kv_copy_pages(self._ref, stream, sources.data_ptr(),
                                          targets.data_ptr(), sources.numel()), "nmoe_kv_copy_pages")
 
     def sync_status(self) -> int:

@@ -6,8 +6,11 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
+
+#include "kernels.h"
 
 namespace nmoe {
 
@@ -120,6 +123,19 @@ __device__ __forceinline__ int2 locate_unit(int n, int64_t u, Units units) {
 }
 
 #endif  // __CUDACC__
+
+// allow_shared_memory(), once for each device (a bit of `allowed`): it takes a tenth of a short call.
+template <typename Kernel>
+inline cudaError_t allow_shared_memory_once(Kernel* kernel, std::atomic<uint64_t>& allowed) {
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (allowed.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  err = allow_shared_memory(kernel);
+  if (err == cudaSuccess && device < 64) allowed.fetch_or(bit, std::memory_order_release);
+  return err;
+}
 
 struct PrefillArgs {
   const __nv_bfloat16* q;

@@ -455,7 +455,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks)
 
 template <typename S>
 cudaError_t launch(const CUtensorMap& map, const CachedArgs& args, const Split& split, int sms, cudaStream_t stream) {
-  cudaError_t err = allow_shared_memory(cached_kernel<S>);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t err = allow_shared_memory_once(cached_kernel<S>, allowed);
   if (err != cudaSuccess) return err;
   cached_kernel<S><<<sms * S::kBlocks, S::kThreads, shared_bytes<S>(), stream>>>(map, args, split);
   return cudaGetLastError();

@@ -350,7 +350,8 @@ __global__ void __launch_bounds__(S::kThreads, 1)
 }  // namespace
 
 cudaError_t launch_cached_rows(const CUtensorMap& map, const CachedArgs& args, const Split& split, int sms, cudaStream_t stream) {
-  cudaError_t err = allow_shared_memory(cached_rows_kernel);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t err = allow_shared_memory_once(cached_rows_kernel, allowed);
   if (err != cudaSuccess) return err;
   cached_rows_kernel<<<sms, S::kThreads, kSharedBytes, stream>>>(map, args, split);
   return cudaGetLastError();
