@@ -40,102 +40,135 @@ __device__ __forceinline__ float2 decode_two(uint32_t codes) {
 }
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendChunks = 128 * kHeadDim / 8 / kAppendThreads;  // of 8 values, the largest page
+constexpr int kAppendBlocks = 6;  // on an SM
 
-// A block per page that gets new rows, head, and keys or values.  The page's new values stay in
-// registers between the maximum that gives the exponent and their rounding, so they are read once.
+// A block per page that gets new rows and `per_block` of its heads' keys and values.  A page and head's new
+// values stay in registers between the maximum that gives the exponent and their rounding, so they are read
+// once; finding the page is a chain of loads, which the heads share where there are blocks enough.
 // A page that held tokens may get a larger exponent: its older codes are rounded again then, which
 // is exact but for values that fall among the subnormal codes.
-__global__ void __launch_bounds__(kAppendThreads)
+// The largest 16-bit half of all threads' words; `parts` is not in use by another call.
+__device__ __forceinline__ uint32_t block_max(uint32_t two, uint32_t* parts) {
+  __syncthreads();  // (the parts of the call before are read)
+  const uint32_t mine = __reduce_max_sync(0xffffffffu, max(two & 0xffffu, two >> 16));
+  if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (int w = 0; w < kAppendThreads / 32; ++w) all = max(all, parts[w]);
+  return all;
+}
+
+// Magnitudes of two bf16, 0 for an infinity or NaN.
+__device__ __forceinline__ uint32_t finite_only(uint32_t two) {
+  const uint32_t lo = two & 0x7fffu, hi = two & 0x7fff0000u;
+  return (lo < 0x7f80u ? lo : 0u) | (hi < 0x7f800000u ? hi : 0u);
+}
+
+template <int PageTokens>
+__global__ void __launch_bounds__(kAppendThreads, PageTokens <= 64 ? kAppendBlocks : 4)
     kv_append_kernel(PagedCache c, Batch b, int layer, const __nv_bfloat16* k, int64_t k_stride,
-                     const __nv_bfloat16* v, int64_t v_stride) {
-  __shared__ float warp_max[kAppendThreads / 32];
-  if (*c.error != 0) return;  // a reservation failed: these rows have no place of their own
-  const int half = blockIdx.y & 1, head = blockIdx.y >> 1;
+                     const __nv_bfloat16* v, int64_t v_stride, int per_block) {
+  constexpr int kAppendChunks = PageTokens * kHeadDim / 8 / kAppendThreads;  // of 8 values, to a thread
+  __shared__ uint32_t warp_max[2][kAppendThreads / 32];
+  const int pending = *c.error;
   const int2 unit = locate_unit(b.count, blockIdx.x, [&](int i) {
     const BatchEntry e = batch_entry(c, b, i);
     if (!e.valid) report_cache_error(c.error, kCacheBadSequence);
     if (e.rows == 0) return 0;
     return ((e.length - 1) >> c.page_shift) - ((e.length - e.rows) >> c.page_shift) + 1;
   });
-  if (unit.x < 0) return;
+  // (after a reservation that failed these rows have no place of their own)
+  if (pending != 0 || unit.x < 0) return;
   const BatchEntry e = batch_entry(c, b, unit.x);
   const int place = ((e.length - e.rows) >> c.page_shift) + unit.y;
   const int begin = max(e.length - e.rows, place << c.page_shift);  // positions in the sequence
   const int end = min(e.length, (place + 1) << c.page_shift);
   const int held = begin & (c.page_tokens - 1);
+  const int last = min(static_cast<int>(blockIdx.y + 1) * per_block, 2 * c.kv_heads);
+  const int chunks = (end - begin) * (kHeadDim / 8), first_row = e.first + begin - (e.length - e.rows);
+  auto read = [&](int of, uint4(&raw)[kAppendChunks]) {
+    const int64_t stride = of & 1 ? v_stride : k_stride;
+    const __nv_bfloat16* from = (of & 1 ? v : k) + (of >> 1) * kHeadDim + first_row * stride;
+#pragma unroll
+    for (int i = 0; i < kAppendChunks; ++i) {
+      const int chunk = i * kAppendThreads + threadIdx.x;
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (chunk < chunks) raw[i] = *reinterpret_cast<const uint4*>(from + (chunk / 16) * stride + (chunk % 16) * 8);
+    }
+  };
+  uint4 raw[kAppendChunks];
+  read(blockIdx.y * per_block, raw);  // (under way while the page is looked up)
   const int page = page_at(c, e.sequence, place);
   if (page < 0) {
     report_cache_error(c.error, kCacheBadSequence);
     return;
   }
-  const size_t block = block_of_page(c, layer, page, half, head);
-  uint8_t* codes = c.codes + block * c.page_tokens * kHeadDim;
-  const int before = c.exponents[block];
-  const int64_t stride = half ? v_stride : k_stride;
-  const __nv_bfloat16* from = (half ? v : k) + head * kHeadDim +
-                              (e.first + begin - (e.length - e.rows)) * stride;
-  const int chunks = (end - begin) * (kHeadDim / 8);
-  uint4 raw[kAppendChunks];
-  float amax = 0.0f;
+#pragma unroll 1
+  for (int of = blockIdx.y * per_block; of < last; ++of) {
+    const size_t block = block_of_page(c, layer, page, of & 1, of >> 1);
+    uint8_t* codes = c.codes + block * c.page_tokens * kHeadDim;
+    const int before = held > 0 ? c.exponents[block] : 0;
+    // magnitudes as whole numbers, two at a time; those of infinities and NaN are beyond all others
+    uint32_t two_max = 0;
 #pragma unroll
-  for (int i = 0; i < kAppendChunks; ++i) {
-    const int chunk = i * kAppendThreads + threadIdx.x;
-    if (chunk < chunks) {
-      raw[i] = *reinterpret_cast<const uint4*>(from + (chunk / 16) * stride + (chunk % 16) * 8);
+    for (int i = 0; i < kAppendChunks; ++i) {
       const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float lo = fabsf(__uint_as_float(words[w] << 16));
-        const float hi = fabsf(__uint_as_float(words[w] & 0xffff0000u));
-        if (lo < INFINITY) amax = fmaxf(amax, lo);
-        if (hi < INFINITY) amax = fmaxf(amax, hi);
+      for (int w = 0; w < 4; ++w) two_max = __vmaxu2(two_max, words[w] & 0x7fff7fffu);
+    }
+    uint32_t largest = block_max(two_max, warp_max[0]);
+    const bool special = largest >= 0x7f80u;
+    if (special) {
+      two_max = 0;
+#pragma unroll
+      for (int i = 0; i < kAppendChunks; ++i) {
+        const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) two_max = __vmaxu2(two_max, finite_only(words[w]));
+      }
+      largest = block_max(two_max, warp_max[1]);
+    }
+    const float amax = __uint_as_float(largest << 16);
+    int after = exponent_for(amax);
+    if (held > 0) after = max(after, before);
+    if (threadIdx.x == 0) c.exponents[block] = static_cast<int8_t>(after);
+    if (held > 0 && after > before) {
+      const float lower = power_of_two(before - after);
+      uint4* older = reinterpret_cast<uint4*>(codes);
+      for (int i = threadIdx.x; i < held * (kHeadDim / 16); i += kAppendThreads) {
+        uint4 x = older[i];
+        uint32_t* words = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float2 a = decode_two(words[w]), z = decode_two(words[w] >> 16);
+          words[w] = encode_two(a.x * lower, a.y * lower) | (encode_two(z.x * lower, z.y * lower) << 16);
+        }
+        older[i] = x;
       }
     }
-  }
+    const uint64_t factor2 = pack2(power_of_two(-after), power_of_two(-after));
 #pragma unroll
-  for (int step = 16; step > 0; step /= 2) {
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, step));
-  }
-  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
-  __syncthreads();
+    for (int i = 0; i < kAppendChunks; ++i) {
+      const int chunk = i * kAppendThreads + threadIdx.x;
+      if (chunk < chunks) {
+        const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        uint32_t two[4];
 #pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, warp_max[w]);
-  int after = exponent_for(amax);
-  if (held > 0) after = max(after, before);
-  if (threadIdx.x == 0) c.exponents[block] = static_cast<int8_t>(after);
-  if (held > 0 && after > before) {
-    const float lower = power_of_two(before - after);
-    uint4* older = reinterpret_cast<uint4*>(codes);
-    for (int i = threadIdx.x; i < held * (kHeadDim / 16); i += kAppendThreads) {
-      uint4 x = older[i];
-      uint32_t* words = reinterpret_cast<uint32_t*>(&x);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float2 a = decode_two(words[w]), z = decode_two(words[w] >> 16);
-        words[w] = encode_two(a.x * lower, a.y * lower) | (encode_two(z.x * lower, z.y * lower) << 16);
+        for (int w = 0; w < 4; ++w) {
+          float lo, hi;
+          unpack2(mul2(pack2(__uint_as_float(words[w] << 16), __uint_as_float(words[w] & 0xffff0000u)), factor2), lo, hi);
+          if (special) {  // an infinity is not hidden behind the largest code
+            if ((words[w] & 0x7f80u) == 0x7f80u) lo = NAN;
+            if ((words[w] & 0x7f800000u) == 0x7f800000u) hi = NAN;
+          }
+          two[w] = encode_two(lo, hi);
+        }
+        *reinterpret_cast<uint2*>(codes + held * kHeadDim + chunk * 8) =
+            make_uint2(two[0] | (two[1] << 16), two[2] | (two[3] << 16));
       }
-      older[i] = x;
     }
-  }
-  const float factor = power_of_two(-after);
-#pragma unroll
-  for (int i = 0; i < kAppendChunks; ++i) {
-    const int chunk = i * kAppendThreads + threadIdx.x;
-    if (chunk < chunks) {
-      const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-      uint32_t two[4];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        float lo = __uint_as_float(words[w] << 16), hi = __uint_as_float(words[w] & 0xffff0000u);
-        // an infinity is not hidden behind the largest code
-        lo = fabsf(lo) < INFINITY ? lo * factor : NAN;
-        hi = fabsf(hi) < INFINITY ? hi * factor : NAN;
-        two[w] = encode_two(lo, hi);
-      }
-      *reinterpret_cast<uint2*>(codes + held * kHeadDim + chunk * 8) =
-          make_uint2(two[0] | (two[1] << 16), two[2] | (two[3] << 16));
-    }
+    if (of + 1 < last) read(of + 1, raw);
   }
 }
 
@@ -326,6 +359,7 @@ __global__ void __launch_bounds__(kBookThreads)
 __global__ void __launch_bounds__(kBookThreads)
     kv_fork_kernel(PagedCache c, const int* parents, const int* children, int count) {
   __shared__ BookShared s;
+  release_successor();
   if (threadIdx.x == 0) {
     s.flag = 0;
     *c.move_count = 0;
@@ -403,6 +437,7 @@ __global__ void __launch_bounds__(kBookThreads)
 // one below L.  The block table follows in the copy kernel, which has the threads for it.
 __global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) {
   __shared__ BookShared s;
+  release_successor();
   if (threadIdx.x == 0) *c.move_count = 0;
   if (*c.error != 0) return;
   int live = 0;
@@ -440,29 +475,46 @@ __global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) 
 // ---------------------------------------------------------------------------
 
 constexpr int kCopyThreads = 256;
+constexpr int kCopyChunk = kCopyThreads * 4;  // of 16 bytes: four loads under way in each thread
 
 __global__ void __launch_bounds__(kCopyThreads)
     kv_copy_kernel(PagedCache c, const int* sources, const int* targets, const int* count_at,
                    int count, bool rewrite_table) {
   if (count_at != nullptr) {
+    wait_for_predecessor();  // (the books)
     if (*c.error != 0) return;
     count = *count_at;
   }
   const int heads2 = 2 * c.kv_heads;
-  const size_t page_bytes = static_cast<size_t>(heads2) * c.page_tokens * kHeadDim;
-  for (int64_t u = blockIdx.x; u < static_cast<int64_t>(count) * c.layers; u += gridDim.x) {
-    const int from = sources[u / c.layers], to = targets[u / c.layers];
-    const size_t layer = u % c.layers;
+  const size_t page_words = static_cast<size_t>(heads2) * c.page_tokens * kHeadDim / 16;
+  const int chunks = static_cast<int>((page_words + kCopyChunk - 1) / kCopyChunk);
+  const int64_t of_layer = static_cast<int64_t>(count) * chunks;
+  for (int64_t u = blockIdx.x; u < of_layer * c.layers; u += gridDim.x) {
+    const size_t layer = u / of_layer;
+    const int move = static_cast<int>(u % of_layer / chunks), chunk = static_cast<int>(u % chunks);
+    const int from = sources[move], to = targets[move];
     if (static_cast<unsigned>(from) >= static_cast<unsigned>(c.pages) ||
         static_cast<unsigned>(to) >= static_cast<unsigned>(c.pages)) {
       report_cache_error(c.error, kCacheBadSequence);
       continue;
     }
-    const uint4* read = reinterpret_cast<const uint4*>(c.codes + (layer * c.pages + from) * page_bytes);
-    uint4* write = reinterpret_cast<uint4*>(c.codes + (layer * c.pages + to) * page_bytes);
-    for (size_t i = threadIdx.x; i < page_bytes / 16; i += kCopyThreads) write[i] = read[i];
-    for (int i = threadIdx.x; i < heads2; i += kCopyThreads) {
-      c.exponents[(layer * c.pages + to) * heads2 + i] = c.exponents[(layer * c.pages + from) * heads2 + i];
+    const size_t read_page = layer * c.pages + from, write_page = layer * c.pages + to;
+    const size_t at = static_cast<size_t>(chunk) * kCopyChunk + threadIdx.x;
+    const uint4* read = reinterpret_cast<const uint4*>(c.codes) + read_page * page_words + at;
+    uint4* write = reinterpret_cast<uint4*>(c.codes) + write_page * page_words + at;
+    uint4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (at + i * kCopyThreads < page_words) x[i] = __ldcs(read + i * kCopyThreads);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (at + i * kCopyThreads < page_words) __stcs(write + i * kCopyThreads, x[i]);
+    }
+    if (chunk == 0) {
+      for (int i = threadIdx.x; i < heads2; i += kCopyThreads) {
+        c.exponents[write_page * heads2 + i] = c.exponents[read_page * heads2 + i];
+      }
     }
   }
   if (!rewrite_table) return;
@@ -479,9 +531,9 @@ __global__ void __launch_bounds__(kCopyThreads)
 
 cudaError_t launch_copy(const PagedCache& cache, const int* sources, const int* targets,
                         const int* count_at, int count, bool rewrite_table, cudaStream_t stream) {
-  kv_copy_kernel<<<device_sms() * 8, kCopyThreads, 0, stream>>>(cache, sources, targets, count_at,
-                                                                count, rewrite_table);
-  return cudaGetLastError();
+  return launch_kernel(kv_copy_kernel, dim3(device_sms() * 8), kCopyThreads, 0,
+                       LaunchStream(stream, count_at != nullptr), cache, sources, targets, count_at,
+                       count, rewrite_table);
 }
 
 }  // namespace
@@ -492,8 +544,16 @@ cudaError_t launch_kv_append(const PagedCache& cache, const Batch& batch, int la
   // c rows of a sequence touch at most c / page_tokens + 2 pages, and no more than c
   const int64_t units = std::min<int64_t>(
       batch.rows, (batch.rows >> cache.page_shift) + 2 * static_cast<int64_t>(batch.count));
-  kv_append_kernel<<<dim3(static_cast<unsigned>(units), 2 * cache.kv_heads), kAppendThreads, 0,
-                     stream>>>(cache, batch, layer, k, k_stride, v, v_stride);
+  // as many heads to a block as it takes for all blocks to be resident at once
+  const int64_t of = 2 * cache.kv_heads, resident = kAppendBlocks * device_sms();
+  const int64_t groups = std::clamp<int64_t>(resident / units, 1, of);
+  const int per_block = static_cast<int>((of + groups - 1) / groups);
+  const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>((of + per_block - 1) / per_block));
+  auto* kernel = cache.page_tokens == 16   ? kv_append_kernel<16>
+                 : cache.page_tokens == 32 ? kv_append_kernel<32>
+                 : cache.page_tokens == 64 ? kv_append_kernel<64>
+                                           : kv_append_kernel<128>;
+  kernel<<<grid, kAppendThreads, 0, stream>>>(cache, batch, layer, k, k_stride, v, v_stride, per_block);
   return cudaGetLastError();
 }
 
