@@ -167,28 +167,32 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
   const uint64_t* fades = reinterpret_cast<const uint64_t*>(c->fade);
   volatile int* failed = &c->failed;
   int joins = 0;
-  const uint64_t* factors = reinterpret_cast<const uint64_t*>(c->factor);
-  const int* limits = c->limit;
   uint32_t no = 0;  // tiles so far
   bool ok = mbar_wait_warp(smem_u32(&c->segment_full[0]), 0);
   int some = ok && c->has_segment[0];
   uint2 queries[S::kBatch];
-  if (some) load_queries<S>(args, c->segment[0], 0, queries);
+  c->first_bad[token] = INT32_MAX;
+  if (some) {
+    load_queries<S>(args, c->segment[0], 0, queries);
+    prepare_queries<S, 16>(args, c->segment[0], 0, queries, q, c);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&c->q_full);
+  }
 #pragma unroll 1
   for (uint32_t segments = 0;; ++segments) {
     const Segment& s = c->segment[segments % kSegments];
+    const uint32_t following = segments + 1;
+    const uint64_t* factors = reinterpret_cast<const uint64_t*>(c->factor[segments & 1]);
+    const int* limits = c->limit[segments & 1];
     if (!ok) *failed = 1;
-    softmax_sync<S>();
-    if (*failed) return false;
-    if (!some) break;
-    prepare_queries<S, 16>(args, s, queries, q, c);
     if (token < R) {
       c->shift[token] = 0.0f;
       c->highest[token] = kLowest;
     }
-    fence_proxy_async_smem();
     softmax_sync<S>();
-    if (lane == 0) mbar_arrive(&c->q_full);
+    if (*failed) return false;
+    if (!some) break;
     uint64_t sum[R / 2];
 #pragma unroll
     for (int r = 0; r < R / 2; ++r) sum[r] = 0;
@@ -209,6 +213,12 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       const uint64_t v2 = pack2(v_power, v_power);
       const float v_inverse = exp2_approx(-v_power);
       const uint64_t v2_inverse = pack2(v_inverse, v_inverse);
+      if (j + 1 == s.tiles) {  // the next segment's queries are on their way meanwhile
+        const bool known = mbar_wait_warp(smem_u32(&c->segment_full[following % kSegments]), (following / kSegments) & 1);
+        some = known && c->has_segment[following % kSegments];
+        if (some) load_queries<S>(args, c->segment[following % kSegments], 0, queries);
+        ok = ok && known;
+      }
       if (at_end) clean_values<S>(values + slot * kKeyTileBytes, token, position, s, c);
       // exponents of the weights, rows in pairs: score + power of the values - reference + kWeightBits
       uint64_t y[R / 2];
@@ -337,18 +347,19 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       __syncwarp();
       if (lane == 0) mbar_arrive(&c->p_full);
     }
-    // the next segment's queries are on their way during the end of this one
-    const uint32_t following = segments + 1;
-    const bool known = mbar_wait_warp(smem_u32(&c->segment_full[following % kSegments]), (following / kSegments) & 1);
-    some = known && c->has_segment[following % kSegments];
-    if (some) load_queries<S>(args, c->segment[following % kSegments], 0, queries);
+    if (some) {  // (all scores of this segment are done)
+      prepare_queries<S, 16>(args, c->segment[following % kSegments], following & 1, queries, q, c);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c->q_full);
+    }
     // the rows' sums of weights over the 128 threads, in a fixed order
     float each[R];
 #pragma unroll
     for (int r = 0; r < R; r += 2) unpack2(sum[r / 2], each[r], each[r + 1]);
     warp_sums<R>(each, lane);
     c->warp_sum[warp][sum_row<R>(lane, 0)] = each[0];
-    ok = mbar_wait_warp(smem_u32(&c->p_empty), (no & 1) ^ 1) && known;
+    ok = mbar_wait_warp(smem_u32(&c->p_empty), (no & 1) ^ 1);
     tcgen05_fence_after();
     if (!ok) *failed = 1;
     softmax_sync<S>();
@@ -363,9 +374,11 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
     // a thread per dimension now
     const bool alone = s.part < 0;
     float* slot = split.slots + slot_floats(R) * max(s.part, 0);
+    const int* out_rows = c->out_row[segments & 1];
     const int bad = c->first_bad[token];
+    c->first_bad[token] = INT32_MAX;
 #pragma unroll 1
-    for (int i = 0; i < R && c->out_row[i] >= 0; i += 8) {
+    for (int i = 0; i < R && out_rows[i] >= 0; i += 8) {
       uint32_t a[16];
       tmem_ld_x8_async(o_at + i, a);
       tmem_ld_x8_async(o_at + R + i, a + 8);
@@ -373,7 +386,7 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       registers_loaded<16>(a);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int r = i + k, to = c->out_row[r];
+        const int r = i + k, to = out_rows[r];
         float o = fmaf(__uint_as_float(a[k + 8]), 0.0625f, __uint_as_float(a[k]));
         if (limits[r] >= bad) o = NAN;
         if (to < 0) continue;

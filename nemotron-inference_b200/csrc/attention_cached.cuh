@@ -13,8 +13,9 @@
 // together, so it does not matter how far powers lie apart.  The sums of the weights without the values'
 // powers are kept in FP32 beside.
 //
-// With R rows of queries (new rows x heads that share the key head) at a time, W tiles of 128 tokens in all
-// and G blocks, block g takes the tiles [W g / G, W (g + 1) / G) in order, whatever the sequences' lengths.
+// With R rows of queries (new rows x heads that share the key head) at a time, W tiles of 128 tokens in all (and
+// one more for each sequence, key head and rows) and G blocks, block g takes the tiles [W g / G, W (g + 1) / G)
+// in order, whatever the sequences' lengths.
 // Where a (sequence, key head) is cut, each piece leaves its sums in the workspace; when all have, each of
 // these blocks joins a share of the rows, piece by piece in order, so results never depend on timing.
 #pragma once
@@ -32,6 +33,9 @@ constexpr int kKeyTileBytes = kKeyTile * kHeadDim;
 constexpr int kMaxPagesPerTile = kKeyTile / 16;
 constexpr int kMaxRows = 128;
 constexpr int kSegments = 4;
+// What a (sequence, key head, rows) costs a block beside its tiles, in tiles: its queries, and its results on their
+// way out.  Counted where tiles are shared, or blocks that meet many short sequences come last by 20 %.
+constexpr int kUnitCost = 1;
 constexpr int kSlotsPerBlock = 2;      // of the workspace: a piece that began in a block before, one that goes on
 constexpr float kWeightBits = -1.5f;  // a row's largest weight is 2^-1.5 when its reference is set ...
 constexpr float kLargestBits = 0.0f;  // ... and at most 1 before it is set anew
@@ -66,9 +70,10 @@ struct WorkControl {
   int has_segment[kSegments];
   Segment to_join[2];          // the (at most two) that other blocks have pieces of
   int powers[S::kValueSlots][2][kMaxPagesPerTile];  // of a tile's pages, keys and values
-  alignas(16) float factor[S::kRows];  // what a row's product of codes is multiplied by
-  int out_row[S::kRows];               // of the result, -1: none
-  int limit[S::kRows];                 // a row's position: the last token it sees
+  // of this segment's rows and the next one's
+  alignas(16) float factor[2][S::kRows];  // what a row's product of codes is multiplied by
+  int out_row[2][S::kRows];               // of the result, -1: none
+  int limit[2][S::kRows];                 // a row's position: the last token it sees
   int first_bad[kHeadDim];             // position of the first masked value that is no number, by dimension
   int found_bad;
   int joined;
@@ -183,12 +188,14 @@ __device__ __forceinline__ float power_of_two(int e) {  // -126 <= e <= 127
 template <typename S>
 struct EntryTiles {
   int tiles, row_tiles;  // of tokens, of rows
+  int cost;              // of one (key head, rows): the tiles lie behind kUnitCost
   int64_t all;
 
   __device__ EntryTiles(const CachedArgs& args, const BatchEntry& e) {
     tiles = (e.length + kKeyTile - 1) / kKeyTile;
     row_tiles = (e.rows * (args.heads / args.cache.kv_heads) + S::kRows - 1) / S::kRows;
-    all = static_cast<int64_t>(tiles) * row_tiles * args.cache.kv_heads;
+    cost = tiles + kUnitCost;
+    all = static_cast<int64_t>(cost) * row_tiles * args.cache.kv_heads;
   }
 };
 
@@ -268,27 +275,29 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
   while (entry_at < stop && ok) {
     const EntryTiles<S> t(args, e);
     // the first (key head, rows) that reach into this block's share
-    const int unit = max(begin - entry_at, 0) / t.tiles;
+    const int unit = max(begin - entry_at, 0) / t.cost;
     int head = unit / t.row_tiles, row_tile = unit % t.row_tiles;
-    int unit_at = entry_at + unit * t.tiles;
+    int unit_at = entry_at + unit * t.cost;
     const int last_page = pages_of(cache, e.length);
 #pragma unroll 1
-    for (; head < cache.kv_heads && unit_at < stop && ok; unit_at += t.tiles) {
+    for (; head < cache.kv_heads && unit_at < stop && ok; unit_at += t.cost) {
       Segment s;
       s.first = e.first;
       s.rows = e.rows;
       s.length = e.length;
       s.kv_head = head;
       s.row0 = row_tile * S::kRows;
-      s.tile = max(begin - unit_at, 0);
-      s.tiles = min(stop - unit_at, t.tiles) - s.tile;
-      s.lead = shares.block_of(unit_at);
-      s.parts = shares.block_of(unit_at + t.tiles - 1) - s.lead + 1;
+      const int tiles_at = unit_at + kUnitCost;
+      s.tile = max(begin - tiles_at, 0);
+      s.tiles = min(stop - tiles_at, t.tiles) - s.tile;
+      s.lead = shares.block_of(tiles_at);
+      s.parts = shares.block_of(tiles_at + t.tiles - 1) - s.lead + 1;
       s.part = s.parts == 1 ? -1 : kSlotsPerBlock * g + (g == s.lead);
       if (++row_tile == t.row_tiles) {
         row_tile = 0;
         ++head;
       }
+      if (s.tiles <= 0) continue;
       const uint32_t place = segments % kSegments;
       if (!(ok = mbar_wait_warp(smem_u32(&c->segment_empty[place]), ((segments / kSegments) & 1) ^ 1))) break;
       if (lane == 0) {
@@ -406,7 +415,7 @@ __device__ __forceinline__ void load_queries(const CachedArgs& args, const Segme
 // ... and put into shared memory as two terms, each row scaled by a power of two.  The second terms, kRows rows
 // behind the first, are multiplied by `Second`.
 template <typename S, int Second>
-__device__ __forceinline__ void store_queries(const CachedArgs& args, const Segment& s, int batch,
+__device__ __forceinline__ void store_queries(const CachedArgs& args, const Segment& s, int which, int batch,
                                               const uint2 (&raw)[S::kBatch], uint8_t* q, WorkControl<S>* c) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = args.heads / args.cache.kv_heads;
@@ -438,18 +447,18 @@ __device__ __forceinline__ void store_queries(const CachedArgs& args, const Segm
     *reinterpret_cast<uint32_t*>(q + r2 * 128 + ((chunk ^ (r2 & 7)) << 4) + inside) = b[0] | (b[1] << 16);
     if (lane == 0) {
       // (a row that is no number: its scores are none)
-      c->factor[r] = largest < 0x7f80 ? args.scale * kLog2e * power_of_two(some) * power_of_two(rest) : NAN;
+      c->factor[which][r] = largest < 0x7f80 ? args.scale * kLog2e * power_of_two(some) * power_of_two(rest) : NAN;
       const int token = (s.row0 + r) / group;
       const bool valid = token < s.rows;
-      c->limit[r] = s.length - s.rows + (valid ? token : 0);
-      c->out_row[r] = valid ? (s.first + token) * args.heads + s.kv_head * group + (s.row0 + r) % group : -1;
+      c->limit[which][r] = s.length - s.rows + (valid ? token : 0);
+      c->out_row[which][r] = valid ? (s.first + token) * args.heads + s.kv_head * group + (s.row0 + r) % group : -1;
     }
   }
 }
 
-// All of them, the first batch having been read.
+// All of them, the first batch having been read; `which` of the row arrays takes what belongs to them.
 template <typename S, int Second>
-__device__ __forceinline__ void prepare_queries(const CachedArgs& args, const Segment& s, uint2 (&raw)[S::kBatch], uint8_t* q,
+__device__ __forceinline__ void prepare_queries(const CachedArgs& args, const Segment& s, int which, uint2 (&raw)[S::kBatch], uint8_t* q,
                                                 WorkControl<S>* c) {
   const int rows = s.rows * (args.heads / args.cache.kv_heads) - s.row0;
 #pragma unroll 1
@@ -457,10 +466,8 @@ __device__ __forceinline__ void prepare_queries(const CachedArgs& args, const Se
     // (rows of warps that have none are not read by anybody)
     if (batch * S::kBatch * S::kSoftmaxWarps >= (rows + 31) / 32 * 32) break;
     if (batch > 0) load_queries<S>(args, s, batch, raw);
-    store_queries<S, Second>(args, s, batch, raw, q, c);
+    store_queries<S, Second>(args, s, which, batch, raw, q, c);
   }
-  if (threadIdx.x < kHeadDim) c->first_bad[threadIdx.x] = INT32_MAX;
-  if (threadIdx.x == 0) c->found_bad = 0;
 }
 
 

@@ -113,7 +113,9 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
     softmax_sync<S>();
     if (*failed) return false;
     if (!some) break;
-    prepare_queries<S, 1>(args, s, queries, q, c);
+    if (threadIdx.x < kHeadDim) c->first_bad[threadIdx.x] = INT32_MAX;
+    if (threadIdx.x == 0) c->found_bad = 0;
+    prepare_queries<S, 1>(args, s, 0, queries, q, c);
     fence_proxy_async_smem();
     softmax_sync<S>();
     if (lane == 0) mbar_arrive(&c->q_full);
@@ -122,8 +124,8 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
     float factor = 0.0f, shift = 0.0f, sum = 0.0f;
     int limit = -1;
     if (has_rows) {
-      factor = c->factor[row];
-      limit = c->limit[row];
+      factor = c->factor[0][row];
+      limit = c->limit[0][row];
     }
 #pragma unroll 1
     for (int j = 0; j < s.tiles; ++j, ++no) {
@@ -249,7 +251,7 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
     softmax_sync<S>();
     const bool alone = s.part < 0;
     if (has_rows) {
-      const int to = c->out_row[row];
+      const int to = c->out_row[0][row];
       const float all = (c->sum[0][row] + c->sum[1][row]) * kCodeScale, inverse = 1.0f / all;
       const bool bad = c->found_bad != 0;
       float* slot = split.slots + slot_floats(S::kRows) * max(s.part, 0);
