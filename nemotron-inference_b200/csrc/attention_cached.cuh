@@ -481,16 +481,20 @@ __device__ __forceinline__ void clean_values(uint8_t* values, int token, int pos
 #pragma unroll
     for (int i = 0; i < 8; ++i) row[i] = make_uint4(0, 0, 0, 0);
   } else if (position > s.length - s.rows) {
-    uint32_t* words = reinterpret_cast<uint32_t*>(row);
+    uint32_t any = 0;  // bit 7 of a byte for a code that is no number
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 x = row[i];
+      any |= ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u) |
+             ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
+    }
+    if (any & 0x80808080u) {
+      uint8_t* codes = reinterpret_cast<uint8_t*>(row);
 #pragma unroll 1
-    for (int i = 0; i < kHeadDim / 4; ++i) {
-      const uint32_t x = words[i];
-      if ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0) continue;
-#pragma unroll 1
-      for (int k = 0; k < 4; ++k) {
-        if (((x >> (8 * k)) & 0x7fu) != 0x7fu) continue;
-        atomicMin(&c->first_bad[(((i >> 2) ^ (token & 7)) << 4) + 4 * (i & 3) + k], position);
-        reinterpret_cast<uint8_t*>(words + i)[k] = 0;
+      for (int i = 0; i < kHeadDim; ++i) {
+        if ((codes[i] & 0x7fu) != 0x7fu) continue;
+        atomicMin(&c->first_bad[(((i >> 4) ^ (token & 7)) << 4) + (i & 15)], position);
+        codes[i] = 0;
         c->found_bad = 1;
       }
     }
@@ -498,11 +502,12 @@ __device__ __forceinline__ void clean_values(uint8_t* values, int token, int pos
   fence_proxy_async_smem();
 }
 
-// Joins the pieces of a (sequence, key head): this block its share of the rows, a warp per row.  With few pieces
-// the next row's are on their way meanwhile.
+// Joins the pieces of a (sequence, key head): this block its share of the rows, a warp per row.  Of few rows many
+// pieces are read at once, of many the next row's are on their way meanwhile.
 template <typename S>
 __device__ void join(const CachedArgs& args, const Split& split, const Segment& s) {
-  constexpr int kAtOnce = 8;
+  constexpr bool kManyRows = S::kRows > 16;
+  constexpr int kAtOnce = kManyRows ? 4 : 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pieces = s.parts, piece = static_cast<int>(blockIdx.x) - s.lead;
   const int rows = min(S::kRows, s.rows * (args.heads / args.cache.kv_heads) - s.row0);
@@ -530,7 +535,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
   };
   Read read;
   int r = rows * piece / pieces + warp;
-  if (r < end) read_start(read, r, 0);
+  if (kManyRows && r < end) read_start(read, r, 0);
 #pragma unroll 1
   for (; r < end; r += S::kSoftmaxWarps) {
     const int next = r + S::kSoftmaxWarps, row = s.row0 + r;
@@ -538,7 +543,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
     float top = -INFINITY, sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
     for (int start = 0; start < pieces; start += 32) {
-      if (start > 0) read_start(read, r, start);
+      if (!kManyRows || start > 0) read_start(read, r, start);
       const int count = min(32, pieces - start);
       const float higher = fmaxf(top, warp_max(read.reference));
       const float keep = top > -INFINITY ? exp2_approx(top - higher) : 0.0f;
@@ -554,7 +559,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
         float4 x[kAtOnce];
 #pragma unroll
         for (int p = 0; p < kAtOnce; ++p) x[p] = read.x[p];
-        if (start + first + kAtOnce >= pieces && next < end) read_start(read, next, 0);
+        if (kManyRows && start + first + kAtOnce >= pieces && next < end) read_start(read, next, 0);
 #pragma unroll
         for (int p = 0; p < kAtOnce; ++p) {
           const float f = __shfl_sync(0xffffffffu, scale, first + p);
