@@ -507,7 +507,7 @@ __device__ __forceinline__ void clean_values(uint8_t* values, int token, int pos
 template <typename S>
 __device__ void join(const CachedArgs& args, const Split& split, const Segment& s) {
   constexpr bool kManyRows = S::kRows > 16;
-  constexpr int kAtOnce = kManyRows ? 4 : 16;
+  constexpr int kAtOnce = kManyRows ? 8 : 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pieces = s.parts, piece = static_cast<int>(blockIdx.x) - s.lead;
   const int rows = min(S::kRows, s.rows * (args.heads / args.cache.kv_heads) - s.row0);

@@ -1,10 +1,10 @@
 // Attention over the 8-bit cache for up to 128 rows of queries to a key head (drafted tokens, chunks of prompts);
 // what there is to both kernels is in attention_cached.cuh.
 //
-// A thread per row, two for its halves of a tile of 128 tokens:
+// A thread per row, four for its quarters of a tile of 128 tokens:
 //   S = a K^T + b K^T   M = 128 rows, N = 128 tokens, K = 128, twice: the queries' terms from shared memory, into
 //                       one sum (b is not scaled up: what lies 2^10 below the largest element ends at 2^-18 of it)
-//   softmax             a row's scores, reference and sum are in registers of the two threads
+//   softmax             a row's scores, reference and sum are in registers of the four threads
 //   O_a += a V, O_b += b V   M = 128 rows, N = 128 dimensions, K = 128 tokens: weights from TMEM, written over the
 //                       scores; the values' tile is read along its rows
 // A tile takes some 1000 MMA cycles and, by the softmax warps, some 800 issue slots of each scheduler, beside the
@@ -17,21 +17,21 @@ namespace {
 struct Rows {
   static constexpr int kRows = kMaxRows;
   static constexpr int kKeySlots = 5, kValueSlots = 5;  // tiles in flight
-  static constexpr int kSoftmaxWarps = 8;               // of four, each has half of the tokens
-  static constexpr int kBatch = 4;                      // rows of queries to a warp at a time
+  static constexpr int kSoftmaxWarps = 16;              // each four have a quarter of the tokens
+  static constexpr int kBatch = 2;                      // rows of queries to a warp at a time
   static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
   static constexpr uint32_t kQueryBytes = 2 * kRows * kHeadDim;
 };
 using S = Rows;
 
-constexpr int kHalf = kKeyTile / 2;
+constexpr int kQuarter = kKeyTile / 4;
 constexpr uint32_t kTermBytes = S::kRows * kHeadDim;  // of the queries
 constexpr int kPart = 16;  // tokens that never lie in two pages
 constexpr int kColumns = 512, kSums = 2 * kKeyTile;  // two buffers of S; then O_a, O_b
 
 struct Control : WorkControl<S> {
   uint64_t s_full[2], p_full, o_full;
-  float top[2][S::kRows], sum[2][S::kRows];  // by half
+  float top[4][S::kRows], sum[4][S::kRows];  // by quarter
   int failed;
 };
 
@@ -95,7 +95,7 @@ __device__ bool mma_role(uint32_t keys_at, uint32_t values_at, uint32_t q_at, ui
 }
 
 __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t* values, uint8_t* q, uint32_t tmem, Control* c) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp >> 2;
   const int row = threadIdx.x & (S::kRows - 1);
   const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
   const int page_shift = args.cache.page_shift;
@@ -130,25 +130,25 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
 #pragma unroll 1
     for (int j = 0; j < s.tiles; ++j, ++no) {
       const uint32_t slot = no % S::kValueSlots, buffer = no & 1;
-      const int first = (s.tile + j) * kKeyTile, begin = first + half * kHalf;
+      const int first = (s.tile + j) * kKeyTile, begin = first + quarter * kQuarter;
       const bool at_end = first + kKeyTile - 1 > clear, is_first = j == 0;
       ok = mbar_wait_warp(smem_u32(&c->v_full[slot]), (no / S::kValueSlots) & 1);
-      if (at_end && half == 0) clean_values<S>(values + slot * kKeyTileBytes, row, first + row, s, c);
+      if (at_end && quarter == 0) clean_values<S>(values + slot * kKeyTileBytes, row, first + row, s, c);
       ok = mbar_wait_warp(smem_u32(&c->s_full[buffer]), (no >> 1) & 1) && ok;
       tcgen05_fence_after();
       // exponents of the weights, tokens in pairs: score + power of the values - reference + kWeightBits
       const uint32_t s_at = lanes + buffer * kKeyTile;
-      uint32_t y[kHalf];
-      float v_inverse[kHalf / kPart], high = -INFINITY;
+      uint32_t y[kQuarter];
+      float v_inverse[kQuarter / kPart], high = -INFINITY;
       if (has_rows) {
 #pragma unroll
-        for (int i = 0; i < kHalf; i += 32) tmem_ld_x32_async(s_at + half * kHalf + i, y + i);
+        for (int i = 0; i < kQuarter; i += 32) tmem_ld_x32_async(s_at + quarter * kQuarter + i, y + i);
         tmem_ld_wait();
-        registers_loaded<kHalf>(y);
+        registers_loaded<kQuarter>(y);
 #pragma unroll
-        for (int p = 0; p < kHalf / kPart; ++p) {
+        for (int p = 0; p < kQuarter / kPart; ++p) {
           // (places behind the sequence may lie in pages that it does not have)
-          const int page = (half * kHalf + p * kPart) >> page_shift;
+          const int page = (quarter * kQuarter + p * kPart) >> page_shift;
           const bool there = begin + p * kPart < s.length;
           const int k_power = there ? c->powers[slot][0][page] : 0, v_power = there ? c->powers[slot][1][page] : 0;
           v_inverse[p] = power_of_two(-v_power);
@@ -164,37 +164,37 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
         }
         if (at_end) {
 #pragma unroll
-          for (int i = 0; i < kHalf; ++i) {
+          for (int i = 0; i < kQuarter; ++i) {
             if (begin + i > limit) y[i] = 0xff800000u;
           }
         }
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) high = fmaxf(high, __uint_as_float(y[i]));
+        for (int i = 0; i < kQuarter; ++i) high = fmaxf(high, __uint_as_float(y[i]));
       }
       // (all scores are read behind this: weights may be written over them)
       if (!ok) *failed = 1;
       const bool rise = softmax_any<S>(is_first || high > kLargestBits);
       if (*failed) return false;
       if (rise) {
-        c->top[half][row] = high;
+        c->top[quarter][row] = high;
         softmax_sync<S>();
-        const float top = fmaxf(c->top[0][row], c->top[1][row]);
+        const float top = fmaxf(fmaxf(c->top[0][row], c->top[1][row]), fmaxf(c->top[2][row], c->top[3][row]));
         // a row's first tile sets its reference (unless it sees none of it), others may raise it
         const float by = has_rows && top > (is_first ? -INFINITY : kLargestBits) ? top - kWeightBits : 0.0f;
         shift -= by;
         if (__any_sync(0xffffffffu, by != 0.0f)) {
 #pragma unroll
-          for (int i = 0; i < kHalf; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) - by);
+          for (int i = 0; i < kQuarter; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) - by);
           if (!is_first) {
             const float fade = exp2_approx(-by);
             sum *= fade;
-            // O of the tiles before is complete; each half takes one of its terms
+            // O of the tiles before is complete; each quarter takes half of one of its terms
             ok = mbar_wait_warp(smem_u32(&c->o_full), (no & 1) ^ 1);
             tcgen05_fence_after();
             if (!ok) *failed = 1;
-            const uint32_t o_at = lanes + kSums + half * kHeadDim;
+            const uint32_t o_at = lanes + kSums + quarter * (kHeadDim / 2);
 #pragma unroll 1
-            for (int i = 0; i < kHeadDim; i += 32) {
+            for (int i = 0; i < kHeadDim / 2; i += 32) {
               uint32_t o[32];
               tmem_ld_x32_async(o_at + i, o);
               tmem_ld_wait();
@@ -209,9 +209,9 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       }
       if (has_rows) {
         // four codes to a column: the first terms of the tile's 128 tokens, then the second terms
-        uint32_t a[kHalf / 4], b[kHalf / 4];
+        uint32_t a[kQuarter / 4], b[kQuarter / 4];
 #pragma unroll
-        for (int p = 0; p < kHalf / kPart; ++p) {
+        for (int p = 0; p < kQuarter / kPart; ++p) {
           uint64_t of_part = 0;
 #pragma unroll
           for (int i = p * kPart; i < (p + 1) * kPart; i += 4) {
@@ -231,8 +231,8 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
           unpack2(of_part, s0, s1);
           sum = fmaf(s0 + s1, v_inverse[p], sum);
         }
-        tmem_st_x16(s_at + half * (kHalf / 4), a);
-        tmem_st_x16(s_at + kKeyTile / 4 + half * (kHalf / 4), b);
+        tmem_st_x8(s_at + quarter * (kQuarter / 4), a);
+        tmem_st_x8(s_at + kKeyTile / 4 + quarter * (kQuarter / 4), b);
         tmem_st_wait();
       }
       tcgen05_fence_before();
@@ -244,7 +244,7 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
     const bool known = mbar_wait_warp(smem_u32(&c->segment_full[following % kSegments]), (following / kSegments) & 1);
     some = known && c->has_segment[following % kSegments];
     if (some) load_queries<S>(args, c->segment[following % kSegments], 0, queries);
-    c->sum[half][row] = sum;
+    c->sum[quarter][row] = sum;
     ok = mbar_wait_warp(smem_u32(&c->o_full), (no & 1) ^ 1) && known;
     tcgen05_fence_after();
     if (!ok) *failed = 1;
@@ -252,12 +252,12 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
     const bool alone = s.part < 0;
     if (has_rows) {
       const int to = c->out_row[0][row];
-      const float all = (c->sum[0][row] + c->sum[1][row]) * kCodeScale, inverse = 1.0f / all;
+      const float all = ((c->sum[0][row] + c->sum[1][row]) + (c->sum[2][row] + c->sum[3][row])) * kCodeScale, inverse = 1.0f / all;
       const bool bad = c->found_bad != 0;
       float* slot = split.slots + slot_floats(S::kRows) * max(s.part, 0);
-      // each half has 64 of the dimensions
+      // each quarter has 32 of the dimensions
 #pragma unroll 1
-      for (int d = half * 64; d < half * 64 + 64; d += 16) {
+      for (int d = quarter * 32; d < quarter * 32 + 32; d += 16) {
         uint32_t a[16], b[16];
         tmem_ld_x16_async(lanes + kSums + d, a);
         tmem_ld_x16_async(lanes + kSums + kHeadDim + d, b);
@@ -284,7 +284,7 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
           for (int i = 0; i < 4; ++i) __stcg(out + i, make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
         }
       }
-      if (!alone && half == 0) {  // (a row that has seen no token, all being behind its mask, leaves nothing)
+      if (!alone && quarter == 0) {  // (a row that has seen no token, all being behind its mask, leaves nothing)
         __stcg(slot + S::kRows * kHeadDim + row, all == 0.0f ? -INFINITY : -shift);
         __stcg(slot + S::kRows * (kHeadDim + 1) + row, all);
       }
