@@ -409,7 +409,8 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
     __syncwarp();
     if (lane == 0) mbar_arrive(&c->segment_empty[segments % kSegments]);
   }
-  return announce_and_join<S>(args, split, joins, c);
+  announce_and_join<S>(args, split, joins, c);
+  return true;
 }
 
 template <typename S>
@@ -484,10 +485,10 @@ size_t attention_cached_workspace_bytes() {
 
 cudaError_t launch_attention_cached(const CachedArgs& args, cudaStream_t stream) {
   const int sms = device_sms();
-  if (sms * 2 * sizeof(int) > kAttendCounterBytes) return cudaErrorInvalidValue;
+  if (sms * 2 > kMaxBlocks) return cudaErrorInvalidValue;
   CUtensorMap map;
   if (!pages_tensor_map(args.cache, &map)) return cudaErrorInvalidValue;
-  const Split split{reinterpret_cast<int*>(args.cache.attend_workspace),
+  const Split split{reinterpret_cast<JoinCounters*>(args.cache.attend_workspace),
                     reinterpret_cast<float*>(args.cache.attend_workspace + kAttendCounterBytes)};
   // By the query rows that the entries have on average.  Entries with more are taken 8, 16 or 128 at a time
   // and read their keys and values again each time.

@@ -16,8 +16,11 @@
 // With R rows of queries (new rows x heads that share the key head) at a time, W tiles of 128 tokens in all (and
 // one more for each sequence, key head and rows) and G blocks, block g takes the tiles [W g / G, W (g + 1) / G)
 // in order, whatever the sequences' lengths.
-// Where a (sequence, key head) is cut, each piece leaves its sums in the workspace; when all have, each of
-// these blocks joins a share of the rows, piece by piece in order, so results never depend on timing.
+// Where a (sequence, key head) is cut, each piece leaves its sums in the workspace.  When all have, these blocks
+// join them, a share of the rows at a time; each row is joined piece by piece in order, so results never depend
+// on timing or on who joins.  Nobody has to wait: a block that sees pieces missing for some 30 us leaves, and the
+// one that brings the last piece joins what nobody else does.  (All blocks run at once only if no other kernel
+// holds SMs; two calls on two streams could otherwise each wait for blocks that the other keeps out.)
 #pragma once
 
 #include <cuda_fp16.h>
@@ -76,7 +79,7 @@ struct WorkControl {
   int limit[2][S::kRows];                 // a row's position: the last token it sees
   int first_bad[kHeadDim];             // position of the first masked value that is no number, by dimension
   int found_bad;
-  int joined;
+  int share, pieces_before[2];
   uint32_t tmem;
   int64_t before[S::kThreads / 32];
   Shares shares;      // of all tiles
@@ -87,8 +90,17 @@ struct WorkControl {
 // What a block leaves for the join: 128 sums a row, then the references and the sums of weights.
 __host__ __device__ constexpr size_t slot_floats(int rows) { return static_cast<size_t>(rows) * (kHeadDim + 2); }
 
+// By the block in which a (sequence, key head) begins, all 0 between calls.
+struct JoinCounters {
+  int pieces;  // that are there
+  int taken;   // shares of rows asked for, and kLeftEarly for each block that left without asking
+};
+constexpr int kLeftEarly = 1 << 16;
+constexpr int kMaxBlocks = static_cast<int>(kAttendCounterBytes / sizeof(JoinCounters));
+constexpr int kJoinPatience = 1 << 16;  // cycles
+
 struct Split {
-  int* counters;  // by the block in which a (sequence, key head) begins: pieces that are done, twice
+  JoinCounters* counters;
   float* slots;
 };
 
@@ -502,17 +514,22 @@ __device__ __forceinline__ void clean_values(uint8_t* values, int token, int pos
   fence_proxy_async_smem();
 }
 
-// Joins the pieces of a (sequence, key head): this block its share of the rows, a warp per row.  Of few rows many
+// How many shares the rows of a segment's (sequence, key head) are joined in.
+template <typename S>
+__device__ __forceinline__ int rows_to_join(const CachedArgs& args, const Segment& s) {
+  return min(S::kRows, s.rows * (args.heads / args.cache.kv_heads) - s.row0);
+}
+
+// Joins the pieces of a (sequence, key head), one of `shares` shares of the rows, a warp per row.  Of few rows many
 // pieces are read at once, of many the next row's are on their way meanwhile.
 template <typename S>
-__device__ void join(const CachedArgs& args, const Split& split, const Segment& s) {
+__device__ void join(const CachedArgs& args, const Split& split, const Segment& s, int share, int shares) {
   constexpr bool kManyRows = S::kRows > 16;
   constexpr int kAtOnce = kManyRows ? 8 : 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int pieces = s.parts, piece = static_cast<int>(blockIdx.x) - s.lead;
-  const int rows = min(S::kRows, s.rows * (args.heads / args.cache.kv_heads) - s.row0);
+  const int pieces = s.parts, rows = rows_to_join<S>(args, s);
   auto sums_of = [&](int p) { return split.slots + slot_floats(S::kRows) * (kSlotsPerBlock * (s.lead + p) + (p == 0)); };
-  const int end = rows * (piece + 1) / pieces;
+  const int end = rows * (share + 1) / shares;
   struct Read {
     float reference, weight;  // a lane per piece
     float4 x[kAtOnce];        // the sums of pieces `first` on
@@ -534,7 +551,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
     read_x(read, r, start);
   };
   Read read;
-  int r = rows * piece / pieces + warp;
+  int r = rows * share / shares + warp;
   if (kManyRows && r < end) read_start(read, r, 0);
 #pragma unroll 1
   for (; r < end; r += S::kSoftmaxWarps) {
@@ -580,42 +597,53 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
   }
 }
 
-// Waits until every piece of a segment's (sequence, key head) has left its sums, then joins.  All blocks
-// with tiles run at once (as many as the SMs hold, and none waits before its own tiles are done).  The
-// counter is 0 again when the last of them has joined.
+// A block's part in the join of a segment's (sequence, key head), of whose pieces `pieces_before` were there when its
+// own was left.  The last who asks for a share, or leaves, sets the counters back.
 template <typename S>
-__device__ bool wait_and_join(const CachedArgs& args, const Split& split, const Segment& s, WorkControl<S>* c) {
+__device__ void help_join(const CachedArgs& args, const Split& split, const Segment& s, const int& pieces_before, WorkControl<S>* c) {
+  JoinCounters* counters = &split.counters[s.lead];
+  const int shares = min(s.parts, rows_to_join<S>(args, s));
+  bool all = false;  // thread 0's
   if (threadIdx.x == 0) {
-    volatile int* done = split.counters + s.lead;
+    volatile int* pieces = &counters->pieces;
     const long long start = clock64();
-    bool there = *done >= s.parts;
-    while (!there && clock64() - start < (1ll << 31)) there = *done >= s.parts;
-    __threadfence();
-    c->joined = there;
+    all = pieces_before == s.parts - 1 || *pieces >= s.parts;
+    while (!all && clock64() - start < kJoinPatience) all = *pieces >= s.parts;
   }
-  softmax_sync<S>();
-  if (!c->joined) return false;
-  join<S>(args, split, s);
-  softmax_sync<S>();
-  if (threadIdx.x == 0 && atomicAdd(&split.counters[s.lead], 1) == 2 * s.parts - 1) split.counters[s.lead] = 0;
-  return true;
+#pragma unroll 1
+  for (;;) {
+    if (threadIdx.x == 0) {
+      const int mine = all ? 1 : kLeftEarly, asked = atomicAdd(&counters->taken, mine), now = asked + mine;
+      __threadfence();
+      c->share = all && (asked & (kLeftEarly - 1)) < shares ? asked & (kLeftEarly - 1) : -1;
+      if ((now & (kLeftEarly - 1)) + now / kLeftEarly == shares + s.parts) {
+        counters->pieces = 0;
+        counters->taken = 0;
+      }
+    }
+    softmax_sync<S>();
+    const int share = c->share;
+    if (share < 0) return;
+    join<S>(args, split, s, share, shares);
+    softmax_sync<S>();
+  }
 }
 
 // The end of a block's softmax warps: its pieces are there (all threads' sums are behind a barrier, so one
 // thread speaks for them), and are joined with the others'.
 template <typename S>
-__device__ bool announce_and_join(const CachedArgs& args, const Split& split, int joins, WorkControl<S>* c) {
-  if (joins == 0) return true;
+__device__ void announce_and_join(const CachedArgs& args, const Split& split, int joins, WorkControl<S>* c) {
+  if (joins == 0) return;
   if (threadIdx.x == 0) {
     __threadfence();
 #pragma unroll 1
-    for (int i = 0; i < joins; ++i) atomicAdd(&split.counters[c->to_join[i].lead], 1);
+    for (int i = 0; i < joins; ++i) c->pieces_before[i] = atomicAdd(&split.counters[c->to_join[i].lead].pieces, 1);
   }
 #pragma unroll 1
   for (int i = 0; i < joins; ++i) {
-    if (!wait_and_join<S>(args, split, c->to_join[i], c)) return false;
+    if (i > 0) softmax_sync<S>();  // (the share of the first is read)
+    help_join<S>(args, split, c->to_join[i], c->pieces_before[i], c);
   }
-  return true;
 }
 
 // Barriers of WorkControl; one thread.

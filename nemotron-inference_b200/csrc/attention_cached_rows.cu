@@ -297,7 +297,8 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
     __syncwarp();
     if (lane == 0) mbar_arrive(&c->segment_empty[segments % kSegments]);
   }
-  return announce_and_join<S>(args, split, joins, c);
+  announce_and_join<S>(args, split, joins, c);
+  return true;
 }
 
 __global__ void __launch_bounds__(S::kThreads, 1)

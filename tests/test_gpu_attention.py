@@ -693,3 +693,30 @@ def test_a_decode_step_is_replayed_from_a_graph(attention):
         graph.replay()
     assert cache.sync_status() == 0 and cache.lengths.tolist() == [41, 41]
     _check_attend(cache, 0, q, [0, 1], [1, 1], out)
+
+
+@pytest.mark.parametrize("heads", [4, 32, 64])
+def test_two_caches_on_two_streams(attention, heads):
+    """Both calls' sequences are cut between blocks that the other call may keep from running."""
+    caches, queries, alone = [], [], []
+    for seed in range(2):
+        cache = attention.KvCache.allocate(1, 64, 2, 3, 40, page_tokens=64)
+        lengths = [1500, 7, 900]
+        kv = _normal(40 + seed, 2, sum(lengths), 2, D).to(torch.bfloat16)
+        everyone = _int([0, 1, 2])
+        cache.extend(everyone, _offsets(lengths), sum(lengths))
+        cache.append(0, kv[0], kv[1], everyone, _offsets(lengths))
+        caches.append(cache)
+        queries.append(_normal(50 + seed, 3, heads, D).to(torch.bfloat16))
+        alone.append(cache.attend(0, queries[seed], everyone, _offsets([1, 1, 1])))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    offsets, results = _offsets([1, 1, 1]), [[], []]
+    for _ in range(50):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                results[i].append(caches[i].attend(0, queries[i], everyone, offsets))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(r, alone[i]) for r in results[i])
+        assert caches[i].sync_status() == 0
