@@ -439,9 +439,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks)
     tmem_alloc(&c->tmem, S::kColumns);
     tmem_relinquish();
   }
-  find_begin<S>(args, c);
   tcgen05_fence_before();
+  wait_for_predecessor();
+  find_begin<S>(args, c);
   __syncthreads();
+  release_successor();  // (the columns of TMEM are there)
   tcgen05_fence_after();
   const uint32_t tmem = c->tmem;
   if (warp < S::kSoftmaxWarps) {
@@ -472,8 +474,8 @@ cudaError_t launch(const CUtensorMap& map, const CachedArgs& args, const Split& 
   static std::atomic<uint64_t> allowed{0};
   cudaError_t err = allow_shared_memory_once(cached_kernel<S>, allowed);
   if (err != cudaSuccess) return err;
-  cached_kernel<S><<<sms * S::kBlocks, S::kThreads, shared_bytes<S>(), stream>>>(map, args, split);
-  return cudaGetLastError();
+  return launch_kernel(cached_kernel<S>, dim3(sms * S::kBlocks), S::kThreads, shared_bytes<S>(),
+                       LaunchStream(stream, true), map, args, split);
 }
 
 }  // namespace

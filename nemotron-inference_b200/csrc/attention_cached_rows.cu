@@ -322,9 +322,11 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     tmem_alloc(&c->tmem, kColumns);
     tmem_relinquish();
   }
-  find_begin<S>(args, c);
   tcgen05_fence_before();
+  wait_for_predecessor();
+  find_begin<S>(args, c);
   __syncthreads();
+  release_successor();  // (the columns of TMEM are there)
   tcgen05_fence_after();
   const uint32_t tmem = c->tmem;
   if (warp < S::kSoftmaxWarps) {
@@ -356,8 +358,8 @@ cudaError_t launch_cached_rows(const CUtensorMap& map, const CachedArgs& args, c
   static std::atomic<uint64_t> allowed{0};
   cudaError_t err = allow_shared_memory_once(cached_rows_kernel, allowed);
   if (err != cudaSuccess) return err;
-  cached_rows_kernel<<<sms, S::kThreads, kSharedBytes, stream>>>(map, args, split);
-  return cudaGetLastError();
+  return launch_kernel(cached_rows_kernel, dim3(sms), S::kThreads, kSharedBytes, LaunchStream(stream, true),
+                       map, args, split);
 }
 
 }  // namespace nmoe

@@ -55,6 +55,7 @@ struct Control {
   int has_work[2];
   uint32_t tmem;
   int bad_values;  // a value in a masked tile is no number
+  int stopped;
 };
 
 constexpr size_t kSharedBytes = 1024 + (2 + kSlots) * kTileBytes + sizeof(Control);
@@ -492,7 +493,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* slots = shared + 2 * kTileBytes;
   Control* c = reinterpret_cast<Control*>(slots + kSlots * kTileBytes);
   const int warp = threadIdx.x >> 5;
-  if (*args.error != 0) return;  // a wait of an earlier call ran out
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&c->q_full[t], 1);
@@ -520,10 +520,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
   }
   tcgen05_fence_before();
+  wait_for_predecessor();
+  if (threadIdx.x == 0) c->stopped = *args.error != 0;  // a wait of an earlier call ran out
   __syncthreads();
+  release_successor();  // (the columns of TMEM are there)
   tcgen05_fence_after();
   const uint32_t tmem = c->tmem;
-  if (warp < kSoftmaxWarps) {
+  if (c->stopped) {
+  } else if (warp < kSoftmaxWarps) {
     more_registers<kSoftmaxRegisters>();
     softmax_role(args, tmem, c);
   } else if (warp == kMmaWarp) {
@@ -576,9 +580,8 @@ cudaError_t launch_attention_prefill(const PrefillArgs& args, cudaStream_t strea
   static std::atomic<uint64_t> allowed{0};
   cudaError_t err = allow_shared_memory_once(prefill_kernel, allowed);
   if (err != cudaSuccess) return err;
-  prefill_kernel<<<static_cast<unsigned>(blocks), kThreads, kSharedBytes, stream>>>(q, k, v, args,
-                                                                                    two_heads);
-  return cudaGetLastError();
+  return launch_kernel(prefill_kernel, dim3(static_cast<unsigned>(blocks)), kThreads, kSharedBytes,
+                       LaunchStream(stream, true), q, k, v, args, two_heads);
 }
 
 }  // namespace nmoe

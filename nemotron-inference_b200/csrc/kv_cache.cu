@@ -71,6 +71,8 @@ __global__ void __launch_bounds__(kAppendThreads, PageTokens <= 64 ? kAppendBloc
                      const __nv_bfloat16* v, int64_t v_stride, int per_block) {
   constexpr int kAppendChunks = PageTokens * kHeadDim / 8 / kAppendThreads;  // of 8 values, to a thread
   __shared__ uint32_t warp_max[2][kAppendThreads / 32];
+  release_successor();
+  wait_for_predecessor();
   const int pending = *c.error;
   const int2 unit = locate_unit(b.count, blockIdx.x, [&](int i) {
     const BatchEntry e = batch_entry(c, b, i);
@@ -261,6 +263,8 @@ __device__ int extension(const PagedCache& c, const Batch& b, int i, int& old_le
 
 __global__ void __launch_bounds__(kBookThreads) kv_extend_kernel(PagedCache c, Batch b) {
   __shared__ BookShared s;
+  release_successor();
+  wait_for_predecessor();
   if (*c.error != 0) return;
   if (threadIdx.x == 0) s.flag = 0;
   __syncthreads();
@@ -332,6 +336,8 @@ __device__ void count_pages(const PagedCache& c, const int* sequences, int count
 __global__ void __launch_bounds__(kBookThreads)
     kv_free_kernel(PagedCache c, const int* sequences, int count) {
   __shared__ BookShared s;
+  release_successor();
+  wait_for_predecessor();
   if (*c.error != 0) return;
   if (threadIdx.x == 0) s.flag = 0;
   __syncthreads();
@@ -360,6 +366,7 @@ __global__ void __launch_bounds__(kBookThreads)
     kv_fork_kernel(PagedCache c, const int* parents, const int* children, int count) {
   __shared__ BookShared s;
   release_successor();
+  wait_for_predecessor();
   if (threadIdx.x == 0) {
     s.flag = 0;
     *c.move_count = 0;
@@ -438,6 +445,7 @@ __global__ void __launch_bounds__(kBookThreads)
 __global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) {
   __shared__ BookShared s;
   release_successor();
+  wait_for_predecessor();
   if (threadIdx.x == 0) *c.move_count = 0;
   if (*c.error != 0) return;
   int live = 0;
@@ -480,8 +488,9 @@ constexpr int kCopyChunk = kCopyThreads * 4;  // of 16 bytes: four loads under w
 __global__ void __launch_bounds__(kCopyThreads)
     kv_copy_kernel(PagedCache c, const int* sources, const int* targets, const int* count_at,
                    int count, bool rewrite_table) {
+  release_successor();
+  wait_for_predecessor();  // (the books)
   if (count_at != nullptr) {
-    wait_for_predecessor();  // (the books)
     if (*c.error != 0) return;
     count = *count_at;
   }
@@ -532,7 +541,7 @@ __global__ void __launch_bounds__(kCopyThreads)
 cudaError_t launch_copy(const PagedCache& cache, const int* sources, const int* targets,
                         const int* count_at, int count, bool rewrite_table, cudaStream_t stream) {
   return launch_kernel(kv_copy_kernel, dim3(device_sms() * 8), kCopyThreads, 0,
-                       LaunchStream(stream, count_at != nullptr), cache, sources, targets, count_at,
+                       LaunchStream(stream, true), cache, sources, targets, count_at,
                        count, rewrite_table);
 }
 
@@ -553,32 +562,28 @@ cudaError_t launch_kv_append(const PagedCache& cache, const Batch& batch, int la
                  : cache.page_tokens == 32 ? kv_append_kernel<32>
                  : cache.page_tokens == 64 ? kv_append_kernel<64>
                                            : kv_append_kernel<128>;
-  kernel<<<grid, kAppendThreads, 0, stream>>>(cache, batch, layer, k, k_stride, v, v_stride, per_block);
-  return cudaGetLastError();
+  return launch_kernel(kernel, grid, kAppendThreads, 0, LaunchStream(stream, true), cache, batch, layer, k,
+                       k_stride, v, v_stride, per_block);
 }
 
 cudaError_t launch_kv_extend(const PagedCache& cache, const Batch& batch, cudaStream_t stream) {
-  kv_extend_kernel<<<1, kBookThreads, 0, stream>>>(cache, batch);
-  return cudaGetLastError();
+  return launch_kernel(kv_extend_kernel, dim3(1), kBookThreads, 0, LaunchStream(stream, true), cache, batch);
 }
 
 cudaError_t launch_kv_fork(const PagedCache& cache, const int* parents, const int* children, int count,
                            cudaStream_t stream) {
-  kv_fork_kernel<<<1, kBookThreads, 0, stream>>>(cache, parents, children, count);
-  const cudaError_t err = cudaGetLastError();
+  const cudaError_t err = launch_kernel(kv_fork_kernel, dim3(1), kBookThreads, 0, LaunchStream(stream, true), cache, parents, children, count);
   if (err != cudaSuccess) return err;
   return launch_copy(cache, cache.move_source, cache.move_target, cache.move_count, 0, false, stream);
 }
 
 cudaError_t launch_kv_free(const PagedCache& cache, const int* sequences, int count,
                            cudaStream_t stream) {
-  kv_free_kernel<<<1, kBookThreads, 0, stream>>>(cache, sequences, count);
-  return cudaGetLastError();
+  return launch_kernel(kv_free_kernel, dim3(1), kBookThreads, 0, LaunchStream(stream, true), cache, sequences, count);
 }
 
 cudaError_t launch_kv_compact(const PagedCache& cache, cudaStream_t stream) {
-  kv_compact_kernel<<<1, kBookThreads, 0, stream>>>(cache);
-  const cudaError_t err = cudaGetLastError();
+  const cudaError_t err = launch_kernel(kv_compact_kernel, dim3(1), kBookThreads, 0, LaunchStream(stream, true), cache);
   if (err != cudaSuccess) return err;
   return launch_copy(cache, cache.move_source, cache.move_target, cache.move_count, 0, true, stream);
 }
