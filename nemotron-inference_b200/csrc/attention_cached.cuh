@@ -79,7 +79,7 @@ struct WorkControl {
   int limit[2][S::kRows];                 // a row's position: the last token it sees
   int first_bad[kHeadDim];             // position of the first masked value that is no number, by dimension
   int found_bad;
-  int share, pieces_before[2];
+  int share, pieces_before[2];  // of a join
   uint32_t tmem;
   int64_t before[S::kThreads / 32];
   Shares shares;      // of all tiles
@@ -92,10 +92,11 @@ __host__ __device__ constexpr size_t slot_floats(int rows) { return static_cast<
 
 // By the block in which a (sequence, key head) begins, all 0 between calls.
 struct JoinCounters {
-  int pieces;  // that are there
-  int taken;   // shares of rows asked for, and kLeftEarly for each block that left without asking
+  int pieces;  // that are there, and kLeft for each block that left before all were; stands once all are
+  int taken;   // shares of rows, where a block has left
+  int done;    // blocks that ask for nothing more
 };
-constexpr int kLeftEarly = 1 << 16;
+constexpr int kLeft = 1 << 16;
 constexpr int kMaxBlocks = static_cast<int>(kAttendCounterBytes / sizeof(JoinCounters));
 constexpr int kJoinPatience = 1 << 16;  // cycles
 
@@ -514,22 +515,16 @@ __device__ __forceinline__ void clean_values(uint8_t* values, int token, int pos
   fence_proxy_async_smem();
 }
 
-// How many shares the rows of a segment's (sequence, key head) are joined in.
-template <typename S>
-__device__ __forceinline__ int rows_to_join(const CachedArgs& args, const Segment& s) {
-  return min(S::kRows, s.rows * (args.heads / args.cache.kv_heads) - s.row0);
-}
-
-// Joins the pieces of a (sequence, key head), one of `shares` shares of the rows, a warp per row.  Of few rows many
+// Joins the pieces of a (sequence, key head), one of as many shares of the rows, a warp per row.  Of few rows many
 // pieces are read at once, of many the next row's are on their way meanwhile.
 template <typename S>
-__device__ void join(const CachedArgs& args, const Split& split, const Segment& s, int share, int shares) {
+__device__ void join(const CachedArgs& args, const Split& split, const Segment& s, int share) {
   constexpr bool kManyRows = S::kRows > 16;
   constexpr int kAtOnce = kManyRows ? 8 : 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int pieces = s.parts, rows = rows_to_join<S>(args, s);
+  const int pieces = s.parts, rows = min(S::kRows, s.rows * (args.heads / args.cache.kv_heads) - s.row0);
   auto sums_of = [&](int p) { return split.slots + slot_floats(S::kRows) * (kSlotsPerBlock * (s.lead + p) + (p == 0)); };
-  const int end = rows * (share + 1) / shares;
+  const int end = rows * (share + 1) / pieces;
   struct Read {
     float reference, weight;  // a lane per piece
     float4 x[kAtOnce];        // the sums of pieces `first` on
@@ -551,7 +546,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
     read_x(read, r, start);
   };
   Read read;
-  int r = rows * share / shares + warp;
+  int r = rows * share / pieces + warp;
   if (kManyRows && r < end) read_start(read, r, 0);
 #pragma unroll 1
   for (; r < end; r += S::kSoftmaxWarps) {
@@ -597,35 +592,44 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
   }
 }
 
+// One thread: waits a while for the pieces that are missing when `word` was read.  The word when all are there, or
+// -1: this block has left.
+__device__ __forceinline__ int wait_for_pieces(JoinCounters* counters, int word, int parts) {
+  volatile int* pieces = &counters->pieces;
+  const long long start = clock64();
+  while ((word & (kLeft - 1)) < parts && clock64() - start < kJoinPatience) word = *pieces;
+  while ((word & (kLeft - 1)) < parts) {  // (it can have changed as often as there are blocks)
+    const int seen = atomicCAS(&counters->pieces, word, word + kLeft);
+    if (seen == word) return -1;
+    word = seen;
+  }
+  return word;
+}
+
 // A block's part in the join of a segment's (sequence, key head), of whose pieces `pieces_before` were there when its
-// own was left.  The last who asks for a share, or leaves, sets the counters back.
+// own was left.  If nobody has left, each block has the share of its own piece; else they take them in turn.  The
+// last block that is done sets the counters back.
 template <typename S>
 __device__ void help_join(const CachedArgs& args, const Split& split, const Segment& s, const int& pieces_before, WorkControl<S>* c) {
   JoinCounters* counters = &split.counters[s.lead];
-  const int shares = min(s.parts, rows_to_join<S>(args, s));
-  bool all = false;  // thread 0's
+  int done = 0, word = 0;  // thread 0's
   if (threadIdx.x == 0) {
-    volatile int* pieces = &counters->pieces;
-    const long long start = clock64();
-    all = pieces_before == s.parts - 1 || *pieces >= s.parts;
-    while (!all && clock64() - start < kJoinPatience) all = *pieces >= s.parts;
+    word = wait_for_pieces(counters, pieces_before + 1, s.parts);
+    __threadfence();
+    c->share = word >= kLeft ? atomicAdd(&counters->taken, 1) : word >= 0 ? static_cast<int>(blockIdx.x) - s.lead : -1;
+    if (word < kLeft) done = atomicAdd(&counters->done, 1);
   }
+  softmax_sync<S>();
 #pragma unroll 1
-  for (;;) {
-    if (threadIdx.x == 0) {
-      const int mine = all ? 1 : kLeftEarly, asked = atomicAdd(&counters->taken, mine), now = asked + mine;
-      __threadfence();
-      c->share = all && (asked & (kLeftEarly - 1)) < shares ? asked & (kLeftEarly - 1) : -1;
-      if ((now & (kLeftEarly - 1)) + now / kLeftEarly == shares + s.parts) {
-        counters->pieces = 0;
-        counters->taken = 0;
-      }
-    }
+  for (int share = c->share; share >= 0 && share < s.parts; share = c->share) {
+    join<S>(args, split, s, share);
     softmax_sync<S>();
-    const int share = c->share;
-    if (share < 0) return;
-    join<S>(args, split, s, share, shares);
+    if (threadIdx.x == 0) c->share = word >= kLeft ? atomicAdd(&counters->taken, 1) : -1;
     softmax_sync<S>();
+  }
+  if (threadIdx.x == 0) {
+    if (word >= kLeft) done = atomicAdd(&counters->done, 1);
+    if (done == s.parts - 1) counters->pieces = counters->taken = counters->done = 0;
   }
 }
 
