@@ -184,8 +184,21 @@ constexpr int kBookThreads = 1024;
 struct BookShared {
   int warp_sums[kBookThreads / 32];
   int flag;
-  int released;
+  int list[kBookThreads];  // pages
 };
+
+// Asks for a word that a later step of the books reads: they are chains of loads, some 0.6 us each.
+__device__ __forceinline__ void ask_for(const int* p) {
+  asm volatile("{\n\t.reg .b32 unused;\n\tld.global.b32 unused, [%0];\n\t}" ::"l"(p));
+}
+
+// For the lists' sequences: their lengths.  (Counts of references and claims are not asked for ahead: they change
+// by atomics.)
+__device__ __forceinline__ void ask_for_lengths(const PagedCache& c, const int* sequences, int count) {
+  if (static_cast<int>(threadIdx.x) >= count) return;
+  const int sequence = sequences[threadIdx.x];
+  if (static_cast<unsigned>(sequence) < static_cast<unsigned>(c.max_sequences)) ask_for(c.lengths + sequence);
+}
 
 // Exclusive sum of `mine` over the block; `total` is the whole sum.
 __device__ int block_prefix(int mine, BookShared& s, int& total) {
@@ -265,12 +278,15 @@ __global__ void __launch_bounds__(kBookThreads) kv_extend_kernel(PagedCache c, B
   __shared__ BookShared s;
   release_successor();
   wait_for_predecessor();
-  if (*c.error != 0) return;
+  const int error = *c.error;
+  ask_for_lengths(c, b.sequences, b.count);
+  if (error != 0) return;
   if (threadIdx.x == 0) s.flag = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < b.count; i += kBookThreads) claim(c, b.sequences[i], s);
   __syncthreads();
   int need = 0;
+  int* list = nullptr;
   if (s.flag == 0) {
     __syncthreads();
     for (int start = 0; start < b.count; start += kBookThreads) {
@@ -287,7 +303,8 @@ __global__ void __launch_bounds__(kBookThreads) kv_extend_kernel(PagedCache c, B
     __syncthreads();
     if (s.flag == 0) {
       __syncthreads();
-      if (!list_free_pages(c, need, c.move_target, s) && threadIdx.x == 0) s.flag = kCacheNoPages;
+      list = need <= kBookThreads ? s.list : c.move_target;
+      if (!list_free_pages(c, need, list, s) && threadIdx.x == 0) s.flag = kCacheNoPages;
     }
   }
   __syncthreads();
@@ -306,7 +323,7 @@ __global__ void __launch_bounds__(kBookThreads) kv_extend_kernel(PagedCache c, B
         const int sequence = b.sequences[i];
         int* row = c.table + static_cast<size_t>(sequence) * c.max_pages + pages_of(c, held);
         for (int j = 0; j < mine; ++j) {
-          const int page = c.move_target[at + j];
+          const int page = list[at + j];
           row[j] = page;
           c.references[page] = 1;
         }
@@ -338,7 +355,9 @@ __global__ void __launch_bounds__(kBookThreads)
   __shared__ BookShared s;
   release_successor();
   wait_for_predecessor();
-  if (*c.error != 0) return;
+  const int error = *c.error;
+  ask_for_lengths(c, sequences, count);
+  if (error != 0) return;
   if (threadIdx.x == 0) s.flag = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += kBookThreads) claim(c, sequences[i], s);
@@ -371,7 +390,10 @@ __global__ void __launch_bounds__(kBookThreads)
     s.flag = 0;
     *c.move_count = 0;
   }
-  if (*c.error != 0) return;
+  const int error = *c.error;
+  ask_for_lengths(c, parents, count);
+  ask_for_lengths(c, children, count);
+  if (error != 0) return;
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += kBookThreads) claim(c, children[i], s);
   __syncthreads();
@@ -388,33 +410,39 @@ __global__ void __launch_bounds__(kBookThreads)
     int need = 0;
     for (int start = 0; start < count; start += kBookThreads) {
       const int i = start + threadIdx.x;
-      const int mine = i < count && (held_tokens(c, parents[i]) & (c.page_tokens - 1)) != 0;
+      const int tokens = i < count ? held_tokens(c, parents[i]) : 0;
+      const int mine = (tokens & (c.page_tokens - 1)) != 0;
+      const int source = mine ? page_at(c, parents[i], tokens >> c.page_shift) : 0;
       int total;
       const int at = need + block_prefix(mine, s, total);
-      if (mine && at < c.pages) {
-        const int sequence = parents[i];
-        c.move_source[at] = page_at(c, sequence, pages_of(c, held_tokens(c, sequence)) - 1);
-        if (c.move_source[at] < 0) s.flag = kCacheBadSequence;
-      }
+      if (mine && at < c.pages) c.move_source[at] = source;
+      if (source < 0) s.flag = kCacheBadSequence;
       need += total;
     }
     __syncthreads();
-    const bool enough = need <= c.pages && list_free_pages(c, need, c.move_target, s);
+    int* list = need <= kBookThreads ? s.list : c.move_target;
+    const bool enough = need <= c.pages && list_free_pages(c, need, list, s);
     if (!enough && threadIdx.x == 0) s.flag = kCacheNoPages;
     __syncthreads();
     if (s.flag != 0) {
       count_pages(c, children, count, 1);
     } else {
+      // a partly filled last page's copy, then the full pages
       int before = 0;
       for (int start = 0; start < count; start += kBookThreads) {
         const int i = start + threadIdx.x;
-        const int mine = i < count && (held_tokens(c, parents[i]) & (c.page_tokens - 1)) != 0;
+        const int tokens = i < count ? held_tokens(c, parents[i]) : 0;
+        const int mine = (tokens & (c.page_tokens - 1)) != 0;
         int total;
         const int at = before + block_prefix(mine, s, total);
-        if (mine) c.remap[i] = c.move_target[at];  // (count <= pages where every parent has one)
+        if (mine) {
+          const int page = list[at];
+          c.table[static_cast<size_t>(children[i]) * c.max_pages + (tokens >> c.page_shift)] = page;
+          c.references[page] = 1;
+          c.move_target[at] = page;
+        }
         before += total;
       }
-      __syncthreads();
       for (int i = threadIdx.x >> 5; i < count; i += kBookThreads / 32) {
         const int tokens = held_tokens(c, parents[i]), full = tokens >> c.page_shift;
         const bool partial = (tokens & (c.page_tokens - 1)) != 0;
@@ -425,8 +453,7 @@ __global__ void __launch_bounds__(kBookThreads)
             page = max(page_at(c, parents[i], place), 0);
             atomicAdd(&c.references[page], 1);
           } else if (place == full && partial) {
-            page = c.remap[i];
-            c.references[page] = 1;
+            continue;
           }
           row[place] = page;
         }
@@ -447,12 +474,13 @@ __global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) 
   release_successor();
   wait_for_predecessor();
   if (threadIdx.x == 0) *c.move_count = 0;
-  if (*c.error != 0) return;
+  const int error = *c.error;
   int live = 0;
   for (int page = threadIdx.x; page < c.pages; page += kBookThreads) {
     live += c.references[page] > 0;
     c.remap[page] = page;
   }
+  if (error != 0) return;
   int total;
   block_prefix(live, s, total);
   live = total;
@@ -461,12 +489,11 @@ __global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) 
     const int page = start + threadIdx.x;
     const bool used = page < c.pages && c.references[page] > 0;
     const bool source = used && page >= live, target = page < live && !used;
-    const int s_at = sources + block_prefix(source, s, total);
-    sources += total;
-    const int t_at = targets + block_prefix(target, s, total);
-    targets += total;
-    if (source) c.move_source[s_at] = page;
-    if (target) c.move_target[t_at] = page;
+    const int before = block_prefix(source | (target << 16), s, total);  // (at most 1024 of each)
+    if (source) c.move_source[sources + (before & 0xffff)] = page;
+    if (target) c.move_target[targets + (before >> 16)] = page;
+    sources += total & 0xffff;
+    targets += total >> 16;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < sources; i += kBookThreads) {
@@ -491,8 +518,9 @@ __global__ void __launch_bounds__(kCopyThreads)
   release_successor();
   wait_for_predecessor();  // (the books)
   if (count_at != nullptr) {
-    if (*c.error != 0) return;
+    const int error = *c.error;
     count = *count_at;
+    if (error != 0) return;
   }
   const int heads2 = 2 * c.kv_heads;
   const size_t page_words = static_cast<size_t>(heads2) * c.page_tokens * kHeadDim / 16;
@@ -528,7 +556,8 @@ __global__ void __launch_bounds__(kCopyThreads)
   }
   if (!rewrite_table) return;
   const int warps = gridDim.x * (kCopyThreads / 32);
-  for (int i = (blockIdx.x * kCopyThreads + threadIdx.x) >> 5; i < c.max_sequences; i += warps) {
+  // (from the last block down: of few pages and sequences other blocks do the copies)
+  for (int i = warps - 1 - static_cast<int>((blockIdx.x * kCopyThreads + threadIdx.x) >> 5); i < c.max_sequences; i += warps) {
     const int held = pages_of(c, held_tokens(c, i));
     int* row = c.table + static_cast<size_t>(i) * c.max_pages;
     for (int place = threadIdx.x & 31; place < held; place += 32) {
