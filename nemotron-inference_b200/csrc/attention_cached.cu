@@ -7,6 +7,11 @@
 //   O^T += V^T [a | b]  M = 128 dimensions, N = 2R, K = 128 tokens: the values' tile is read along its rows
 // Rows being few, all 128 threads have work and the tensor cores run far below what they can do, while the memory
 // is read at its rate.  Two blocks to an SM, a tile's chain of some 1500 cycles in one beside the other's.
+//
+// Measured, 32 heads on 8 key heads, pages of 64: 64 sequences of 2048 tokens on average 56 us (268 MB: 4.8 TB/s, 0.73
+// of the copy rate; some 11 us of it before the first tiles arrive and after the last), one of 65536 tokens 36 us
+// (134 MB).  One of 1500 tokens on 2 key heads 11.5 us: launch, the chain sequence - length - page - tile, and the
+// join of 12 pieces.
 #include <algorithm>
 
 #include "attention_cached.cuh"
@@ -44,7 +49,7 @@ constexpr size_t shared_bytes() {
   return 1024 + (S::kKeySlots + S::kValueSlots) * kKeyTileBytes + S::kQueryBytes + S::kWeightBytes + sizeof(Control<S>);
 }
 
-// All blocks of a launch run at once.
+// The blocks fit beside each other.
 template <typename S>
 constexpr bool fits_on_sm() {
   return S::kBlocks * (shared_bytes<S>() + 1024) <= 228 * 1024 && S::kBlocks * S::kColumns <= 512;
