@@ -6,7 +6,8 @@ own input RMSNorm and residual add, so the stack is layer(layer(...layer(x))).
 Works over single-device layers (`ExpertLayerSlice`), over expert-parallel engines
 (`ExpertParallelEngine`) and over plain callables `f(x, out)`: the model's layer loop
 interleaves MoE layers with Mamba and attention layers (:603-636), which stay the caller's
-own code and enter the stack as callbacks on the same device buffers.  The hidden state
+own code and enter the stack as callbacks on the same device buffers (`AttentionLayer` of
+attention_layer.py is one).  The hidden state
 stays on the device in FP32 between layers; nothing synchronises with the host except the
 split-size exchange inside a compact expert-parallel step.
 """
