@@ -720,3 +720,60 @@ def test_two_caches_on_two_streams(attention, heads):
     for i in range(2):
         assert all(torch.equal(r, alone[i]) for r in results[i])
         assert caches[i].sync_status() == 0
+
+
+def test_a_cache_of_more_than_4_gb(attention):
+    """The last pages of a large pool, of which something else holds the others, do what those of a
+    small pool do."""
+    kv_heads, heads, few, pages, layers = 2, 8, 24, 75000, 2
+    lengths = [130, 0, 300]
+    kv = _normal(60, sum(lengths), 2, kv_heads, D).to(torch.bfloat16)
+    more = _normal(61, 4, 2, kv_heads, D).to(torch.bfloat16)
+    q = _normal(62, 4, heads, D).to(torch.bfloat16)
+    caches, results = [], []
+    for n in (few, pages):
+        cache = attention.KvCache.allocate(layers, n, kv_heads, 4, 8, 64)
+        cache.references[:n - few] = 1
+        prompts = (_int([0, 1, 2]), _offsets(lengths))
+        cache.extend(*prompts, rows=sum(lengths))
+        for layer in range(layers):
+            cache.append(layer, kv[:, 0], kv[:, 1], *prompts)
+        cache.fork(_int([2]), _int([3]))
+        step = (_int([3, 0, 2]), _offsets([2, 1, 1]))
+        cache.extend(*step, rows=4)
+        for layer in range(layers):
+            cache.append(layer, more[:, 0], more[:, 1], *step)
+            results.append(cache.attend(layer, q, *step))
+        cache.free(_int([0]))
+        cache.compact()
+        results.append(cache.attend(layers - 1, q[:3], _int([3, 2]), _offsets([2, 1])))
+        assert cache.sync_status() == 0
+        caches.append(cache)
+    small, large = caches
+    assert large.codes.numel() > 2 ** 32
+    assert torch.equal(large.block_table[2:] - small.block_table[2:],
+                       (small.block_table[2:] > 0) * (pages - few) +
+                       (small.block_table[2:] == 0) * large.block_table[2:])
+    assert torch.equal(large.references[-few:], small.references)
+    assert torch.equal(large.exponents[:, -few:], small.exponents)
+    assert torch.equal(large.codes[:, -few:].view(torch.uint8), small.codes.view(torch.uint8))
+    for a, b in zip(results[:3], results[3:]):
+        assert torch.equal(a, b)
+    del small
+    _check_attend(large, 1, torch.cat((q[:2], q[3:])), [3, 2], [2, 1],
+                  large.attend(1, torch.cat((q[:2], q[3:])), _int([3, 2]), _offsets([2, 1])))
+
+
+def test_prefill_of_rows_beyond_4_gb(attention):
+    """Prompts at the end of a batch whose queries and results are larger than 4 GB."""
+    rows, heads, kv_heads, lengths = 600000, 32, 2, [200, 0, 77]
+    used = sum(lengths)
+    small = [_normal(70 + i, used, h, D).to(torch.bfloat16) for i, h in enumerate((heads, kv_heads, kv_heads))]
+    large = [torch.zeros((rows,) + t.shape[1:], dtype=t.dtype, device="cuda") for t in small]
+    for a, b in zip(large, small):
+        a[-used:] = b
+    got, lse = attention.attention_prefill(*large, _offsets(lengths) + (rows - used), return_lse=True)
+    want, sums = attention.attention_prefill(*small, _offsets(lengths), return_lse=True)
+    assert attention.prefill_sync_status() == 0
+    assert torch.equal(got[-used:], want) and torch.equal(lse[-used:], sums)
+    _check_prefill(*small, lengths, got[-used:], lse[-used:])
