@@ -79,7 +79,7 @@ struct WorkControl {
   int limit[2][S::kRows];                 // a row's position: the last token it sees
   int first_bad[kHeadDim];             // position of the first masked value that is no number, by dimension
   int found_bad;
-  int share, pieces_before[2];  // of a join
+  int share, pieces;  // of a join
   uint32_t tmem;
   int64_t before[S::kThreads / 32];
   Shares shares;      // of all tiles
@@ -478,8 +478,11 @@ __device__ __forceinline__ void prepare_queries(const CachedArgs& args, const Se
   for (int batch = 0; batch < S::kRows / (S::kBatch * S::kSoftmaxWarps); ++batch) {
     // (rows of warps that have none are not read by anybody)
     if (batch * S::kBatch * S::kSoftmaxWarps >= (rows + 31) / 32 * 32) break;
-    if (batch > 0) load_queries<S>(args, s, batch, raw);
+    uint2 next[S::kBatch];
+    if (batch + 1 < S::kRows / (S::kBatch * S::kSoftmaxWarps)) load_queries<S>(args, s, batch + 1, next);
     store_queries<S, Second>(args, s, which, batch, raw, q, c);
+#pragma unroll
+    for (int k = 0; k < S::kBatch; ++k) raw[k] = next[k];
   }
 }
 
@@ -592,45 +595,64 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
   }
 }
 
-// One thread: waits a while for the pieces that are missing when `word` was read.  The word when all are there, or
-// -1: this block has left.
-__device__ __forceinline__ int wait_for_pieces(JoinCounters* counters, int word, int parts) {
-  volatile int* pieces = &counters->pieces;
+// (a fence behind a plain load took 900 cycles)
+__device__ __forceinline__ int load_acquire(const int* p) {
+  int x;
+  asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(x) : "l"(p) : "memory");
+  return x;
+}
+
+// One thread: waits a while for the pieces that are missing.  The counter's word when all are there, or -1: this block
+// has left.
+__device__ __forceinline__ int wait_for_pieces(JoinCounters* counters, int parts) {
   const long long start = clock64();
-  while ((word & (kLeft - 1)) < parts && clock64() - start < kJoinPatience) word = *pieces;
+  int word = load_acquire(&counters->pieces);
+  while ((word & (kLeft - 1)) < parts && clock64() - start < kJoinPatience) word = load_acquire(&counters->pieces);
   while ((word & (kLeft - 1)) < parts) {  // (it can have changed as often as there are blocks)
     const int seen = atomicCAS(&counters->pieces, word, word + kLeft);
     if (seen == word) return -1;
     word = seen;
+    __threadfence();
   }
   return word;
 }
 
-// A block's part in the join of a segment's (sequence, key head), of whose pieces `pieces_before` were there when its
-// own was left.  If nobody has left, each block has the share of its own piece; else they take them in turn.  The
-// last block that is done sets the counters back.
+// A block's part in the join of a segment's (sequence, key head).  If nobody has left, each block has the share of its
+// own piece; else they take them in turn.  The last block that is done sets the counters back.
 template <typename S>
-__device__ void help_join(const CachedArgs& args, const Split& split, const Segment& s, const int& pieces_before, WorkControl<S>* c) {
+__device__ void help_join(const CachedArgs& args, const Split& split, const Segment& s, WorkControl<S>* c) {
   JoinCounters* counters = &split.counters[s.lead];
-  int done = 0, word = 0;  // thread 0's
-  if (threadIdx.x == 0) {
-    word = wait_for_pieces(counters, pieces_before + 1, s.parts);
-    __threadfence();
-    c->share = word >= kLeft ? atomicAdd(&counters->taken, 1) : word >= 0 ? static_cast<int>(blockIdx.x) - s.lead : -1;
-    if (word < kLeft) done = atomicAdd(&counters->done, 1);
-  }
+  if (threadIdx.x == 0) c->pieces = wait_for_pieces(counters, s.parts);
   softmax_sync<S>();
+  const int word = c->pieces;
+  // The last warp counts the block as done; where it joins rows first, the counter's answer is on its way meanwhile.
+  const bool counts = threadIdx.x == 32 * (S::kSoftmaxWarps - 1);
+  int done = 0;
+  auto count = [&] {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %2, 0;\n\t"
+        "@p atom.global.add.u32 %0, [%1], 1;\n\t}"
+        : "+r"(done)
+        : "l"(&counters->done), "r"(static_cast<uint32_t>(counts))
+        : "memory");
+  };
+  if (word < kLeft) count();
+  int share = word < 0 ? s.parts : static_cast<int>(blockIdx.x) - s.lead;
 #pragma unroll 1
-  for (int share = c->share; share >= 0 && share < s.parts; share = c->share) {
+  for (;;) {
+    if (word >= kLeft) {
+      if (threadIdx.x == 0) c->share = atomicAdd(&counters->taken, 1);
+      softmax_sync<S>();
+      share = c->share;
+    }
+    if (share >= s.parts) break;
     join<S>(args, split, s, share);
-    softmax_sync<S>();
-    if (threadIdx.x == 0) c->share = word >= kLeft ? atomicAdd(&counters->taken, 1) : -1;
+    if (word < kLeft) break;
     softmax_sync<S>();
   }
-  if (threadIdx.x == 0) {
-    if (word >= kLeft) done = atomicAdd(&counters->done, 1);
-    if (done == s.parts - 1) counters->pieces = counters->taken = counters->done = 0;
-  }
+  if (word >= kLeft) count();
+  if (counts && done == s.parts - 1) counters->pieces = counters->taken = counters->done = 0;
 }
 
 // The end of a block's softmax warps: its pieces are there (all threads' sums are behind a barrier, so one
@@ -641,12 +663,12 @@ __device__ void announce_and_join(const CachedArgs& args, const Split& split, in
   if (threadIdx.x == 0) {
     __threadfence();
 #pragma unroll 1
-    for (int i = 0; i < joins; ++i) c->pieces_before[i] = atomicAdd(&split.counters[c->to_join[i].lead].pieces, 1);
+    for (int i = 0; i < joins; ++i) atomicAdd(&split.counters[c->to_join[i].lead].pieces, 1);
   }
 #pragma unroll 1
   for (int i = 0; i < joins; ++i) {
-    if (i > 0) softmax_sync<S>();  // (the share of the first is read)
-    help_join<S>(args, split, c->to_join[i], c->pieces_before[i], c);
+    if (i > 0) softmax_sync<S>();  // (the counters' words of the first are read)
+    help_join<S>(args, split, c->to_join[i], c);
   }
 }
 
