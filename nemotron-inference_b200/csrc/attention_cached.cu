@@ -24,6 +24,9 @@ struct Shape {
   static constexpr int kRows = R;
   static constexpr int kWidth = 2 * R;  // columns of S and O, bytes of a token's weights
   static constexpr int kBlocks = 2;     // on an SM
+  // What a (sequence, key head, rows) costs a block beside its tiles, in tiles: its queries, and its results on their way
+  // out.  Counted where tiles are shared, or blocks that meet many come last by 20 %.
+  static constexpr int kUnitCost = 1;
   static constexpr int kKeySlots = 3, kValueSlots = 3;  // tiles in flight
   static constexpr int kSoftmaxWarps = 4;
   static constexpr int kBatch = R / kSoftmaxWarps;  // rows of queries to a warp

@@ -14,7 +14,7 @@
 // powers are kept in FP32 beside.
 //
 // With R rows of queries (new rows x heads that share the key head) at a time, W tiles of 128 tokens in all (and
-// one more for each sequence, key head and rows) and G blocks, block g takes the tiles [W g / G, W (g + 1) / G)
+// some more for what each sequence, key head and rows cost beside) and G blocks, block g takes the tiles [W g / G, W (g + 1) / G)
 // in order, whatever the sequences' lengths.
 // Where a (sequence, key head) is cut, each piece leaves its sums in the workspace.  When all have, these blocks
 // join them, a share of the rows at a time; each row is joined piece by piece in order, so results never depend
@@ -36,9 +36,6 @@ constexpr int kKeyTileBytes = kKeyTile * kHeadDim;
 constexpr int kMaxPagesPerTile = kKeyTile / 16;
 constexpr int kMaxRows = 128;
 constexpr int kSegments = 4;
-// What a (sequence, key head, rows) costs a block beside its tiles, in tiles: its queries, and its results on their
-// way out.  Counted where tiles are shared, or blocks that meet many short sequences come last by 20 %.
-constexpr int kUnitCost = 1;
 constexpr int kSlotsPerBlock = 2;      // of the workspace: a piece that began in a block before, one that goes on
 constexpr float kWeightBits = -1.5f;  // a row's largest weight is 2^-1.5 when its reference is set ...
 constexpr float kLargestBits = 0.0f;  // ... and at most 1 before it is set anew
@@ -201,13 +198,13 @@ __device__ __forceinline__ float power_of_two(int e) {  // -126 <= e <= 127
 template <typename S>
 struct EntryTiles {
   int tiles, row_tiles;  // of tokens, of rows
-  int cost;              // of one (key head, rows): the tiles lie behind kUnitCost
+  int cost;              // of one (key head, rows): the tiles lie behind S::kUnitCost
   int64_t all;
 
   __device__ EntryTiles(const CachedArgs& args, const BatchEntry& e) {
     tiles = (e.length + kKeyTile - 1) / kKeyTile;
     row_tiles = (e.rows * (args.heads / args.cache.kv_heads) + S::kRows - 1) / S::kRows;
-    cost = tiles + kUnitCost;
+    cost = tiles + S::kUnitCost;
     all = static_cast<int64_t>(cost) * row_tiles * args.cache.kv_heads;
   }
 };
@@ -300,7 +297,7 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
       s.length = e.length;
       s.kv_head = head;
       s.row0 = row_tile * S::kRows;
-      const int tiles_at = unit_at + kUnitCost;
+      const int tiles_at = unit_at + S::kUnitCost;
       s.tile = max(begin - tiles_at, 0);
       s.tiles = min(stop - tiles_at, t.tiles) - s.tile;
       s.lead = shares.block_of(tiles_at);
@@ -518,80 +515,84 @@ __device__ __forceinline__ void clean_values(uint8_t* values, int token, int pos
   fence_proxy_async_smem();
 }
 
-// Joins the pieces of a (sequence, key head), one of as many shares of the rows, a warp per row.  Of few rows many
-// pieces are read at once, of many the next row's are on their way meanwhile.
+// Joins the pieces of a (sequence, key head), one of as many shares of the rows.  Lanes per row: all 32 where there are
+// few rows, or eight, so that four of a warp's many rows are on their way at once (a row after the other, asked for one
+// ahead, took 6500 cycles for three of them: 48 sequences of 8192 tokens 113 -> 101 us).
 template <typename S>
 __device__ void join(const CachedArgs& args, const Split& split, const Segment& s, int share) {
-  constexpr bool kManyRows = S::kRows > 16;
-  constexpr int kAtOnce = kManyRows ? 8 : 16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int pieces = s.parts, rows = min(S::kRows, s.rows * (args.heads / args.cache.kv_heads) - s.row0);
-  auto sums_of = [&](int p) { return split.slots + slot_floats(S::kRows) * (kSlotsPerBlock * (s.lead + p) + (p == 0)); };
+  constexpr int kLanes = S::kRows > 16 ? 8 : 32;
+  constexpr int kVectors = kHeadDim / 4 / kLanes;   // of four dimensions, to a lane
+  constexpr int kAtOnce = kLanes == 32 ? 16 : 2;    // pieces (of many rows four spill: 112 us where two take 100)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = lane & (kLanes - 1), leader = lane - mine;
+  const int group = args.heads / args.cache.kv_heads;
+  const int pieces = s.parts, rows = min(S::kRows, s.rows * group - s.row0);
   const int end = rows * (share + 1) / pieces;
-  struct Read {
-    float reference, weight;  // a lane per piece
-    float4 x[kAtOnce];        // the sums of pieces `first` on
-  };
-  auto read_x = [&](Read& read, int r, int first) {
-#pragma unroll
-    for (int p = 0; p < kAtOnce; ++p) {
-      if (first + p < pieces) read.x[p] = __ldcg(reinterpret_cast<const float4*>(sums_of(first + p) + r * kHeadDim) + lane);
-    }
-  };
-  auto read_start = [&](Read& read, int r, int start) {
-    read.reference = -INFINITY;
-    read.weight = 0.0f;
-    if (start + lane < pieces) {
-      const float* at = sums_of(start + lane) + S::kRows * kHeadDim + r;
-      read.reference = __ldcg(at);
-      read.weight = __ldcg(at + S::kRows);
-    }
-    read_x(read, r, start);
-  };
-  Read read;
-  int r = rows * share / pieces + warp;
-  if (kManyRows && r < end) read_start(read, r, 0);
+  auto sums_of = [&](int p) { return split.slots + slot_floats(S::kRows) * (kSlotsPerBlock * (s.lead + p) + (p == 0)); };
 #pragma unroll 1
-  for (; r < end; r += S::kSoftmaxWarps) {
-    const int next = r + S::kSoftmaxWarps, row = s.row0 + r;
-    // the maximum so far is raised where there are over 32 pieces
-    float top = -INFINITY, sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-    for (int start = 0; start < pieces; start += 32) {
-      if (!kManyRows || start > 0) read_start(read, r, start);
-      const int count = min(32, pieces - start);
-      const float higher = fmaxf(top, warp_max(read.reference));
-      const float keep = top > -INFINITY ? exp2_approx(top - higher) : 0.0f;
-      const float scale = read.reference > -INFINITY ? exp2_approx(read.reference - higher) : 0.0f;
-      const float weight = scale != 0.0f ? read.weight * scale : 0.0f;
-      top = higher;
-      sum *= keep;
+  for (int base = rows * share / pieces + warp * (32 / kLanes); base < end; base += S::kSoftmaxWarps * (32 / kLanes)) {
+    const int r = min(base + leader / kLanes, end - 1), row = s.row0 + r;
+    // the maximum so far is raised from chunk to chunk of pieces
+    float top = -INFINITY, sum = 0.0f, o[4 * kVectors];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] *= keep;
+    for (int i = 0; i < 4 * kVectors; ++i) o[i] = 0.0f;
+#pragma unroll 1
+    for (int start = 0; start < pieces; start += kLanes) {
+      float reference = -INFINITY, weight = 0.0f;  // a lane per piece
+      if (start + mine < pieces) {
+        const float* at = sums_of(start + mine) + S::kRows * kHeadDim + r;
+        reference = __ldcg(at);
+        weight = __ldcg(at + S::kRows);
+      }
+      const int count = min(kLanes, pieces - start);
+      float scale = 0.0f;
 #pragma unroll 1
       for (int first = 0; first < count; first += kAtOnce) {
-        if (first > 0) read_x(read, r, start + first);
-        float4 x[kAtOnce];
-#pragma unroll
-        for (int p = 0; p < kAtOnce; ++p) x[p] = read.x[p];
-        if (kManyRows && start + first + kAtOnce >= pieces && next < end) read_start(read, next, 0);
+        float4 x[kAtOnce][kVectors];
 #pragma unroll
         for (int p = 0; p < kAtOnce; ++p) {
-          const float f = __shfl_sync(0xffffffffu, scale, first + p);
+          const float4* at = reinterpret_cast<const float4*>(sums_of(start + first + p) + r * kHeadDim) + mine;
+#pragma unroll
+          for (int i = 0; i < kVectors; ++i) {
+            if (first + p < count) x[p][i] = __ldcg(at + i * kLanes);
+          }
+        }
+        if (first == 0) {
+          float higher = reference;
+#pragma unroll
+          for (int step = kLanes / 2; step > 0; step /= 2) higher = fmaxf(higher, __shfl_xor_sync(0xffffffffu, higher, step));
+          higher = fmaxf(higher, top);
+          const float keep = top > -INFINITY ? exp2_approx(top - higher) : 0.0f;
+          scale = reference > -INFINITY ? exp2_approx(reference - higher) : 0.0f;
+          weight = scale != 0.0f ? weight * scale : 0.0f;
+          top = higher;
+          sum *= keep;
+#pragma unroll
+          for (int i = 0; i < 4 * kVectors; ++i) o[i] *= keep;
+        }
+#pragma unroll
+        for (int p = 0; p < kAtOnce; ++p) {
+          const float f = __shfl_sync(0xffffffffu, scale, leader + ((first + p) & (kLanes - 1)));
+          const float w = __shfl_sync(0xffffffffu, weight, leader + ((first + p) & (kLanes - 1)));
           if (first + p >= count || f == 0.0f) continue;
-          sum += __shfl_sync(0xffffffffu, weight, first + p);
-          o[0] = fmaf(x[p].x, f, o[0]);
-          o[1] = fmaf(x[p].y, f, o[1]);
-          o[2] = fmaf(x[p].z, f, o[2]);
-          o[3] = fmaf(x[p].w, f, o[3]);
+          sum += w;
+#pragma unroll
+          for (int i = 0; i < kVectors; ++i) {
+            o[4 * i] = fmaf(x[p][i].x, f, o[4 * i]);
+            o[4 * i + 1] = fmaf(x[p][i].y, f, o[4 * i + 1]);
+            o[4 * i + 2] = fmaf(x[p][i].z, f, o[4 * i + 2]);
+            o[4 * i + 3] = fmaf(x[p][i].w, f, o[4 * i + 3]);
+          }
         }
       }
     }
+    if (base + leader / kLanes >= end) continue;
     const float inverse = 1.0f / sum;
-    const int group = args.heads / args.cache.kv_heads;
     const size_t at = static_cast<size_t>(s.first + row / group) * args.heads + s.kv_head * group + row % group;
-    *reinterpret_cast<uint2*>(args.out + at * kHeadDim + lane * 4) =
-        make_uint2(pack_bf16(o[0] * inverse, o[1] * inverse), pack_bf16(o[2] * inverse, o[3] * inverse));
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+      *reinterpret_cast<uint2*>(args.out + at * kHeadDim + (mine + i * kLanes) * 4) =
+          make_uint2(pack_bf16(o[4 * i] * inverse, o[4 * i + 1] * inverse), pack_bf16(o[4 * i + 2] * inverse, o[4 * i + 3] * inverse));
+    }
   }
 }
 
