@@ -517,7 +517,8 @@ __device__ __forceinline__ void clean_values(uint8_t* values, int token, int pos
 
 // Joins the pieces of a (sequence, key head), one of as many shares of the rows.  Lanes per row: all 32 where there are
 // few rows, or eight, so that four of a warp's many rows are on their way at once (a row after the other, asked for one
-// ahead, took 6500 cycles for three of them: 48 sequences of 8192 tokens 113 -> 101 us).
+// ahead, took 6500 cycles for three of them: 48 sequences of 8192 tokens 113 -> 101 us).  A share of no more rows than
+// there are warps spreads a row's pieces over the four instead, a quarter each.
 template <typename S>
 __device__ void join(const CachedArgs& args, const Split& split, const Segment& s, int share) {
   constexpr int kLanes = S::kRows > 16 ? 8 : 32;
@@ -526,24 +527,28 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = lane & (kLanes - 1), leader = lane - mine;
   const int group = args.heads / args.cache.kv_heads;
   const int pieces = s.parts, rows = min(S::kRows, s.rows * group - s.row0);
-  const int end = rows * (share + 1) / pieces;
+  const int end = rows * (share + 1) / pieces, slot = lane / kLanes;
+  const bool spread = kLanes < 32 && rows <= pieces * S::kSoftmaxWarps;
+  const int at_once = spread ? 1 : 32 / kLanes;  // rows
+  const int from = spread ? pieces * slot / (32 / kLanes) : 0, to = spread ? pieces * (slot + 1) / (32 / kLanes) : pieces;
+  const int longest = spread ? (pieces + 32 / kLanes - 1) / (32 / kLanes) : pieces;
   auto sums_of = [&](int p) { return split.slots + slot_floats(S::kRows) * (kSlotsPerBlock * (s.lead + p) + (p == 0)); };
 #pragma unroll 1
-  for (int base = rows * share / pieces + warp * (32 / kLanes); base < end; base += S::kSoftmaxWarps * (32 / kLanes)) {
-    const int r = min(base + leader / kLanes, end - 1), row = s.row0 + r;
+  for (int base = rows * share / pieces + warp * at_once; base < end; base += S::kSoftmaxWarps * at_once) {
+    const int r = min(base + (spread ? 0 : slot), end - 1), row = s.row0 + r;
     // the maximum so far is raised from chunk to chunk of pieces
     float top = -INFINITY, sum = 0.0f, o[4 * kVectors];
 #pragma unroll
     for (int i = 0; i < 4 * kVectors; ++i) o[i] = 0.0f;
 #pragma unroll 1
-    for (int start = 0; start < pieces; start += kLanes) {
+    for (int start = from; start < from + longest; start += kLanes) {
       float reference = -INFINITY, weight = 0.0f;  // a lane per piece
-      if (start + mine < pieces) {
+      if (start + mine < to) {
         const float* at = sums_of(start + mine) + S::kRows * kHeadDim + r;
         reference = __ldcg(at);
         weight = __ldcg(at + S::kRows);
       }
-      const int count = min(kLanes, pieces - start);
+      const int count = min(kLanes, from + longest - start);
       float scale = 0.0f;
 #pragma unroll 1
       for (int first = 0; first < count; first += kAtOnce) {
@@ -553,7 +558,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
           const float4* at = reinterpret_cast<const float4*>(sums_of(start + first + p) + r * kHeadDim) + mine;
 #pragma unroll
           for (int i = 0; i < kVectors; ++i) {
-            if (first + p < count) x[p][i] = __ldcg(at + i * kLanes);
+            if (start + first + p < to) x[p][i] = __ldcg(at + i * kLanes);
           }
         }
         if (first == 0) {
@@ -573,7 +578,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
         for (int p = 0; p < kAtOnce; ++p) {
           const float f = __shfl_sync(0xffffffffu, scale, leader + ((first + p) & (kLanes - 1)));
           const float w = __shfl_sync(0xffffffffu, weight, leader + ((first + p) & (kLanes - 1)));
-          if (first + p >= count || f == 0.0f) continue;
+          if (first + p >= count || f == 0.0f) continue;  // (f is 0 behind the last piece)
           sum += w;
 #pragma unroll
           for (int i = 0; i < kVectors; ++i) {
@@ -585,7 +590,22 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
         }
       }
     }
-    if (base + leader / kLanes >= end) continue;
+    if (spread) {
+#pragma unroll
+      for (int step = kLanes; step < 32; step *= 2) {
+        const float higher = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+        const float keep = top > -INFINITY ? exp2_approx(top - higher) : 0.0f;
+        top = higher;
+        sum *= keep;
+        sum += __shfl_xor_sync(0xffffffffu, sum, step);
+#pragma unroll
+        for (int i = 0; i < 4 * kVectors; ++i) {
+          o[i] *= keep;
+          o[i] += __shfl_xor_sync(0xffffffffu, o[i], step);
+        }
+      }
+    }
+    if (spread ? slot > 0 : base + slot >= end) continue;
     const float inverse = 1.0f / sum;
     const size_t at = static_cast<size_t>(s.first + row / group) * args.heads + s.kv_head * group + row % group;
 #pragma unroll
