@@ -777,3 +777,15 @@ def test_prefill_of_rows_beyond_4_gb(attention):
     assert attention.prefill_sync_status() == 0
     assert torch.equal(got[-used:], want) and torch.equal(lse[-used:], sums)
     _check_prefill(*small, lengths, got[-used:], lse[-used:])
+
+
+@pytest.mark.parametrize("lengths,counts,heads,kv_heads", [
+    ([30000], [8], 16, 1), ([9000, 20011], [3, 5], 8, 1), ([40000], [2], 18, 1), ([1000] * 40, [7] * 40, 32, 2)])
+def test_attend_joins_many_pieces_of_many_rows(attention, lengths, counts, heads, kv_heads):
+    cache = _filled(attention, lengths, kv_heads, 64, seed=2, layers=1)
+    q = (2 * _normal(11, sum(counts), heads, D)).to(torch.bfloat16)
+    batch = (_int(list(range(len(lengths)))), _offsets(counts))
+    got = cache.attend(0, q, *batch, scale=0.05)
+    assert cache.sync_status() == 0
+    _check_attend(cache, 0, q, list(range(len(lengths))), counts, got, scale=0.05)
+    assert torch.equal(cache.attend(0, q, *batch, scale=0.05), got)
