@@ -515,10 +515,14 @@ NMOE_API nmoe_status nmoe_route_tokens_noalloc(
  * at most once in a list), `offsets` [count + 1] the rows that belong to each:
  * entry i has the rows [offsets[i], offsets[i+1]) of `rows`, possibly none.
  *
- * What only the device can see is wrong (a list entry out of range or named
- * twice, too few pages) leaves a status in the workspace: nmoe_kv_sync_status
- * returns and clears it.  Until then nmoe_kv_extend, _append, _fork, _free and
- * _compact do nothing, so that rows without a place are not written over others.
+ * What only the device can see is wrong leaves a status in the workspace:
+ * nmoe_kv_sync_status returns and clears it, and until then nmoe_kv_extend, _fork,
+ * _free and _compact change nothing.  Where one of these found it (a list entry out
+ * of range or named twice, too few pages), nmoe_kv_append does nothing either, so
+ * that rows without a place are not written over others.  An entry or a page out
+ * of range that an append, attention or a copy of pages comes upon is that entry's
+ * or page's alone: all others of the call, and of such calls behind it, are done
+ * all the same.  (That no sequence is named twice is not checked by these.)
  */
 typedef struct nmoe_kv_cache {
   int32_t layers;

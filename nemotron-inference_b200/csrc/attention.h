@@ -17,7 +17,7 @@ namespace nmoe {
 constexpr int kHeadDim = 128;
 constexpr int kMinExponent = -32, kMaxExponent = 32;  // of a page and head's scale, 2^exponent
 
-// What a kernel can leave in a cache's error word, beside kDevWaitTimeout.
+// What a kernel can leave in a cache's words `error` and `raised`, beside kDevWaitTimeout.
 enum CacheError : int {
   kCacheNoPages = 16,      // fewer free pages, or places in the block table, than asked for
   kCacheBadSequence = 17,  // a sequence out of range or twice in a list, a page out of range
@@ -31,7 +31,12 @@ struct PagedCache {
   int* table;       // [max_sequences][max_pages]
   int* lengths;     // [max_sequences]
   int* references;  // [pages]; 0: free
+  // Two words, of which the first code stays.  `error`: the books could not be kept, or a wait ran out; appends and
+  // attention read it and do nothing then.  `raised`: an entry or a page that appends, attention or copies of pages
+  // found wrong and left out; the books read it, too.  None of a launch's blocks reads what others of it write, so
+  // a wrong entry changes nothing for the rest of its batch.
   int* error;
+  int* raised;
   int* move_count;   // pages for the copy kernel: the first *move_count of the two lists
   int* move_source;  // [pages]
   int* move_target;  // [pages]
@@ -58,6 +63,9 @@ struct BatchEntry {
 __device__ __forceinline__ void report_cache_error(int* error, int code) {
   if (error != nullptr) atomicCAS(error, 0, code);
 }
+
+// What the books go by.
+__device__ __forceinline__ bool error_pending(const PagedCache& c) { return (*c.error | *c.raised) != 0; }
 
 // Entry i of a batch, brought into range: whatever the arrays hold, its rows lie within the batch's
 // and its tokens within the block table.

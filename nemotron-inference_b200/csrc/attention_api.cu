@@ -28,7 +28,9 @@ struct Layout {
   size_t move_source, move_target, remap, claims, attend, total;
 };
 
-// Header (error word, number of pages to copy), the lists of the page kernels, the attention's parts.
+// Header (the words below), the lists of the page kernels, the attention's parts.
+enum HeaderWord { kErrorWord, kMoveCountWord, kRaisedWord, kHeaderWords };
+
 Layout layout_of(const nmoe_kv_cache& c) {
   const size_t pages = sizeof(int) * static_cast<size_t>(c.pages);
   const size_t sequences = sizeof(int) * static_cast<size_t>(c.max_sequences);
@@ -65,8 +67,9 @@ bool view_of(const nmoe_kv_cache* c, PagedCache& view) {
   view.table = c->block_table;
   view.lengths = c->lengths;
   view.references = c->references;
-  view.error = reinterpret_cast<int*>(w);
-  view.move_count = reinterpret_cast<int*>(w) + 1;
+  view.error = reinterpret_cast<int*>(w) + kErrorWord;
+  view.move_count = reinterpret_cast<int*>(w) + kMoveCountWord;
+  view.raised = reinterpret_cast<int*>(w) + kRaisedWord;
   view.move_source = reinterpret_cast<int*>(w + l.move_source);
   view.move_target = reinterpret_cast<int*>(w + l.move_target);
   view.remap = reinterpret_cast<int*>(w + l.remap);
@@ -105,16 +108,28 @@ nmoe_status device_status(int code) {
   }
 }
 
-// Waits for the stream, reads an error word and clears it, with what a call that gave up may have left.
-nmoe_status sync_error_word(int* word, cudaStream_t stream, void* counters = nullptr) {
+// Waits for the stream, reads an error word and clears it.
+nmoe_status sync_error_word(int* word, cudaStream_t stream) {
   int code = 0;
   cudaError_t err = cudaMemcpyAsync(&code, word, sizeof(code), cudaMemcpyDeviceToHost, stream);
   if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
   if (err == cudaSuccess && code != 0) {
     err = cudaMemsetAsync(word, 0, sizeof(code), stream);
-    if (err == cudaSuccess && counters != nullptr) {
-      err = cudaMemsetAsync(counters, 0, nmoe::kAttendCounterBytes, stream);
-    }
+    if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
+  }
+  return err == cudaSuccess ? device_status(code) : status_of(err);
+}
+
+// The same for a cache's words, with what a call that gave up may have left.
+nmoe_status sync_cache(const PagedCache& cache, cudaStream_t stream) {
+  int words[kHeaderWords] = {};
+  cudaError_t err = cudaMemcpyAsync(words, cache.error, sizeof(words), cudaMemcpyDeviceToHost, stream);
+  if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
+  const int code = words[kErrorWord] != 0 ? words[kErrorWord] : words[kRaisedWord];
+  if (err == cudaSuccess && code != 0) {
+    err = cudaMemsetAsync(cache.error, 0, sizeof(int), stream);
+    if (err == cudaSuccess) err = cudaMemsetAsync(cache.raised, 0, sizeof(int), stream);
+    if (err == cudaSuccess) err = cudaMemsetAsync(cache.attend_workspace, 0, nmoe::kAttendCounterBytes, stream);
     if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
   }
   return err == cudaSuccess ? device_status(code) : status_of(err);
@@ -257,7 +272,7 @@ nmoe_status nmoe_kv_copy_pages(const nmoe_kv_cache* cache, void* stream, const i
 nmoe_status nmoe_kv_sync_status(const nmoe_kv_cache* cache, void* stream) {
   PagedCache view;
   if (!view_of(cache, view)) return NMOE_ERR_INVALID_ARGUMENT;
-  return sync_error_word(view.error, static_cast<cudaStream_t>(stream), view.attend_workspace);
+  return sync_cache(view, static_cast<cudaStream_t>(stream));
 }
 
 nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* stream, int32_t layer,

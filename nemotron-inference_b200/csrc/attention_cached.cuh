@@ -220,7 +220,7 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
 #pragma unroll 1
   for (int i = begin; i < end; ++i) {
     e = batch_entry(args.cache, args.batch, i);
-    if (!e.valid && blockIdx.x == 0) report_cache_error(args.cache.error, kCacheBadSequence);
+    if (!e.valid && blockIdx.x == 0) report_cache_error(args.cache.raised, kCacheBadSequence);
     mine += EntryTiles<S>(args, e).all;
   }
   int64_t upto = mine;
@@ -240,7 +240,7 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
   // (more than 2^31 tiles are some 70 TB of codes to be read; with fewer tiles than blocks, the first blocks have
   // one each)
   if (total > INT32_MAX) {
-    if (threadIdx.x == 0) report_cache_error(args.cache.error, kCacheBadSequence);
+    if (threadIdx.x == 0) report_cache_error(args.cache.raised, kCacheBadSequence);
     total = 0;
   }
   Shares shares;
@@ -327,7 +327,7 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
           if (wanted + lane < last_page) {
             page = page_at(cache, e.sequence, wanted + lane);
             if (page < 0) {
-              report_cache_error(cache.error, kCacheBadSequence);
+              report_cache_error(cache.raised, kCacheBadSequence);
               page = 0;
             }
           }

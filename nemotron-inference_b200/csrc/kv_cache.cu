@@ -79,11 +79,12 @@ __global__ void __launch_bounds__(kAppendThreads, PageTokens <= 64 ? kAppendBloc
   const int pending = *c.error;
   const int2 unit = locate_unit(b.count, blockIdx.x, [&](int i) {
     const BatchEntry e = batch_entry(c, b, i);
-    if (!e.valid) report_cache_error(c.error, kCacheBadSequence);
+    if (!e.valid) report_cache_error(c.raised, kCacheBadSequence);
     if (e.rows == 0) return 0;
     return ((e.length - 1) >> c.page_shift) - ((e.length - e.rows) >> c.page_shift) + 1;
   });
-  // (after a reservation that failed these rows have no place of their own)
+  // (after a reservation that failed these rows have no place of their own; no block of an append writes this word,
+  // so all of them see the same)
   if (pending != 0 || unit.x < 0) return;
   const BatchEntry e = batch_entry(c, b, unit.x);
   const int place = ((e.length - e.rows) >> c.page_shift) + unit.y;
@@ -106,7 +107,7 @@ __global__ void __launch_bounds__(kAppendThreads, PageTokens <= 64 ? kAppendBloc
   read(blockIdx.y * per_block, raw);  // (under way while the page is looked up)
   const int page = page_at(c, e.sequence, place);
   if (page < 0) {
-    report_cache_error(c.error, kCacheBadSequence);
+    report_cache_error(c.raised, kCacheBadSequence);
     return;
   }
 #pragma unroll 1
@@ -281,9 +282,9 @@ __global__ void __launch_bounds__(kBookThreads) kv_extend_kernel(PagedCache c, B
   __shared__ BookShared s;
   release_successor();
   wait_for_predecessor();
-  const int error = *c.error;
+  const bool pending = error_pending(c);
   ask_for_lengths(c, b.sequences, b.count);
-  if (error != 0) return;
+  if (pending) return;
   if (threadIdx.x == 0) s.flag = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < b.count; i += kBookThreads) claim(c, b.sequences[i], s);
@@ -358,9 +359,9 @@ __global__ void __launch_bounds__(kBookThreads)
   __shared__ BookShared s;
   release_successor();
   wait_for_predecessor();
-  const int error = *c.error;
+  const bool pending = error_pending(c);
   ask_for_lengths(c, sequences, count);
-  if (error != 0) return;
+  if (pending) return;
   if (threadIdx.x == 0) s.flag = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += kBookThreads) claim(c, sequences[i], s);
@@ -393,10 +394,10 @@ __global__ void __launch_bounds__(kBookThreads)
     s.flag = 0;
     *c.move_count = 0;
   }
-  const int error = *c.error;
+  const bool pending = error_pending(c);
   ask_for_lengths(c, parents, count);
   ask_for_lengths(c, children, count);
-  if (error != 0) return;
+  if (pending) return;
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += kBookThreads) claim(c, children[i], s);
   __syncthreads();
@@ -477,13 +478,13 @@ __global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) 
   release_successor();
   wait_for_predecessor();
   if (threadIdx.x == 0) *c.move_count = 0;
-  const int error = *c.error;
+  const bool pending = error_pending(c);
   int live = 0;
   for (int page = threadIdx.x; page < c.pages; page += kBookThreads) {
     live += c.references[page] > 0;
     c.remap[page] = page;
   }
-  if (error != 0) return;
+  if (pending) return;
   int total;
   block_prefix(live, s, total);
   live = total;
@@ -524,9 +525,9 @@ __global__ void __launch_bounds__(kCopyThreads)
   release_successor();
   wait_for_predecessor();  // (the books)
   if (count_at != nullptr) {
-    const int error = *c.error;
+    const bool pending = error_pending(c);
     count = *count_at;
-    if (error != 0) return;
+    if (pending) return;
   }
   const int heads2 = 2 * c.kv_heads;
   const size_t page_words = static_cast<size_t>(heads2) * c.page_tokens * kHeadDim / 16;
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(kCopyThreads)
     const int from = sources[move], to = targets[move];
     if (static_cast<unsigned>(from) >= static_cast<unsigned>(c.pages) ||
         static_cast<unsigned>(to) >= static_cast<unsigned>(c.pages)) {
-      report_cache_error(c.error, kCacheBadSequence);
+      report_cache_error(c.raised, kCacheBadSequence);
       continue;
     }
     const size_t read_page = layer * c.pages + from, write_page = layer * c.pages + to;
