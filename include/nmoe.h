@@ -592,7 +592,8 @@ NMOE_API nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* str
  * i in rows [offsets[i], offsets[i+1]) (device, rising from 0 to `tokens`).
  * out [tokens][heads][128]; lse [tokens][heads], nullable: the logarithms of
  * the rows' sums of exponentials; error: a device word, zero at first, for
- * nmoe_attention_sync_status (until which nothing more is computed). */
+ * nmoe_attention_sync_status.  Until it has returned what a call left there,
+ * calls with this word compute nothing and write zeros (lse: -infinity). */
 NMOE_API nmoe_status nmoe_attention_prefill(void* stream, const void* q, int64_t q_stride,
                                             const void* k, int64_t k_stride, const void* v,
                                             int64_t v_stride, int64_t tokens, int32_t heads,

@@ -17,12 +17,14 @@ layer runs between its projections, over the C ABI of include/nmoe.h:
 q is [rows, heads, 128] bf16, k and v [rows, kv_heads, 128]; slices of a fused projection's
 rows are taken as they lie.  `sequences` [n] (rows of the block table, each at most once) and
 `offsets` [n + 1] (rows of each) are int32 tensors on the device; the host reads neither, so
-a step can be recorded in a CUDA graph.  Calls run on the current stream; a cache is used by
-one stream at a time.
+a step can be recorded in a CUDA graph; what a call keeps on the device (a cache's workspace, the
+word of `attention_prefill`) is made before that, by a `KvCache` or a call that is not recorded.
+Calls run on the current stream; a cache is used by one stream at a time.
 """
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import Dict, Optional
 
 import torch
@@ -92,6 +94,11 @@ def _require_list(t: torch.Tensor, name: str, device: torch.device) -> None:
         raise ValueError(f"{name} must be a contiguous int32 vector on {device}")
 
 
+def _require_word(t: torch.Tensor, device: torch.device) -> None:
+    if t.dtype is not torch.int32 or t.numel() != 1 or t.device != device:
+        raise ValueError(f"error must be one int32 on {device}")
+
+
 def _stream_of(device: torch.device, what: str) -> int:
     """The current stream, if `device` is the current device."""
     if device.type != "cuda":
@@ -111,17 +118,43 @@ def _output(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _zeros(elements: int, dtype: torch.dtype, device: torch.device, what: str) -> torch.Tensor:
+    """Memory that every stream finds zero: the fill is over when this returns, and no node of a graph."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} is made before anything that uses it is recorded in a CUDA graph")
+    made = torch.zeros(elements, dtype=dtype, device=device)
+    torch.cuda.current_stream(device).synchronize()
+    return made
+
+
 _error_words: Dict[int, torch.Tensor] = {}
+_error_words_lock = threading.Lock()
+
+
+def _error_word(device: torch.device) -> torch.Tensor:
+    """The word of the calls of `attention_prefill` on a device that are given none."""
+    error = _error_words.get(device.index)
+    if error is None:
+        with _error_words_lock:
+            error = _error_words.get(device.index)
+            if error is None:
+                error = _error_words[device.index] = _zeros(1, torch.int32, device, "the word of attention_prefill")
+    return error
 
 
 def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
                       scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-                      return_lse: bool = False):
+                      return_lse: bool = False, error: Optional[torch.Tensor] = None):
     """Causal attention over whole prompts packed one behind the other: prompt i is the rows
     [offsets[i], offsets[i + 1]), and each of its rows sees those up to itself.  Query head h
     attends key head h // (heads // kv_heads).  Returns [rows, heads, 128] bf16 and, if asked
     for, the FP32 logarithms [rows, heads] of the rows' sums of exponentials.  `scale` is
-    1 / sqrt(128) unless given."""
+    1 / sqrt(128) unless given.
+
+    `error`: an int32 word on the device, zero at first, in which a call whose waits run out leaves
+    a status; calls compute nothing while it holds one (`prefill_sync_status`).  Without it all calls
+    on a device have one word together: streams or models that should not stop each other are
+    given words of their own."""
     device = q.device
     stream = _stream_of(device, "q")
     rows, heads, q_stride = _row_layout(q, "q", device)
@@ -134,9 +167,12 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets
                                                 "offsets one entry more than there are prompts")
     out = _output(out, q)
     lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
-    error = _error_words.get(device.index)
     if error is None:
-        error = _error_words[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        error = _error_words.get(device.index)
+        if error is None:
+            error = _error_word(device)
+    else:
+        _require_word(error, device)
     _check((_library or _lib()).nmoe_attention_prefill(
         stream, q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, rows, heads,
         kv_heads, offsets.data_ptr(), prompts, DEFAULT_SCALE if scale is None else scale,
@@ -145,9 +181,13 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets
     return (out, lse) if return_lse else out
 
 
-def prefill_sync_status() -> int:
-    """Waits for the current stream; the status of `attention_prefill` on this device."""
-    error = _error_words.get(torch.cuda.current_device())
+def prefill_sync_status(error: Optional[torch.Tensor] = None) -> int:
+    """Waits for the current stream; what calls of `attention_prefill` with this word, or with none on
+    this device, could not do, and clears it."""
+    if error is None:
+        error = _error_words.get(torch.cuda.current_device())
+    else:
+        _require_word(error, torch.device("cuda", torch.cuda.current_device()))
     return NMOE_OK if error is None else _lib().nmoe_attention_sync_status(error.data_ptr(), _stream())
 
 
@@ -191,9 +231,10 @@ class KvCache:
         needed = _lib().nmoe_kv_workspace_bytes(ctypes.byref(self._c))
         if needed == 0:
             raise NmoeError(1, "KvCache", "a size is zero or too large")
-        self._workspace = torch.zeros(needed, dtype=torch.uint8, device=device)
+        self._workspace = _zeros(needed, torch.uint8, device, "a cache's workspace")
         self._c.workspace, self._c.workspace_bytes = self._workspace.data_ptr(), needed
         self._ref = ctypes.byref(self._c)
+        _error_word(device)  # (what records a step with a cache may begin with prompts)
 
     @staticmethod
     def allocate(layers: int, pages: int, kv_heads: int, max_sequences: int,
@@ -201,6 +242,8 @@ class KvCache:
         """An empty cache on the current device."""
         if not torch.cuda.is_available():
             raise RuntimeError("KvCache needs a CUDA device: there is no CPU path")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a cache is made before anything that uses it is recorded in a CUDA graph")
         device = device or torch.device("cuda", torch.cuda.current_device())
         int32 = dict(dtype=torch.int32, device=device)
         codes = torch.zeros((layers, pages, 2, kv_heads, page_tokens, HEAD_DIM), dtype=torch.uint8,

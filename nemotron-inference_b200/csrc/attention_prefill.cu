@@ -492,6 +492,19 @@ __device__ void softmax_role(const PrefillArgs& args, uint32_t tmem, Control* c)
   if (lane == 0) report_cache_error(args.error, kDevWaitTimeout);
 }
 
+// Of a call that computes nothing: zeros, and no sums.  (Nobody asks for another's block then: all of the grid run.)
+__device__ void clear_results(const PrefillArgs& args) {
+  const int from = min(max(args.offsets[0], 0), args.tokens), to = min(args.offsets[args.sequences], args.tokens);
+  for (int row = from + static_cast<int>(blockIdx.x); row < to; row += gridDim.x) {
+    const size_t at = static_cast<size_t>(row) * args.heads;
+    for (int i = threadIdx.x; i < args.heads * (kHeadDim / 8); i += kThreads) {
+      reinterpret_cast<uint4*>(args.out + at * kHeadDim)[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (args.lse == nullptr) continue;
+    for (int i = threadIdx.x; i < args.heads; i += kThreads) args.lse[at + i] = -INFINITY;
+  }
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                    const __grid_constant__ CUtensorMap v_map, const PrefillArgs args, bool two_heads) {
@@ -534,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tcgen05_fence_after();
   const uint32_t tmem = c->tmem;
   if (c->stopped) {
+    clear_results(args);
   } else if (warp < kSoftmaxWarps) {
     more_registers<kSoftmaxRegisters>();
     softmax_role(args, tmem, c);

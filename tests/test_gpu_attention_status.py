@@ -68,3 +68,121 @@ def test_what_an_append_finds_wrong_keeps_the_books_as_they_are(attention):
         assert torch.equal(a, b)
     cache.free(_int([1]))
     assert cache.sync_status() == 0 and cache.lengths.tolist() == [100, 0, 30]
+
+
+def _alone(script):
+    """Runs a script in a process of its own: nothing has called the operators before."""
+    head = ("import importlib, sys, torch\n"
+            "sys.path.insert(0, %r)\n"
+            "import __graft_entry__ as entry\n"
+            "package = entry.load_package()\n"
+            "attention = importlib.import_module('nemotron_inference_b200.attention')\n"
+            "def rows(seed, n, heads):\n"
+            "    g = torch.Generator(device='cuda').manual_seed(seed)\n"
+            "    return torch.randn((n, heads, 128), generator=g, device='cuda').to(torch.bfloat16)\n"
+            "q, k, v = rows(1, 40, 4), rows(2, 40, 2), rows(3, 40, 2)\n"
+            "offsets = torch.tensor([0, 30, 40], dtype=torch.int32, device='cuda')\n" % ROOT)
+    done = subprocess.run([sys.executable, "-c", head + script], capture_output=True, text=True, timeout=300,
+                          cwd=ROOT)
+    assert done.returncode == 0, done.stdout[-2000:] + done.stderr[-2000:]
+
+
+def test_prompts_on_a_stream_that_is_ahead_of_the_first_call():
+    # the first call stands behind other work of its stream; memory that it takes held something before
+    _alone("""
+outs = [torch.full((40, 4, 128), 7.0, dtype=torch.bfloat16, device='cuda') for _ in range(2)]
+mine = torch.zeros(1, dtype=torch.int32, device='cuda')
+# (a first launch loads the kernel, which would wait for the device; it is given a word of its own)
+attention._lib().nmoe_attention_prefill(0, q.data_ptr(), 512, k.data_ptr(), 256, v.data_ptr(), 256, 40, 4, 2,
+                                        offsets.data_ptr(), 2, 0.1, outs[0].data_ptr(), None, mine.data_ptr())
+a, b = torch.cuda.Stream(), torch.cuda.Stream()
+torch.cuda.synchronize()
+with torch.cuda.stream(a):
+    used = [torch.full((1 << 18,), 7, dtype=torch.int32, device='cuda') for _ in range(4)]
+    used += [torch.full((1,), 7, dtype=torch.int32, device='cuda') for _ in range(200)]
+    torch.cuda.synchronize()
+    del used
+    torch.cuda._sleep(300000000)
+    attention.attention_prefill(q, k, v, offsets, out=outs[0])
+with torch.cuda.stream(b):
+    attention.attention_prefill(q, k, v, offsets, out=outs[1])
+torch.cuda.synchronize()
+want = attention.attention_prefill(q, k, v, offsets)
+assert attention.prefill_sync_status() == 0
+assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+""")
+
+
+def test_a_first_call_in_a_recording_is_refused():
+    _alone("""
+def recorded(call):
+    graph, refused = torch.cuda.CUDAGraph(), False
+    with torch.cuda.graph(graph):
+        keep = torch.zeros(8, device='cuda')
+        try:
+            call()
+        except RuntimeError as error:
+            refused = 'record' in str(error)
+    torch.cuda.synchronize()
+    return graph, not refused
+out = torch.zeros_like(q)
+assert not recorded(lambda: attention.attention_prefill(q, k, v, offsets, out=out))[1]
+assert not recorded(lambda: attention.KvCache.allocate(1, 4, 2, 2, 2))[1]
+want = attention.attention_prefill(q, k, v, offsets)
+graph, done = recorded(lambda: attention.attention_prefill(q, k, v, offsets, out=out))
+assert done
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, want) and attention.prefill_sync_status() == 0
+""")
+
+
+def test_a_cache_makes_the_word_of_prompts_as_well():
+    # (whoever records a step has its cache before)
+    _alone("""
+cache = attention.KvCache.allocate(1, 4, 2, 2, 2)
+out = torch.zeros_like(q)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    attention.attention_prefill(q, k, v, offsets, out=out)
+graph.replay()
+assert attention.prefill_sync_status() == 0
+assert torch.equal(out, attention.attention_prefill(q, k, v, offsets))
+""")
+
+
+def test_two_threads_make_one_word():
+    _alone("""
+import threading, time
+zeros, made = torch.zeros, []
+def slow(*args, **kwargs):
+    made.append(args)
+    time.sleep(0.2)
+    return zeros(*args, **kwargs)
+torch.zeros = slow
+def call():
+    attention.attention_prefill(q, k, v, offsets, out=torch.empty_like(q))
+threads = [threading.Thread(target=call) for _ in range(4)]
+for t in threads: t.start()
+for t in threads: t.join()
+assert len(made) == 1, made
+""")
+
+
+def test_a_word_of_the_callers_own(attention):
+    q, k, v = (_normal(30 + i, 200, h, D).to(torch.bfloat16) for i, h in enumerate((4, 2, 2)))
+    offsets = _offsets([120, 80])
+    want, sums = attention.attention_prefill(q, k, v, offsets, return_lse=True)
+    mine = _int([1])  # as a wait that ran out leaves it
+    out, lse = attention.attention_prefill(q, k, v, offsets, return_lse=True, error=mine,
+                                           out=torch.full_like(q, 7.0))
+    # nothing is computed, and nothing is handed out that nobody wrote
+    assert not bool(out.any()) and bool((lse == -float("inf")).all())
+    assert torch.equal(attention.attention_prefill(q, k, v, offsets), want)  # others go on
+    assert attention.prefill_sync_status() == 0
+    assert attention.prefill_sync_status(mine) == 4 and int(mine) == 0
+    out, lse = attention.attention_prefill(q, k, v, offsets, return_lse=True, error=mine)
+    assert torch.equal(out, want) and torch.equal(lse, sums) and attention.prefill_sync_status(mine) == 0
+    for bad in (torch.zeros(1, device="cuda"), _int([0, 0]), torch.zeros(1, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            attention.attention_prefill(q, k, v, offsets, error=bad)
