@@ -519,10 +519,11 @@ NMOE_API nmoe_status nmoe_route_tokens_noalloc(
  * nmoe_kv_sync_status returns and clears it, and until then nmoe_kv_extend, _fork,
  * _free and _compact change nothing.  Where one of these found it (a list entry out
  * of range or named twice, too few pages), nmoe_kv_append does nothing either, so
- * that rows without a place are not written over others.  An entry or a page out
- * of range that an append, attention or a copy of pages comes upon is that entry's
- * or page's alone: all others of the call, and of such calls behind it, are done
- * all the same.  (That no sequence is named twice is not checked by these.)
+ * that rows without a place are not written over others, and nmoe_attention_cached
+ * writes zeros.  An entry or a page out of range that an append, attention or a
+ * copy of pages comes upon is that entry's or page's alone: all others of the call,
+ * and of such calls behind it, are done all the same.  (That no sequence is named
+ * twice is not checked by these.)
  */
 typedef struct nmoe_kv_cache {
   int32_t layers;
@@ -583,7 +584,8 @@ NMOE_API nmoe_status nmoe_kv_sync_status(const nmoe_kv_cache* cache, void* strea
 /* Attention of new rows over the cache: row j of an entry with c rows stands at
  * position length - c + j of its sequence and sees every token up to itself
  * (which nmoe_kv_append has written).  out [rows][heads][128]:
- * softmax(scale * q k^T) v, sums in FP32. */
+ * softmax(scale * q k^T) v, sums in FP32.  The rows of an entry that names what is
+ * not there become zeros; rows of no entry stay as they are. */
 NMOE_API nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* stream, int32_t layer,
                                            const void* q, int64_t q_stride, int32_t heads,
                                            const int32_t* sequences, const int32_t* offsets,

@@ -79,6 +79,7 @@ struct WorkControl {
   int share, pieces;  // of a join
   uint32_t tmem;
   int64_t before[S::kThreads / 32];
+  int stopped;        // an error was pending before this call
   Shares shares;      // of all tiles
   BatchEntry entry;   // the entry in which this block's begin,
   int found, found_before;  // which it is, and the tiles of those before it
@@ -209,18 +210,32 @@ struct EntryTiles {
   }
 };
 
+// Rows that get no results become zeros, each block's share of them by one or all threads.
+static __device__ __noinline__ void clear_rows(__nv_bfloat16* out, int heads, int from, int to, int thread, int threads) {
+  const int64_t of_row = static_cast<int64_t>(heads) * (kHeadDim / 8);
+  for (int64_t row = from + static_cast<int64_t>(blockIdx.x); row < to; row += gridDim.x) {
+    for (int64_t i = thread; i < of_row; i += threads) reinterpret_cast<uint4*>(out)[row * of_row + i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // All threads: the number of tiles, and the entry in which this block's begin.
 template <typename S>
 __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
   const int n = args.batch.count, each = (n + S::kThreads - 1) / S::kThreads;
   const int begin = min(n, static_cast<int>(threadIdx.x) * each), end = min(n, begin + each);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // (one thread's word: a wait that runs out in another block of this launch writes it)
+  if (threadIdx.x == 0) c->stopped = *args.cache.error;
   int64_t mine = 0;
   BatchEntry e;
 #pragma unroll 1
   for (int i = begin; i < end; ++i) {
     e = batch_entry(args.cache, args.batch, i);
-    if (!e.valid && blockIdx.x == 0) report_cache_error(args.cache.raised, kCacheBadSequence);
+    if (!e.valid) {
+      if (blockIdx.x == 0) report_cache_error(args.cache.raised, kCacheBadSequence);
+      const int from = args.batch.offsets[i], to = args.batch.offsets[i + 1];
+      if (from >= 0 && to <= args.batch.rows) clear_rows(args.out, args.heads, from, to, 0, 1);
+    }
     mine += EntryTiles<S>(args, e).all;
   }
   int64_t upto = mine;
@@ -239,9 +254,11 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
   }
   // (more than 2^31 tiles are some 70 TB of codes to be read; with fewer tiles than blocks, the first blocks have
   // one each)
-  if (total > INT32_MAX) {
-    if (threadIdx.x == 0) report_cache_error(args.cache.raised, kCacheBadSequence);
+  if (total > INT32_MAX && threadIdx.x == 0) report_cache_error(args.cache.raised, kCacheBadSequence);
+  if (total > INT32_MAX || c->stopped != 0) {
     total = 0;
+    clear_rows(args.out, args.heads, max(args.batch.offsets[0], 0), min(args.batch.offsets[n], args.batch.rows), threadIdx.x,
+               S::kThreads);
   }
   Shares shares;
   shares.total = static_cast<int>(total);

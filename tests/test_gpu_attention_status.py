@@ -186,3 +186,51 @@ def test_a_word_of_the_callers_own(attention):
     for bad in (torch.zeros(1, device="cuda"), _int([0, 0]), torch.zeros(1, dtype=torch.int32)):
         with pytest.raises(ValueError):
             attention.attention_prefill(q, k, v, offsets, error=bad)
+
+
+@pytest.mark.parametrize("heads", [4, 64])
+def test_attention_does_nothing_after_books_that_failed(attention, heads):
+    cache = _filled(attention, [100, 50], 2, 32, seed=9, layers=1)
+    q = _normal(10, 6, heads, D).to(torch.bfloat16)
+    batch = (_int([0, 1]), _offsets([4, 2]))
+    want = cache.attend(0, q, *batch)
+    cache.extend(_int([0]), _offsets([32 * 40]), rows=32 * 40)  # more than there are pages
+    out = cache.attend(0, q, *batch, out=torch.full_like(q, 7.0))
+    assert not bool(out.any())  # (of rows that have no place, no plausible results)
+    assert cache.sync_status() == 6
+    assert torch.equal(cache.attend(0, q, *batch), want) and cache.sync_status() == 0
+
+
+@pytest.mark.parametrize("heads", [4, 64])
+def test_attention_beside_a_bad_entry(attention, heads):
+    cache = _filled(attention, [100, 5000, 50, 2], 2, 32, seed=9, layers=1)
+    counts = [4, 3, 5, 2]
+    q = _normal(10, sum(counts), heads, D).to(torch.bfloat16)
+    want = cache.attend(0, q, _int([0, 1, 2, 3]), _offsets(counts))
+    for place in range(4):
+        sequences = [0, 1, 2, 3]
+        sequences[place] = (-1, 4, 10 ** 9, -5)[place]
+        got = cache.attend(0, q, _int(sequences), _offsets(counts), out=torch.full_like(q, 7.0))
+        assert cache.sync_status() == 1
+        rows = slice(sum(counts[:place]), sum(counts[:place + 1]))
+        assert not bool(got[rows].any())
+        got[rows] = want[rows]
+        # (with other tiles in the batch a sequence may be cut elsewhere: the last bit of a sum)
+        assert torch.allclose(got.float(), want.float(), rtol=2 ** -7, atol=2 ** -7)
+
+
+def test_what_a_call_that_gave_up_left_is_cleared(attention):
+    # as blocks leave it that stopped in the middle of a join: counters that are not zero
+    cache = _filled(attention, [6000], 1, 64, seed=9, layers=1)
+    q = _normal(10, 1, 8, D).to(torch.bfloat16)
+    batch = (_int([0]), _offsets([1]))
+    want = cache.attend(0, q, *batch)
+    words = cache._workspace.view(torch.int32)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    counters = words[-(4096 // 4 + 128 * (D + 2) * 2 * sms):][:1024]  # (in front of the pieces)
+    assert not bool(counters.any())
+    counters.fill_(3)
+    words[0] = 1
+    assert not bool(cache.attend(0, q, *batch).any())
+    assert cache.sync_status() == 4 and not bool(counters.any())
+    assert torch.equal(cache.attend(0, q, *batch), want) and cache.sync_status() == 0
