@@ -127,6 +127,11 @@ def _zeros(elements: int, dtype: torch.dtype, device: torch.device, what: str) -
     return made
 
 
+def new_error_word(device: torch.device) -> torch.Tensor:
+    """A word for `attention_prefill`."""
+    return _zeros(1, torch.int32, device, "the word of attention_prefill")
+
+
 _error_words: Dict[int, torch.Tensor] = {}
 _error_words_lock = threading.Lock()
 
@@ -138,7 +143,7 @@ def _error_word(device: torch.device) -> torch.Tensor:
         with _error_words_lock:
             error = _error_words.get(device.index)
             if error is None:
-                error = _error_words[device.index] = _zeros(1, torch.int32, device, "the word of attention_prefill")
+                error = _error_words[device.index] = new_error_word(device)
     return error
 
 
@@ -151,7 +156,7 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets
     for, the FP32 logarithms [rows, heads] of the rows' sums of exponentials.  `scale` is
     1 / sqrt(128) unless given.
 
-    `error`: an int32 word on the device, zero at first, in which a call whose waits run out leaves
+    `error`: an int32 word on the device, zero at first (`new_error_word`), in which a call whose waits run out leaves
     a status; calls compute nothing while it holds one (`prefill_sync_status`).  Without it all calls
     on a device have one word together: streams or models that should not stop each other are
     given words of their own."""

@@ -13,6 +13,9 @@ attention, the projection back and the residual.  The projections are plain bf16
     batch.begin()
     stack.run(x, out)
     batch = TokenBatch(cache, sequences, one_each, len(sequences))     # ... a token at a time
+
+`stack.sync_status()` says what a pass could not do: a batch for which there were too few pages leaves
+the cache and its lengths as they were, and its results are of no use.
 """
 from __future__ import annotations
 
@@ -22,7 +25,7 @@ from typing import Optional
 import torch
 
 from . import rmsnorm
-from .attention import HEAD_DIM, KvCache, attention_prefill
+from .attention import HEAD_DIM, KvCache, attention_prefill, new_error_word, prefill_sync_status
 
 
 @dataclass
@@ -59,6 +62,13 @@ class AttentionLayer:
                              "128], norm [hidden], with the cache's kv_heads")
         self.weights, self.cache, self.layer = weights, cache, layer
         self.batch: Optional[TokenBatch] = None
+        self.error = new_error_word(cache.device)  # of this layer's prompts
+
+    def sync_status(self) -> int:
+        """Waits for the current stream; what this layer, or its cache for any layer, could not do, and
+        clears it (`MoeLayerStack.sync_status` asks every layer)."""
+        of_cache, of_prompts = self.cache.sync_status(), prefill_sync_status(self.error)
+        return of_cache or of_prompts
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor) -> None:
         """x, out: [rows, hidden] FP32 or bf16, the rows of `batch`."""
@@ -70,7 +80,7 @@ class AttentionLayer:
         q, k, v = qkv.split((self.heads, cache.kv_heads, cache.kv_heads), dim=1)
         cache.append(self.layer, k, v, batch.sequences, batch.offsets)
         if batch.prompts:
-            attended = attention_prefill(q, k, v, batch.offsets)
+            attended = attention_prefill(q, k, v, batch.offsets, error=self.error)
         else:
             attended = cache.attend(self.layer, q, batch.sequences, batch.offsets)
         torch.add(x, attended.flatten(1) @ w.out.t(), out=out)

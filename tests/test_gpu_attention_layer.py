@@ -131,3 +131,43 @@ def test_attention_layer_refusals(modules):
     layer.batch = layers.TokenBatch(cache, _int([0]), _int([0, 1]), 1)
     with pytest.raises(ValueError):
         layer(x, torch.empty_like(x))  # another one's rows
+
+
+def _layer(modules, cache):
+    attention, layers, stacks = modules
+    layer = layers.AttentionLayer(_weights(layers, 1), cache, 0)
+    return layer, stacks.MoeLayerStack([layer], HIDDEN, 64)
+
+
+def _batch(modules, layer, sequences, counts, prompts=False):
+    offsets = [0]
+    for c in counts:
+        offsets.append(offsets[-1] + c)
+    layer.batch = modules[1].TokenBatch(layer.cache, _int(sequences), _int(offsets), offsets[-1], prompts)
+    layer.batch.begin()
+    x = torch.randn((offsets[-1], HIDDEN), device="cuda")
+    return x, torch.empty_like(x)
+
+
+def test_a_stack_reports_what_its_cache_could_not_do(modules):
+    attention = modules[0]
+    cache = attention.KvCache.allocate(1, 4, KV_HEADS, 2, 4, page_tokens=16)
+    layer, stack = _layer(modules, cache)
+    stack.run(*_batch(modules, layer, [0], [40], prompts=True))
+    assert stack.sync_status() == 0
+    x, out = _batch(modules, layer, [0, 1], [1, 30])  # two more pages, of which there is one
+    stack.run(x, out)
+    assert stack.sync_status() == 6 and cache.lengths.tolist() == [40, 0]
+    assert torch.equal(out, x)  # (no attended rows were added)
+    stack.run(*_batch(modules, layer, [0], [1]))
+    assert stack.sync_status() == 0 and cache.lengths.tolist() == [41, 0]
+
+
+def test_a_stack_reports_a_wait_of_its_prompts_that_ran_out(modules):
+    attention = modules[0]
+    cache = attention.KvCache.allocate(1, 8, KV_HEADS, 2, 4, page_tokens=16)
+    layer, stack = _layer(modules, cache)
+    layer.error.fill_(1)  # as the kernel leaves it
+    stack.run(*_batch(modules, layer, [0], [20], prompts=True))
+    assert attention.prefill_sync_status() == 0  # (another one's)
+    assert stack.sync_status() == 4 and stack.sync_status() == 0
