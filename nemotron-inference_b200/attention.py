@@ -33,6 +33,7 @@ from . import NMOE_OK, NmoeError, _check, _stream, load_library
 
 HEAD_DIM = 128
 DEFAULT_SCALE = HEAD_DIM ** -0.5
+_BAD_SEQUENCE = 17  # kCacheBadSequence of csrc/attention.h
 
 
 class _KvCache(ctypes.Structure):
@@ -237,6 +238,7 @@ class KvCache:
         if needed == 0:
             raise NmoeError(1, "KvCache", "a size is zero or too large")
         self._workspace = _zeros(needed, torch.uint8, device, "a cache's workspace")
+        self._error = self._workspace[:4].view(torch.int32)  # what the books go by
         self._c.workspace, self._c.workspace_bytes = self._workspace.data_ptr(), needed
         self._ref = ctypes.byref(self._c)
         _error_word(device)  # (what records a step with a cache may begin with prompts)
@@ -273,6 +275,14 @@ class KvCache:
         stream = self._batch(sequences, offsets)
         _check(_lib().nmoe_kv_extend(self._ref, stream, sequences.data_ptr(), offsets.data_ptr(),
                                      sequences.numel(), rows), "nmoe_kv_extend")
+
+    def require_empty(self, sequences: torch.Tensor, offsets: torch.Tensor) -> None:
+        """NMOE_ERR_INVALID_ARGUMENT from `sync_status`, and books that change no more until then, if
+        one of the sequences that get rows holds tokens already."""
+        self._batch(sequences, offsets)
+        held = self.lengths.index_select(0, sequences.clamp(0, self.lengths.shape[0] - 1))
+        wrong = ((held != 0) & (offsets[1:] != offsets[:-1])).any()
+        self._error.masked_fill_(wrong & (self._error == 0), _BAD_SEQUENCE)
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, sequences: torch.Tensor,
                offsets: torch.Tensor) -> None:

@@ -32,7 +32,8 @@ from .attention import HEAD_DIM, KvCache, attention_prefill, new_error_word, pre
 class TokenBatch:
     """What a pass through the stack works on: `rows` new tokens, those of sequence sequences[i] in
     rows [offsets[i], offsets[i + 1]).  `prompts`: they are whole prompts, of sequences that held
-    nothing before."""
+    nothing before (where one did, the cache stays as it was and its status is
+    NMOE_ERR_INVALID_ARGUMENT: such rows are attended with `prompts` off)."""
     cache: KvCache
     sequences: torch.Tensor
     offsets: torch.Tensor
@@ -41,6 +42,8 @@ class TokenBatch:
 
     def begin(self) -> None:
         """Makes room for the new tokens, once for all layers."""
+        if self.prompts:
+            self.cache.require_empty(self.sequences, self.offsets)
         self.cache.extend(self.sequences, self.offsets, self.rows)
 
 

@@ -171,3 +171,21 @@ def test_a_stack_reports_a_wait_of_its_prompts_that_ran_out(modules):
     stack.run(*_batch(modules, layer, [0], [20], prompts=True))
     assert attention.prefill_sync_status() == 0  # (another one's)
     assert stack.sync_status() == 4 and stack.sync_status() == 0
+
+
+def test_whole_prompts_of_sequences_that_hold_tokens_are_refused(modules):
+    attention = modules[0]
+    cache = attention.KvCache.allocate(1, 16, KV_HEADS, 4, 4, page_tokens=16)
+    layer, stack = _layer(modules, cache)
+    stack.run(*_batch(modules, layer, [0, 2], [20, 5], prompts=True))
+    assert stack.sync_status() == 0
+    codes = cache.codes.view(torch.uint8).clone()
+    for sequences, counts in (([1, 0], [3, 4]), ([2], [1]), ([0, 1], [1, 0])):
+        stack.run(*_batch(modules, layer, sequences, counts, prompts=True))
+        assert stack.sync_status() == 1
+        assert cache.lengths.tolist() == [20, 0, 5, 0] and torch.equal(cache.codes.view(torch.uint8), codes)
+    # no rows for it: nothing of it is left out; a list that names what is not there is the books' to refuse
+    stack.run(*_batch(modules, layer, [0, 1], [0, 7], prompts=True))
+    assert stack.sync_status() == 0 and cache.lengths.tolist() == [20, 7, 5, 0]
+    stack.run(*_batch(modules, layer, [9, -1], [2, 3], prompts=True))
+    assert stack.sync_status() == 1 and cache.lengths.tolist() == [20, 7, 5, 0]
