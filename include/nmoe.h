@@ -591,7 +591,8 @@ NMOE_API nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* str
                                            const int32_t* sequences, const int32_t* offsets,
                                            int32_t count, int64_t rows, float scale, void* out);
 /* Causal attention over `count` whole prompts packed one behind the other, prompt
- * i in rows [offsets[i], offsets[i+1]) (device, rising from 0 to `tokens`).
+ * i in rows [offsets[i], offsets[i+1]) (device, rising within 0 to `tokens`; rows of
+ * no prompt stay as they are).
  * out [tokens][heads][128]; lse [tokens][heads], nullable: the logarithms of
  * the rows' sums of exponentials; error: a device word, zero at first, for
  * nmoe_attention_sync_status.  Until it has returned what a call left there,

@@ -154,13 +154,13 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets
     """Causal attention over whole prompts packed one behind the other: prompt i is the rows
     [offsets[i], offsets[i + 1]), and each of its rows sees those up to itself.  Query head h
     attends key head h // (heads // kv_heads).  Returns [rows, heads, 128] bf16 and, if asked
-    for, the FP32 logarithms [rows, heads] of the rows' sums of exponentials.  `scale` is
-    1 / sqrt(128) unless given.
+    for, the FP32 logarithms [rows, heads] of the rows' sums of exponentials.  Rows of no prompt
+    are as `out` had them, undefined without it.  `scale` is 1 / sqrt(128) unless given.
 
-    `error`: an int32 word on the device, zero at first (`new_error_word`), in which a call whose waits run out leaves
-    a status; calls compute nothing while it holds one (`prefill_sync_status`).  Without it all calls
-    on a device have one word together: streams or models that should not stop each other are
-    given words of their own."""
+    `error`: an int32 word on the device, zero at first (`new_error_word`), in which a call whose
+    waits run out leaves a status; calls compute nothing while it holds one
+    (`prefill_sync_status`).  Without it all calls on a device have one word together: streams or
+    models that should not stop each other are given words of their own."""
     device = q.device
     stream = _stream_of(device, "q")
     rows, heads, q_stride = _row_layout(q, "q", device)
@@ -168,9 +168,9 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets
     v_rows, v_heads, v_stride = _row_layout(v, "v", device)
     _require_list(offsets, "offsets", device)
     prompts = offsets.shape[0] - 1
-    if k_rows != rows or v_rows != rows or v_heads != kv_heads or heads % kv_heads or prompts < 0:
+    if k_rows != rows or v_rows != rows or v_heads != kv_heads or heads % kv_heads or prompts < (rows > 0):
         raise NmoeError(1, "attention_prefill", "k and v need q's rows and a divisor of its heads, "
-                                                "offsets one entry more than there are prompts")
+                                                "offsets one entry more than there are prompts, rows a prompt")
     out = _output(out, q)
     lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
     if error is None:
@@ -299,11 +299,12 @@ class KvCache:
     def attend(self, layer: int, q: torch.Tensor, sequences: torch.Tensor, offsets: torch.Tensor,
                scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of new rows, the last tokens of their sequences: row j of c sees every token
-        up to position length - c + j.  Returns [rows, heads, 128] bf16."""
+        up to position length - c + j.  Returns [rows, heads, 128] bf16; rows of no entry are as `out`
+        had them, undefined without it."""
         stream = self._batch(sequences, offsets)
         rows, heads, q_stride = _row_layout(q, "q", self.device)
-        if heads % self.kv_heads:
-            raise NmoeError(1, "KvCache.attend", "heads must be a multiple of kv_heads")
+        if heads % self.kv_heads or (rows and sequences.shape[0] == 0):
+            raise NmoeError(1, "KvCache.attend", "heads must be a multiple of kv_heads, rows need a sequence")
         out = _output(out, q)
         _check(_lib().nmoe_attention_cached(
             self._ref, stream, layer, q.data_ptr(), q_stride, heads, sequences.data_ptr(),

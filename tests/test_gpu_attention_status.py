@@ -234,3 +234,14 @@ def test_what_a_call_that_gave_up_left_is_cleared(attention):
     assert not bool(cache.attend(0, q, *batch).any())
     assert cache.sync_status() == 4 and not bool(counters.any())
     assert torch.equal(cache.attend(0, q, *batch), want) and cache.sync_status() == 0
+
+
+def test_rows_without_a_list_are_refused(attention, package):
+    cache = attention.KvCache.allocate(1, 10, 2, 3, 4, 16)
+    q = torch.zeros((3, 4, D), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(package.NmoeError):
+        cache.attend(0, q, _int([]), _int([0]))
+    with pytest.raises(package.NmoeError):
+        attention.attention_prefill(q, q[:, :2], q[:, :2], _int([0]))
+    assert cache.attend(0, q[:0], _int([]), _int([0])).shape == (0, 4, D)
+    assert attention.attention_prefill(q[:0], q[:0, :2], q[:0, :2], _int([0])).shape == (0, 4, D)
