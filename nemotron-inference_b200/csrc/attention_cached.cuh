@@ -585,7 +585,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
           higher = fmaxf(higher, top);
           const float keep = top > -INFINITY ? exp2_approx(top - higher) : 0.0f;
           scale = reference > -INFINITY ? exp2_approx(reference - higher) : 0.0f;
-          weight = scale != 0.0f ? weight * scale : 0.0f;
+          weight *= scale;  // (of a piece far below the others 0, or what is no number)
           top = higher;
           sum *= keep;
 #pragma unroll
@@ -595,7 +595,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
         for (int p = 0; p < kAtOnce; ++p) {
           const float f = __shfl_sync(0xffffffffu, scale, leader + ((first + p) & (kLanes - 1)));
           const float w = __shfl_sync(0xffffffffu, weight, leader + ((first + p) & (kLanes - 1)));
-          if (first + p >= count || f == 0.0f) continue;  // (f is 0 behind the last piece)
+          if (start + first + p >= to) continue;
           sum += w;
 #pragma unroll
           for (int i = 0; i < kVectors; ++i) {

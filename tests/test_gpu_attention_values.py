@@ -1,0 +1,44 @@
+"""GPU tests of attention at the ends of the numbers: keys and values that are none, scores beyond
+FP32, powers and queries far apart, in both kernels over the cache (up to 16 rows of queries to a
+key head, and more)."""
+import importlib
+import math
+
+import pytest
+import torch
+
+from test_gpu_attention import _check_attend, _filled, _int, _normal, _offsets, _rows, _values
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+
+
+@pytest.fixture(scope="module")
+def attention(package):
+    return importlib.import_module("nemotron_inference_b200.attention")
+
+
+@pytest.mark.parametrize("heads", [4, 32])
+@pytest.mark.parametrize("half", [0, 1])
+def test_no_number_far_below_the_largest_score(attention, heads, half):
+    # the sequence is cut between blocks; the key or value stands in a first piece whose weights are all 2^-500
+    # of those of the pieces that are joined with it: the formula multiplies by it all the same
+    n = 20000
+    cache = _filled(attention, [n, 30], 1, 64, seed=31, layers=1)
+    pages = cache.block_table[0, :-(-n // 64)].long()
+    codes = cache.codes.view(torch.uint8)
+    low, high = (int(torch.tensor(x).to(torch.float8_e4m3fn).view(torch.uint8)) for x in (-16.0, 16.0))
+    codes[0, pages, 0] = high
+    codes[0, pages[:4], 0] = low
+    cache.exponents[0, pages] = 0
+    q = torch.ones((2, heads, D), dtype=torch.bfloat16, device="cuda")
+    batch = (_int([0, 1]), _offsets([1, 1]))
+    clean = cache.attend(0, q, *batch, scale=0.1)
+    assert bool(clean.isfinite().all())
+    codes[0, pages[1], half, 0, 40, 9] = 0x7F
+    got = cache.attend(0, q, *batch, scale=0.1)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[0, :, slice(None) if half == 0 else 9] = True
+    assert torch.equal(got[~hit], clean[~hit]) and bool(got[hit].float().isnan().all())
+    assert cache.sync_status() == 0
