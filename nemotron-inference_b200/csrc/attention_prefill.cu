@@ -377,7 +377,7 @@ __device__ void softmax_role(const PrefillArgs& args, uint32_t tmem, Control* c)
       } else if (__any_sync(0xffffffffu, (highest - top) * factor > kRescale)) {
         // (S of this tile is complete, so O of those before it is)
         const float higher = fmaxf(highest, top);
-        const float keep = exp2_approx((top - higher) * factor);
+        const float keep = top > -INFINITY ? exp2_approx((top - higher) * factor) : 0.0f;  // (or both are -infinity)
         top = higher;
         const uint64_t keep2 = pack2(keep, keep);
         sum2 = mul2(sum2, keep2);

@@ -42,3 +42,30 @@ def test_no_number_far_below_the_largest_score(attention, heads, half):
     hit[0, :, slice(None) if half == 0 else 9] = True
     assert torch.equal(got[~hit], clean[~hit]) and bool(got[hit].float().isnan().all())
     assert cache.sync_status() == 0
+
+
+def _lowest(attention, lowest, of_even, check):
+    # keys that are masked by a large negative value in a dimension of its own, which rows of even places
+    # read; those of odd ones read another, and raise their references with the second tile
+    n = 420
+    k, v = (_normal(33 + i, n, 1, D) for i in range(2))
+    q = _normal(35, n, 2, D)
+    q[:, :, :2], k[:, :, :2] = 0, 0
+    k[:256, 0, 0] = lowest
+    k[128:256, 0, 1] = 100.0
+    q[0::2, :, 0] = of_even
+    q[1::2, :, 1] = 10.0
+    q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
+    got, lse = attention.attention_prefill(q, k, v, _offsets([n]), return_lse=True)
+    assert attention.prefill_sync_status() == 0
+    for h in range(2):
+        want, sums, bound = _rows(q[:, h].double(), k[:, 0].double(), v[:, 0].double(), 0, D ** -0.5)
+        error = (got[:, h].double() - want).abs()
+        assert bool((error <= bound)[check].all()), float((error / bound)[check].max())
+        off = (lse[:, h].double() - sums).abs() / sums.abs().clamp(min=64)
+        assert float(off[check].max()) <= 2 ** -17
+
+
+def test_prefill_of_rows_whose_first_scores_are_infinite(attention):
+    # FP32 has no such number: -infinity, and those that a row sees later are finite
+    _lowest(attention, -3.3895e38, 2.0, slice(256, None))
