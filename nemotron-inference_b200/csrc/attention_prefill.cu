@@ -331,6 +331,15 @@ __device__ __forceinline__ void add_bad_values(const PrefillArgs& args, const Wo
   }
 }
 
+// Weights are 2^(s c - round(m c)), one fma each.  What the rounding adds to all of a row's exponents cancels, as
+// long as references that follow one another are told apart by their rounded products, and it stays below 64.  Where
+// |m c| is 2^30 or more (keys that are masked by the type's lowest value), scores that differ at all do so by 2^6
+// orders; c is cut to a power of two there, so that m c is exact.
+__device__ __forceinline__ float factor_for(float top, float factor) {
+  const bool far = fabsf(top * factor) >= 1073741824.0f;
+  return far ? __uint_as_float(__float_as_uint(factor) & 0x7f800000u) : factor;
+}
+
 // Four warps per query tile, a thread per row.
 __device__ void softmax_role(const PrefillArgs& args, uint32_t tmem, Control* c) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -338,7 +347,6 @@ __device__ void softmax_role(const PrefillArgs& args, uint32_t tmem, Control* c)
   const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp, from bit 16
   const uint32_t s_at = tmem + lanes + t * kTile, o_at = tmem + lanes + 2 * kTile + t * kHeadDim;
   const float factor = args.scale * kLog2e;
-  const uint64_t factor2 = pack2(factor, factor);
   uint32_t s_uses = 0, o_uses = 0;
   for (uint32_t items = 0;; ++items) {
     const uint32_t place = items & 1;
@@ -348,7 +356,7 @@ __device__ void softmax_role(const PrefillArgs& args, uint32_t tmem, Control* c)
     __syncwarp();
     if (lane == 0) mbar_arrive(&c->work_empty[place]);
     const int tiles = w.tiles[t];
-    float top = 0.0f;
+    float top = 0.0f, own_factor = factor;
     uint64_t sum2 = 0, by_rounding2 = 0;
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
@@ -374,11 +382,16 @@ __device__ void softmax_role(const PrefillArgs& args, uint32_t tmem, Control* c)
       const float highest = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
       if (j == 0) {
         top = highest;
+        own_factor = factor_for(top, factor);
       } else if (__any_sync(0xffffffffu, (highest - top) * factor > kRescale)) {
         // (S of this tile is complete, so O of those before it is)
         const float higher = fmaxf(highest, top);
-        const float keep = top > -INFINITY ? exp2_approx((top - higher) * factor) : 0.0f;  // (or both are -infinity)
+        const float next_factor = factor_for(higher, factor);
+        const float by = own_factor == next_factor ? __fmul_rn(top, own_factor) - __fmul_rn(higher, own_factor)
+                                                   : (top - higher) * factor;
+        const float keep = top > -INFINITY ? exp2_approx(by) : 0.0f;  // (or both are -infinity)
         top = higher;
+        own_factor = next_factor;
         const uint64_t keep2 = pack2(keep, keep);
         sum2 = mul2(sum2, keep2);
 #pragma unroll 1
@@ -392,8 +405,8 @@ __device__ void softmax_role(const PrefillArgs& args, uint32_t tmem, Control* c)
           tmem_st_x32(o_at + part * 32, o);
         }
       }
-      const float shift = top == -INFINITY ? 0.0f : -top * factor;
-      const uint64_t shift2 = pack2(shift, shift);
+      const float shift = top == -INFINITY ? 0.0f : -__fmul_rn(top, own_factor);
+      const uint64_t shift2 = pack2(shift, shift), factor2 = pack2(own_factor, own_factor);
       uint64_t part2[2] = {0, 0};
 #pragma unroll
       for (int part = 0; part < 4; ++part) {

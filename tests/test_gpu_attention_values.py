@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_attention import _check_attend, _filled, _int, _normal, _offsets, _rows, _values
+from test_gpu_attention import _filled, _int, _normal, _offsets
 
 pytestmark = pytest.mark.gpu
 
@@ -59,9 +59,16 @@ def _lowest(attention, lowest, of_even, check):
     got, lse = attention.attention_prefill(q, k, v, _offsets([n]), return_lse=True)
     assert attention.prefill_sync_status() == 0
     for h in range(2):
-        want, sums, bound = _rows(q[:, h].double(), k[:, 0].double(), v[:, 0].double(), 0, D ** -0.5)
+        scores = (q[:, h].double() @ k[:, 0].double().T) * D ** -0.5
+        scores.masked_fill_(~torch.ones((n, n), dtype=torch.bool, device="cuda").tril(), -math.inf)
+        # (by the maximum: a logarithm of the sum is lost beside a score of 1e30, in 64 bits as well)
+        w = torch.exp(scores - scores.amax(1, keepdim=True))
+        total = w.sum(1, keepdim=True)
+        want, spread = (w @ v[:, 0].double()) / total, (w @ v[:, 0].double().abs()) / total
+        bound = 1.75 * 2 ** -8 * spread + 2 ** -22 * v[:, 0].double().abs().sum(0) / total
         error = (got[:, h].double() - want).abs()
         assert bool((error <= bound)[check].all()), float((error / bound)[check].max())
+        sums = scores.amax(1) + total[:, 0].log()
         off = (lse[:, h].double() - sums).abs() / sums.abs().clamp(min=64)
         assert float(off[check].max()) <= 2 ** -17
 
@@ -69,3 +76,9 @@ def _lowest(attention, lowest, of_even, check):
 def test_prefill_of_rows_whose_first_scores_are_infinite(attention):
     # FP32 has no such number: -infinity, and those that a row sees later are finite
     _lowest(attention, -3.3895e38, 2.0, slice(256, None))
+
+
+@pytest.mark.parametrize("lowest", [-1e4, -1e6, -1e9, -1e12, -1e30, -3.3895e38])
+def test_prefill_of_scores_very_far_below_zero(attention, lowest):
+    # the rows up to 256 see nothing else; between, FP32 holds such a sum's other terms in part
+    _lowest(attention, lowest, 0.5, slice(256 if -1e30 < lowest < -1e4 else 0, None))
