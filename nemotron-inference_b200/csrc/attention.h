@@ -35,9 +35,9 @@ struct PagedCache {
   // attention read it and do nothing then.  `raised`: an entry or a page that appends, attention or copies of pages
   // found wrong and left out; the books read it, too.  None of a launch's blocks reads what others of it write, so
   // a wrong entry changes nothing for the rest of its batch.
-  int* error;
-  int* raised;
+  int* error;        // the first of four words that are read together:
   int* move_count;   // pages for the copy kernel: the first *move_count of the two lists
+  int* raised;
   int* move_source;  // [pages]
   int* move_target;  // [pages]
   int* remap;        // [max(pages, max_sequences)]: where a page went, a child's copy
@@ -64,8 +64,15 @@ __device__ __forceinline__ void report_cache_error(int* error, int code) {
   if (error != nullptr) atomicCAS(error, 0, code);
 }
 
-// What the books go by.
-__device__ __forceinline__ bool error_pending(const PagedCache& c) { return (*c.error | *c.raised) != 0; }
+// The words at c.error, in one load.
+struct CacheWords {
+  int error, move_count, raised, unused;
+  __device__ bool pending() const { return (error | raised) != 0; }  // what the books go by
+};
+__device__ __forceinline__ CacheWords cache_words(const PagedCache& c) {
+  const int4 words = *reinterpret_cast<const int4*>(c.error);
+  return {words.x, words.y, words.z, words.w};
+}
 
 // Entry i of a batch, brought into range: whatever the arrays hold, its rows lie within the batch's
 // and its tokens within the block table.

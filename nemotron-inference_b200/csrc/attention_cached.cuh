@@ -225,7 +225,8 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
   const int begin = min(n, static_cast<int>(threadIdx.x) * each), end = min(n, begin + each);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // (one thread's word: a wait that runs out in another block of this launch writes it)
-  if (threadIdx.x == 0) c->stopped = *args.cache.error;
+  int stopped = 0;
+  if (threadIdx.x == 0) stopped = *args.cache.error;
   int64_t mine = 0;
   BatchEntry e;
 #pragma unroll 1
@@ -245,6 +246,7 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
     if (lane >= step) upto += other;
   }
   if (lane == 31) c->before[warp] = upto;
+  if (threadIdx.x == 0) c->stopped = stopped;
   __syncthreads();
   int64_t total = 0, below = upto - mine;
 #pragma unroll 1
@@ -595,7 +597,7 @@ __device__ void join(const CachedArgs& args, const Split& split, const Segment& 
         for (int p = 0; p < kAtOnce; ++p) {
           const float f = __shfl_sync(0xffffffffu, scale, leader + ((first + p) & (kLanes - 1)));
           const float w = __shfl_sync(0xffffffffu, weight, leader + ((first + p) & (kLanes - 1)));
-          if (start + first + p >= to) continue;
+          if (spread ? start + first + p >= to : first + p >= count) continue;
           sum += w;
 #pragma unroll
           for (int i = 0; i < kVectors; ++i) {

@@ -282,9 +282,9 @@ __global__ void __launch_bounds__(kBookThreads) kv_extend_kernel(PagedCache c, B
   __shared__ BookShared s;
   release_successor();
   wait_for_predecessor();
-  const bool pending = error_pending(c);
+  const CacheWords words = cache_words(c);
   ask_for_lengths(c, b.sequences, b.count);
-  if (pending) return;
+  if (words.pending()) return;
   if (threadIdx.x == 0) s.flag = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < b.count; i += kBookThreads) claim(c, b.sequences[i], s);
@@ -359,9 +359,9 @@ __global__ void __launch_bounds__(kBookThreads)
   __shared__ BookShared s;
   release_successor();
   wait_for_predecessor();
-  const bool pending = error_pending(c);
+  const CacheWords words = cache_words(c);
   ask_for_lengths(c, sequences, count);
-  if (pending) return;
+  if (words.pending()) return;
   if (threadIdx.x == 0) s.flag = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += kBookThreads) claim(c, sequences[i], s);
@@ -390,14 +390,14 @@ __global__ void __launch_bounds__(kBookThreads)
   __shared__ BookShared s;
   release_successor();
   wait_for_predecessor();
+  const CacheWords words = cache_words(c);
+  ask_for_lengths(c, parents, count);
+  ask_for_lengths(c, children, count);
   if (threadIdx.x == 0) {
     s.flag = 0;
     *c.move_count = 0;
   }
-  const bool pending = error_pending(c);
-  ask_for_lengths(c, parents, count);
-  ask_for_lengths(c, children, count);
-  if (pending) return;
+  if (words.pending()) return;
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += kBookThreads) claim(c, children[i], s);
   __syncthreads();
@@ -477,14 +477,14 @@ __global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) 
   __shared__ BookShared s;
   release_successor();
   wait_for_predecessor();
+  const CacheWords words = cache_words(c);
   if (threadIdx.x == 0) *c.move_count = 0;
-  const bool pending = error_pending(c);
   int live = 0;
   for (int page = threadIdx.x; page < c.pages; page += kBookThreads) {
     live += c.references[page] > 0;
     c.remap[page] = page;
   }
-  if (pending) return;
+  if (words.pending()) return;
   int total;
   block_prefix(live, s, total);
   live = total;
@@ -520,14 +520,13 @@ constexpr int kCopyChunk = kCopyThreads * 4;  // of 16 bytes: four loads under w
 // copies in 8 layers, or a few, are spread evenly.  It is launched while the books are kept and waits for them.
 
 __global__ void __launch_bounds__(kCopyThreads)
-    kv_copy_kernel(PagedCache c, const int* sources, const int* targets, const int* count_at,
-                   int count, bool rewrite_table) {
+    kv_copy_kernel(PagedCache c, const int* sources, const int* targets, bool of_books, int count, bool rewrite_table) {
   release_successor();
   wait_for_predecessor();  // (the books)
-  if (count_at != nullptr) {
-    const bool pending = error_pending(c);
-    count = *count_at;
-    if (pending) return;
+  if (of_books) {
+    const CacheWords words = cache_words(c);
+    count = words.move_count;
+    if (words.pending()) return;
   }
   const int heads2 = 2 * c.kv_heads;
   const size_t page_words = static_cast<size_t>(heads2) * c.page_tokens * kHeadDim / 16;
@@ -575,9 +574,9 @@ __global__ void __launch_bounds__(kCopyThreads)
 }
 
 cudaError_t launch_copy(const PagedCache& cache, const int* sources, const int* targets,
-                        const int* count_at, int count, bool rewrite_table, cudaStream_t stream) {
+                        bool of_books, int count, bool rewrite_table, cudaStream_t stream) {
   return launch_kernel(kv_copy_kernel, dim3(device_sms() * 8), kCopyThreads, 0,
-                       LaunchStream(stream, true), cache, sources, targets, count_at,
+                       LaunchStream(stream, true), cache, sources, targets, of_books,
                        count, rewrite_table);
 }
 
@@ -610,7 +609,7 @@ cudaError_t launch_kv_fork(const PagedCache& cache, const int* parents, const in
                            cudaStream_t stream) {
   const cudaError_t err = launch_kernel(kv_fork_kernel, dim3(1), kBookThreads, 0, LaunchStream(stream, true), cache, parents, children, count);
   if (err != cudaSuccess) return err;
-  return launch_copy(cache, cache.move_source, cache.move_target, cache.move_count, 0, false, stream);
+  return launch_copy(cache, cache.move_source, cache.move_target, true, 0, false, stream);
 }
 
 cudaError_t launch_kv_free(const PagedCache& cache, const int* sequences, int count,
@@ -621,12 +620,12 @@ cudaError_t launch_kv_free(const PagedCache& cache, const int* sequences, int co
 cudaError_t launch_kv_compact(const PagedCache& cache, cudaStream_t stream) {
   const cudaError_t err = launch_kernel(kv_compact_kernel, dim3(1), kBookThreads, 0, LaunchStream(stream, true), cache);
   if (err != cudaSuccess) return err;
-  return launch_copy(cache, cache.move_source, cache.move_target, cache.move_count, 0, true, stream);
+  return launch_copy(cache, cache.move_source, cache.move_target, true, 0, true, stream);
 }
 
 cudaError_t launch_kv_copy_pages(const PagedCache& cache, const int* sources, const int* targets,
                                  int count, cudaStream_t stream) {
-  return launch_copy(cache, sources, targets, nullptr, count, false, stream);
+  return launch_copy(cache, sources, targets, false, count, false, stream);
 }
 
 }  // namespace nmoe
