@@ -565,7 +565,8 @@ NMOE_API nmoe_status nmoe_kv_append(const nmoe_kv_cache* cache, void* stream, in
 /* children[i] becomes a copy of parents[i]: what it held is given up, full
  * pages are shared (references), a partly filled last page is copied in every
  * layer to the lowest free one.  Children are distinct and no parents.
- * NMOE_ERR_CAPACITY leaves everything as it was. */
+ * NMOE_ERR_CAPACITY leaves everything as it was; an entry of a parent's that is no
+ * page is reported, and the child's as well. */
 NMOE_API nmoe_status nmoe_kv_fork(const nmoe_kv_cache* cache, void* stream, const int32_t* parents,
                                   const int32_t* children, int32_t count);
 /* Gives up the sequences' pages: lengths and table entries become 0, a page

@@ -36,7 +36,7 @@ struct PagedCache {
   // found wrong and left out; the books read it, too.  None of a launch's blocks reads what others of it write, so
   // a wrong entry changes nothing for the rest of its batch.
   int* error;        // the first of four words that are read together:
-  int* move_count;   // pages for the copy kernel: the first *move_count of the two lists
+  int* move_count;   // pages for the copy kernel: the first *move_count of the two lists; -1: the books stay as they are
   int* raised;
   int* move_source;  // [pages]
   int* move_target;  // [pages]

@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kBookThreads)
   ask_for_lengths(c, children, count);
   if (threadIdx.x == 0) {
     s.flag = 0;
-    *c.move_count = 0;
+    *c.move_count = -1;
   }
   if (words.pending()) return;
   __syncthreads();
@@ -454,8 +454,12 @@ __global__ void __launch_bounds__(kBookThreads)
         for (int place = threadIdx.x & 31; place < c.max_pages; place += 32) {
           int page = 0;
           if (place < full) {
-            page = max(page_at(c, parents[i], place), 0);
-            atomicAdd(&c.references[page], 1);
+            page = c.table[static_cast<size_t>(parents[i]) * c.max_pages + place];
+            if (static_cast<unsigned>(page) < static_cast<unsigned>(c.pages)) {
+              atomicAdd(&c.references[page], 1);
+            } else {  // (copied as it stands: it is no page of the child's, either)
+              report_cache_error(c.raised, kCacheBadSequence);
+            }
           } else if (place == full && partial) {
             continue;
           }
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) 
   release_successor();
   wait_for_predecessor();
   const CacheWords words = cache_words(c);
-  if (threadIdx.x == 0) *c.move_count = 0;
+  if (threadIdx.x == 0) *c.move_count = -1;
   int live = 0;
   for (int page = threadIdx.x; page < c.pages; page += kBookThreads) {
     live += c.references[page] > 0;
@@ -524,9 +528,8 @@ __global__ void __launch_bounds__(kCopyThreads)
   release_successor();
   wait_for_predecessor();  // (the books)
   if (of_books) {
-    const CacheWords words = cache_words(c);
-    count = words.move_count;
-    if (words.pending()) return;
+    count = *c.move_count;
+    if (count < 0) return;
   }
   const int heads2 = 2 * c.kv_heads;
   const size_t page_words = static_cast<size_t>(heads2) * c.page_tokens * kHeadDim / 16;

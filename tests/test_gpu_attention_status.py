@@ -245,3 +245,25 @@ def test_rows_without_a_list_are_refused(attention, package):
         attention.attention_prefill(q, q[:, :2], q[:, :2], _int([0]))
     assert cache.attend(0, q[:0], _int([]), _int([0])).shape == (0, 4, D)
     assert attention.attention_prefill(q[:0], q[:0, :2], q[:0, :2], _int([0])).shape == (0, 4, D)
+
+
+def test_a_fork_of_a_page_that_does_not_exist(attention):
+    cache = _filled(attention, [100, 0, 40], 1, 16, seed=3, layers=2)
+    row = cache.block_table[0].tolist()
+    row[2] = cache.block_table[0, 2] = 10 ** 6
+    references = cache.references.tolist()
+    page = references.index(0)
+    cache.fork(_int([0]), _int([1]))
+    assert cache.sync_status() == 1  # and no other page has taken its place
+    assert cache.block_table[0].tolist() == row and cache.lengths.tolist() == [100, 100, 40]
+    for shared in row[:2] + row[3:6]:
+        references[shared] += 1
+    references[page] = 1
+    assert cache.references.tolist() == references
+    assert cache.block_table[1].tolist() == row[:6] + [page, 0]
+    bits = cache.codes.view(torch.uint8)
+    assert torch.equal(bits[:, page], bits[:, row[6]])
+    cache.free(_int([1]))
+    assert cache.sync_status() == 0 and cache.references.tolist()[page] == 0
+    cache.fork(_int([2]), _int([1]))
+    assert cache.sync_status() == 0
