@@ -35,7 +35,7 @@ struct PagedCache {
   // attention read it and do nothing then.  `raised`: an entry or a page that appends, attention or copies of pages
   // found wrong and left out; the books read it, too.  None of a launch's blocks reads what others of it write, so
   // a wrong entry changes nothing for the rest of its batch.
-  int* error;        // the first of four words that are read together:
+  int* error;        // the first of four words that are read together: error, move_count, raised, impatient
   int* move_count;   // pages for the copy kernel: the first *move_count of the two lists; -1: the books stay as they are
   int* raised;
   int* move_source;  // [pages]
@@ -66,7 +66,8 @@ __device__ __forceinline__ void report_cache_error(int* error, int code) {
 
 // The words at c.error, in one load.
 struct CacheWords {
-  int error, move_count, raised, unused;
+  int error, move_count, raised;
+  int impatient;  // tests set it: a block leaves a join at once where pieces are missing
   __device__ bool pending() const { return (error | raised) != 0; }  // what the books go by
 };
 __device__ __forceinline__ CacheWords cache_words(const PagedCache& c) {

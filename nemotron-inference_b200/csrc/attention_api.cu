@@ -29,7 +29,7 @@ struct Layout {
 };
 
 // Header (the words below), the lists of the page kernels, the attention's parts.
-enum HeaderWord { kErrorWord, kMoveCountWord, kRaisedWord, kHeaderWords = 4 };
+enum HeaderWord { kErrorWord, kMoveCountWord, kRaisedWord, kImpatientWord, kHeaderWords };
 
 Layout layout_of(const nmoe_kv_cache& c) {
   const size_t pages = sizeof(int) * static_cast<size_t>(c.pages);

@@ -80,6 +80,7 @@ struct WorkControl {
   uint32_t tmem;
   int64_t before[S::kThreads / 32];
   int stopped;        // an error was pending before this call
+  int patience;       // cycles that a block waits for the pieces of a join
   Shares shares;      // of all tiles
   BatchEntry entry;   // the entry in which this block's begin,
   int found, found_before;  // which it is, and the tiles of those before it
@@ -225,8 +226,8 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
   const int begin = min(n, static_cast<int>(threadIdx.x) * each), end = min(n, begin + each);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // (one thread's word: a wait that runs out in another block of this launch writes it)
-  int stopped = 0;
-  if (threadIdx.x == 0) stopped = *args.cache.error;
+  CacheWords words{};
+  if (threadIdx.x == 0) words = cache_words(args.cache);
   int64_t mine = 0;
   BatchEntry e;
 #pragma unroll 1
@@ -246,7 +247,10 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
     if (lane >= step) upto += other;
   }
   if (lane == 31) c->before[warp] = upto;
-  if (threadIdx.x == 0) c->stopped = stopped;
+  if (threadIdx.x == 0) {
+    c->stopped = words.error;
+    c->patience = words.impatient ? 0 : kJoinPatience;
+  }
   __syncthreads();
   int64_t total = 0, below = upto - mine;
 #pragma unroll 1
@@ -644,10 +648,10 @@ __device__ __forceinline__ int load_acquire(const int* p) {
 
 // One thread: waits a while for the pieces that are missing.  The counter's word when all are there, or -1: this block
 // has left.
-__device__ __forceinline__ int wait_for_pieces(JoinCounters* counters, int parts) {
+__device__ __forceinline__ int wait_for_pieces(JoinCounters* counters, int parts, int patience) {
   const long long start = clock64();
   int word = load_acquire(&counters->pieces);
-  while ((word & (kLeft - 1)) < parts && clock64() - start < kJoinPatience) word = load_acquire(&counters->pieces);
+  while ((word & (kLeft - 1)) < parts && clock64() - start < patience) word = load_acquire(&counters->pieces);
   while ((word & (kLeft - 1)) < parts) {  // (it can have changed as often as there are blocks)
     const int seen = atomicCAS(&counters->pieces, word, word + kLeft);
     if (seen == word) return -1;
@@ -662,7 +666,7 @@ __device__ __forceinline__ int wait_for_pieces(JoinCounters* counters, int parts
 template <typename S>
 __device__ void help_join(const CachedArgs& args, const Split& split, const Segment& s, WorkControl<S>* c) {
   JoinCounters* counters = &split.counters[s.lead];
-  if (threadIdx.x == 0) c->pieces = wait_for_pieces(counters, s.parts);
+  if (threadIdx.x == 0) c->pieces = wait_for_pieces(counters, s.parts, c->patience);
   softmax_sync<S>();
   const int word = c->pieces;
   // The last warp counts the block as done; where it joins rows first, the counter's answer is on its way meanwhile.

@@ -267,3 +267,21 @@ def test_a_fork_of_a_page_that_does_not_exist(attention):
     assert cache.sync_status() == 0 and cache.references.tolist()[page] == 0
     cache.fork(_int([2]), _int([1]))
     assert cache.sync_status() == 0
+
+
+@pytest.mark.parametrize("lengths,counts,heads,kv_heads", [
+    ([20000], [1], 8, 1), ([9000, 20011], [3, 5], 8, 1), ([700] * 70, [1] * 70, 8, 1), ([30000, 5, 800], [8, 1, 2], 32, 2),
+    ([2500], [300], 16, 2)])
+def test_joins_that_blocks_leave(attention, lengths, counts, heads, kv_heads):
+    # blocks that find pieces missing go at once, and those that bring the last ones join what is left
+    cache = _filled(attention, lengths, kv_heads, 64, seed=2, layers=1)
+    q = (2 * _normal(11, sum(counts), heads, D)).to(torch.bfloat16)
+    batch = (_int(list(range(len(lengths)))), _offsets(counts))
+    want = cache.attend(0, q, *batch, scale=0.05)
+    impatient = cache._workspace.view(torch.int32)[3]
+    for _ in range(10):
+        impatient.fill_(1)
+        assert torch.equal(cache.attend(0, q, *batch, scale=0.05, out=torch.full_like(q, 7.0)), want)
+        impatient.fill_(0)
+        assert torch.equal(cache.attend(0, q, *batch, scale=0.05, out=torch.full_like(q, 7.0)), want)
+    assert cache.sync_status() == 0
