@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_attention import _filled, _int, _normal, _offsets
+from test_gpu_attention import _check_attend, _filled, _int, _normal, _offsets, _rows, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,85 @@ def test_prefill_of_rows_whose_first_scores_are_infinite(attention):
 def test_prefill_of_scores_very_far_below_zero(attention, lowest):
     # the rows up to 256 see nothing else; between, FP32 holds such a sum's other terms in part
     _lowest(attention, lowest, 0.5, slice(256 if -1e30 < lowest < -1e4 else 0, None))
+
+
+# 32 query heads to a key head: more than 16 rows of queries in every entry
+@pytest.mark.parametrize("heads,kv_heads", [(32, 1), (64, 2)])
+@pytest.mark.parametrize("length", [133, 9000])
+def test_many_rows_keep_what_is_masked_out(attention, heads, kv_heads, length):
+    rows, other, at = 6, 2, length - 3  # row 3 and later ones see the token
+    cache = _filled(attention, [length, 70], kv_heads, 64, seed=5, layers=1)
+    group, head = heads // kv_heads, kv_heads - 1
+    q = _normal(13, rows + other, heads, D).to(torch.bfloat16)
+    batch = (_int([0, 1]), _offsets([rows, other]))
+    clean = cache.attend(0, q, *batch)
+    bits = cache.codes.view(torch.uint8)
+    page = int(cache.block_table[0, at // 64])
+    for half in (0, 1):
+        place = (0, page, half, head, at % 64, 9)
+        before = int(bits[place])
+        bits[place] = 0xFF if half else 0x7F
+        got = cache.attend(0, q, *batch)
+        bits[place] = before
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[3:rows, head * group:(head + 1) * group, 9 if half else slice(None)] = True
+        assert torch.equal(got[~hit], clean[~hit]) and bool(got[hit].float().isnan().all())
+    assert torch.equal(cache.attend(0, q, *batch), clean) and cache.sync_status() == 0
+
+
+@pytest.mark.parametrize("page_tokens", [16, 64])
+@pytest.mark.parametrize("heads,counts", [(32, [3, 1]), (128, [1, 1])])
+def test_many_rows_over_pages_of_very_different_scales(attention, page_tokens, heads, counts):
+    n = 4000
+    cache = _filled(attention, [n, 90], 1, page_tokens, seed=3, layers=1)
+    pages = cache.block_table[0, :-(-n // page_tokens)].long()
+    # values up to 2^64 apart; the largest keys stand where the values are small
+    g = torch.Generator().manual_seed(4)
+    big = torch.rand(pages.numel(), generator=g) < 0.3
+    powers = torch.randint(-32, 33, (pages.numel(),), generator=g)
+    cache.exponents[0, pages, 1, 0] = torch.where(big, -32, powers).to(torch.int8).cuda()
+    cache.exponents[0, pages, 0, 0] = torch.where(big, -5, torch.randint(-32, -6, (pages.numel(),), generator=g)).to(
+        torch.int8).cuda()
+    q = _normal(11, sum(counts), heads, D).to(torch.bfloat16)
+    got = cache.attend(0, q, _int([0, 1]), _offsets(counts))
+    _check_attend(cache, 0, q, [0, 1], counts, got)
+
+
+def _check_many_rows(cache, q, scale, got):
+    """One row of 32 or more heads of sequence 0.  The queries of this kernel are two E4M3 terms with the row's
+    largest element between 2^7 and 2^8, of which the second is rounded to 2^-10 at worst: each element is off by
+    at most 2^-17 of the largest.  That moves a score by delta = scale 2^-17 max|q| sum|k| at most, a weight by a
+    factor e^(+-delta), and the result by 2 delta of the weighted |v| to first order (2.2 here: delta < 0.1).  The
+    rest is as for the others: 1.75 2^-8 of it, and 2^-22 of the largest weight for each token."""
+    k, v = _values(cache, 0, 0)
+    group = q.shape[1] // cache.kv_heads
+    for h in range(q.shape[1]):
+        x = q[0, h].double()
+        want, _, bound = _rows(x[None], k[h // group], v[h // group], k.shape[1] - 1, scale)
+        delta = scale * 2 ** -17 * float(x.abs().max()) * float(k[h // group].abs().sum(1).max())
+        assert delta < 0.1
+        scores = (k[h // group] @ x) * scale
+        spread = torch.softmax(scores, 0) @ v[h // group].abs()
+        error = (got[0, h].double() - want[0]).abs()
+        assert bool((error <= bound[0] + 2.2 * delta * spread).all()), (h, float((error / bound[0]).max()))
+
+
+def test_many_rows_of_queries_of_any_size(attention):
+    # rows whose elements lie many powers of two apart, rows of zeros, rows near bf16's ends, outliers
+    heads = 64
+    cache = _filled(attention, [300, 300], 2, 32, seed=4, layers=1)
+    q = _normal(12, 6, heads, D)
+    q[0] *= torch.exp2(torch.linspace(-30, 0, D, device="cuda"))
+    q[1] = 0
+    q[2] *= 2.0 ** -100
+    q[3] *= 2.0 ** 20
+    q[4, :, 5] = 2.0 ** 9
+    q[5, :, 5] = torch.exp2(torch.arange(heads, device="cuda") / 8.0 + 2)
+    q = q.to(torch.bfloat16)
+    pages = cache.block_table[0, :10].long()
+    for row, scale in ((0, 0.1), (1, 0.1), (2, 0.1), (2, 2.0 ** 97), (3, 2.0 ** -23), (4, 0.01), (5, 0.01)):
+        if row >= 4:  # (the outlier meets keys of nothing: what is left depends on the other elements)
+            cache.codes.view(torch.uint8)[0, pages, 0, :, :, 5] = 0
+        got = cache.attend(0, q[row:row + 1], _int([0]), _offsets([1]), scale=scale)
+        _check_many_rows(cache, q[row:row + 1], scale, got)
+    assert cache.sync_status() == 0
