@@ -7,7 +7,8 @@
 //
 // What bounds it is reading the cache once.  So the codes go from memory to the tensor cores as they lie
 // in their pages, and what they are multiplied by is made 8-bit as well, as a sum of two E4M3 terms: a bf16
-// query's eight bits of significand fit the two exactly, scaled to its row's largest element; a weight
+// query's eight bits of significand fit the two exactly where it lies within 2^13 of its row's largest element (2^9
+// in the kernel for many rows) and are off by 2^-21 (2^-17) of that at most where it does not; a weight
 // e^(s - reference) is rounded to within 2^-8 of itself, or 2^-20 of the largest.  The keys' powers enter the
 // scores and those of the values the exponents of the weights, whose reference is a running maximum of both
 // together, so it does not matter how far powers lie apart.  The sums of the weights without the values'
@@ -137,11 +138,6 @@ __device__ __forceinline__ int ordered(float x) {
 }
 __device__ __forceinline__ float from_ordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
 constexpr int kLowest = static_cast<int>(0x807fffffu);  // of -infinity
-
-// The largest over the warp, in all lanes.
-__device__ __forceinline__ float warp_max(float x) {
-  return from_ordered(__reduce_max_sync(0xffffffffu, ordered(x)));
-}
 
 // All softmax warps.
 template <typename S>
@@ -429,7 +425,7 @@ __device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t* r) {
                : "memory");
 }
 
-// Four rows of a segment's queries to each warp: read ...
+// kBatch rows of a segment's queries to each warp: read ...
 template <typename S>
 __device__ __forceinline__ void load_queries(const CachedArgs& args, const Segment& s, int batch, uint2 (&raw)[S::kBatch]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -3,7 +3,9 @@
 //
 // A thread per row, four for its quarters of a tile of 128 tokens:
 //   S = a K^T + b K^T   M = 128 rows, N = 128 tokens, K = 128, twice: the queries' terms from shared memory, into
-//                       one sum (b is not scaled up: what lies 2^10 below the largest element ends at 2^-18 of it)
+//                       one sum, so b is not scaled up: its codes are 2^-9 apart and the row's largest element is
+//                       between 2^7 and 2^8, which leaves 2^-17 of that in each element.  A score is off by
+//                       scale 2^-17 max|q| sum|k| at worst
 //   softmax             a row's scores, reference and sum are in registers of the four threads
 //   O_a += a V, O_b += b V   M = 128 rows, N = 128 dimensions, K = 128 tokens: weights from TMEM, written over the
 //                       scores; the values' tile is read along its rows

@@ -42,14 +42,6 @@ __device__ __forceinline__ float2 decode_two(uint32_t codes) {
 constexpr int kAppendThreads = 256;
 constexpr int kAppendBlocks = 6;  // on an SM
 
-// A block per page that gets new rows and `per_block` of its heads' keys and values.  A page and head's new
-// values stay in registers between the maximum that gives the exponent and their rounding, so they are read
-// once; finding the page is a chain of loads, which the heads share where there are blocks enough.
-// A page that held tokens may get a larger exponent: its older codes are rounded again then, which
-// is exact but for values that fall among the subnormal codes.
-// 8190 rows of 23 sequences and 8 heads: 16 to 18 us for 49 MB, 0.4 of the copy rate: each block's chain (error word,
-// entry, length, page, exponent) is some 5 us and the loads' own latency comes once for each head; the issue slots
-// are busy in 39 % of the cycles.  64 rows: 7.3 us, the chain and a launch.
 // The largest 16-bit half of all threads' words; `parts` is not in use by another call.
 __device__ __forceinline__ uint32_t block_max(uint32_t two, uint32_t* parts) {
   __syncthreads();  // (the parts of the call before are read)
@@ -68,6 +60,14 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t two) {
   return (lo < 0x7f80u ? lo : 0u) | (hi < 0x7f800000u ? hi : 0u);
 }
 
+// A block per page that gets new rows and `per_block` of its heads' keys and values.  A page and head's new
+// values stay in registers between the maximum that gives the exponent and their rounding, so they are read
+// once; finding the page is a chain of loads, which the heads share where there are blocks enough.
+// A page that held tokens may get a larger exponent: its older codes are rounded again then, which
+// is exact but for values that fall among the subnormal codes.
+// 8190 rows of 23 sequences and 8 heads: 18 us for 49 MB, 0.4 of the copy rate: each block's chain (error word,
+// entry, length, page, exponent) is some 5 us and the loads' own latency comes once for each head; the issue slots
+// are busy in 39 % of the cycles.  64 rows: 7.4 us, the chain and a launch.
 template <int PageTokens>
 __global__ void __launch_bounds__(kAppendThreads, PageTokens <= 64 ? kAppendBlocks : 4)
     kv_append_kernel(PagedCache c, Batch b, int layer, const __nv_bfloat16* k, int64_t k_stride,
