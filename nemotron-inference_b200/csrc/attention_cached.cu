@@ -42,6 +42,7 @@ struct Control : WorkControl<S> {
   alignas(16) float rise[S::kRows], fade[S::kRows];  // of a reference, and what that leaves of its sums
   int highest[S::kRows];                             // largest exponents of a tile, as ordered()
   uint32_t risen;                                    // the rows whose references have changed
+  uint32_t anew;                                     // those that begin anew
   float warp_sum[S::kSoftmaxWarps][S::kRows];
   float sum[S::kRows], inverse[S::kRows];
   int failed;
@@ -231,7 +232,7 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       // exponents of the weights, rows in pairs: score + power of the values - reference + kWeightBits
       uint64_t y[R / 2];
       float high = -INFINITY;
-      {  // (the second terms are sixteen fold)
+      auto exponents = [&] {  // (the second terms are sixteen fold)
         uint32_t a[R], b[R];
 #pragma unroll
         for (int i = 0; i < R; i += 8) {
@@ -248,20 +249,18 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
                    mul2(pack2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), k2));
           y[i] = fma2(product, factors[i], add2(shifts[i], v2));
         }
-      }
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c->s_empty[buffer]);
-      if (at_end) {
+        if (at_end) {
 #pragma unroll
-        for (int r = 0; r < R; r += 2) {
-          float y0, y1;
-          unpack2(y[r / 2], y0, y1);
-          if (position > limits[r]) y0 = -INFINITY;
-          if (position > limits[r + 1]) y1 = -INFINITY;
-          y[r / 2] = pack2(y0, y1);
+          for (int r = 0; r < R; r += 2) {
+            float y0, y1;
+            unpack2(y[r / 2], y0, y1);
+            if (position > limits[r]) y0 = -INFINITY;
+            if (position > limits[r + 1]) y1 = -INFINITY;
+            y[r / 2] = pack2(y0, y1);
+          }
         }
-      }
+      };
+      exponents();
 #pragma unroll
       for (int r = 0; r < R / 2; ++r) {
         float y0, y1;
@@ -276,37 +275,44 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       if (*failed) return false;
       if (rise) {
         // the largest of each row that it may be, eight rows at a time
+        auto find_highest = [&](bool all) {
 #pragma unroll
-        for (int i = 0; i < R; i += 8) {
-          float z[8];
+          for (int i = 0; i < R; i += 8) {
+            float z[8];
 #pragma unroll
-          for (int k = 0; k < 8; k += 2) unpack2(y[(i + k) / 2], z[k], z[k + 1]);
-          const float of_eight = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])),
-                                       fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
-          if (!__any_sync(0xffffffffu, is_first || of_eight > kLargestBits)) continue;
-          int mine = kLowest;
+            for (int k = 0; k < 8; k += 2) unpack2(y[(i + k) / 2], z[k], z[k + 1]);
+            const float of_eight = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])),
+                                         fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
+            if (!__any_sync(0xffffffffu, all || of_eight > kLargestBits)) continue;
+            int mine = kLowest;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int largest = __reduce_max_sync(0xffffffffu, ordered(z[k]));
-            if (lane == k) mine = largest;
+            for (int k = 0; k < 8; ++k) {
+              const int largest = __reduce_max_sync(0xffffffffu, ordered(z[k]));
+              if (lane == k) mine = largest;
+            }
+            if (lane < 8 && (all || mine > ordered(kLargestBits))) atomicMax(&c->highest[i + lane], mine);
           }
-          if (lane < 8 && (is_first || mine > ordered(kLargestBits))) atomicMax(&c->highest[i + lane], mine);
-        }
-        softmax_sync<S>();
+          softmax_sync<S>();
+        };
+        find_highest(is_first);
         if (token < 32) {
-          bool risen = false;
+          bool risen = false, far = false;
           if (token < R) {
             const int r = token;
             const float top = from_ordered(c->highest[r]);
             c->highest[r] = kLowest;
             risen = top > -INFINITY;
-            const float by = risen ? top - kWeightBits : 0.0f;  // (in a first tile a reference may fall, too)
+            far = !is_first && top > kFarBits;
+            const float by = risen && !far ? top - kWeightBits : 0.0f;  // (in a first tile a reference may fall, too)
             c->rise[r] = -by;
-            c->fade[r] = is_first ? 1.0f : exp2_approx(-by);
-            c->shift[r] -= by;
+            c->fade[r] = is_first ? 1.0f : far ? 0.0f : exp2_approx(-by);
+            c->shift[r] = far ? 0.0f : is_first && top == -INFINITY ? -kNoReference : c->shift[r] - by;
           }
-          const uint32_t rows = __ballot_sync(0xffffffffu, risen);
-          if (lane == 0) c->risen = rows;
+          const uint32_t rows = __ballot_sync(0xffffffffu, risen), rows_anew = __ballot_sync(0xffffffffu, far);
+          if (lane == 0) {
+            c->risen = rows;
+            c->anew = rows_anew;
+          }
         }
         softmax_sync<S>();
 #pragma unroll
@@ -329,8 +335,25 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
             tmem_st_x8(o_at + R + i, o + 8);
           }
           tmem_st_wait();
+          if (c->anew != 0) {  // (hardly ever) as in a first tile, for these rows
+            exponents();
+            find_highest(true);
+            if (token < R) {
+              const float top = from_ordered(c->highest[token]);
+              c->highest[token] = kLowest;
+              const float by = (c->anew >> token & 1) && top > -INFINITY ? top - kWeightBits : 0.0f;
+              c->rise[token] = -by;
+              c->shift[token] -= by;
+            }
+            softmax_sync<S>();
+#pragma unroll
+            for (int r = 0; r < R / 2; ++r) y[r] = add2(y[r], rises[r]);
+          }
         }
       }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c->s_empty[buffer]);
 #pragma unroll
       for (int i = 0; i < R; i += 8) {
         uint32_t a[2], b[2];

@@ -41,6 +41,11 @@ constexpr int kSlotsPerBlock = 2;      // of the workspace: a piece that began i
 constexpr float kWeightBits = -1.5f;  // a row's largest weight is 2^-1.5 when its reference is set ...
 constexpr float kLargestBits = 0.0f;  // ... and at most 1 before it is set anew
 constexpr float kCodeScale = 256.0f;  // of weights as codes
+// An exponent is score - reference by one fma, off by 2^-24 of what comes out.  In a tile that lies this many orders
+// above its row's reference so far (keys before it that are masked by values of their own), that would be 2^-10 and
+// more: what the row has summed up is worth nothing there, and it begins anew.
+constexpr float kFarBits = 8192.0f;
+constexpr float kNoReference = -3e38f;  // of a row whose scores so far are all -infinity
 
 // The tiles of one (sequence, key head, rows) that a block works on.
 struct Segment {

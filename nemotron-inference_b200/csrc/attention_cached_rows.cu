@@ -151,7 +151,7 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       const uint32_t s_at = lanes + buffer * kKeyTile;
       uint32_t y[kQuarter];
       float v_inverse[kQuarter / kPart], high = -INFINITY;
-      if (has_rows) {
+      auto exponents = [&] {
 #pragma unroll
         for (int i = 0; i < kQuarter; i += 32) tmem_ld_x32_async(s_at + quarter * kQuarter + i, y + i);
         tmem_ld_wait();
@@ -179,9 +179,11 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
             if (begin + i > limit) y[i] = 0xff800000u;
           }
         }
+        high = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kQuarter; ++i) high = fmaxf(high, __uint_as_float(y[i]));
-      }
+      };
+      if (has_rows) exponents();
       // (all scores are read behind this: weights may be written over them)
       if (!ok) *failed = 1;
       const bool rise = softmax_any<S>(is_first || high > kLargestBits);
@@ -189,15 +191,23 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       if (rise) {
         c->top[quarter][row] = high;
         softmax_sync<S>();
-        const float top = fmaxf(fmaxf(c->top[0][row], c->top[1][row]), fmaxf(c->top[2][row], c->top[3][row]));
+        float top = fmaxf(fmaxf(c->top[0][row], c->top[1][row]), fmaxf(c->top[2][row], c->top[3][row]));
+        const bool anew = has_rows && !is_first && top > kFarBits;
+        if (!is_first && softmax_any<S>(anew)) {  // (hardly ever)
+          if (anew) shift = 0.0f;
+          if (has_rows) exponents();
+          c->top[quarter][row] = high;
+          softmax_sync<S>();
+          top = fmaxf(fmaxf(c->top[0][row], c->top[1][row]), fmaxf(c->top[2][row], c->top[3][row]));
+        }
         // a row's first tile sets its reference (unless it sees none of it), others may raise it
-        const float by = has_rows && top > (is_first ? -INFINITY : kLargestBits) ? top - kWeightBits : 0.0f;
-        shift -= by;
-        if (__any_sync(0xffffffffu, by != 0.0f)) {
+        const float by = has_rows && top > (is_first || anew ? -INFINITY : kLargestBits) ? top - kWeightBits : 0.0f;
+        shift = is_first && top == -INFINITY ? -kNoReference : shift - by;
+        if (__any_sync(0xffffffffu, by != 0.0f || anew)) {
 #pragma unroll
           for (int i = 0; i < kQuarter; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) - by);
           if (!is_first) {
-            const float fade = exp2_approx(-by);
+            const float fade = anew ? 0.0f : exp2_approx(-by);
             sum *= fade;
             // O of the tiles before is complete; each quarter takes half of one of its terms
             ok = mbar_wait_warp(smem_u32(&c->o_full), (no & 1) ^ 1);

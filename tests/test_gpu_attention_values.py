@@ -164,3 +164,38 @@ def test_many_rows_of_queries_of_any_size(attention):
         got = cache.attend(0, q[row:row + 1], _int([0]), _offsets([1]), scale=scale)
         _check_many_rows(cache, q[row:row + 1], scale, got)
     assert cache.sync_status() == 0
+
+
+@pytest.mark.parametrize("heads", [16, 128])
+@pytest.mark.parametrize("power", [4, 14, 24, 32])
+def test_scores_far_above_those_of_the_tiles_before(attention, heads, power):
+    # the first 192 tokens are masked by keys that are lowest in one dimension: their scores are -448 x 2^power
+    # x scale, and the tokens behind them alone count.  Blocks have several tiles of a sequence each.
+    n, kv_heads, masked, scale = 700, 4, 192, D ** -0.5
+    cache = _filled(attention, [n] * 40, kv_heads, 64, seed=41, layers=1)
+    codes = cache.codes.view(torch.uint8)
+    codes[0, :, 0, :, :, 0] = 0
+    pages = cache.block_table[:, :masked // 64].flatten().long()
+    codes[0, pages, 0] = 0
+    codes[0, pages, 0, :, :, 0] = 0xFE  # -448
+    cache.exponents[0, pages, 0] = power
+    q = _normal(42, 40, heads, D)
+    q[:, :, 0] = 1.0
+    q = q.to(torch.bfloat16)
+    everyone = list(range(40))
+    got = cache.attend(0, q, _int(everyone), _offsets([1] * 40))
+    assert cache.sync_status() == 0
+    group = heads // kv_heads
+    for s in everyone:
+        k, v = _values(cache, 0, s)
+        for h in range(kv_heads):
+            of = slice(h * group, (h + 1) * group)
+            x = q[s, of].double()
+            scores = (x @ k[h].T) * scale
+            w = torch.softmax(scores, 1)
+            spread = w @ v[h].abs()
+            # (a score's error is that of the tokens that count, as in _check_many_rows)
+            delta = scale * 2 ** -17 * float(x.abs().max()) * float(k[h, masked:].abs().sum(1).max())
+            bound = (1.75 * 2 ** -8 + 2.2 * delta) * spread + 2 ** -22 * w.amax(1, keepdim=True) * v[h].abs().sum(0)
+            error = (got[s, of].double() - w @ v[h]).abs()
+            assert bool((error <= bound).all()), (s, h, float((error / bound).max()))
