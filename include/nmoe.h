@@ -585,8 +585,9 @@ NMOE_API nmoe_status nmoe_kv_sync_status(const nmoe_kv_cache* cache, void* strea
 /* Attention of new rows over the cache: row j of an entry with c rows stands at
  * position length - c + j of its sequence and sees every token up to itself
  * (which nmoe_kv_append has written).  out [rows][heads][128]:
- * softmax(scale * q k^T) v, sums in FP32.  The rows of an entry that names what is
- * not there become zeros; rows of no entry stay as they are. */
+ * softmax(scale * q k^T) v, sums in FP32; a weight enters the product with v to
+ * within 2^-8 of itself, or 2^-20.5 of its row's largest.  The rows of an entry that
+ * names what is not there become zeros; rows of no entry stay as they are. */
 NMOE_API nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* stream, int32_t layer,
                                            const void* q, int64_t q_stride, int32_t heads,
                                            const int32_t* sequences, const int32_t* offsets,

@@ -8,9 +8,9 @@
 // Rows being few, all 128 threads have work and the tensor cores run far below what they can do, while the memory
 // is read at its rate.  Two blocks to an SM, a tile's chain of some 1500 cycles in one beside the other's.
 //
-// Measured, 32 heads on 8 key heads, pages of 64: 64 sequences of 2048 tokens on average 55 us (268 MB: 4.8 TB/s, 0.74
+// Measured, 32 heads on 8 key heads, pages of 64: 64 sequences of 2048 tokens on average 56 us (268 MB: 4.8 TB/s, 0.73
 // of the copy rate; some 11 us of it before the first tiles arrive and after the last), one of 65536 tokens 34 us
-// (134 MB).  One of 1500 tokens on 2 key heads 11.4 us: launch, the chain sequence - length - page - tile, and the
+// (134 MB).  One of 1500 tokens on 2 key heads 10.9 us: launch, the chain sequence - length - page - tile, and the
 // join of 12 pieces.
 #include <algorithm>
 

@@ -9,7 +9,8 @@
 // in their pages, and what they are multiplied by is made 8-bit as well, as a sum of two E4M3 terms: a bf16
 // query's eight bits of significand fit the two exactly where it lies within 2^13 of its row's largest element (2^9
 // in the kernel for many rows) and are off by 2^-21 (2^-17) of that at most where it does not; a weight
-// e^(s - reference) is rounded to within 2^-8 of itself, or 2^-20 of the largest.  The keys' powers enter the
+// e^(s - reference) is rounded to within 2^-8 of itself, or 2^-22 (2^-20.5 of the row's largest, which is 2^-1.5 at
+// least).  The keys' powers enter the
 // scores and those of the values the exponents of the weights, whose reference is a running maximum of both
 // together, so it does not matter how far powers lie apart.  The sums of the weights without the values'
 // powers are kept in FP32 beside.

@@ -12,8 +12,8 @@
 // A tile takes some 1000 MMA cycles and, by the softmax warps, some 800 issue slots of each scheduler, beside the
 // 1400 cycles that the memory takes to bring one to an SM.  Scores are a tile ahead of the values.
 //
-// Measured, 48 sequences of 8192 tokens on average with up to 8 new rows each, 16 heads on each of 2 key heads: 103 us
-// (201 MB: 2.0 TB/s).  A tile takes some 2900 cycles: the warps go through a tile's steps together (scores and
+// Measured, 48 sequences of 8192 tokens on average with up to 8 new rows each, 16 heads on each of 2 key heads: 104 us
+// (201 MB: 1.9 TB/s).  A tile takes some 2900 cycles: the warps go through a tile's steps together (scores and
 // maximum 600 cycles, exponentials and codes 1400, barriers between), so the special function unit and the issue slots
 // are idle in turn.  With 8 softmax warps 119 us where 16 took 114; four pipelines of 128 rows and instructions for the
 // conversions to codes, 162 where this form took 128.

@@ -23,7 +23,7 @@
 // in FP32, the rest take the special function unit's 16 a cycle; alone the unit would take as long as the
 // tile's 1024 MMA cycles.  8192 tokens, 32 heads on 2 key heads: 433 us alone = 1.27 PFLOP/s = 0.76 of the measured
 // bf16 rate, the tensor pipe active in 68 % of the cycles.  Short prompts: some 5000 cycles of a block's item beside
-// its tiles (queries in, the first tile's scores, the last one's results out), 8190 tokens in 23 prompts 80 us, the
+// its tiles (queries in, the first tile's scores, the last one's results out), 8190 tokens in 23 prompts 81 us, the
 // tensor pipe active in 33 %.  17 tokens: 10 us, a launch and one item.
 #include <algorithm>
 

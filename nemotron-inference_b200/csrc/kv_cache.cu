@@ -67,7 +67,7 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t two) {
 // is exact but for values that fall among the subnormal codes.
 // 8190 rows of 23 sequences and 8 heads: 18 us for 49 MB, 0.4 of the copy rate: each block's chain (error word,
 // entry, length, page, exponent) is some 5 us and the loads' own latency comes once for each head; the issue slots
-// are busy in 39 % of the cycles.  64 rows: 7.4 us, the chain and a launch.
+// are busy in 40 % of the cycles.  64 rows: 7.4 us, the chain and a launch.
 template <int PageTokens>
 __global__ void __launch_bounds__(kAppendThreads, PageTokens <= 64 ? kAppendBlocks : 4)
     kv_append_kernel(PagedCache c, Batch b, int layer, const __nv_bfloat16* k, int64_t k_stride,
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) 
 constexpr int kCopyThreads = 256;
 constexpr int kCopyChunk = kCopyThreads * 4;  // of 16 bytes: four loads under way in each thread
 
-// Bound by memory: 781 MB of a compaction in 135 us, 0.89 of the copy rate.  A chunk is a page's part, not a page: 128
+// Bound by memory: 781 MB of a compaction in 131 us, 0.91 of the copy rate.  A chunk is a page's part, not a page: 128
 // copies in 8 layers, or a few, are spread evenly.  It is launched while the books are kept and waits for them.
 
 __global__ void __launch_bounds__(kCopyThreads)
