@@ -522,7 +522,7 @@ NMOE_API nmoe_status nmoe_route_tokens_noalloc(
  * that rows without a place are not written over others, and nmoe_attention_cached
  * writes zeros.  An entry or a page out of range that an append, attention or a
  * copy of pages comes upon is that entry's or page's alone: all others of the call,
- * and of such calls behind it, are done all the same.  (That no sequence is named
+ * and of such calls up to the next of the former, are done all the same.  (That no sequence is named
  * twice is not checked by these.)
  */
 typedef struct nmoe_kv_cache {

@@ -196,6 +196,13 @@ __device__ __forceinline__ void ask_for(const int* p) {
   asm volatile("{\n\t.reg .b32 unused;\n\tld.global.b32 unused, [%0];\n\t}" ::"l"(p));
 }
 
+// Whether the books stay as they are.  What follows (an append of rows for which no room was made) does nothing
+// either, even if it was an append that found something wrong: so that goes where appends and attention look.
+__device__ __forceinline__ bool books_closed(const PagedCache& c, const CacheWords& words) {
+  if (words.pending() && threadIdx.x == 0) report_cache_error(c.error, words.raised);
+  return words.pending();
+}
+
 // For the lists' sequences: their lengths.  (Counts of references and claims are not asked for ahead: they change
 // by atomics.)
 __device__ __forceinline__ void ask_for_lengths(const PagedCache& c, const int* sequences, int count) {
@@ -284,7 +291,7 @@ __global__ void __launch_bounds__(kBookThreads) kv_extend_kernel(PagedCache c, B
   wait_for_predecessor();
   const CacheWords words = cache_words(c);
   ask_for_lengths(c, b.sequences, b.count);
-  if (words.pending()) return;
+  if (books_closed(c, words)) return;
   if (threadIdx.x == 0) s.flag = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < b.count; i += kBookThreads) claim(c, b.sequences[i], s);
@@ -361,7 +368,7 @@ __global__ void __launch_bounds__(kBookThreads)
   wait_for_predecessor();
   const CacheWords words = cache_words(c);
   ask_for_lengths(c, sequences, count);
-  if (words.pending()) return;
+  if (books_closed(c, words)) return;
   if (threadIdx.x == 0) s.flag = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += kBookThreads) claim(c, sequences[i], s);
@@ -397,7 +404,7 @@ __global__ void __launch_bounds__(kBookThreads)
     s.flag = 0;
     *c.move_count = -1;
   }
-  if (words.pending()) return;
+  if (books_closed(c, words)) return;
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += kBookThreads) claim(c, children[i], s);
   __syncthreads();
@@ -488,7 +495,7 @@ __global__ void __launch_bounds__(kBookThreads) kv_compact_kernel(PagedCache c) 
     live += c.references[page] > 0;
     c.remap[page] = page;
   }
-  if (words.pending()) return;
+  if (books_closed(c, words)) return;
   int total;
   block_prefix(live, s, total);
   live = total;

@@ -285,3 +285,27 @@ def test_joins_that_blocks_leave(attention, lengths, counts, heads, kv_heads):
         impatient.fill_(0)
         assert torch.equal(cache.attend(0, q, *batch, scale=0.05, out=torch.full_like(q, 7.0)), want)
     assert cache.sync_status() == 0
+
+
+@pytest.mark.parametrize("find", ["append", "attend"])
+def test_no_row_is_written_where_no_room_was_made(attention, find):
+    # a step whose append or attention finds something wrong, and the steps behind it, whose extension does nothing
+    cache = _filled(attention, [40, 20], 2, 16, seed=9, layers=1)
+    kv = torch.ones((2, 2, D), dtype=torch.bfloat16, device="cuda")
+    q = torch.ones((2, 8, D), dtype=torch.bfloat16, device="cuda")
+    bad, good = (_int([5, 1]), _offsets([1, 1])), (_int([0, 1]), _offsets([1, 1]))
+    if find == "append":
+        cache.append(0, kv, kv, *bad)
+    else:
+        cache.attend(0, q, *bad)
+    codes, exponents = cache.codes.view(torch.uint8).clone(), cache.exponents.clone()
+    for _ in range(2):
+        cache.extend(*good, rows=2)
+        cache.append(0, 3 * kv, 3 * kv, *good)
+        assert not bool(cache.attend(0, q, *good).any())
+    assert cache.lengths.tolist() == [40, 20]
+    assert torch.equal(cache.codes.view(torch.uint8), codes) and torch.equal(cache.exponents, exponents)
+    assert cache.sync_status() == 1 and cache.sync_status() == 0
+    cache.extend(*good, rows=2)
+    cache.append(0, kv, kv, *good)
+    assert cache.sync_status() == 0 and cache.lengths.tolist() == [41, 21]
