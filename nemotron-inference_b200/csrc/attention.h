@@ -33,8 +33,8 @@ struct PagedCache {
   int* references;  // [pages]; 0: free
   // Two words, of which the first code stays.  `error`: the books could not be kept, or a wait ran out; appends and
   // attention read it and do nothing then.  `raised`: an entry or a page that appends, attention or copies of pages
-  // found wrong and left out; the books read it, too, and pass it on to `error` when they do nothing.  None of a launch's blocks reads what others of it write, so
-  // a wrong entry changes nothing for the rest of its batch.
+  // found wrong and left out; the books read it, too, and pass it on to `error` when they do nothing.  None of a
+  // launch's blocks reads what others of it write, so a wrong entry changes nothing for the rest of its batch.
   int* error;        // the first of four words that are read together: error, move_count, raised, impatient
   int* move_count;   // pages for the copy kernel: the first *move_count of the two lists; -1: the books stay as they are
   int* raised;
