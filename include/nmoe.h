@@ -606,6 +606,30 @@ NMOE_API nmoe_status nmoe_attention_prefill(void* stream, const void* q, int64_t
                                             float scale, void* out, float* lse, int32_t* error);
 NMOE_API nmoe_status nmoe_attention_sync_status(int32_t* error, void* stream);
 
+/* --- sampling ---------------------------------------------------------------------
+ * A token for each row of logits [rows][vocab] (FP32 or bf16, `stride` elements
+ * from row to row): in falling order of the logits, equal ones by rising
+ * number, the first top_k tokens (all where top_k < 1); of these as many as
+ * reach top_p of the sum of their weights e^(logit / temperature) (a token
+ * stays if those before it sum up to less; all where top_p >= 1); of these
+ * those of at least min_p times the largest weight, which always stays.  What is
+ * left shares out [0, 1) in rising order of the tokens, by weight, and
+ * uniform[row] falls on one (values outside [0, 1): on the first, the last).  A
+ * temperature that is not above 0 takes the first of the largest logits.
+ *
+ * Each parameter is a device array of one for each row or, where that is null,
+ * `*_all` for every row.  Weights are 64-bit whole numbers of 2^-44 of the
+ * largest: the token is the formula's, whatever the batch.  A row that holds a NaN, or
+ * whose largest logit is infinite, gets token -1 and logprob NaN.
+ * logprobs [rows] (nullable): log of the token's softmax over all logits, at
+ * temperature 1.  A row's size is at most 1.5 MB (NMOE_ERR_UNSUPPORTED). */
+NMOE_API nmoe_status nmoe_sample(void* stream, const void* logits, nmoe_dtype dtype, int64_t stride,
+                                 int64_t rows, int32_t vocab, const float* uniform,
+                                 const float* temperature, float temperature_all,
+                                 const int32_t* top_k, int32_t top_k_all, const float* top_p,
+                                 float top_p_all, const float* min_p, float min_p_all,
+                                 int32_t* tokens, float* logprobs);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif
