@@ -592,6 +592,33 @@ NMOE_API nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* str
                                            const void* q, int64_t q_stride, int32_t heads,
                                            const int32_t* sequences, const int32_t* offsets,
                                            int32_t count, int64_t rows, float scale, void* out);
+/* The same for sequences that hold the same first pages, as children of one
+ * parent do.  Entries [groups[g], groups[g+1]) of the batch are a group (groups
+ * [group_count + 1], device, rising within 0 to count; entries of no group share
+ * with nobody).  nmoe_kv_find_shared finds how many tokens the members of a group
+ * with new rows have in common, shared [count] (each entry's group's): the pages that
+ * all their rows of the block table begin with, up to the first of all new rows,
+ * as whole runs of 128 tokens, and 0 where fewer than two members have rows.  It
+ * is called once a step, behind nmoe_kv_extend; nmoe_attention_shared then
+ * gives the results of nmoe_attention_cached in every layer, reading what is
+ * shared once for all rows of a group.
+ *
+ * `workspace` (256-byte aligned, nmoe_attention_shared_workspace_bytes() bytes,
+ * anything in it) is this call's alone until it is done.  A `shared` that is not what
+ * nmoe_kv_find_shared finds, but within the sequences' lengths, gives attention over the pages
+ * of a group's first member with rows; one beyond them, or that members have
+ * different ones of, leaves zeros and NMOE_ERR_INVALID_ARGUMENT. */
+NMOE_API nmoe_status nmoe_kv_find_shared(const nmoe_kv_cache* cache, void* stream,
+                                         const int32_t* sequences, const int32_t* offsets,
+                                         int32_t count, int64_t rows, const int32_t* groups,
+                                         int32_t group_count, int32_t* shared);
+NMOE_API size_t nmoe_attention_shared_workspace_bytes(int64_t rows, int32_t heads);
+NMOE_API nmoe_status nmoe_attention_shared(const nmoe_kv_cache* cache, void* stream, int32_t layer,
+                                           const void* q, int64_t q_stride, int32_t heads,
+                                           const int32_t* sequences, const int32_t* offsets,
+                                           int32_t count, int64_t rows, const int32_t* groups,
+                                           int32_t group_count, const int32_t* shared, float scale,
+                                           void* workspace, size_t workspace_bytes, void* out);
 /* Causal attention over `count` whole prompts packed one behind the other, prompt
  * i in rows [offsets[i], offsets[i+1]) (device, rising within 0 to `tokens`; rows of
  * no prompt stay as they are).

@@ -47,7 +47,8 @@ EXPORTED_SYMBOLS = (
     "nmoe_layer_set_unfused_activation", "nmoe_layer_export_unfused", "nmoe_layer_keep_trace",
     "nmoe_kv_workspace_bytes", "nmoe_kv_extend", "nmoe_kv_append", "nmoe_kv_fork", "nmoe_kv_free",
     "nmoe_kv_compact", "nmoe_kv_copy_pages", "nmoe_kv_sync_status", "nmoe_attention_cached",
-    "nmoe_attention_prefill", "nmoe_attention_sync_status", "nmoe_sample",
+    "nmoe_attention_prefill", "nmoe_attention_sync_status", "nmoe_kv_find_shared",
+    "nmoe_attention_shared_workspace_bytes", "nmoe_attention_shared", "nmoe_sample",
 )
 
 

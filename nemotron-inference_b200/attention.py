@@ -10,6 +10,8 @@ layer runs between its projections, over the C ABI of include/nmoe.h:
         cache.append(layer, k, v, sequences, offsets)     # the new rows, as 8-bit codes
         out = attention_prefill(q, k, v, offsets)         # whole prompts, or
         out = cache.attend(layer, q, sequences, offsets)  # new rows over all tokens so far
+        out = cache.attend_shared(layer, q, sequences, offsets, groups, shared)  # the same, or
+                                                          # continuations of a prompt together
     cache.fork(parents, children)                     # several continuations of a prompt
     cache.free(sequences)                             # finished
     cache.compact()                                   # the pages in use, without holes
@@ -33,6 +35,7 @@ from . import NMOE_OK, NmoeError, _check, _stream, load_library
 
 HEAD_DIM = 128
 DEFAULT_SCALE = HEAD_DIM ** -0.5
+_MOST_ROWS = 2 ** 30 - 1
 _BAD_SEQUENCE = 17  # kCacheBadSequence of csrc/attention.h
 
 
@@ -65,6 +68,11 @@ def _lib() -> ctypes.CDLL:
         lib.nmoe_kv_copy_pages.argtypes = [cache, vp, vp, vp, i32]
         lib.nmoe_kv_sync_status.argtypes = [cache, vp]
         lib.nmoe_attention_cached.argtypes = [cache, vp, i32, vp, i64, i32, vp, vp, i32, i64, f32, vp]
+        lib.nmoe_kv_find_shared.argtypes = [cache, vp, vp, vp, i32, i64, vp, i32, vp]
+        lib.nmoe_attention_shared_workspace_bytes.restype = ctypes.c_size_t
+        lib.nmoe_attention_shared_workspace_bytes.argtypes = [i64, i32]
+        lib.nmoe_attention_shared.argtypes = [cache, vp, i32, vp, i64, i32, vp, vp, i32, i64, vp, i32, vp, f32,
+                                              vp, ctypes.c_size_t, vp]
         lib.nmoe_attention_prefill.argtypes = [vp, vp, i64, vp, i64, vp, i64, i64, i32, i32, vp, i32,
                                                f32, vp, vp, vp]
         lib.nmoe_attention_sync_status.argtypes = [vp, vp]
@@ -311,6 +319,56 @@ class KvCache:
             offsets.data_ptr(), sequences.shape[0], rows, DEFAULT_SCALE if scale is None else scale,
             out.data_ptr()), "nmoe_attention_cached")
         return out
+
+    def find_shared(self, sequences: torch.Tensor, offsets: torch.Tensor, groups: torch.Tensor,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """How many tokens the entries of a batch have in common with their groups, [n] int32, for
+        `attend_shared`: entries [groups[g], groups[g + 1]) are a group, such as the children of one
+        parent, and what its members with new rows share are the pages with which all their rows of the
+        block table begin, before all new rows, as whole runs of 128 tokens.  0 for entries of no group,
+        and where fewer than two members have rows.  Once a step, behind `extend`, for all layers."""
+        stream = self._batch(sequences, offsets)
+        self._groups(sequences, groups)
+        if out is None:
+            out = torch.empty_like(sequences)
+        else:
+            _require_list(out, "out", self.device)
+            if out.shape != sequences.shape:
+                raise ValueError("out must have as many entries as sequences")
+        # (rows: the lists are within what they say themselves)
+        _check(_lib().nmoe_kv_find_shared(self._ref, stream, sequences.data_ptr(), offsets.data_ptr(), sequences.shape[0],
+                                          _MOST_ROWS, groups.data_ptr(), groups.shape[0] - 1, out.data_ptr()),
+               "nmoe_kv_find_shared")
+        return out
+
+    def attend_shared(self, layer: int, q: torch.Tensor, sequences: torch.Tensor, offsets: torch.Tensor,
+                      groups: torch.Tensor, shared: torch.Tensor, scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """`attend` for a batch in groups, with what `find_shared` found for it: the tokens that a group
+        shares are read once for all of its rows."""
+        stream = self._batch(sequences, offsets)
+        self._groups(sequences, groups)
+        _require_list(shared, "shared", self.device)
+        if shared.shape != sequences.shape:
+            raise ValueError("shared must have as many entries as sequences")
+        rows, heads, q_stride = _row_layout(q, "q", self.device)
+        if heads % self.kv_heads or (rows and sequences.shape[0] == 0):
+            raise NmoeError(1, "KvCache.attend_shared", "heads must be a multiple of kv_heads, rows need a sequence")
+        out = _output(out, q)
+        library = _library or _lib()
+        needed = library.nmoe_attention_shared_workspace_bytes(rows, heads) if rows else 0
+        workspace = torch.empty(needed, dtype=torch.uint8, device=self.device)
+        _check(library.nmoe_attention_shared(
+            self._ref, stream, layer, q.data_ptr(), q_stride, heads, sequences.data_ptr(), offsets.data_ptr(),
+            sequences.shape[0], rows, groups.data_ptr(), groups.shape[0] - 1, shared.data_ptr(),
+            DEFAULT_SCALE if scale is None else scale, workspace.data_ptr(), needed, out.data_ptr()),
+            "nmoe_attention_shared")
+        return out
+
+    def _groups(self, sequences: torch.Tensor, groups: torch.Tensor) -> None:
+        _require_list(groups, "groups", self.device)
+        if not 1 <= groups.shape[0] <= sequences.shape[0] + 1:
+            raise ValueError("groups must have one entry more than there are groups, no more of them than sequences")
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
         """children[i] becomes a copy of parents[i]: full pages are shared, a partly filled last

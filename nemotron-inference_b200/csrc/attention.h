@@ -55,6 +55,7 @@ struct Batch {
 
 struct BatchEntry {
   int sequence, first, rows, length;  // length: tokens in the cache, these rows among them
+  int skip;                           // tokens before the first that is attended
   bool valid;
 };
 
@@ -79,6 +80,7 @@ __device__ __forceinline__ CacheWords cache_words(const PagedCache& c) {
 // and its tokens within the block table.
 __device__ __forceinline__ BatchEntry batch_entry(const PagedCache& c, const Batch& b, int i) {
   BatchEntry e;
+  e.skip = 0;
   e.sequence = b.sequences[i];
   const int from = b.offsets[i], to = b.offsets[i + 1];
   e.first = min(max(from, 0), b.rows);
@@ -168,6 +170,17 @@ struct PrefillArgs {
   int* error;
 };
 
+// Attention over a cache may be taken in parts: what the sequences of a group share, once for all of their rows, and
+// what each has of its own.
+enum class Part { kAll, kShared, kOwn };
+
+// Where a row's sums of a part are (csrc/attention_shared.cu).
+struct alignas(16) RowPart {
+  float reference, sum;
+  int parts_row;  // 1: beside the other rows'; else 256 times the number of pieces in the workspace, and its row there
+  int lead;       // first block that has one
+};
+
 struct CachedArgs {
   PagedCache cache;
   Batch batch;
@@ -177,6 +190,12 @@ struct CachedArgs {
   int heads;
   float scale;
   __nv_bfloat16* out;
+  // Of a batch in groups: entries [groups[g], groups[g + 1]) share the first shared[i] tokens, whole tiles.
+  const int* groups;
+  int group_count;
+  const int* shared;
+  float* sums;        // of this part, [rows][heads][128]
+  RowPart* row_parts;  // [rows][heads]
 };
 
 // bf16 rows of heads x 128 as [rows][heads * 128], boxes of 64 columns x box_rows, 128-byte swizzle.
@@ -191,6 +210,17 @@ cudaError_t launch_attention_prefill(const PrefillArgs& args, cudaStream_t strea
 constexpr size_t kAttendCounterBytes = 4096;
 size_t attention_cached_workspace_bytes();
 cudaError_t launch_attention_cached(const CachedArgs& args, cudaStream_t stream);
+// The kernels behind it by the rows of queries that an entry, or a group, has on average; `slots` of the workspace for
+// pieces, attention_cached_slot_bytes() bytes.
+size_t attention_cached_slot_bytes();
+int attention_cached_slot_rows(int64_t rows);  // that a piece has room for
+cudaError_t launch_cached_part(const CachedArgs& args, Part part, int64_t rows, float* slots, cudaStream_t stream);
+// The same results for a batch whose sequences share their first pages; `workspace`:
+// attention_shared_workspace_bytes().
+size_t attention_shared_workspace_bytes(int64_t rows, int heads);
+cudaError_t launch_attention_shared(const CachedArgs& args, char* workspace, cudaStream_t stream);
+cudaError_t launch_kv_find_shared(const PagedCache& cache, const Batch& batch, const int* groups, int group_count, int* shared,
+                                  cudaStream_t stream);
 cudaError_t launch_kv_append(const PagedCache& cache, const Batch& batch, int layer,
                              const __nv_bfloat16* k, int64_t k_stride, const __nv_bfloat16* v,
                              int64_t v_stride, cudaStream_t stream);

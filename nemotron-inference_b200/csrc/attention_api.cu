@@ -137,6 +137,13 @@ nmoe_status sync_cache(const PagedCache& cache, cudaStream_t stream) {
 
 bool scale_valid(float scale) { return std::isfinite(scale) && scale > 0.0f; }
 
+// Entries of a batch in groups.
+bool groups_valid(const int32_t* groups, int32_t group_count, int32_t count) {
+  return group_count >= 0 && group_count <= count && (group_count == 0 || groups != nullptr) && !misaligned(groups, 4);
+}
+
+constexpr int64_t kMostSharedPairs = 1ll << 32;  // rows x heads: 2 TB of sums
+
 }  // namespace
 
 namespace nmoe {
@@ -279,7 +286,7 @@ nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* stream, int3
                                   const void* q, int64_t q_stride, int32_t heads,
                                   const int32_t* sequences, const int32_t* offsets, int32_t count,
                                   int64_t rows, float scale, void* out) {
-  nmoe::CachedArgs args;
+  nmoe::CachedArgs args{};
   if (!view_of(cache, args.cache) || !batch_of(sequences, offsets, count, rows, args.batch) ||
       layer < 0 || layer >= args.cache.layers || heads <= 0 || heads % args.cache.kv_heads != 0 ||
       heads > 65535 || !scale_valid(scale)) {
@@ -296,6 +303,65 @@ nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* stream, int3
   args.scale = scale;
   args.out = static_cast<__nv_bfloat16*>(out);
   return status_of(nmoe::launch_attention_cached(args, static_cast<cudaStream_t>(stream)));
+}
+
+nmoe_status nmoe_kv_find_shared(const nmoe_kv_cache* cache, void* stream, const int32_t* sequences,
+                                const int32_t* offsets, int32_t count, int64_t rows,
+                                const int32_t* groups, int32_t group_count, int32_t* shared) {
+  PagedCache view;
+  Batch batch;
+  if (!view_of(cache, view) || !batch_of(sequences, offsets, count, rows, batch) ||
+      !groups_valid(groups, group_count, count) || misaligned(shared, 4)) {
+    return NMOE_ERR_INVALID_ARGUMENT;
+  }
+  if (count == 0) return NMOE_OK;
+  if (shared == nullptr) return NMOE_ERR_INVALID_ARGUMENT;
+  if (group_count == 0) {
+    return status_of(cudaMemsetAsync(shared, 0, sizeof(int32_t) * count, static_cast<cudaStream_t>(stream)));
+  }
+  return status_of(nmoe::launch_kv_find_shared(view, batch, groups, group_count, shared,
+                                               static_cast<cudaStream_t>(stream)));
+}
+
+size_t nmoe_attention_shared_workspace_bytes(int64_t rows, int32_t heads) {
+  if (rows <= 0 || heads <= 0 || heads > 65535 || rows > kMostSharedPairs / heads) return 0;
+  return nmoe::attention_shared_workspace_bytes(rows, heads);
+}
+
+nmoe_status nmoe_attention_shared(const nmoe_kv_cache* cache, void* stream, int32_t layer,
+                                  const void* q, int64_t q_stride, int32_t heads,
+                                  const int32_t* sequences, const int32_t* offsets, int32_t count,
+                                  int64_t rows, const int32_t* groups, int32_t group_count,
+                                  const int32_t* shared, float scale, void* workspace,
+                                  size_t workspace_bytes, void* out) {
+  if (group_count == 0) {
+    return nmoe_attention_cached(cache, stream, layer, q, q_stride, heads, sequences, offsets, count, rows,
+                                 scale, out);
+  }
+  nmoe::CachedArgs args{};
+  if (!view_of(cache, args.cache) || !batch_of(sequences, offsets, count, rows, args.batch) ||
+      layer < 0 || layer >= args.cache.layers || heads <= 0 || heads % args.cache.kv_heads != 0 ||
+      heads > 65535 || !scale_valid(scale) || !groups_valid(groups, group_count, count) ||
+      misaligned(shared, 4) || misaligned(workspace, kAlign)) {
+    return NMOE_ERR_INVALID_ARGUMENT;
+  }
+  if (count == 0 || rows == 0) return NMOE_OK;
+  if (!rows_valid(q, q_stride, heads) || out == nullptr || misaligned(out, 16) || shared == nullptr ||
+      workspace == nullptr || rows > kMostSharedPairs / heads ||
+      workspace_bytes < nmoe::attention_shared_workspace_bytes(rows, heads)) {
+    return NMOE_ERR_INVALID_ARGUMENT;
+  }
+  args.layer = layer;
+  args.q = static_cast<const __nv_bfloat16*>(q);
+  args.q_stride = q_stride;
+  args.heads = heads;
+  args.scale = scale;
+  args.out = static_cast<__nv_bfloat16*>(out);
+  args.groups = groups;
+  args.group_count = group_count;
+  args.shared = shared;
+  return status_of(nmoe::launch_attention_shared(args, static_cast<char*>(workspace),
+                                                 static_cast<cudaStream_t>(stream)));
 }
 
 nmoe_status nmoe_attention_prefill(void* stream, const void* q, int64_t q_stride, const void* k,

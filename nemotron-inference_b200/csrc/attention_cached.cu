@@ -162,7 +162,7 @@ __device__ __forceinline__ uint32_t weight_offset(int token, int column) {
   return at ^ ((at >> 3) & mask);
 }
 
-template <typename S>
+template <typename S, Part P>
 __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t* values, uint8_t* q, uint8_t* weights,
                              uint32_t tmem, Control<S>* c) {
   constexpr int R = S::kRows;
@@ -205,7 +205,7 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
     uint64_t sum[R / 2];
 #pragma unroll
     for (int r = 0; r < R / 2; ++r) sum[r] = 0;
-    const int clear = s.length - s.rows;  // the last token that every row sees
+    const int clear = P == Part::kShared ? s.length : s.length - s.rows;  // the last token that every row sees
 #pragma unroll 1
     for (int j = 0; j < s.tiles; ++j, ++no) {
       const uint32_t slot = no % S::kValueSlots, buffer = no & 1;
@@ -421,7 +421,9 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
         float o = fmaf(__uint_as_float(a[k + 8]), 0.0625f, __uint_as_float(a[k]));
         if (limits[r] >= bad) o = NAN;
         if (to < 0) continue;
-        if (alone) {
+        if (P != Part::kAll && alone) {
+          __stcg(args.sums + static_cast<size_t>(to) * kHeadDim + token, o);
+        } else if (alone) {
           args.out[static_cast<size_t>(to) * kHeadDim + token] = __float2bfloat16(o * c->inverse[r]);
         } else {
           __stcg(slot + r * kHeadDim + token, o);
@@ -429,22 +431,27 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
       }
     }
     tcgen05_fence_before();
+    if (P != Part::kAll && token < R) {
+      leave_row_part(args, s, out_rows[token], token, c->sum[token] == 0.0f ? -INFINITY : -c->shift[token], c->sum[token]);
+    }
     if (!alone) {
       if (token < R) {  // (a row that has seen no token, all being behind its mask, leaves nothing)
         __stcg(slot + R * kHeadDim + token, c->sum[token] == 0.0f ? -INFINITY : -c->shift[token]);
         __stcg(slot + R * (kHeadDim + 1) + token, c->sum[token]);
       }
-      if (threadIdx.x == 0) c->to_join[joins] = s;
-      ++joins;
+      if (P == Part::kAll) {
+        if (threadIdx.x == 0) c->to_join[joins] = s;
+        ++joins;
+      }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&c->segment_empty[segments % kSegments]);
   }
-  announce_and_join<S>(args, split, joins, c);
+  if (P == Part::kAll) announce_and_join<S>(args, split, joins, c);
   return true;
 }
 
-template <typename S>
+template <typename S, Part P>
 __global__ void __launch_bounds__(S::kThreads, S::kBlocks)
     cached_kernel(const __grid_constant__ CUtensorMap map, const CachedArgs args, const Split split) {
   static_assert(fits_on_sm<S>());
@@ -471,14 +478,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks)
     tmem_relinquish();
   }
   tcgen05_fence_before();
-  wait_for_predecessor();
-  find_begin<S>(args, c);
+  if (P != Part::kOwn) wait_for_predecessor();  // (kOwn: see launch_attention_shared())
+  find_begin<S, P>(args, c);
   __syncthreads();
   release_successor();  // (the columns of TMEM are there)
   tcgen05_fence_after();
   const uint32_t tmem = c->tmem;
   if (warp < S::kSoftmaxWarps) {
-    if (!softmax_role<S>(args, split, values, q, weights, tmem, c) && (threadIdx.x & 31) == 0) {
+    if (!softmax_role<S, P>(args, split, values, q, weights, tmem, c) && (threadIdx.x & 31) == 0) {
       report_cache_error(args.cache.error, kDevWaitTimeout);
     }
   } else if (warp == S::kSoftmaxWarps) {
@@ -490,7 +497,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks)
     __syncwarp();
     mbar_wait_warp(smem_u32(&c->drained), 0);
   } else {
-    load_role<S>(args, &map, smem_u32(keys), smem_u32(values), c);
+    load_role<S, P>(args, &map, smem_u32(keys), smem_u32(values), c);
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -498,31 +505,37 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks)
     tcgen05_fence_after();
     tmem_dealloc(tmem, S::kColumns);
   }
+  if (P == Part::kOwn) wait_for_predecessor();
+}
+
+template <typename S, Part P>
+cudaError_t launch(const CUtensorMap& map, const CachedArgs& args, const Split& split, int sms, cudaStream_t stream) {
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t err = allow_shared_memory_once(cached_kernel<S, P>, allowed);
+  if (err != cudaSuccess) return err;
+  return launch_kernel(cached_kernel<S, P>, dim3(sms * S::kBlocks), S::kThreads, shared_bytes<S>(),
+                       LaunchStream(stream, true), map, args, split);
 }
 
 template <typename S>
-cudaError_t launch(const CUtensorMap& map, const CachedArgs& args, const Split& split, int sms, cudaStream_t stream) {
-  static std::atomic<uint64_t> allowed{0};
-  cudaError_t err = allow_shared_memory_once(cached_kernel<S>, allowed);
-  if (err != cudaSuccess) return err;
-  return launch_kernel(cached_kernel<S>, dim3(sms * S::kBlocks), S::kThreads, shared_bytes<S>(),
-                       LaunchStream(stream, true), map, args, split);
+cudaError_t launch(const CUtensorMap& map, const CachedArgs& args, Part part, const Split& split, int sms, cudaStream_t stream) {
+  return part == Part::kAll      ? launch<S, Part::kAll>(map, args, split, sms, stream)
+         : part == Part::kShared ? launch<S, Part::kShared>(map, args, split, sms, stream)
+                                 : launch<S, Part::kOwn>(map, args, split, sms, stream);
 }
 
 }  // namespace
 
-size_t attention_cached_workspace_bytes() {
+size_t attention_cached_slot_bytes() {
   // (two blocks of 16 rows need less than one of 128)
-  return kAttendCounterBytes + sizeof(float) * slot_floats(kMaxRows) * kSlotsPerBlock * device_sms();
+  return sizeof(float) * slot_floats(kMaxRows) * kSlotsPerBlock * device_sms();
 }
 
+size_t attention_cached_workspace_bytes() { return kAttendCounterBytes + attention_cached_slot_bytes(); }
+
+int attention_cached_slot_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : kMaxRows; }
+
 cudaError_t launch_attention_cached(const CachedArgs& args, cudaStream_t stream) {
-  const int sms = device_sms();
-  if (sms * 2 > kMaxBlocks) return cudaErrorInvalidValue;
-  CUtensorMap map;
-  if (!pages_tensor_map(args.cache, &map)) return cudaErrorInvalidValue;
-  const Split split{reinterpret_cast<JoinCounters*>(args.cache.attend_workspace),
-                    reinterpret_cast<float*>(args.cache.attend_workspace + kAttendCounterBytes)};
   // By the query rows that the entries have on average.  Entries with more are taken 8, 16 or 128 at a time
   // and read their keys and values again each time.  64 sequences of 2048 tokens, 8 key heads, cold, in us, by 8 / 16 /
   // 128 at a time: 8 rows 72 / 74 / 113, 12 rows 110 / 76 / 113, 16 rows 109 / 76 / 115, 24 rows 149 / 113 / 117, 32 rows
@@ -531,9 +544,21 @@ cudaError_t launch_attention_cached(const CachedArgs& args, cudaStream_t stream)
   // rows x 16 heads among 64 places, 8192 tokens each, are taken 8 at a time, 43 us where 128 at a time take 33.
   const int64_t rows = (args.batch.rows + args.batch.count - 1) / args.batch.count *
                        static_cast<int64_t>(args.heads / args.cache.kv_heads);
-  if (rows <= 8) return launch<Shape<8>>(map, args, split, sms, stream);
-  if (rows <= 16) return launch<Shape<16>>(map, args, split, sms, stream);
-  return launch_cached_rows(map, args, split, sms, stream);
+  return launch_cached_part(args, Part::kAll, rows, reinterpret_cast<float*>(args.cache.attend_workspace + kAttendCounterBytes),
+                            stream);
+}
+
+cudaError_t launch_cached_part(const CachedArgs& args, Part part, int64_t rows, float* slots, cudaStream_t stream) {
+  const int sms = device_sms();
+  if (sms * 2 > kMaxBlocks) return cudaErrorInvalidValue;
+  CUtensorMap map;
+  if (!pages_tensor_map(args.cache, &map)) return cudaErrorInvalidValue;
+  const Split split{reinterpret_cast<JoinCounters*>(args.cache.attend_workspace), slots};
+  switch (attention_cached_slot_rows(rows)) {
+    case 8: return launch<Shape<8>>(map, args, part, split, sms, stream);
+    case 16: return launch<Shape<16>>(map, args, part, split, sms, stream);
+    default: return launch_cached_rows(map, args, part, split, sms, stream);
+  }
 }
 
 }  // namespace nmoe

@@ -198,6 +198,49 @@ __device__ __forceinline__ float power_of_two(int e) {  // -126 <= e <= 127
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
+// Entry i of a part of the work: of the batch, or a group as one, whose rows are all its members' and whose tokens those
+// that they share, as the first of them with rows has them.
+static __device__ __noinline__ BatchEntry group_entry(const CachedArgs& args, int g) {
+  const Batch& b = args.batch;
+  BatchEntry e;
+  e.sequence = e.first = e.rows = e.length = e.skip = 0;
+  const int from = args.groups[g], to = args.groups[g + 1];
+  e.valid = from >= 0 && from <= to && to <= b.count;
+  if (!e.valid || from == to) return e;
+  int leader = from;
+  while (leader + 1 < to && b.offsets[leader + 1] <= b.offsets[leader]) ++leader;
+  const int first = b.offsets[from], rows = b.offsets[to] - first, shared = args.shared[leader];
+  const int sequence = b.sequences[leader];
+  e.valid = first >= 0 && rows >= 0 && rows <= b.rows - first && shared >= 0 && shared % kKeyTile == 0 &&
+            static_cast<unsigned>(sequence) < static_cast<unsigned>(args.cache.max_sequences);
+  if (!e.valid || shared == 0) return e;
+  const int64_t room = static_cast<int64_t>(args.cache.max_pages) << args.cache.page_shift;
+  e.valid = shared <= args.cache.lengths[sequence] && shared <= room;
+  if (!e.valid) return e;
+  e.sequence = sequence;
+  e.first = first;
+  e.rows = rows;
+  e.length = shared;
+  return e;
+}
+template <Part P>
+__device__ __forceinline__ BatchEntry part_entry(const CachedArgs& args, int i) {
+  if constexpr (P == Part::kShared) return group_entry(args, i);
+  BatchEntry e = batch_entry(args.cache, args.batch, i);
+  if constexpr (P == Part::kOwn) {
+    if (e.valid) {
+      e.skip = args.shared[i];
+      e.valid = e.skip >= 0 && e.skip % kKeyTile == 0 && e.skip <= e.length - e.rows;
+    }
+    if (!e.valid) e.rows = e.length = e.skip = 0;
+  }
+  return e;
+}
+template <Part P>
+__device__ __forceinline__ int part_count(const CachedArgs& args) {
+  return P == Part::kShared ? args.group_count : args.batch.count;
+}
+
 // How a batch entry's tiles lie in the order of all: by key head, then by rows, kRows at a time.
 template <typename S>
 struct EntryTiles {
@@ -206,7 +249,7 @@ struct EntryTiles {
   int64_t all;
 
   __device__ EntryTiles(const CachedArgs& args, const BatchEntry& e) {
-    tiles = (e.length + kKeyTile - 1) / kKeyTile;
+    tiles = (e.length + kKeyTile - 1) / kKeyTile - e.skip / kKeyTile;
     row_tiles = (e.rows * (args.heads / args.cache.kv_heads) + S::kRows - 1) / S::kRows;
     cost = tiles + S::kUnitCost;
     all = static_cast<int64_t>(cost) * row_tiles * args.cache.kv_heads;
@@ -222,9 +265,9 @@ static __device__ __noinline__ void clear_rows(__nv_bfloat16* out, int heads, in
 }
 
 // All threads: the number of tiles, and the entry in which this block's begin.
-template <typename S>
+template <typename S, Part P>
 __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
-  const int n = args.batch.count, each = (n + S::kThreads - 1) / S::kThreads;
+  const int n = part_count<P>(args), each = (n + S::kThreads - 1) / S::kThreads;
   const int begin = min(n, static_cast<int>(threadIdx.x) * each), end = min(n, begin + each);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // (one thread's word: a wait that runs out in another block of this launch writes it)
@@ -234,11 +277,13 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
   BatchEntry e;
 #pragma unroll 1
   for (int i = begin; i < end; ++i) {
-    e = batch_entry(args.cache, args.batch, i);
+    e = part_entry<P>(args, i);
     if (!e.valid) {
       if (blockIdx.x == 0) report_cache_error(args.cache.raised, kCacheBadSequence);
-      const int from = args.batch.offsets[i], to = args.batch.offsets[i + 1];
-      if (from >= 0 && to <= args.batch.rows) clear_rows(args.out, args.heads, from, to, 0, 1);
+      if (P != Part::kShared) {
+        const int from = args.batch.offsets[i], to = args.batch.offsets[i + 1];
+        if (from >= 0 && to <= args.batch.rows) clear_rows(args.out, args.heads, from, to, 0, 1);
+      }
     }
     mine += EntryTiles<S>(args, e).all;
   }
@@ -265,8 +310,10 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
   if (total > INT32_MAX && threadIdx.x == 0) report_cache_error(args.cache.raised, kCacheBadSequence);
   if (total > INT32_MAX || c->stopped != 0) {
     total = 0;
-    clear_rows(args.out, args.heads, max(args.batch.offsets[0], 0), min(args.batch.offsets[n], args.batch.rows), threadIdx.x,
-               S::kThreads);
+    if (P != Part::kShared) {
+      clear_rows(args.out, args.heads, max(args.batch.offsets[0], 0), min(args.batch.offsets[n], args.batch.rows), threadIdx.x,
+                 S::kThreads);
+    }
   }
   Shares shares;
   shares.total = static_cast<int>(total);
@@ -279,7 +326,7 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
   if (start >= below && start < below + mine) {  // one thread's
 #pragma unroll 1
     for (int i = begin; i < end; ++i) {
-      if (each > 1) e = batch_entry(args.cache, args.batch, i);
+      if (each > 1) e = part_entry<P>(args, i);
       const int64_t tiles = EntryTiles<S>(args, e).all;
       if (start < below + tiles) {
         c->found = i;
@@ -293,7 +340,7 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
 }
 
 // The warp that brings keys and values in, a page at a time.
-template <typename S>
+template <typename S, Part P>
 __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32_t keys_at, uint32_t values_at, WorkControl<S>* c) {
   const PagedCache& cache = args.cache;
   const int lane = threadIdx.x & 31, g = blockIdx.x;
@@ -333,6 +380,7 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
         ++head;
       }
       if (s.tiles <= 0) continue;
+      s.tile += e.skip / kKeyTile;
       const uint32_t place = segments % kSegments;
       if (!(ok = mbar_wait_warp(smem_u32(&c->segment_empty[place]), ((segments / kSegments) & 1) ^ 1))) break;
       if (lane == 0) {
@@ -394,7 +442,7 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
     }
     entry_at += static_cast<int>(t.all);
     while (entry_at < stop && ok) {  // (entries without rows have no tiles)
-      e = batch_entry(cache, args.batch, ++i);
+      e = part_entry<P>(args, ++i);
       if (e.rows > 0) break;
     }
   }
@@ -718,6 +766,12 @@ __device__ void announce_and_join(const CachedArgs& args, const Split& split, in
   }
 }
 
+// What a row leaves of a part: where its sums are, and whether in pieces.
+__device__ __forceinline__ void leave_row_part(const CachedArgs& args, const Segment& s, int to, int row, float reference, float sum) {
+  if (to < 0 || (s.part >= 0 && static_cast<int>(blockIdx.x) != s.lead)) return;
+  args.row_parts[to] = {reference, sum, s.part < 0 ? 1 : s.parts << 8 | row, s.lead};
+}
+
 // Barriers of WorkControl; one thread.
 template <typename S>
 __device__ void init_work(WorkControl<S>* c) {
@@ -743,6 +797,6 @@ __device__ void init_work(WorkControl<S>* c) {
 }
 
 // For the kernel of more than 16 rows.
-cudaError_t launch_cached_rows(const CUtensorMap& map, const CachedArgs& args, const Split& split, int sms, cudaStream_t stream);
+cudaError_t launch_cached_rows(const CUtensorMap& map, const CachedArgs& args, Part part, const Split& split, int sms, cudaStream_t stream);
 
 }  // namespace nmoe

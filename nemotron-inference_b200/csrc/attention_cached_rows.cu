@@ -105,6 +105,7 @@ __device__ bool mma_role(uint32_t keys_at, uint32_t values_at, uint32_t q_at, ui
   }
 }
 
+template <Part P>
 __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t* values, uint8_t* q, uint32_t tmem, Control* c) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp >> 2;
   const int row = threadIdx.x & (S::kRows - 1);
@@ -131,7 +132,7 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
     softmax_sync<S>();
     if (lane == 0) mbar_arrive(&c->q_full);
     const bool has_rows = s.row0 + (row & ~31) < s.rows * (args.heads / args.cache.kv_heads);  // the warp
-    const int clear = s.length - s.rows;  // the last token that every row sees
+    const int clear = P == Part::kShared ? s.length : s.length - s.rows;  // the last token that every row sees
     float factor = 0.0f, shift = 0.0f, sum = 0.0f;
     int limit = -1;
     if (has_rows) {
@@ -292,7 +293,7 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
           if (bad && limit >= c->first_bad[d + i]) o[i] = NAN;
         }
         if (to < 0) continue;
-        if (alone) {
+        if (alone && P == Part::kAll) {
           uint32_t two[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) two[i] = pack_bf16(o[2 * i] * inverse, o[2 * i + 1] * inverse);
@@ -300,28 +301,30 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, uint8_t
           out[0] = make_uint4(two[0], two[1], two[2], two[3]);
           out[1] = make_uint4(two[4], two[5], two[6], two[7]);
         } else {
-          float4* out = reinterpret_cast<float4*>(slot + row * kHeadDim + d);
+          float4* out = reinterpret_cast<float4*>((alone ? args.sums + static_cast<size_t>(to) * kHeadDim : slot + row * kHeadDim) + d);
 #pragma unroll
           for (int i = 0; i < 4; ++i) __stcg(out + i, make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
         }
       }
+      if (P != Part::kAll && quarter == 0) leave_row_part(args, s, to, row, all == 0.0f ? -INFINITY : -shift, all);
       if (!alone && quarter == 0) {  // (a row that has seen no token, all being behind its mask, leaves nothing)
         __stcg(slot + S::kRows * kHeadDim + row, all == 0.0f ? -INFINITY : -shift);
         __stcg(slot + S::kRows * (kHeadDim + 1) + row, all);
       }
     }
     tcgen05_fence_before();
-    if (!alone) {
+    if (!alone && P == Part::kAll) {
       if (threadIdx.x == 0) c->to_join[joins] = s;
       ++joins;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&c->segment_empty[segments % kSegments]);
   }
-  announce_and_join<S>(args, split, joins, c);
+  if (P == Part::kAll) announce_and_join<S>(args, split, joins, c);
   return true;
 }
 
+template <Part P>
 __global__ void __launch_bounds__(S::kThreads, 1)
     cached_rows_kernel(const __grid_constant__ CUtensorMap map, const CachedArgs args, const Split split) {
   extern __shared__ uint8_t raw[];
@@ -344,14 +347,14 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     tmem_relinquish();
   }
   tcgen05_fence_before();
-  wait_for_predecessor();
-  find_begin<S>(args, c);
+  if (P != Part::kOwn) wait_for_predecessor();  // (kOwn: see launch_attention_shared())
+  find_begin<S, P>(args, c);
   __syncthreads();
   release_successor();  // (the columns of TMEM are there)
   tcgen05_fence_after();
   const uint32_t tmem = c->tmem;
   if (warp < S::kSoftmaxWarps) {
-    if (!softmax_role(args, split, values, q, tmem, c) && (threadIdx.x & 31) == 0) {
+    if (!softmax_role<P>(args, split, values, q, tmem, c) && (threadIdx.x & 31) == 0) {
       report_cache_error(args.cache.error, kDevWaitTimeout);
     }
   } else if (warp == S::kSoftmaxWarps) {
@@ -363,7 +366,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     __syncwarp();
     mbar_wait_warp(smem_u32(&c->drained), 0);
   } else {
-    load_role<S>(args, &map, smem_u32(keys), smem_u32(values), c);
+    load_role<S, P>(args, &map, smem_u32(keys), smem_u32(values), c);
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -371,16 +374,24 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     tcgen05_fence_after();
     tmem_dealloc(tmem, kColumns);
   }
+  if (P == Part::kOwn) wait_for_predecessor();
+}
+
+template <Part P>
+cudaError_t launch(const CUtensorMap& map, const CachedArgs& args, const Split& split, int sms, cudaStream_t stream) {
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t err = allow_shared_memory_once(cached_rows_kernel<P>, allowed);
+  if (err != cudaSuccess) return err;
+  return launch_kernel(cached_rows_kernel<P>, dim3(sms), S::kThreads, kSharedBytes, LaunchStream(stream, true),
+                       map, args, split);
 }
 
 }  // namespace
 
-cudaError_t launch_cached_rows(const CUtensorMap& map, const CachedArgs& args, const Split& split, int sms, cudaStream_t stream) {
-  static std::atomic<uint64_t> allowed{0};
-  cudaError_t err = allow_shared_memory_once(cached_rows_kernel, allowed);
-  if (err != cudaSuccess) return err;
-  return launch_kernel(cached_rows_kernel, dim3(sms), S::kThreads, kSharedBytes, LaunchStream(stream, true),
-                       map, args, split);
+cudaError_t launch_cached_rows(const CUtensorMap& map, const CachedArgs& args, Part part, const Split& split, int sms, cudaStream_t stream) {
+  return part == Part::kAll      ? launch<Part::kAll>(map, args, split, sms, stream)
+         : part == Part::kShared ? launch<Part::kShared>(map, args, split, sms, stream)
+                                 : launch<Part::kOwn>(map, args, split, sms, stream);
 }
 
 }  // namespace nmoe
