@@ -633,6 +633,40 @@ NMOE_API nmoe_status nmoe_attention_prefill(void* stream, const void* q, int64_t
                                             float scale, void* out, float* lse, int32_t* error);
 NMOE_API nmoe_status nmoe_attention_sync_status(int32_t* error, void* stream);
 
+/* --- low-rank adapters --------------------------------------------------------------
+ * Beside a projection that many requests share, what each one's own adapter adds:
+ * out = y + scales[id] (x A[id]^T) B[id]^T for the rows [offsets[i], offsets[i+1]) of
+ * entry i with id = ids[i] (device; entries may have the same; -1: none, the rows of y
+ * as they are).  x [rows][inner], y and out [rows][outer] bf16, out may be y; `*_stride`
+ * elements from row to row, a multiple of 8.  A [adapters][rank][inner],
+ * B [adapters][outer][rank] bf16, scales [adapters] FP32; inner, outer and rank are
+ * multiples of 8, rank at most 128.  Sums are FP32, the result is rounded once.  Rows of no entry
+ * stay as they are.
+ *
+ * `workspace`: nmoe_adapters_workspace_bytes() bytes, 256-byte aligned, anything
+ * in it, this call's alone until it is done.  `error`: a device word, zero at first,
+ * for nmoe_adapters_sync_status: an id that is none (its rows get none) and offsets
+ * that do not rise within 0 to `rows` (such an entry's rows stay as they are). */
+typedef struct nmoe_adapters {
+  int32_t adapters;
+  int32_t rank;
+  int32_t inner;
+  int32_t outer;
+  const void* a;
+  const void* b;
+  const float* scales;
+} nmoe_adapters;
+
+/* 0 for sizes that are none. */
+NMOE_API size_t nmoe_adapters_workspace_bytes(const nmoe_adapters* pool, int64_t rows, int32_t count);
+NMOE_API nmoe_status nmoe_adapters_add(const nmoe_adapters* pool, void* stream, const void* x,
+                                       int64_t x_stride, const void* y, int64_t y_stride, void* out,
+                                       int64_t out_stride, int64_t rows, const int32_t* ids,
+                                       const int32_t* offsets, int32_t count, void* workspace,
+                                       size_t workspace_bytes, int32_t* error);
+/* Waits for the stream; what calls with this word found wrong, and clears it. */
+NMOE_API nmoe_status nmoe_adapters_sync_status(int32_t* error, void* stream);
+
 /* --- sampling ---------------------------------------------------------------------
  * A token for each row of logits [rows][vocab] (FP32 or bf16, `stride` elements
  * from row to row): in falling order of the logits, equal ones by rising

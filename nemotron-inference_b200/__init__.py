@@ -49,6 +49,7 @@ EXPORTED_SYMBOLS = (
     "nmoe_kv_compact", "nmoe_kv_copy_pages", "nmoe_kv_sync_status", "nmoe_attention_cached",
     "nmoe_attention_prefill", "nmoe_attention_sync_status", "nmoe_kv_find_shared",
     "nmoe_attention_shared_workspace_bytes", "nmoe_attention_shared", "nmoe_sample",
+    "nmoe_adapters_workspace_bytes", "nmoe_adapters_add", "nmoe_adapters_sync_status",
 )
 
 

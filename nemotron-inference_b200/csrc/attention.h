@@ -201,6 +201,9 @@ struct CachedArgs {
 // bf16 rows of heads x 128 as [rows][heads * 128], boxes of 64 columns x box_rows, 128-byte swizzle.
 bool rows_tensor_map(const void* base, int64_t rows, int64_t heads, int64_t stride, int box_rows,
                      CUtensorMap* map);
+// The same of any bf16 matrix [rows][columns]; what lies beside it reads as zeros.
+bool matrix_tensor_map(const void* base, int64_t rows, int64_t columns, int64_t stride, int box_rows,
+                       CUtensorMap* map);
 
 // A cache's codes as rows of 128 bytes, boxes of a page and head, 128-byte swizzle.
 bool pages_tensor_map(const PagedCache& cache, CUtensorMap* map);

@@ -170,7 +170,12 @@ static EncodeTiled encode_tiled() {
 
 bool rows_tensor_map(const void* base, int64_t rows, int64_t heads, int64_t stride, int box_rows,
                      CUtensorMap* map) {
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(heads) * kHeadDim, static_cast<cuuint64_t>(rows)};
+  return matrix_tensor_map(base, rows, heads * kHeadDim, stride, box_rows, map);
+}
+
+bool matrix_tensor_map(const void* base, int64_t rows, int64_t columns, int64_t stride, int box_rows,
+                       CUtensorMap* map) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
   const cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t steps[2] = {1u, 1u};
