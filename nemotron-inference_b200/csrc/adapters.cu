@@ -7,8 +7,8 @@
 //            ranks; those behind the rank are whatever lies there and their results are not read) and the rows of x as the
 //            one of 16 or 128, so that a single token costs no more than its own bytes.  The contraction is cut
 //            into parts where tiles are few; each leaves FP32 sums.
-//   outside  out = y + (scale t) B^T for a tile of 128 rows and 128 columns at a time.  t, summed up in a fixed order,
-//            is two bf16 terms (within 2^-17 of it; as one it would be off by 2^-9, of the size of what y's own rounding
+//   outside  out = y + (scale t) B^T, a block to an SM with an even share of all tiles of 128 rows and 128 columns, y and B
+//            on their way tiles ahead.  t, summed up in a fixed order, is two bf16 terms (within 2^-17 of it; as one it would be off by 2^-9, of the size of what y's own rounding
 //            leaves), both multiplied with the same tile of B into one sum; y is added in FP32 and the result rounded
 //            once.  Rows without an adapter are copied.
 #include <algorithm>
@@ -26,8 +26,7 @@ constexpr int kTile = 128;
 constexpr int kChunk = 64;  // columns of x and A at a time: rows of 128 bytes
 constexpr int kMostSplits = 16;
 constexpr int kMostStages = 8;
-constexpr int kInsideThreads = 192, kOutsideThreads = 320;
-constexpr int kOutsideStages = 3;
+constexpr int kInsideThreads = 192;
 constexpr uint32_t kPanelBytes = kTile * 128;  // 128 rows of 64 bf16
 
 // A tile of rows of one entry.
@@ -194,10 +193,39 @@ __global__ void __launch_bounds__(kInsideThreads)
   }
 }
 
+// Rows of one entry that a block works on, and their tiles of columns.
+struct Piece {
+  int first, rows, adapter;  // adapter -1: none
+  int from, to;              // tiles of columns
+};
+
+constexpr int kPieces = 4;  // known ahead
+constexpr int kMostOutsideStages = 3;
+constexpr int kSumWarps = 8, kTermWarps = 4;
+constexpr int kLoadWarp = kSumWarps, kMmaWarp = kSumWarps + 1, kFirstTermWarp = kSumWarps + 2;
+constexpr int kOutsideThreads = 32 * (kSumWarps + 2 + kTermWarps);
+constexpr uint32_t kTileBytes = 2 * kPanelBytes;  // 128 rows of 128 columns of y
+
 struct OutsideControl {
-  uint64_t full[kOutsideStages], empty[kOutsideStages], d_full[2], d_empty[2], t_full, drained;
+  uint64_t piece_full[kPieces], piece_empty[kPieces];
+  uint64_t y_full[kMostOutsideStages], y_empty[kMostOutsideStages], b_full[kMostOutsideStages], b_empty[kMostOutsideStages];
+  uint64_t d_full[2], d_empty[2], t_full[2], t_empty[2], drained;
+  Piece piece[kPieces];
+  int some[kPieces];
   uint32_t tmem;
-  Found found;
+  int before[32];
+  int64_t begin, end;        // this block's tiles, in order of the rows
+  int entry;                 // the entry in which they begin, and the first tile of its
+  int64_t entry_begin;
+};
+
+// Stages of a block's shared memory, by the panels of 64 ranks.
+struct OutsideLayout {
+  int panels, stages, terms;  // stages of y and B, buffers of t
+  __host__ __device__ explicit OutsideLayout(int rank) : panels((rank + kChunk - 1) / kChunk), stages(panels > 1 ? 2 : 3), terms(panels > 1 ? 1 : 2) {}
+  __host__ __device__ uint32_t b_bytes() const { return panels * kPanelBytes; }
+  __host__ __device__ uint32_t t_bytes() const { return 2 * panels * kPanelBytes; }
+  __host__ __device__ uint32_t total() const { return stages * (kTileBytes + b_bytes()) + terms * t_bytes(); }
 };
 
 // 16 bytes of y and sums of eight columns.
@@ -212,172 +240,360 @@ __device__ __forceinline__ uint4 add_eight(const uint4& y, const uint32_t* d) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// blockIdx.y: `tiles_each` tiles of columns.
-__global__ void __launch_bounds__(kOutsideThreads, 2)
-    outside_kernel(const __grid_constant__ CUtensorMap map_b, const AdapterArgs args, int splits, int tiles_each) {
-  extern __shared__ uint8_t raw[];
-  OutsideControl* c = reinterpret_cast<OutsideControl*>(raw);
-  const int panels = (args.rank + kChunk - 1) / kChunk;
-  uint8_t* terms = raw + sizeof(OutsideControl);  // of t: first terms, second terms, `panels` panels each
-  terms += (1024 - (smem_u32(terms) & 1023)) & 1023;
-  uint8_t* ring = terms + 2 * panels * kPanelBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Entry i, empty where its offsets do not rise within the rows.
+__device__ __forceinline__ Piece entry_of(const AdapterArgs& args, int i) {
+  Piece p;
+  const int from = args.offsets[i], to = args.offsets[i + 1], id = args.ids[i];
+  p.first = from;
+  p.rows = from >= 0 && from <= to && to <= args.rows ? to - from : 0;
+  p.adapter = static_cast<unsigned>(id) < static_cast<unsigned>(args.adapters) ? id : -1;
+  p.from = p.to = 0;
+  return p;
+}
+
+// All threads: this block's share of all tiles of 128 rows and columns.
+__device__ void find_share(const AdapterArgs& args, int columns, OutsideControl* c) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = (args.count + kOutsideThreads - 1) / kOutsideThreads;
+  const int begin = min(static_cast<int>(threadIdx.x) * each, args.count), end = min(begin + each, args.count);
+  int mine = 0;
+#pragma unroll 4
+  for (int i = begin; i < end; ++i) mine += (entry_of(args, i).rows + kTile - 1) / kTile;
+  int upto = mine;
+#pragma unroll
+  for (int step = 1; step < 32; step *= 2) {
+    const int other = __shfl_up_sync(0xffffffffu, upto, step);
+    if (lane >= step) upto += other;
+  }
+  if (lane == 31) c->before[warp] = upto;
+  __syncthreads();
+  int at = upto - mine, total = 0;
+  for (int w = 0; w < kOutsideThreads / 32; ++w) {
+    if (w < warp) at += c->before[w];
+    total += c->before[w];
+  }
+  const int64_t all = static_cast<int64_t>(total) * columns;
+  const int64_t from = all * blockIdx.x / gridDim.x, to = all * (blockIdx.x + 1) / gridDim.x;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kOutsideStages; ++i) {
-      mbar_init(&c->full[i], 1);
-      mbar_init(&c->empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&c->d_full[i], 1);
-      mbar_init(&c->d_empty[i], 8);
-    }
-    mbar_init(&c->t_full, 8);
-    mbar_init(&c->drained, 1);
-    fence_barrier_init();
+    c->begin = from;
+    c->end = to;
   }
-  if (warp == 9) {
-    tmem_alloc(&c->tmem, 2 * kTile);
-    tmem_relinquish();
+  if (from < to && from >= static_cast<int64_t>(at) * columns && from < static_cast<int64_t>(at + mine) * columns) {  // one thread's
+    for (int i = begin; i < end; ++i) {
+      const int tiles = (entry_of(args, i).rows + kTile - 1) / kTile;
+      if (from < static_cast<int64_t>(at + tiles) * columns) {
+        c->entry = i;
+        c->entry_begin = static_cast<int64_t>(at) * columns;
+        break;
+      }
+      at += tiles;
+    }
   }
-  tcgen05_fence_before();
-  wait_for_predecessor();
-  const RowsTile t = find_tile(args, blockIdx.x, kTile, &c->found);
-  release_successor();  // (the columns of TMEM are there)
-  tcgen05_fence_after();
-  const uint32_t tmem = c->tmem;
-  const int all = (args.outer + kTile - 1) / kTile, from = blockIdx.y * tiles_each;
-  const int count = t.rows > 0 ? min(tiles_each, all - from) : 0;
-  const bool adapted = t.adapter >= 0;
-  const int steps = (args.rank + 15) / 16;
-  const uint32_t stage_bytes = panels * kPanelBytes;
-  if (warp == 8) {
-    bool ok = true;
-    int i = 0;
-    for (; adapted && i < count && ok; ++i) {
-      const int stage = i % kOutsideStages;
-      ok = mbar_wait_warp(smem_u32(&c->empty[stage]), ((i / kOutsideStages) & 1) ^ 1);
-      if (ok && elect_one()) {
-        const uint32_t bar = smem_u32(&c->full[stage]), to = smem_u32(ring) + stage * stage_bytes;
-        mbar_arrive_expect_tx_at(bar, stage_bytes);
-        for (int p = 0; p < panels; ++p) {
-          tma_load_2d_at(to + p * kPanelBytes, &map_b, p * kChunk, t.adapter * args.outer + (from + i) * kTile, bar);
-        }
+  __syncthreads();
+}
+
+// The warp that finds the block's pieces, and brings in y and B.
+__device__ bool load_role(const AdapterArgs& args, const CUtensorMap* y_rows, const CUtensorMap* y_few, const CUtensorMap* b_map, uint32_t y_at,
+                          uint32_t b_at, const OutsideLayout& layout, int columns, OutsideControl* c) {
+  const int lane = threadIdx.x & 31;
+  const bool in_place = args.out == args.y;
+  uint32_t pieces = 0, units = 0, adapted = 0;
+  int64_t at = c->begin;
+  const int64_t stop = c->end;
+  int64_t entry_at = c->entry_begin;
+  bool ok = true;
+#pragma unroll 1
+  for (int i = c->entry; at < stop && i < args.count; ++i) {
+    const Piece e = entry_of(args, i);
+    const int row_tiles = (e.rows + kTile - 1) / kTile;
+#pragma unroll 1
+    for (int tile = static_cast<int>((at - entry_at) / columns); tile < row_tiles && at < stop; ++tile) {
+      const int64_t tile_at = entry_at + static_cast<int64_t>(tile) * columns;
+      Piece p;
+      p.first = e.first + tile * kTile;
+      p.rows = min(e.rows - tile * kTile, kTile);
+      p.adapter = e.adapter;
+      p.from = static_cast<int>(at - tile_at);
+      p.to = static_cast<int>(min(stop - tile_at, static_cast<int64_t>(columns)));
+      at = tile_at + p.to;
+      if (in_place && p.adapter < 0) continue;  // (these stay)
+      const uint32_t place = pieces % kPieces;
+      if (!mbar_wait_warp(smem_u32(&c->piece_empty[place]), ((pieces / kPieces) & 1) ^ 1)) return false;
+      if (lane == 0) {
+        c->piece[place] = p;
+        c->some[place] = 1;
+        mbar_arrive(&c->piece_full[place]);
       }
       __syncwarp();
-    }
-    if (!ok) {  // what is in flight arrives before the block's shared memory is given up
-      if (lane == 0) report_cache_error(args.error, kDevWaitTimeout);
-      for (int back = max(0, i - 1 - kOutsideStages); back < i - 1; ++back) {
-        mbar_wait_warp(smem_u32(&c->full[back % kOutsideStages]), (back / kOutsideStages) & 1);
+      ++pieces;
+      const int boxes = p.rows > kTile / 2 ? 1 : (p.rows + 7) / 8;  // of 128 rows, or of 8
+      const uint32_t bytes = boxes == 1 && p.rows > 8 ? kTileBytes : boxes * 2048;
+#pragma unroll 1
+      for (int column = p.from; column < p.to; ++column, ++units) {
+        const uint32_t stage = units % layout.stages, y_bar = smem_u32(&c->y_full[stage]), to = y_at + stage * kTileBytes;
+        if (!mbar_wait_warp(smem_u32(&c->y_empty[stage]), ((units / layout.stages) & 1) ^ 1)) return false;
+        if (elect_one()) {
+          mbar_arrive_expect_tx_at(y_bar, bytes);
+          for (int half = 0; half < 2; ++half) {
+            if (bytes == kTileBytes) {
+              tma_load_2d_at(to + half * kPanelBytes, y_rows, column * kTile + half * 64, p.first, y_bar);
+            } else {
+              for (int k = 0; k < boxes; ++k) {
+                tma_load_2d_at(to + half * kPanelBytes + k * 1024, y_few, column * kTile + half * 64, p.first + 8 * k, y_bar);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (p.adapter < 0) continue;
+        const uint32_t b_stage = adapted % layout.stages, b_bar = smem_u32(&c->b_full[b_stage]);
+        if (!mbar_wait_warp(smem_u32(&c->b_empty[b_stage]), ((adapted / layout.stages) & 1) ^ 1)) return false;
+        if (elect_one()) {
+          mbar_arrive_expect_tx_at(b_bar, layout.b_bytes());
+          for (int k = 0; k < layout.panels; ++k) {
+            tma_load_2d_at(b_at + b_stage * layout.b_bytes() + k * kPanelBytes, b_map, k * kChunk, p.adapter * args.outer + column * kTile,
+                           b_bar);
+          }
+        }
+        __syncwarp();
+        ++adapted;
       }
     }
-  } else if (warp == 9) {
-    constexpr uint32_t kDesc = make_idesc_bf16(kTile, false);
-    bool ok = !adapted || count <= 0 || mbar_wait_warp(smem_u32(&c->t_full), 0);
-    for (int i = 0; adapted && i < count && ok; ++i) {
-      const int stage = i % kOutsideStages, buffer = i & 1;
-      ok = mbar_wait_warp(smem_u32(&c->full[stage]), (i / kOutsideStages) & 1);
-      ok = ok && mbar_wait_warp(smem_u32(&c->d_empty[buffer]), ((i >> 1) & 1) ^ 1);
+    entry_at += static_cast<int64_t>(row_tiles) * columns;
+  }
+  const uint32_t place = pieces % kPieces;
+  if (!mbar_wait_warp(smem_u32(&c->piece_empty[place]), ((pieces / kPieces) & 1) ^ 1)) return false;
+  if (lane == 0) {
+    c->some[place] = 0;
+    mbar_arrive(&c->piece_full[place]);
+  }
+  return ok;
+}
+
+// The next piece; false behind the last. `ok` falls where the wait runs out.
+__device__ __forceinline__ bool next_piece(OutsideControl* c, uint32_t pieces, Piece& p, bool& ok) {
+  const uint32_t place = pieces % kPieces;
+  ok = mbar_wait_warp(smem_u32(&c->piece_full[place]), (pieces / kPieces) & 1);
+  if (!ok || !c->some[place]) return false;
+  p = c->piece[place];
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&c->piece_empty[place]);
+  return true;
+}
+
+__device__ bool mma_role(uint32_t t_at, uint32_t b_at, uint32_t tmem, const OutsideLayout& layout, int rank, OutsideControl* c) {
+  constexpr uint32_t kDesc = make_idesc_bf16(kTile, false);
+  const int steps = (rank + 15) / 16;
+  uint32_t adapted = 0, records = 0;
+  bool ok;
+  Piece p;
+#pragma unroll 1
+  for (uint32_t pieces = 0; next_piece(c, pieces, p, ok); ++pieces) {
+    if (p.adapter < 0) continue;
+    const uint32_t buffer_t = records % layout.terms;
+    if (!mbar_wait_warp(smem_u32(&c->t_full[buffer_t]), (records / layout.terms) & 1)) return false;
+    const uint64_t t_desc = make_smem_desc(t_at + buffer_t * layout.t_bytes(), 16, 1024, 2);
+#pragma unroll 1
+    for (int column = p.from; column < p.to; ++column, ++adapted) {
+      const uint32_t stage = adapted % layout.stages, buffer = adapted & 1;
+      if (!mbar_wait_warp(smem_u32(&c->b_full[stage]), (adapted / layout.stages) & 1)) return false;
+      if (!mbar_wait_warp(smem_u32(&c->d_empty[buffer]), ((adapted >> 1) & 1) ^ 1)) return false;
       tcgen05_fence_after();
-      if (ok && elect_one()) {
-        const uint64_t t_desc = make_smem_desc(smem_u32(terms), 16, 1024, 2);
-        const uint64_t b_desc = make_smem_desc(smem_u32(ring) + stage * stage_bytes, 16, 1024, 2);
+      if (elect_one()) {
+        const uint64_t b_desc = make_smem_desc(b_at + stage * layout.b_bytes(), 16, 1024, 2);
         for (int term = 0; term < 2; ++term) {
           for (int k = 0; k < steps; ++k) {
             const uint32_t at = k / 4 * kPanelBytes + k % 4 * 32;
-            mma_f16_ss(tmem + buffer * kTile, advance_smem_desc(t_desc, term * panels * kPanelBytes + at), advance_smem_desc(b_desc, at),
-                       kDesc, term > 0 || k > 0);
+            mma_f16_ss(tmem + buffer * kTile, advance_smem_desc(t_desc, term * layout.b_bytes() + at), advance_smem_desc(b_desc, at), kDesc,
+                       term > 0 || k > 0);
           }
         }
         tcgen05_commit(&c->d_full[buffer]);
-        tcgen05_commit(&c->empty[stage]);
+        tcgen05_commit(&c->b_empty[stage]);
+        if (column + 1 == p.to) tcgen05_commit(&c->t_empty[buffer_t]);
       }
       __syncwarp();
     }
-    if (elect_one()) {
-      if (!ok) report_cache_error(args.error, kDevWaitTimeout);
-      tcgen05_commit(&c->drained);
-    }
-    __syncwarp();
-    mbar_wait_warp(smem_u32(&c->drained), 0);
-  } else if (count > 0) {
-    // a thread to a row, and to half of a tile's columns
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
-    const bool valid = row < t.rows;
-    const __nv_bfloat16* y = args.y + static_cast<int64_t>(t.first + row) * args.y_stride;
-    __nv_bfloat16* out = args.out + static_cast<int64_t>(t.first + row) * args.out_stride;
-    if (adapted) {
-      if (valid) {
-        const float scale = args.scales[t.adapter];
-        const float* inside = args.inside + static_cast<size_t>(t.first + row) * args.rank;
-        const size_t split = static_cast<size_t>(args.rows) * args.rank;
-        for (int chunk = half; chunk < 2 * steps; chunk += 2) {  // of eight ranks
-          float v[8];
+    ++records;
+  }
+  return ok;
+}
+
+// Four warps that sum up t and put it into shared memory as two bf16 terms.
+__device__ bool term_role(const AdapterArgs& args, uint8_t* terms, const OutsideLayout& layout, int splits, OutsideControl* c) {
+  const int thread = threadIdx.x - 32 * kFirstTermWarp;
+  const int eights = (args.rank + 15) / 16 * 2;  // of ranks, filled up to whole steps of an MMA
+  const size_t split = static_cast<size_t>(args.rows) * args.rank;
+  uint32_t records = 0;
+  bool ok;
+  Piece p;
+#pragma unroll 1
+  for (uint32_t pieces = 0; next_piece(c, pieces, p, ok); ++pieces) {
+    if (p.adapter < 0) continue;
+    if (records == 0) wait_for_predecessor();  // (the first launch; all else was there before that)
+    const uint32_t buffer = records % layout.terms;
+    if (!mbar_wait_warp(smem_u32(&c->t_empty[buffer]), ((records / layout.terms) & 1) ^ 1)) return false;
+    const float scale = args.scales[p.adapter];
+    const float* inside = args.inside + static_cast<size_t>(p.first) * args.rank;
+#pragma unroll 1
+    for (int i = thread; i < p.rows * eights; i += 32 * kTermWarps) {
+      const int row = i / eights, eight = i - row * eights;
+      float v[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-          if (chunk * 8 < args.rank) {
-            for (int s = 0; s < splits; ++s) {
-              const float4 lo = __ldcg(reinterpret_cast<const float4*>(inside + s * split + chunk * 8));
-              const float4 hi = __ldcg(reinterpret_cast<const float4*>(inside + s * split + chunk * 8) + 1);
-              v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
-              v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+      if (eight * 8 < args.rank) {
+        const float4* from = reinterpret_cast<const float4*>(inside + static_cast<size_t>(row) * args.rank + eight * 8);
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+          const float4 lo = __ldcg(from), hi = __ldcg(from + 1);
+          from = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(from) + split);
+          v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+          v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+        }
+      }
+      uint32_t first[4], second[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float x = v[2 * k] * scale, z = v[2 * k + 1] * scale;
+        first[k] = pack_bf16(x, z);
+        const float x1 = __uint_as_float(first[k] << 16), z1 = __uint_as_float(first[k] & 0xffff0000u);
+        // (nothing is left of what has become infinite)
+        second[k] = pack_bf16(fabsf(x1) < INFINITY ? x - x1 : 0.0f, fabsf(z1) < INFINITY ? z - z1 : 0.0f);
+      }
+      uint8_t* to = terms + buffer * layout.t_bytes() + (eight >> 3) * kPanelBytes + row * 128 + (((eight & 7) ^ (row & 7)) << 4);
+      *reinterpret_cast<uint4*>(to) = make_uint4(first[0], first[1], first[2], first[3]);
+      *reinterpret_cast<uint4*>(to + layout.b_bytes()) = make_uint4(second[0], second[1], second[2], second[3]);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&c->t_full[buffer]);
+    ++records;
+  }
+  return ok;
+}
+
+// Eight warps that add up: a thread to a row and half of a tile's columns, whose results go over y's in shared memory
+// and from there, by the same warp, to memory, whole lines at a time.
+__device__ bool sum_role(const AdapterArgs& args, uint8_t* y, uint32_t tmem, const OutsideLayout& layout, OutsideControl* c) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = (warp & 3) * 32, row = row0 + lane, half = warp >> 2;
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * 64;
+  uint32_t units = 0, adapted = 0;
+  bool ok;
+  Piece p;
+#pragma unroll 1
+  for (uint32_t pieces = 0; next_piece(c, pieces, p, ok); ++pieces) {
+    const bool some = row0 < p.rows, with = p.adapter >= 0;
+    __nv_bfloat16* out = args.out + static_cast<int64_t>(p.first) * args.out_stride;
+#pragma unroll 1
+    for (int column = p.from; column < p.to; ++column, ++units) {
+      const uint32_t stage = units % layout.stages, buffer = adapted & 1;
+      uint8_t* tile = y + stage * kTileBytes + half * kPanelBytes;
+      if (!mbar_wait_warp(smem_u32(&c->y_full[stage]), (units / layout.stages) & 1)) return false;
+      if (with) {
+        if (!mbar_wait_warp(smem_u32(&c->d_full[buffer]), (adapted >> 1) & 1)) return false;
+        tcgen05_fence_after();
+        if (some) {
+#pragma unroll
+          for (int k = 0; k < 8; k += 4) {
+            uint32_t d[32];
+            tmem_ld_x32_async(lanes + buffer * kTile + k * 8, d);
+            tmem_ld_wait();
+            registers_loaded<32>(d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint4* at = reinterpret_cast<uint4*>(tile + row * 128 + (((k + j) ^ (row & 7)) << 4));
+              *at = add_eight(*at, d + 8 * j);
             }
           }
-          uint32_t first[4], second[4];
+        }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c->d_empty[buffer]);
+        ++adapted;
+      }
+      if (some) {
+        const int at = column * kTile + half * 64 + (lane & 7) * 8;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = v[2 * i] * scale, q = v[2 * i + 1] * scale;
-            first[i] = pack_bf16(p, q);
-            const float p1 = __uint_as_float(first[i] << 16), q1 = __uint_as_float(first[i] & 0xffff0000u);
-            // (nothing is left of what has become infinite)
-            second[i] = pack_bf16(fabsf(p1) < INFINITY ? p - p1 : 0.0f, fabsf(q1) < INFINITY ? q - q1 : 0.0f);
+        for (int k = 0; k < 8; ++k) {
+          const int r = row0 + k * 4 + (lane >> 3);
+          if (r < p.rows && at < args.outer) {
+            *reinterpret_cast<uint4*>(out + r * args.out_stride + at) =
+                *reinterpret_cast<const uint4*>(tile + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
           }
-          uint8_t* to = terms + (chunk >> 3) * kPanelBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
-          *reinterpret_cast<uint4*>(to) = make_uint4(first[0], first[1], first[2], first[3]);
-          *reinterpret_cast<uint4*>(to + panels * kPanelBytes) = make_uint4(second[0], second[1], second[2], second[3]);
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&c->t_full);
+      if (lane == 0) mbar_arrive(&c->y_empty[stage]);
     }
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * 64;
-    bool ok = true;
-    for (int i = 0; i < count && ok; ++i) {
-      const int buffer = i & 1, column = (from + i) * kTile + half * 64;
-      uint4 had[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (valid && column + k * 8 < args.outer) had[k] = *reinterpret_cast<const uint4*>(y + column + k * 8);
-      }
-      if (!adapted) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (valid && column + k * 8 < args.outer) *reinterpret_cast<uint4*>(out + column + k * 8) = had[k];
-        }
-        continue;
-      }
-      ok = mbar_wait_warp(smem_u32(&c->d_full[buffer]), (i >> 1) & 1);
-      tcgen05_fence_after();
-#pragma unroll
-      for (int k = 0; k < 8; k += 2) {
-        uint32_t d[16];
-        tmem_ld_x16_async(lanes + buffer * kTile + k * 8, d);
-        tmem_ld_wait();
-        registers_loaded<16>(d);
-        if (!valid || !ok) continue;
-        if (column + k * 8 < args.outer) *reinterpret_cast<uint4*>(out + column + k * 8) = add_eight(had[k], d);
-        if (column + k * 8 + 8 < args.outer) *reinterpret_cast<uint4*>(out + column + k * 8 + 8) = add_eight(had[k + 1], d + 8);
-      }
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c->d_empty[buffer]);
+  }
+  return ok;
+}
+
+// A block to an SM, each with its share of the tiles of 128 rows and columns.
+__global__ void __launch_bounds__(kOutsideThreads, 1)
+    outside_kernel(const __grid_constant__ CUtensorMap y_rows, const __grid_constant__ CUtensorMap y_few,
+                   const __grid_constant__ CUtensorMap b_map, const AdapterArgs args, int splits) {
+  extern __shared__ uint8_t raw[];
+  OutsideControl* c = reinterpret_cast<OutsideControl*>(raw);
+  const OutsideLayout layout(args.rank);
+  uint8_t* y = raw + sizeof(OutsideControl);
+  y += (1024 - (smem_u32(y) & 1023)) & 1023;
+  uint8_t* b = y + layout.stages * kTileBytes;
+  uint8_t* terms = b + layout.stages * layout.b_bytes();
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPieces; ++i) {
+      mbar_init(&c->piece_full[i], 1);
+      mbar_init(&c->piece_empty[i], kSumWarps + 1 + kTermWarps);
     }
-    if (!ok && lane == 0) report_cache_error(args.error, kDevWaitTimeout);
+    for (int i = 0; i < kMostOutsideStages; ++i) {
+      mbar_init(&c->y_full[i], 1);
+      mbar_init(&c->y_empty[i], kSumWarps);
+      mbar_init(&c->b_full[i], 1);
+      mbar_init(&c->b_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&c->d_full[i], 1);
+      mbar_init(&c->d_empty[i], kSumWarps);
+      mbar_init(&c->t_full[i], kTermWarps);
+      mbar_init(&c->t_empty[i], 1);
+    }
+    mbar_init(&c->drained, 1);
+    c->entry = 0;
+    c->entry_begin = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&c->tmem, 2 * kTile);
+    tmem_relinquish();
   }
   tcgen05_fence_before();
+  const int columns = (args.outer + kTile - 1) / kTile;
+  // (the lists, y and B were there before the first launch, whose blocks have all waited for that when this one's begin)
+  find_share(args, columns, c);
+  release_successor();  // (the columns of TMEM are there)
+  tcgen05_fence_after();
+  const uint32_t tmem = c->tmem;
+  bool ok;
+  if (warp < kSumWarps) {
+    ok = sum_role(args, y, tmem, layout, c);
+  } else if (warp == kLoadWarp) {
+    ok = load_role(args, &y_rows, &y_few, &b_map, smem_u32(y), smem_u32(b), layout, columns, c);
+  } else if (warp == kMmaWarp) {
+    ok = mma_role(smem_u32(terms), smem_u32(b), tmem, layout, args.rank, c);
+    if (elect_one()) tcgen05_commit(&c->drained);
+    __syncwarp();
+    mbar_wait_warp(smem_u32(&c->drained), 0);
+  } else {
+    ok = term_role(args, terms, layout, splits, c);
+  }
+  if (!ok && (threadIdx.x & 31) == 0) report_cache_error(args.error, kDevWaitTimeout);
+  wait_for_predecessor();  // (this launch ends behind the first)
+  tcgen05_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tcgen05_fence_after();
     tmem_dealloc(tmem, 2 * kTile);
   }
@@ -386,19 +602,16 @@ __global__ void __launch_bounds__(kOutsideThreads, 2)
 // How a call is cut.
 struct Plan {
   int height;       // rows of a tile of the first launch
-  int tiles[2];     // of both launches, at most
+  int tiles;        // of these, at most
   int chunks_each, splits, stages;
   size_t inside_shared;
 
   Plan(int64_t rows, int count, int inner, int rank, int sms) {
     // A tile of 16 rows holds its sums in fewer columns and less shared memory; one of 128 reads A once for more rows.
     height = rows <= 16 * static_cast<int64_t>(count) ? 16 : kTile;
-    for (int k = 0; k < 2; ++k) {
-      const int h = k ? kTile : height;
-      tiles[k] = static_cast<int>(std::min<int64_t>(rows, rows / h + count));
-    }
+    tiles = static_cast<int>(std::min<int64_t>(rows, rows / height + count));
     const int chunks = (inner + kChunk - 1) / kChunk;
-    splits = std::clamp(2 * sms / std::max(tiles[0], 1), 1, std::min(kMostSplits, std::max(chunks / 3, 1)));
+    splits = std::clamp(2 * sms / tiles, 1, std::min(kMostSplits, std::max(chunks / 3, 1)));
     chunks_each = (chunks + splits - 1) / splits;
     splits = (chunks + chunks_each - 1) / chunks_each;
     const size_t stage = static_cast<size_t>(rank + height) * 128;
@@ -416,10 +629,12 @@ size_t adapter_workspace_bytes(int64_t rows, int count, int inner, int rank) {
 cudaError_t launch_adapters(const AdapterArgs& args, cudaStream_t stream) {
   const int sms = device_sms();
   const Plan plan(args.rows, args.count, args.inner, args.rank, sms);
-  CUtensorMap map_x, map_a, map_b;
+  CUtensorMap map_x, map_a, map_b, y_rows, y_few;
   if (!matrix_tensor_map(args.x, args.rows, args.inner, args.x_stride, 8, &map_x) ||
       !matrix_tensor_map(args.a, static_cast<int64_t>(args.adapters) * args.rank, args.inner, args.inner, args.rank, &map_a) ||
-      !matrix_tensor_map(args.b, static_cast<int64_t>(args.adapters) * args.outer, args.rank, args.rank, kTile, &map_b)) {
+      !matrix_tensor_map(args.b, static_cast<int64_t>(args.adapters) * args.outer, args.rank, args.rank, kTile, &map_b) ||
+      !matrix_tensor_map(args.y, args.rows, args.outer, args.y_stride, kTile, &y_rows) ||
+      !matrix_tensor_map(args.y, args.rows, args.outer, args.y_stride, 8, &y_few)) {
     return cudaErrorInvalidValue;
   }
   static std::atomic<uint64_t> allowed[3];
@@ -428,15 +643,12 @@ cudaError_t launch_adapters(const AdapterArgs& args, cudaStream_t stream) {
   if (err == cudaSuccess) err = allow_shared_memory_once(outside_kernel, allowed[2]);
   if (err != cudaSuccess) return err;
   auto* inside = plan.height == 16 ? inside_kernel<16> : inside_kernel<kTile>;
-  err = launch_kernel(inside, dim3(plan.tiles[0], plan.splits), kInsideThreads, plan.inside_shared, LaunchStream(stream, true), map_x,
+  err = launch_kernel(inside, dim3(plan.tiles, plan.splits), kInsideThreads, plan.inside_shared, LaunchStream(stream, true), map_x,
                       map_a, args, plan.chunks_each, plan.stages);
   if (err != cudaSuccess) return err;
-  const int all = (args.outer + kTile - 1) / kTile;
-  const int groups = std::clamp(4 * sms / plan.tiles[1], 1, all), tiles_each = (all + groups - 1) / groups;
-  const int panels = (args.rank + kChunk - 1) / kChunk;
-  const size_t shared = sizeof(OutsideControl) + 1024 + (2 + kOutsideStages) * static_cast<size_t>(panels) * kPanelBytes;
-  return launch_kernel(outside_kernel, dim3(plan.tiles[1], (all + tiles_each - 1) / tiles_each), kOutsideThreads, shared,
-                       LaunchStream(stream, true), map_b, args, plan.splits, tiles_each);
+  const size_t shared = sizeof(OutsideControl) + 1024 + OutsideLayout(args.rank).total();
+  return launch_kernel(outside_kernel, dim3(sms), kOutsideThreads, shared, LaunchStream(stream, true), y_rows, y_few, map_b, args,
+                       plan.splits);
 }
 
 }  // namespace nmoe
