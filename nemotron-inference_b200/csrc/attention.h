@@ -207,6 +207,8 @@ bool matrix_tensor_map(const void* base, int64_t rows, int64_t columns, int64_t 
 
 // A cache's codes as rows of 128 bytes, boxes of a page and head, 128-byte swizzle.
 bool pages_tensor_map(const PagedCache& cache, CUtensorMap* map);
+// Any rows of 128 codes.
+bool codes_tensor_map(const uint8_t* codes, int64_t rows, int box_rows, CUtensorMap* map);
 
 cudaError_t launch_attention_prefill(const PrefillArgs& args, cudaStream_t stream);
 // The workspace begins with counters, zero between calls.
@@ -218,6 +220,12 @@ cudaError_t launch_attention_cached(const CachedArgs& args, cudaStream_t stream)
 size_t attention_cached_slot_bytes();
 int attention_cached_slot_rows(int64_t rows);  // that a piece has room for
 cudaError_t launch_cached_part(const CachedArgs& args, Part part, int64_t rows, float* slots, cudaStream_t stream);
+// Of shared tokens, for more rows of queries than that (csrc/attention_shared_rows.cu).
+size_t shared_pairs_slot_bytes();
+int shared_pairs_slot_rows();
+size_t shared_pairs_query_bytes(int64_t rows, int heads);  // of `query_space`, 256-byte aligned
+bool shared_pairs_supported(int64_t rows, int heads);
+cudaError_t launch_shared_pairs(const CachedArgs& args, float* slots, char* query_space, cudaStream_t stream);
 // The same results for a batch whose sequences share their first pages; `workspace`:
 // attention_shared_workspace_bytes().
 size_t attention_shared_workspace_bytes(int64_t rows, int heads);

@@ -187,15 +187,19 @@ bool matrix_tensor_map(const void* base, int64_t rows, int64_t columns, int64_t 
 }
 
 bool pages_tensor_map(const PagedCache& cache, CUtensorMap* map) {
-  const uint64_t rows = static_cast<uint64_t>(cache.layers) * cache.pages * 2 * cache.kv_heads * cache.page_tokens;
+  return codes_tensor_map(cache.codes, static_cast<int64_t>(cache.layers) * cache.pages * 2 * cache.kv_heads * cache.page_tokens,
+                          cache.page_tokens, map);
+}
+
+bool codes_tensor_map(const uint8_t* codes, int64_t rows, int box_rows, CUtensorMap* map) {
   if (rows > INT32_MAX) return false;  // a coordinate has 31 bits: 256 GB of codes
-  const cuuint64_t dims[2] = {kHeadDim, rows};
+  const cuuint64_t dims[2] = {kHeadDim, static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {kHeadDim};
-  const cuuint32_t box[2] = {kHeadDim, static_cast<cuuint32_t>(cache.page_tokens)};
+  const cuuint32_t box[2] = {kHeadDim, static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t steps[2] = {1u, 1u};
   const EncodeTiled encode = encode_tiled();
   return encode != nullptr &&
-         encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, cache.codes, dims, strides, box, steps,
+         encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, steps,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

@@ -31,6 +31,7 @@ struct Shape {
   static constexpr int kSoftmaxWarps = 4;
   static constexpr int kBatch = R / kSoftmaxWarps;  // rows of queries to a warp
   static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
+  static constexpr int kValueReaders = 1, kSegmentReaders = kSoftmaxWarps + 1, kQueryWriters = kSoftmaxWarps;
   static constexpr int kColumns = 3 * kWidth <= 64 ? 64 : 128;  // two buffers of S, and O
   static constexpr uint32_t kQueryBytes = 2 * R * kHeadDim, kWeightBytes = 2 * R * kKeyTile;
 };

@@ -200,7 +200,7 @@ __device__ __forceinline__ float power_of_two(int e) {  // -126 <= e <= 127
 
 // Entry i of a part of the work: of the batch, or a group as one, whose rows are all its members' and whose tokens those
 // that they share, as the first of them with rows has them.
-static __device__ __noinline__ BatchEntry group_entry(const CachedArgs& args, int g) {
+__device__ __forceinline__ BatchEntry group_entry(const CachedArgs& args, int g) {
   const Batch& b = args.batch;
   BatchEntry e;
   e.sequence = e.first = e.rows = e.length = e.skip = 0;
@@ -339,9 +339,15 @@ __device__ void find_begin(const CachedArgs& args, WorkControl<S>* c) {
   }
 }
 
-// The warp that brings keys and values in, a page at a time.
-template <typename S, Part P>
-__device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32_t keys_at, uint32_t values_at, WorkControl<S>* c) {
+struct NoQueries {
+  __device__ bool operator()(const Segment&, uint32_t) const { return true; }
+};
+
+// The warp that brings keys and values in, a page at a time, and by `load_queries(segment, number)` what else a segment
+// needs.
+template <typename S, Part P, typename Queries = NoQueries>
+__device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32_t keys_at, uint32_t values_at, WorkControl<S>* c,
+                          Queries load_queries = Queries()) {
   const PagedCache& cache = args.cache;
   const int lane = threadIdx.x & 31, g = blockIdx.x;
   const Shares shares = c->shares;
@@ -389,6 +395,7 @@ __device__ void load_role(const CachedArgs& args, const CUtensorMap* map, uint32
         mbar_arrive(&c->segment_full[place]);
       }
       __syncwarp();
+      if (!(ok = load_queries(s, segments))) break;
       ++segments;
       int first_page = -1, page = 0, k_power = 0, v_power = 0;  // a lane per page, 32 at a time
 #pragma unroll 1
@@ -495,8 +502,37 @@ __device__ __forceinline__ void load_queries(const CachedArgs& args, const Segme
   }
 }
 
-// ... and put into shared memory as two terms, each row scaled by a power of two.  The second terms, kRows rows
-// behind the first, are multiplied by `Second`.
+// Four elements of a row of queries to a lane: their codes as two terms, the row scaled by a power of two, the second
+// terms multiplied by `Second`; `factor`: what the row's products of codes are multiplied by.
+template <int Second>
+__device__ __forceinline__ void query_terms(const uint2& raw, float scale, uint32_t& first, uint32_t& second, float& factor) {
+  float x[4];
+  x[0] = __uint_as_float(raw.x << 16);
+  x[1] = __uint_as_float(raw.x & 0xffff0000u);
+  x[2] = __uint_as_float(raw.y << 16);
+  x[3] = __uint_as_float(raw.y & 0xffff0000u);
+  // (magnitudes as whole numbers: what is no number is beyond them all)
+  const uint32_t m = max(max(raw.x & 0x7fffu, (raw.x >> 16) & 0x7fffu), max(raw.y & 0x7fffu, (raw.y >> 16) & 0x7fffu));
+  const int largest = static_cast<int>(__reduce_max_sync(0xffffffffu, m));
+  // the largest element's exponent becomes 7: below 256
+  const int power = max(largest >> 7, 1) - 134;
+  const int some = max(power, -100), rest = power - some;  // (2^-power may be beyond FP32)
+  const float down = power_of_two(-some), downer = power_of_two(-rest);
+  uint32_t a[2], b[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const __half2 v = __floats2half2_rn(x[2 * i] * down * downer, x[2 * i + 1] * down * downer);
+    a[i] = codes_of(v);
+    b[i] = codes_of(__hmul2(__hsub2(v, halves_of(a[i])), __float2half2_rn(static_cast<float>(Second))));
+  }
+  first = a[0] | (a[1] << 16);
+  second = b[0] | (b[1] << 16);
+  // (a row that is no number: its scores are none)
+  factor = largest < 0x7f80 ? scale * kLog2e * power_of_two(some) * power_of_two(rest) : NAN;
+}
+
+// ... and put into shared memory as two terms.  The second terms, kRows rows behind the first, are multiplied by
+// `Second`.
 template <typename S, int Second>
 __device__ __forceinline__ void store_queries(const CachedArgs& args, const Segment& s, int which, int batch,
                                               const uint2 (&raw)[S::kBatch], uint8_t* q, WorkControl<S>* c) {
@@ -505,32 +541,14 @@ __device__ __forceinline__ void store_queries(const CachedArgs& args, const Segm
 #pragma unroll
   for (int k = 0; k < S::kBatch; ++k) {
     const int r = (batch * S::kBatch + k) * S::kSoftmaxWarps + warp;
-    float x[4];
-    x[0] = __uint_as_float(raw[k].x << 16);
-    x[1] = __uint_as_float(raw[k].x & 0xffff0000u);
-    x[2] = __uint_as_float(raw[k].y << 16);
-    x[3] = __uint_as_float(raw[k].y & 0xffff0000u);
-    // (magnitudes as whole numbers: what is no number is beyond them all)
-    const uint32_t m = max(max(raw[k].x & 0x7fffu, (raw[k].x >> 16) & 0x7fffu),
-                           max(raw[k].y & 0x7fffu, (raw[k].y >> 16) & 0x7fffu));
-    const int largest = static_cast<int>(__reduce_max_sync(0xffffffffu, m));
-    // the largest element's exponent becomes 7: below 256
-    const int power = max(largest >> 7, 1) - 134;
-    const int some = max(power, -100), rest = power - some;  // (2^-power may be beyond FP32)
-    const float down = power_of_two(-some), downer = power_of_two(-rest);
-    uint32_t a[2], b[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const __half2 v = __floats2half2_rn(x[2 * i] * down * downer, x[2 * i + 1] * down * downer);
-      a[i] = codes_of(v);
-      b[i] = codes_of(__hmul2(__hsub2(v, halves_of(a[i])), __float2half2_rn(static_cast<float>(Second))));
-    }
+    uint32_t first, second;
+    float factor;
+    query_terms<Second>(raw[k], args.scale, first, second, factor);
     const int chunk = lane >> 2, inside = (lane & 3) * 4, r2 = S::kRows + r;
-    *reinterpret_cast<uint32_t*>(q + r * 128 + ((chunk ^ (r & 7)) << 4) + inside) = a[0] | (a[1] << 16);
-    *reinterpret_cast<uint32_t*>(q + r2 * 128 + ((chunk ^ (r2 & 7)) << 4) + inside) = b[0] | (b[1] << 16);
+    *reinterpret_cast<uint32_t*>(q + r * 128 + ((chunk ^ (r & 7)) << 4) + inside) = first;
+    *reinterpret_cast<uint32_t*>(q + r2 * 128 + ((chunk ^ (r2 & 7)) << 4) + inside) = second;
     if (lane == 0) {
-      // (a row that is no number: its scores are none)
-      c->factor[which][r] = largest < 0x7f80 ? args.scale * kLog2e * power_of_two(some) * power_of_two(rest) : NAN;
+      c->factor[which][r] = factor;
       const int token = (s.row0 + r) / group;
       const bool valid = token < s.rows;
       c->limit[which][r] = s.length - s.rows + (valid ? token : 0);
@@ -783,14 +801,14 @@ __device__ void init_work(WorkControl<S>* c) {
 #pragma unroll 1
   for (int i = 0; i < S::kValueSlots; ++i) {
     mbar_init(&c->v_full[i], 1);
-    mbar_init(&c->v_empty[i], 1);
+    mbar_init(&c->v_empty[i], S::kValueReaders);
   }
 #pragma unroll 1
   for (int i = 0; i < kSegments; ++i) {
     mbar_init(&c->segment_full[i], 1);
-    mbar_init(&c->segment_empty[i], S::kSoftmaxWarps + 1);
+    mbar_init(&c->segment_empty[i], S::kSegmentReaders);
   }
-  mbar_init(&c->q_full, S::kSoftmaxWarps);
+  mbar_init(&c->q_full, S::kQueryWriters);
   mbar_init(&c->drained, 1);
   c->found = 0;
   c->found_before = 0;

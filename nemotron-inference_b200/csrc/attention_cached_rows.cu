@@ -31,6 +31,7 @@ struct Rows {
   // out.  Counted where tiles are shared.  (1: 101.5 us, 2: 100.3, 3: 100.0, 4: 99.6, 48 sequences of 8192 tokens)
   static constexpr int kUnitCost = 4;
   static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
+  static constexpr int kValueReaders = 1, kSegmentReaders = kSoftmaxWarps + 1, kQueryWriters = kSoftmaxWarps;
   static constexpr uint32_t kQueryBytes = 2 * kRows * kHeadDim;
 };
 using S = Rows;

@@ -194,15 +194,17 @@ __global__ void __launch_bounds__(kFindThreads) find_shared_kernel(PagedCache c,
 constexpr size_t kAlign = 256;
 size_t aligned(size_t bytes) { return (bytes + kAlign - 1) / kAlign * kAlign; }
 
-// Sums and places of both parts, and the pieces of the second (those of the first are in the cache's workspace).
+// Sums and places of both parts, and the pieces of each.
 struct Workspace {
-  size_t places, sums, slots, total;
+  size_t places, sums, queries, slots[2], total;
   Workspace(int64_t rows, int heads) {
     const size_t pairs = static_cast<size_t>(rows) * heads;
     places = aligned(pairs * sizeof(RowPart));
     sums = aligned(pairs * kHeadDim * sizeof(float));
-    slots = 2 * places + 2 * sums;
-    total = slots + attention_cached_slot_bytes();
+    queries = 2 * places + 2 * sums;
+    slots[0] = queries + aligned(shared_pairs_query_bytes(rows, heads));
+    slots[1] = slots[0] + aligned(std::max(shared_pairs_slot_bytes(), attention_cached_slot_bytes()));
+    total = slots[1] + attention_cached_slot_bytes();
   }
 };
 
@@ -222,13 +224,15 @@ cudaError_t launch_attention_shared(const CachedArgs& args, char* workspace, cud
   for (int k = 0; k < 2; ++k) {
     part.row_parts = reinterpret_cast<RowPart*>(workspace + k * w.places);
     part.sums = reinterpret_cast<float*>(workspace + 2 * w.places + k * w.sums);
-    float* slots = reinterpret_cast<float*>(k ? workspace + w.slots : args.cache.attend_workspace + kAttendCounterBytes);
+    float* slots = reinterpret_cast<float*>(workspace + w.slots[k]);
     const int64_t rows = (args.batch.rows + entries[k] - 1) / entries[k] * of_head;
     join.of_row[k] = part.row_parts;
     join.sums[k] = part.sums;
     join.slots[k] = slots;
-    join.slot_rows[k] = attention_cached_slot_rows(rows);
-    const cudaError_t err = launch_cached_part(part, k ? Part::kOwn : Part::kShared, rows, slots, stream);
+    const bool pairs = k == 0 && rows > kMaxRows && shared_pairs_supported(args.batch.rows, args.heads);
+    join.slot_rows[k] = pairs ? shared_pairs_slot_rows() : attention_cached_slot_rows(rows);
+    const cudaError_t err = pairs ? launch_shared_pairs(part, slots, workspace + w.queries, stream)
+                                  : launch_cached_part(part, k ? Part::kOwn : Part::kShared, rows, slots, stream);
     if (err != cudaSuccess) return err;
   }
   // some two pairs to a warp
