@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const JoinArgs
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[d] *= keep;
         const int some = min(all - start, 32);
-#pragma unroll 4
+#pragma unroll 8
         for (int j = 0; j < some; ++j) {
           const float4 x = __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(__shfl_sync(
                                       0xffffffffu, reinterpret_cast<unsigned long long>(from), j))) +
@@ -235,9 +235,9 @@ cudaError_t launch_attention_shared(const CachedArgs& args, char* workspace, cud
                                   : launch_cached_part(part, k ? Part::kOwn : Part::kShared, rows, slots, stream);
     if (err != cudaSuccess) return err;
   }
-  // some two pairs to a warp
+  // a pair to a warp
   const int64_t pairs = (args.batch.rows + args.batch.count - 1) / args.batch.count * args.heads;
-  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((pairs + 2 * kJoinWarps - 1) / (2 * kJoinWarps), 4096));
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((pairs + kJoinWarps - 1) / kJoinWarps, 4096));
   return launch_kernel(join_parts_kernel, dim3(args.batch.count, blocks), kJoinThreads, 0, LaunchStream(stream, true), join);
 }
 

@@ -10,8 +10,8 @@
 //   O += P V            M = 128 rows, N = 128 dimensions, K = 128 tokens
 // Values become binary16 on their way, exactly but for a factor of 2^-8: the seven bits behind a code's sign lie in both
 // formats in the same order.  So a weight needs one term, is within 2^-11 of itself down to 2^-14 of the largest, and
-// is made with half the instructions of two E4M3 terms; both ways take the tensor cores 512 cycles.  Two warps do it,
-// once for both tiles of rows.
+// is made with half the instructions of two E4M3 terms; both ways take the tensor cores 512 cycles.  The softmax
+// warps do it, each its share, while they wait for scores.  (Two warps of their own took 4700 cycles for a tile.)
 //
 // The queries' terms are made once, by a kernel ahead of this one, and copied in by TMA: 256 rows made by each block
 // that needs them took 24000 cycles.
@@ -27,16 +27,14 @@ struct Pair {
   static constexpr int kRows = kTiles * 128;
   static constexpr int kKeySlots = 3, kValueSlots = 2;  // tiles in flight
   static constexpr int kSoftmaxWarps = 16;
-  static constexpr int kConvertWarps = 2;
   static constexpr int kUnitCost = 2;  // what a (group, key head, rows) costs a block beside its tiles, in tiles
-  static constexpr int kThreads = 32 * (kSoftmaxWarps + kConvertWarps + 2);
-  static constexpr int kValueReaders = kSoftmaxWarps + kConvertWarps, kSegmentReaders = kSoftmaxWarps + kConvertWarps + 1;
-  static constexpr int kQueryWriters = 1;
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
+  static constexpr int kValueReaders = kSoftmaxWarps, kSegmentReaders = kSoftmaxWarps + 1, kQueryWriters = 1;
   static constexpr uint32_t kQueryBytes = 2 * kRows * kHeadDim;
 };
 using S = Pair;
 
-constexpr int kMmaWarp = S::kSoftmaxWarps, kLoadWarp = kMmaWarp + 1, kFirstConvertWarp = kMmaWarp + 2;
+constexpr int kMmaWarp = S::kSoftmaxWarps;  // the one behind it loads
 constexpr int kWideSlots = 2;                       // tiles of binary16 values
 constexpr uint32_t kWideBytes = 2 * kKeyTileBytes;  // two panels of 64 dimensions
 constexpr uint32_t kTermBytes = S::kRows * kHeadDim, kTileRowsBytes = 128 * kHeadDim;
@@ -84,6 +82,13 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_kernel(const CachedAr
   *reinterpret_cast<uint32_t*>(queries.codes + at * kHeadDim + lane * 4) = a;
   *reinterpret_cast<uint32_t*>(queries.codes + (terms + at) * kHeadDim + lane * 4) = b;
   if (lane == 0) queries.factors[at] = factor;
+}
+
+// (what is no number does not count)
+__device__ __forceinline__ float largest_of(float a, float b, float c) {
+  float x;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(x) : "f"(a), "f"(b), "f"(c));
+  return x;
 }
 
 // Eight warps of a tile of rows.
@@ -195,53 +200,34 @@ __device__ __forceinline__ uint32_t no_numbers(uint32_t two) {
   return two;
 }
 
-// Warps that turn values into binary16.
-__device__ bool convert_role(const uint8_t* values, uint8_t* wide, Control* c) {
-  const int thread = threadIdx.x - 32 * kFirstConvertWarp, lane = threadIdx.x & 31;
-  uint32_t no = 0;
-#pragma unroll 1
-  for (uint32_t segments = 0;; ++segments) {
-    const uint32_t place = segments % kSegments;
-    if (!mbar_wait_warp(smem_u32(&c->segment_full[place]), (segments / kSegments) & 1)) return false;
-    const int some = c->has_segment[place], tiles = c->segment[place].tiles;
-    __syncwarp();
-    if (!some) return true;
-    if (lane == 0) mbar_arrive(&c->segment_empty[place]);
-#pragma unroll 1
-    for (int j = 0; j < tiles; ++j, ++no) {
-      const uint32_t slot = no % S::kValueSlots, to_slot = no % kWideSlots;
-      if (!mbar_wait_warp(smem_u32(&c->v_full[slot]), (no / S::kValueSlots) & 1)) return false;
-      if (!mbar_wait_warp(smem_u32(&c->wide_empty[to_slot]), ((no / kWideSlots) & 1) ^ 1)) return false;
-      // sixteen codes to a thread: eight threads to a token
-      const int chunk = thread & 7;
-      uint8_t* panel = wide + to_slot * kWideBytes + (chunk >> 2) * kKeyTileBytes;
-#pragma unroll 2
-      for (int token = thread >> 3; token < kKeyTile; token += 4 * S::kConvertWarps) {
-        const uint4 x = *reinterpret_cast<const uint4*>(values + slot * kKeyTileBytes + token * kHeadDim + ((chunk ^ (token & 7)) << 4));
-        uint4 lo = make_uint4(widen(x.x, 0x1404), widen(x.x, 0x3424), widen(x.y, 0x1404), widen(x.y, 0x3424));
-        uint4 hi = make_uint4(widen(x.z, 0x1404), widen(x.z, 0x3424), widen(x.w, 0x1404), widen(x.w, 0x3424));
-        const uint32_t any = ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u) |
-                             ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
-        if (any & 0x80808080u) {  // (hardly ever) codes that are no numbers, 0x3f80 so far
-          lo = make_uint4(no_numbers(lo.x), no_numbers(lo.y), no_numbers(lo.z), no_numbers(lo.w));
-          hi = make_uint4(no_numbers(hi.x), no_numbers(hi.y), no_numbers(hi.z), no_numbers(hi.w));
-        }
-        // (the threads of the two panels in turn: together they meet every bank once)
-        const int first = 2 * (chunk & 3), odd = chunk >> 2;
-        *reinterpret_cast<uint4*>(panel + token * 128 + (((first + odd) ^ (token & 7)) << 4)) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(panel + token * 128 + (((first + 1 - odd) ^ (token & 7)) << 4)) = odd ? lo : hi;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&c->wide_full[to_slot]);
-        mbar_arrive(&c->v_empty[slot]);
-      }
+// A thread's share of a tile of values, as binary16: sixteen codes at a time, eight threads to a token.
+__device__ __forceinline__ void widen_values(const uint8_t* values, uint8_t* wide) {
+  const int chunk = threadIdx.x & 7;
+  uint8_t* panel = wide + (chunk >> 2) * kKeyTileBytes;
+  constexpr int kTokens = 32 * S::kSoftmaxWarps / 8;
+#pragma unroll
+  for (int i = 0; i < kKeyTile / kTokens; ++i) {
+    const int token = (threadIdx.x >> 3) + i * kTokens;
+    const uint4 x = *reinterpret_cast<const uint4*>(values + token * kHeadDim + ((chunk ^ (token & 7)) << 4));
+    uint4 lo = make_uint4(widen(x.x, 0x1404), widen(x.x, 0x3424), widen(x.y, 0x1404), widen(x.y, 0x3424));
+    uint4 hi = make_uint4(widen(x.z, 0x1404), widen(x.z, 0x3424), widen(x.w, 0x1404), widen(x.w, 0x3424));
+    const uint32_t any = ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u) |
+                         ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
+    if (any & 0x80808080u) {  // (hardly ever) codes that are no numbers
+      lo = make_uint4(no_numbers(lo.x), no_numbers(lo.y), no_numbers(lo.z), no_numbers(lo.w));
+      hi = make_uint4(no_numbers(hi.x), no_numbers(hi.y), no_numbers(hi.z), no_numbers(hi.w));
     }
+    // (the threads of the two panels in turn: together they meet every bank once)
+    const int first = 2 * (chunk & 3), odd = chunk >> 2;
+    *reinterpret_cast<uint4*>(panel + token * 128 + (((first + odd) ^ (token & 7)) << 4)) = odd ? hi : lo;
+    *reinterpret_cast<uint4*>(panel + token * 128 + (((first + 1 - odd) ^ (token & 7)) << 4)) = odd ? lo : hi;
   }
+  fence_proxy_async_smem();
+  __syncwarp();
 }
 
-__device__ bool softmax_role(const CachedArgs& args, const Split& split, const Queries& queries, uint32_t tmem, Control* c) {
+__device__ bool softmax_role(const CachedArgs& args, const Split& split, const Queries& queries, const uint8_t* values, uint8_t* wide,
+                             uint32_t tmem, Control* c) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = warp >> 3, half = (warp >> 2) & 1;
   const int row = t * 128 + (warp & 3) * 32 + lane;  // of the segment's
   const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
@@ -267,7 +253,11 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, const Q
 #pragma unroll 1
     for (int j = 0; j < s.tiles; ++j, ++no) {
       const uint32_t slot = no % S::kValueSlots;
+      const uint32_t wide_slot = no % kWideSlots;
       ok = mbar_wait_warp(smem_u32(&c->v_full[slot]), (no / S::kValueSlots) & 1) && ok;
+      ok = mbar_wait_warp(smem_u32(&c->wide_empty[wide_slot]), ((no / kWideSlots) & 1) ^ 1) && ok;
+      widen_values(values + slot * kKeyTileBytes, wide + wide_slot * kWideBytes);
+      if (lane == 0) mbar_arrive(&c->wide_full[wide_slot]);
       if (present) {
         ok = mbar_wait_warp(smem_u32(&c->s_full[t]), s_uses & 1) && ok;
         ++s_uses;
@@ -275,99 +265,78 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, const Q
         const bool is_first = j == 0;
         uint32_t p[kHalf / 2];
         float high = -INFINITY, added = 0.0f;
-        // Exponents, score + power of the values - reference, 32 tokens at a time; use(x, token, power).
-        auto exponents = [&](auto use) {
+        // Weights by exponents, score + power of the values - reference.  A first tile sets the references, others raise
+        // them where that is due, for both halves of a row alike, and the weights are made again.  (One loop: code that
+        // runs once in a while is not in the cache, and a way of its own for it took 8000 cycles.)  A row whose scores
+        // are very far above its reference takes them as they are first, so that no rounding matters.
+        const float before = shift;
+        bool anew = is_first;
+#pragma unroll 1
+        for (int attempt = 0; attempt < 4; ++attempt) {
+          if (has_rows) {
+            high = -INFINITY;
+            added = 0.0f;
+            uint32_t y[2][kPart];  // (sixteen tokens of scores are on their way during the sixteen before)
+            tmem_ld_x16_async(s_at, y[0]);
 #pragma unroll
-          for (int i = 0; i < kHalf; i += 32) {
-            uint32_t y[32];
-            tmem_ld_x32_async(s_at + i, y);
-            tmem_ld_wait();
-            registers_loaded<32>(y);
-#pragma unroll
-            for (int part = 0; part < 32; part += kPart) {
-              const int page = (half * kHalf + i + part) >> page_shift;
+            for (int part = 0; part < kHalf; part += kPart) {
+              uint32_t(&now)[kPart] = y[part / kPart & 1];
+              tmem_ld_wait();
+              registers_loaded<kPart>(now);
+              if (part + kPart < kHalf) tmem_ld_x16_async(s_at + part + kPart, y[(part / kPart + 1) & 1]);
+              const int page = (half * kHalf + part) >> page_shift;
               const int k_power = c->powers[slot][0][page], v_power = c->powers[slot][1][page];
               const float scale = factor * power_of_two(k_power), bias = static_cast<float>(v_power) + shift;
               const uint64_t scale2 = pack2(scale, scale), bias2 = pack2(bias, bias);
-              uint64_t x[kPart / 2];
+              uint64_t of_part = 0;
 #pragma unroll
               for (int k = 0; k < kPart / 2; ++k) {
-                x[k] = fma2(pack2(__uint_as_float(y[part + 2 * k]), __uint_as_float(y[part + 2 * k + 1])), scale2, bias2);
+                const uint64_t x = fma2(pack2(__uint_as_float(now[2 * k]), __uint_as_float(now[2 * k + 1])), scale2, bias2);
+                float a, b;
+                unpack2(x, a, b);
+                high = largest_of(high, a, b);
+                if (k % 4 == 3) {
+                  unpack2(exp2_polynomial2<3>(x), a, b);
+                } else {
+                  a = exp2_approx(a);
+                  b = exp2_approx(b);
+                }
+                of_part = add2(of_part, pack2(a, b));
+                const __half2 two = __floats2half2_rn(a, b);
+                p[part / 2 + k] = *reinterpret_cast<const uint32_t*>(&two);
               }
-              use(x, i + part, v_power);
+              float s0, s1;
+              unpack2(of_part, s0, s1);
+              added = fmaf(s0 + s1, power_of_two(-v_power), added);
             }
           }
-        };
-        auto largest = [&] {
-          high = -INFINITY;
-          exponents([&](const uint64_t (&x)[kPart / 2], int, int) {
-#pragma unroll
-            for (int k = 0; k < kPart / 2; ++k) {
-              float a, b;
-              unpack2(x[k], a, b);
-              high = fmaxf(high, fmaxf(a, b));
-            }
-          });
-        };
-        auto weigh = [&] {
-          high = -INFINITY;
-          added = 0.0f;
-          exponents([&](const uint64_t (&x)[kPart / 2], int at, int v_power) {
-            uint64_t of_part = 0;
-#pragma unroll
-            for (int k = 0; k < kPart / 2; ++k) {
-              float a, b;
-              unpack2(x[k], a, b);
-              high = fmaxf(high, fmaxf(a, b));
-              if (k % 4 == 3) {
-                unpack2(exp2_polynomial2<3>(x[k]), a, b);
-              } else {
-                a = exp2_approx(a);
-                b = exp2_approx(b);
-              }
-              of_part = add2(of_part, pack2(a, b));
-              const __half2 two = __floats2half2_rn(a, b);
-              p[at / 2 + k] = *reinterpret_cast<const uint32_t*>(&two);
-            }
-            float s0, s1;
-            unpack2(of_part, s0, s1);
-            added = fmaf(s0 + s1, power_of_two(-v_power), added);
-          });
-        };
-        if (!is_first && has_rows) weigh();
-        if (tile_any(t, is_first || high > kRiseBits)) {
-          // A first tile sets the references; others raise them where that is due, from the scores anew, both halves of a
-          // row alike.  (O holds the tiles before: their products were asked for ahead of these scores.)
-          c->top[half][row] = is_first ? INFINITY : high;
-          tile_sync(t);
-          const bool raise = fmaxf(c->top[0][row], c->top[1][row]) > kRiseBits;
-          tile_sync(t);
-          const float before = shift;
-          if (raise) shift = 0.0f;
-          if (has_rows) largest();
+          // (behind this both halves have read the scores: weights may be written over them)
+          if (!tile_any(t, anew || high > kRiseBits)) break;
           c->top[half][row] = high;
           tile_sync(t);
-          float keep = 1.0f;
-          if (raise) {
-            const float top = fmaxf(c->top[0][row], c->top[1][row]);
-            shift = top == -INFINITY ? -kNoReference : -top;
-            keep = is_first ? 0.0f : exp2_approx(shift - before);
+          const float top = fmaxf(c->top[0][row], c->top[1][row]);
+          if (!anew && top > kFarBits) {
+            anew = true;
+            shift = 0.0f;
+          } else if (anew || top > kRiseBits) {
+            shift = top == -INFINITY ? -kNoReference : shift - top;
+            anew = false;
           }
-          if (has_rows && !is_first) {
-            sum *= keep;
+        }
+        const float keep = shift == before || is_first ? 1.0f : exp2_approx(shift - before);
+        if (has_rows && __any_sync(0xffffffffu, keep != 1.0f)) {
+          // (O holds the tiles before: their products were asked for ahead of these scores)
+          sum *= keep;
 #pragma unroll 1
-            for (int i = 0; i < kHalf; i += 32) {
-              uint32_t o[32];
-              tmem_ld_x32_async(o_at + i, o);
-              tmem_ld_wait();
-              registers_loaded<32>(o);
+          for (int i = 0; i < kHalf; i += 32) {
+            uint32_t o[32];
+            tmem_ld_x32_async(o_at + i, o);
+            tmem_ld_wait();
+            registers_loaded<32>(o);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-              tmem_st_x32(o_at + i, o);
-            }
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+            tmem_st_x32(o_at + i, o);
           }
-          if (has_rows) weigh();
-          tile_sync(t);  // (both halves have read the scores)
         }
         if (has_rows) {
           sum += added;
@@ -447,7 +416,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     }
     mbar_init(&c->q_empty, 1);
     for (int i = 0; i < kWideSlots; ++i) {
-      mbar_init(&c->wide_full[i], S::kConvertWarps);
+      mbar_init(&c->wide_full[i], S::kSoftmaxWarps);
       mbar_init(&c->wide_empty[i], 1);
     }
     fence_barrier_init();
@@ -465,13 +434,13 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   const uint32_t tmem = c->tmem;
   bool ok = true;
   if (warp < S::kSoftmaxWarps) {
-    ok = softmax_role(args, split, queries, tmem, c);
+    ok = softmax_role(args, split, queries, values, wide, tmem, c);
   } else if (warp == kMmaWarp) {
     ok = mma_role(args, smem_u32(keys), smem_u32(wide), smem_u32(q), tmem, c);
     if (elect_one()) tcgen05_commit(&c->drained);
     __syncwarp();
     mbar_wait_warp(smem_u32(&c->drained), 0);
-  } else if (warp == kLoadWarp) {
+  } else {
     const int group = args.heads / args.cache.kv_heads;
     load_role<S, Part::kShared>(args, &map, smem_u32(keys), smem_u32(values), c, [&](const Segment& s, uint32_t number) {
       if (number == 0) wait_for_predecessor();
@@ -490,8 +459,6 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       __syncwarp();
       return true;
     });
-  } else {
-    ok = convert_role(values, wide, c);
   }
   if (!ok && (threadIdx.x & 31) == 0) report_cache_error(args.cache.error, kDevWaitTimeout);
   wait_for_predecessor();  // (this launch ends behind that of the queries)
