@@ -29,6 +29,7 @@ struct JoinArgs {
   const float* sums[2];
   const float* slots[2];
   int slot_rows[2];
+  int blocks[2];               // that have slots
 };
 
 // The group that entry i belongs to, -1 for none; all lanes of a warp call it with the same i.
@@ -62,20 +63,25 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const JoinArgs
   }
   wait_for_predecessor();
   release_successor();
-  const bool stopped = cache_words(c.cache).error != 0;  // (also where a wait ran out)
   const int pairs = e.rows * c.heads;
+  const CacheWords words = cache_words(c.cache);
 #pragma unroll 1
   for (int p = blockIdx.y * kJoinWarps + warp; p < pairs; p += gridDim.y * kJoinWarps) {
     const size_t at = static_cast<size_t>(e.first) * c.heads + p;
     float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, top = -INFINITY, sum = 0.0f;
-    if (valid && !stopped) {
-      RowPart part[2];
-      part[0].parts_row = 0;
-      if (e.skip > 0) part[0] = args.of_row[0][at];
-      part[1] = args.of_row[1][at];
-      int count[2];
+    RowPart part[2];
+    part[0].parts_row = 0;
+    if (e.skip > 0) part[0] = args.of_row[0][at];
+    part[1] = args.of_row[1][at];
+    int count[2];
+    bool there = valid && words.error == 0;  // (where a wait ran out, there may be nothing, either)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) count[k] = part[k].parts_row > 255 ? part[k].parts_row >> 8 : part[k].parts_row;
+    for (int k = 0; k < 2; ++k) {
+      count[k] = part[k].parts_row > 255 ? part[k].parts_row >> 8 : part[k].parts_row;
+      there = there && count[k] >= 0 && (count[k] < 2 || (part[k].lead >= 0 && part[k].lead <= args.blocks[k] - count[k] &&
+                                                          (part[k].parts_row & 255) < args.slot_rows[k]));
+    }
+    if (there) {
       const int all = count[0] + count[1];
 #pragma unroll 1
       for (int start = 0; start < all; start += 32) {  // a lane to a piece
@@ -107,7 +113,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const JoinArgs
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[d] *= keep;
         const int some = min(all - start, 32);
-#pragma unroll 8
+#pragma unroll 16
         for (int j = 0; j < some; ++j) {
           const float4 x = __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(__shfl_sync(
                                       0xffffffffu, reinterpret_cast<unsigned long long>(from), j))) +
@@ -121,7 +127,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const JoinArgs
         }
       }
     }
-    const float inverse = valid && !stopped ? 1.0f / sum : 0.0f;
+    const float inverse = there ? 1.0f / sum : 0.0f;
     *reinterpret_cast<uint2*>(c.out + at * kHeadDim + lane * 4) =
         make_uint2(pack_bf16(o[0] * inverse, o[1] * inverse), pack_bf16(o[2] * inverse, o[3] * inverse));
   }
@@ -231,6 +237,7 @@ cudaError_t launch_attention_shared(const CachedArgs& args, char* workspace, cud
     join.slots[k] = slots;
     const bool pairs = k == 0 && rows > kMaxRows && shared_pairs_supported(args.batch.rows, args.heads);
     join.slot_rows[k] = pairs ? shared_pairs_slot_rows() : attention_cached_slot_rows(rows);
+    join.blocks[k] = device_sms() * (join.slot_rows[k] <= 16 ? 2 : 1);
     const cudaError_t err = pairs ? launch_shared_pairs(part, slots, workspace + w.queries, stream)
                                   : launch_cached_part(part, k ? Part::kOwn : Part::kShared, rows, slots, stream);
     if (err != cudaSuccess) return err;
