@@ -679,8 +679,9 @@ NMOE_API nmoe_status nmoe_adapters_sync_status(int32_t* error, void* stream);
  * temperature that is not above 0 takes the first of the largest logits.
  *
  * Each parameter is a device array of one for each row or, where that is null,
- * `*_all` for every row.  Weights are 64-bit whole numbers of 2^-44 of the
- * largest: the token is the formula's, whatever the batch.  A row that holds a NaN, or
+ * `*_all` for every row.  Weights are good to 2^-36 of themselves or 2^-44 of the
+ * largest, their sums 64 bits wide: the token is the formula's but where the
+ * random number lies so near to a neighbour.  A row that holds a NaN, or
  * whose largest logit is infinite, gets token -1 and logprob NaN.
  * logprobs [rows] (nullable): log of the token's softmax over all logits, at
  * temperature 1.  A row's size is at most 1.5 MB (NMOE_ERR_UNSUPPORTED). */

@@ -7,23 +7,26 @@
 //
 // Which token that is changes with the last bits of a sum when a row has many likely tokens: of n equal ones an error
 // of e in the sum moves n e of the random numbers to a neighbour, and FP32 sums of 131072 weights would give another
-// token than the formula in one of a hundred such rows.  So weights are whole numbers of 2^-44 of the largest, or
-// smaller units where the vocabulary leaves room, each within 2^-31 of itself and without a bias, and sums are 64-bit
-// integers: they do not depend on an order, and rows come out the same whatever the split.
+// token than the formula in one of a hundred such rows.  So weights are within 2^-36 of themselves, a thread's sums are
+// FP64 and all others whole numbers of 2^-44 of the largest weight.
 //
-// What bounds it is reading the logits once.  A cluster of blocks holds a row in its shared memory and goes over it as
-// often as the parameters ask.  No sort: the border of what stays is found by histograms over the values, whose bin at
-// the border is listed and ranked one by one (or split again while it holds too many; equal values go by their place).
+// What bounds it is reading the logits once, and FP64 where all weights are summed up: 16 of a scheduler's cycles for 32
+// tokens, 9 us for a row of 131072 on an SM.  Below that the steps of a row wait for one another: a barrier of a cluster
+// and the sums behind it take 1.5 us each, and a row with top-p has a dozen.  One block or a cluster goes over a row as often as its parameters ask, the
+// first time for the largest and the sum of all weights (by a reference that the first tokens give).  No sort: the
+// border of what stays is found by histograms over the values, whose bin at the border is listed and ranked one by one
+// (or split again while it holds too many; equal values go by their place).
 //   top-k   the k-th largest of the threads' own largest values is no larger than the k-th largest of all: one entry a
 //           thread finds a bound that few more than k tokens reach, and these are ranked
-//   top-p   a sixteenth of the tokens tells about where the border lies: the pass that takes the exact sums of all weights
-//           and of those above notes the tokens near it, and the rest goes over these.  (If it lies elsewhere: over
-//           all with weights of (1 - p) / n of the largest's, below which no token of n stays.)
-// The sums in order of i come last, of what stays; where all do, they are taken in FP32 first, whose error has a bound
-// (kSumError): only where the random number lies within it of another token the row is gone over with exact weights.
+//   top-p   some thousand of the tokens tell about where the border lies: the pass that sums up the weights above notes
+//           the tokens near it, and the rest goes over these.  (If it lies elsewhere: over all with weights of (1 - p) / n
+//           of the largest's, below which no token of n stays.)
+// The sums in order of i come last, of what stays.
 //
-// Most of the code runs once for a row, so instructions that are not in the cache yet cost more than the work of a
-// pass: loops take a token to a lane, without unrolling, where the arithmetic is long.
+// Measured (B200, FP32): 256 rows of 131072 as they are 68 us, 40 of them for the first pass (two thirds of what copying
+// reaches); 64 rows of as many settings 80 us; one row 31 us; 37 rows of 50001 in BF16, top-k and top-p, 22 us.  Rows that
+// lay in the shared memory of clusters of eight blocks took 145, 102, 33 and 22 us: such clusters left a third of the
+// SMs' room empty, and SMs idle while a row's steps waited.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -47,31 +50,28 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 1024;
 constexpr int kListed = 256;  // tokens ranked one by one
-constexpr int kSpots = 64;    // noted places of a warp
-constexpr int kSamples = 2;   // tokens to a thread that guess() goes by
+constexpr int kAside = 160;   // vectors that wait for each_from()
+constexpr int kSpots = 256;   // noted places of a warp
+constexpr int kSamples = 16;  // tokens to a thread that guess() goes by, over the blocks of a row
 constexpr int kFewK = 160;    // top_k that the bound from the threads' largest values is for
 constexpr int kVector = 16;   // bytes
-constexpr int kSliceBytes = 64 * 1024;  // of a row to a block where clusters suffice: two blocks to an SM
-constexpr int kMostSliceBytes = 192 * 1024;
-// Logarithms of the weights to base 2: 42 bits behind the point, of which ten choose a power in the table.
-constexpr int kTable = 1024;
-constexpr double kPoint = 1536.0;       // 1.5 * 2^10: a sum with it has 2^-42 as its last bit
-constexpr int kPointHigh = 0x40980000;  // its upper word
-constexpr int kMostUnit = 46;           // weights are counted in 2^-46 of the largest at the finest
-// Relative error of a sum of weights 2^y in FP32 at most: y = (x - m) c is off by 3 2^-24 |y|, and the average of |y|
-// by weight is at most log2 of the number of tokens, below 19: 2.4e-6; ex2.approx adds 2^-22, sums of up to 96 in a
-// thread, in fours, 26 2^-24.
-constexpr double kSumError = 5e-6;
+constexpr int kMostSlice = 1 << 17;  // tokens to a block (the histogram's words)
+constexpr int kMostRowBytes = 1536 * 1024;
+constexpr int kTable = 1024;          // powers 2^(i / 1024)
+constexpr double kTenth = 6597069766656.0;  // 1.5 * 2^42: a sum with it is a whole number of 2^-10, its lower word in 32 bits
+constexpr int kMostUnit = 44;         // weights are counted in 2^-44 of the largest at the finest
+constexpr float kAbove = 500.0f;      // binary orders that a weight may lie above the reference's (FP64 has 1023)
+constexpr float kBelow = 64.0f;       // and below, before it is 0
 constexpr float kWhole = 8388608.0f;    // 2^23: a sum with it is a whole number
 constexpr int kWholeBits = 0x4b000000;
 
-enum SearchState { kUnsure, kFound, kTooMany };
+enum SearchState { kFound, kTooMany };
 
 // What the blocks of a cluster tell each other; written for all, read behind the next barrier of the cluster.
 struct Box {
   float top[kMaxCluster];
   int bad[kMaxCluster];
-  float sum[kMaxCluster];            // of e^(x - m)
+  double sum[kMaxCluster];           // of e^(x - m)
   u64 part[kMaxCluster];             // of a sum in order of i
   u64 higher[kMaxCluster];           // of weights above those noted
   float low[kMaxCluster], high[kMaxCluster];  // values in a bin
@@ -83,7 +83,8 @@ struct Box {
 
 struct Shared {
   Box box;
-  unsigned table[kTable];     // 2^(i / 1024), units of 2^-31
+  double table[kTable];
+  uint4 edges[2];
   alignas(16) unsigned bins[3][kBins];  // the histogram: weights in three words of 15 bits and some, or counts
   union {
     u64 sums[kBins];              // of all blocks' histograms
@@ -91,8 +92,12 @@ struct Shared {
   };
   unsigned listed, noted;     // of the cluster's list (in the first block), of this block's
   ulonglong2 list[kListed];   // of the first block: order and weight
+  uint4 aside[kWarps][kAside];
+  uint16_t aside_at[kWarps][kAside];  // vectors from the warp's first on
   uint16_t spots[kWarps][kSpots];  // from the warp's first token on
+  unsigned warp_noted[kWarps];
   u64 warp_part[kWarps];
+  double warp_double[kWarps];
   float warp_top[kWarps], warp_low[kWarps];
   int bad;
   int bin;
@@ -103,7 +108,7 @@ struct Shared {
 struct Border {
   float value;
   int index;
-  __device__ bool keeps(float x, int i) const { return x > value || (x == value && i <= index); }
+  __device__ bool keeps(float x, int i) const { return (x > value) | ((x == value) & (i <= index)); }
 };
 
 // A token's place in falling order, as a whole number that falls; both zeros are one.
@@ -131,6 +136,11 @@ __device__ __forceinline__ u64 warp_upto(u64 x, int lane) {
     const u64 other = __shfl_up_sync(0xffffffffu, x, step);
     if (lane >= step) x += other;
   }
+  return x;
+}
+__device__ __forceinline__ double warp_total(double x) {
+#pragma unroll 1
+  for (int step = 16; step > 0; step /= 2) x += __shfl_xor_sync(0xffffffffu, x, step);
   return x;
 }
 __device__ __forceinline__ float warp_max(float x) {
@@ -163,25 +173,29 @@ struct Bins {
 extern __shared__ __align__(16) uint8_t dynamic_shared[];
 #define s (*reinterpret_cast<Shared*>(dynamic_shared))  // (by name: a pointer in a register has no address space)
 
-template <typename T>
+template <typename T, int kBlocks>
 struct Row {
+  static constexpr int kMany = kBlocks == 1 ? 8 : 4;   // values at once: their steps wait for one another
+  static constexpr int kAhead = kBlocks == 1 ? 4 : 2;  // vectors on their way
+  static_assert(32 * (kAhead + 1) <= kAside);
   static constexpr int kElements = kVector / sizeof(T);
-  int first;             // number of the token at the slice's first sixteen bytes
+  // This block's slice, in sixteen bytes each: `vectors` of them from an aligned address on, at which `lead` elements
+  // of something else come first; `tokens` of its own, the first of them token `first` + `lead`.
+  const uint4* from;
+  int vectors, lead, tokens, first;
   int rank, size;        // of the cluster
-  int warp, lane, begin, end;  // this warp's chunks of sixteen bytes
-  int each_warp;         // chunks
+  int warp, lane, begin, end;  // this warp's vectors
+  int each_warp;
   float top, lowest;     // the largest logit, the last that has a weight
   double scale;          // log2(e) / T
-  float fast_scale;      // the same
-  bool fast;             // sums in FP32 have their bound
   float ratio;           // of all tokens to those that guess() goes by
   int unit;              // weights are counted in 2^-unit
 
-  // This block's slice; places beside it are -infinity.
-  static __device__ __forceinline__ uint4* slice_at() {
-    return reinterpret_cast<uint4*>(dynamic_shared + (sizeof(Shared) + 15) / 16 * 16);
+  __device__ __forceinline__ bool whole(int c) const { return c * kElements >= lead && (c + 1) * kElements <= lead + tokens; }
+  // Token first + at; -infinity beside the slice.
+  __device__ __forceinline__ float value(int at) const {
+    return at >= lead && at < lead + tokens ? static_cast<float>(reinterpret_cast<const T*>(from)[at]) : -INFINITY;
   }
-  __device__ __forceinline__ float value(int at) const { return static_cast<float>(reinterpret_cast<const T*>(slice_at())[at]); }
   // visit(x, index) of this warp's tokens, a lane each; all lanes together, with -infinity behind the end.
   template <typename Visit>
   __device__ __forceinline__ void each(Visit visit) const {
@@ -190,57 +204,175 @@ struct Row {
       visit(at < end * kElements ? value(at) : -INFINITY, first + at);
     }
   }
-  // visit(x[4], index of x[0]), four at a time, all lanes together, with -infinity behind the end.
-  template <typename Visit>
-  __device__ __forceinline__ void each_four(Visit visit) const {
-    constexpr int kFours = kElements / 4;
+  // Sixteen bytes of the slice, -infinity beside it.
+  __device__ __forceinline__ uint4 vector(int c) const {
+    constexpr unsigned kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+    uint4 v = make_uint4(kNone, kNone, kNone, kNone);
+    if (c < end) {
+      if (whole(c)) {
+        v = __ldg(from + c);
+      } else {
+        v = s.edges[c != 0];
+      }
+    }
+    return v;
+  }
+  // The first and the last sixteen bytes, of which some lie beside the slice.
+  __device__ __forceinline__ void set_edges() const {
+    constexpr int kWords = kVector / 4;
+    if (threadIdx.x < 2 * kWords) {
+      const int at = (threadIdx.x / kWords * (vectors - 1)) * kElements + threadIdx.x % kWords * (4 / static_cast<int>(sizeof(T)));
+      unsigned bits;
+      if constexpr (sizeof(T) == 4) {
+        bits = __float_as_uint(value(at));
+      } else {
+        bits = (__float_as_uint(value(at)) >> 16) | (__float_as_uint(value(at + 1)) & 0xffff0000u);
+      }
+      reinterpret_cast<unsigned*>(s.edges)[threadIdx.x] = bits;
+    }
+  }
+  // visit(x, index of x[0]), kMany at a time; all lanes together, with -infinity beside the slice.  The index of x[m] is that
+  // of x[0] + place(m).  `behind`: a function called after each few vectors.  (The next ones are on their way meanwhile.)
+  static __device__ __forceinline__ constexpr int place(int m) { return m + m / kElements * (31 * kElements); }
+  template <typename Visit, typename Behind>
+  __device__ __forceinline__ void each_many(Visit visit, Behind behind) const {
+    constexpr int kTogether = kMany < kElements ? 1 : kMany / kElements;  // vectors
+    uint4 next[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) next[k] = vector(begin + lane + 32 * k);
 #pragma unroll 1
-    for (int at = begin * kFours + lane; at < end * kFours + lane; at += 32) {
-      float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (at < end * kFours) {
+    for (int c = begin + lane; c < end + lane; c += 32 * kAhead) {
+#pragma unroll
+      for (int k = 0; k < kAhead; k += kTogether) {
+        const int at = first + (c + 32 * k) * kElements;
+        unsigned words[kTogether][4];
+#pragma unroll
+        for (int j = 0; j < kTogether; ++j) {
+          words[j][0] = next[k + j].x;
+          words[j][1] = next[k + j].y;
+          words[j][2] = next[k + j].z;
+          words[j][3] = next[k + j].w;
+          next[k + j] = vector(c + 32 * (k + j + kAhead));
+        }
+        float x[kMany];
         if constexpr (sizeof(T) == 4) {
-          const float4 v = reinterpret_cast<const float4*>(slice_at())[at];
-          x[0] = v.x;
-          x[1] = v.y;
-          x[2] = v.z;
-          x[3] = v.w;
+#pragma unroll
+          for (int m = 0; m < kMany; ++m) x[m] = __uint_as_float(words[m / 4][m % 4]);
+          visit(x, at);
         } else {
-          const uint2 v = reinterpret_cast<const uint2*>(slice_at())[at];
-          x[0] = __uint_as_float(v.x << 16);
-          x[1] = __uint_as_float(v.x & 0xffff0000u);
-          x[2] = __uint_as_float(v.y << 16);
-          x[3] = __uint_as_float(v.y & 0xffff0000u);
+#pragma unroll 1
+          for (int part = 0; part < kElements * kTogether / kMany; ++part) {  // (halves of a vector)
+#pragma unroll
+            for (int m = 0; m < kMany; m += 2) {
+              const int in = m % kElements / 2;
+              const unsigned word = kMany < kElements && part != 0 ? words[0][in + 2] : words[m / kElements][in];
+              x[m] = __uint_as_float(word << 16);
+              x[m + 1] = __uint_as_float(word & 0xffff0000u);
+            }
+            visit(x, at + kMany * part);
+          }
         }
       }
-      visit(x, first + 4 * at);
+      behind();
+    }
+  }
+  template <typename Visit>
+  __device__ __forceinline__ void each_many(Visit visit) const {
+    each_many(visit, [] {});
+  }
+  static __device__ __forceinline__ float largest_of(const float (&x)[kMany]) {
+    float largest = x[0];
+#pragma unroll
+    for (int m = 1; m < kMany; ++m) largest = fmaxf(largest, x[m]);
+    return largest;
+  }
+  static __device__ __forceinline__ double sum_of(const double (&w)[kMany]) {
+    double sum = (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+    for (int m = 4; m < kMany; m += 4) sum += (w[m] + w[m + 1]) + (w[m + 2] + w[m + 3]);
+    return sum;
+  }
+
+  // visit(x[4], index of x[0]) of the fours among whose neighbours in sixteen bytes one is `least` or more: few, mostly, so
+  // that these are put aside until each lane has one.  (Visited where they were met, a lane or two of a warp at a time,
+  // they took 18 us of 64 rows' time where they take 7 now.)
+  template <typename Visit>
+  __device__ __forceinline__ void each_from(float least, Visit visit) const {
+    uint4* aside = s.aside[warp];
+    uint16_t* places = s.aside_at[warp];
+    int waiting = 0;
+    uint4 next[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) next[k] = vector(begin + lane + 32 * k);
+#pragma unroll 1
+    for (int c = begin + lane; c < end + lane; c += 32 * kAhead) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const uint4 v = next[k];
+        next[k] = vector(c + 32 * (k + kAhead));
+        float largest;
+        if constexpr (sizeof(T) == 4) {
+          largest = fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+        } else {
+          auto pair = [](unsigned word) { return *reinterpret_cast<const __nv_bfloat162*>(&word); };
+          const float2 two = __bfloat1622float2(__hmax2(__hmax2(pair(v.x), pair(v.y)), __hmax2(pair(v.z), pair(v.w))));
+          largest = fmaxf(two.x, two.y);
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, largest >= least);
+        if (largest >= least) {
+          const int at = waiting + __popc(here & ((1u << lane) - 1));
+          aside[at] = v;
+          places[at] = static_cast<uint16_t>(c + 32 * k - begin);
+        }
+        waiting += __popc(here);
+      }
+      const bool last = c - lane + 32 * kAhead >= end;
+#pragma unroll 1
+      while (waiting >= 32 || (last && waiting > 0)) {
+        __syncwarp();
+        constexpr unsigned kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+        uint4 v = make_uint4(kNone, kNone, kNone, kNone);
+        const int at = waiting - 1 - lane;
+        int i = 0;
+        if (at >= 0) {
+          v = aside[at];
+          i = first + (begin + places[at]) * kElements;
+        }
+        if constexpr (sizeof(T) == 4) {
+          const float x[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+          visit(x, i);
+        } else {
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            const unsigned w0 = half ? v.z : v.x, w1 = half ? v.w : v.y;
+            const float x[4] = {__uint_as_float(w0 << 16), __uint_as_float(w0 & 0xffff0000u), __uint_as_float(w1 << 16),
+                                __uint_as_float(w1 & 0xffff0000u)};
+            visit(x, i + 4 * half);
+          }
+        }
+        __syncwarp();
+        waiting -= 32;
+      }
+      waiting = max(waiting, 0);
     }
   }
 
-  // A token's weight.  z holds its logarithm to base 2 as a whole number of 2^-42, the upper word units of 2^-10.
-  // 2^(that) is a power from the table, times 1 + q with q = 2^r - 1 a polynomial of the rest r < 2^-10 (its first
-  // three terms: the fourth is 2^-46).  r is cut off at 2^-33, q rounded to 2^-31.
-  __device__ __forceinline__ u64 weight(float x) const {
-    constexpr float c1 = 6.7690154351557163e-4f, c2 = 2.2909784980808780e-7f, c3 = 5.1691529e-11f;  // ln(2)^n 2^-10n / n!
-    const double z = fma(static_cast<double>(fmaxf(x, lowest)) - static_cast<double>(top), scale, kPoint);
-    const int whole = __double2hiint(z) - kPointHigh;
-    const float r = __uint_as_float(0x3f800000u | (static_cast<unsigned>(__double2loint(z)) >> 9)) - 1.0f;
-    const float q = fmaf(fmaf(fmaf(c3, r, c2), r, c1), r, 0x1p-8f);
-    const unsigned one_and_q = __float_as_uint(q) + (0x80000000u - 0x3b800000u);
-    const u64 w = static_cast<u64>(s.table[whole & (kTable - 1)]) * one_and_q;  // units of 2^-62
-    return x >= lowest ? ((w >> (61 - unit - (whole >> 10))) + 1) >> 1 : 0;
+  // 2^y with y = (x - reference) scale: the nearest whole number of 2^-10 to y is a power of two times one from the table,
+  // the rest r, at most 2^-11, makes a factor of which the first three terms are taken (the fourth is 2^-37).
+  __device__ __forceinline__ double power(float x, float reference) const { return power(x, reference, scale); }
+  __device__ __forceinline__ double power(float x, float reference, double scale) const {
+    constexpr double c1 = 0.6931471805599453, c2 = 0.2402265069591007;  // ln 2, its square / 2
+    const double d = static_cast<double>(x) - static_cast<double>(reference);
+    const double z = fma(d, scale, kTenth);
+    const double r = fma(d, scale, -(z - kTenth));
+    const int tenths = __double2loint(z);
+    const double w = s.table[tenths & (kTable - 1)];
+    const double of_two = __hiloint2double(__double2hiint(w) + ((tenths >> 10) << 20), __double2loint(w));
+    return of_two * fma(fma(c2, r, c1), r, 1.0);
   }
-  // Nearly 2^-unit of it, and that as a whole number.
-  __device__ __forceinline__ float fast_weight(float x) const {
-    return x >= lowest ? exp2_approx((x - top) * fast_scale) : 0.0f;
-  }
-  __device__ u64 whole_of(float w) const { return __double2ull_rn(static_cast<double>(w) * static_cast<double>(1ull << unit)); }
-  __device__ float fast_sum() const {
-    float sum = 0.0f;
-    each_four([&](const float (&x)[4], int) {
-      sum += (fast_weight(x[0]) + fast_weight(x[1])) + (fast_weight(x[2]) + fast_weight(x[3]));
-    });
-    return sum;
-  }
+  __device__ __forceinline__ double weight_of(float x) const { return x >= lowest ? power(fmaxf(x, lowest), top) : 0.0; }
+  __device__ u64 whole_of(double w) const { return __double2ull_rn(w * static_cast<double>(1ull << unit)); }
+  __device__ __forceinline__ u64 weight(float x) const { return whole_of(weight_of(x)); }
 
   // visit(x, index) of the noted tokens, or of all for which `in` holds where they were too many to be noted.
   template <typename In, typename Visit>
@@ -399,60 +531,67 @@ struct Row {
     return part >= 1.0 ? static_cast<u64>(part) : 1;
   }
 
-  // Which tokens a sum in order of i counts, and what each one counts.
-  enum Measure { kEqual, kExact, kFast };
+  // Which tokens a sum in order of i counts: those of a value that `stay` keeps, one each, or those that `border` keeps,
+  // their weights.
   struct Counted {
-    Measure measure;
-    Border border;  // of what counts; kEqual: also the value
-    Border stay;    // (kEqual)
+    bool equal;
+    Border border, stay;
   };
   __device__ __forceinline__ u64 measure(const Counted& what, float x, int i) const {
-    if (what.measure == kEqual) return x == what.border.value && what.stay.keeps(x, i);
-    const u64 w = what.measure == kFast ? whole_of(fast_weight(x)) : weight(x);
-    return what.border.keeps(x, i) ? w : 0;
+    if (what.equal) return x == what.border.value && what.stay.keeps(x, i);
+    return what.border.keeps(x, i) ? weight(x) : 0;
   }
-  // The first token in order of i at which the sum exceeds u of the whole (kEqual: `target`).  `mine`: this thread's part of
-  // the sum.  Left in box.first for all blocks, behind one more barrier; -1 where FP32 sums leave it open.
+  // The first token in order of i at which the sum exceeds u of the whole (equal: `target`).  `mine`: this thread's part of
+  // the sum.
   __device__ __forceinline__ int locate(const Counted& what, u64 mine, float u, u64 target) {
     cg::cluster_group cluster = cg::this_cluster();
     tell_total(&s.box.part[rank], mine);
-    if (threadIdx.x == 0) s.box.first = -1;  // (what was there has been read)
     sync();
-    u64 before = 0, margin = 0;
+    u64 before = 0;
     for (int r = 0; r < rank; ++r) before += s.box.part[r];
     const u64 whole = total(s.box.part);
-    if (what.measure != kEqual) {
+    if (!what.equal) {
       const double at = u > 0.0f ? static_cast<double>(u) * static_cast<double>(whole) : 0.0;
       target = at < static_cast<double>(whole) ? min(static_cast<u64>(at), whole - 1) : whole - 1;
-      if (what.measure == kFast) margin = static_cast<u64>(2.0 * kSumError * static_cast<double>(whole)) + 1;
     }
     if (target >= before && target < before + s.box.part[rank]) {  // this block, ...
       const u64 of_warp = lane < kWarps ? s.warp_part[lane] : 0, upto = warp_upto(of_warp, lane);
       const int owner = __ffs(__ballot_sync(0xffffffffu, target < before + upto)) - 1;
       before += __shfl_sync(0xffffffffu, upto - of_warp, owner);  // ... and this warp's tokens
-      const int from = min(owner * each_warp, chunks()) * kElements, to = min((owner + 1) * each_warp, chunks()) * kElements;
+      const int from = min(owner * each_warp, vectors) * kElements, to = min((owner + 1) * each_warp, vectors) * kElements;
+      if (threadIdx.x == 0) s.bin = -1;
+      // as many tokens to each thread, and then one by one those of the thread at which it is exceeded
+      const int each_thread = (to - from + kThreads - 1) / kThreads;
+      const int my_from = min(from + static_cast<int>(threadIdx.x) * each_thread, to), my_to = min(my_from + each_thread, to);
+      u64 own = 0;
+#pragma unroll 2
+      for (int at = my_from; at < my_to; ++at) own += measure(what, value(at), first + at);
+      u64 sum = warp_upto(own, lane);
+      __syncthreads();  // (what was there has been read)
+      if (lane == 31) s.warp_part[warp] = sum;
+      __syncthreads();
+      sum += before + warp_total(lane < warp ? s.warp_part[lane & (kWarps - 1)] : 0);
+      // (single tokens' weights, rounded one by one, may sum up to a little less than their sum did: the last one then)
+      const bool mine = own != 0 && sum - own <= target;
+      if (mine) atomicMax(&s.bin, static_cast<int>(threadIdx.x));
+      __syncthreads();
+      const bool chosen = mine && s.bin == static_cast<int>(threadIdx.x);
+      __syncthreads();
+      if (chosen) {
+        u64 upto = sum - own;
 #pragma unroll 1
-      for (int start = from; start < to; start += kThreads) {
-        const int at = start + static_cast<int>(threadIdx.x);
-        const float x = at < to ? value(at) : -INFINITY;
-        const u64 own = at < to ? measure(what, x, first + at) : 0;
-        u64 sum = warp_upto(own, lane);
-        __syncthreads();  // (what was there has been read)
-        if (lane == 31) s.warp_part[warp] = sum;
-        __syncthreads();
-        sum += before + warp_total(lane < warp ? s.warp_part[lane & (kWarps - 1)] : 0);
-        if (sum > target && sum - own <= target && sum > target + margin && sum - own + margin <= target) {
-          for (int r = 0; r < size; ++r) *cluster.map_shared_rank(&s.box.first, r) = first + at;
+        for (int at = my_from; at < my_to && upto <= target; ++at) {
+          const u64 one = measure(what, value(at), first + at);
+          if (one != 0) s.bin = first + at;
+          upto += one;
         }
-        before += warp_total(lane < kWarps ? s.warp_part[lane] : 0);
-        if (before > target) break;
       }
+      __syncthreads();
+      if (threadIdx.x < size) *cluster.map_shared_rank(&s.box.first, threadIdx.x) = s.bin;
     }
     sync();
     return s.box.first;
   }
-  __device__ int chunks() const { return all_chunks; }
-  int all_chunks;  // of the block
 
   // What a search by weights leaves for the sums of what stays: this warp's sum above the noted tokens, and these.
   struct Known {
@@ -461,45 +600,54 @@ struct Row {
     int noted;
   };
 
-  // About where the weights reach top_p of their sum, by one in `ratio` of the tokens: false where these say nothing, else
-  // the bins of `bins` before which tokens surely stay and behind which none does, most likely.
-  __device__ __forceinline__ bool guess(const Bins& bins, float top_p, int& from, int& to) {
-    const u64 sum = whole_of(fast_sum());
+  // About where `target` tokens lie, or weights that reach top_p of `sum`, by one in `ratio` of the tokens: the bins of
+  // `bins` before which tokens surely stay and behind which none does, most likely; false where these say nothing.
+  __device__ __forceinline__ bool guess(bool weights, const Bins& bins, u64 target, float top_p, u64 sum, int& from, int& to) {
     clear_histogram();
-#pragma unroll 1
-    for (int at = begin * kElements + lane, k = 0; k < kSamples && at < end * kElements; at += 32, ++k) {
-      const float x = value(at);
-      if (bins.has(x)) count_weight(bins.of(x), weight(x));
+    for (int k = 0; k < kSamples / size; k += 2) {
+      const int at = begin * kElements + lane + 32 * k;
+      const float x[2] = {at < end * kElements ? value(at) : -INFINITY, at + 32 < end * kElements ? value(at + 32) : -INFINITY};
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        if (!bins.has(x[m])) continue;
+        if (weights) {
+          count_weight(bins.of(x[m]), weight(x[m]));
+        } else {
+          atomicAdd(&s.bins[0][bins.of(x[m])], 1u);
+        }
+      }
     }
-    tell_total(&s.box.part[rank], sum);
     sync();
     merge_bins();
-    u64 some = 0;
+    double middle, width;
+    if (weights) {
+      u64 some = 0;
 #pragma unroll 4
-    for (int b = lane; b < kBins; b += 32) some += s.sums[b];
-    some = warp_total(some);
-    // the border is where what lies behind has these parts of it
-    const double part = static_cast<double>(total(s.box.part)) / ratio;
-    // (a sum of such parts of what lies behind is off by about the root of the sum of the weights' squares)
-    const double behind = (1.0 - fmax(static_cast<double>(top_p), 0.0)) * part, middle = static_cast<double>(some) - behind;
-    if (!choose_bin(middle >= 1.0 ? static_cast<u64>(middle) : 1)) return false;
-    const double at_border = static_cast<double>(weight(bins.edge(s.bin)));
-    const double width = fmin(4.0 * sqrt(at_border * behind), 0.5 * behind);
-    __syncthreads();
+      for (int b = lane; b < kBins; b += 32) some += s.sums[b];
+      some = warp_total(some);
+      // what lies behind the border has this part of the sum (off by about the root of the sum of the weights' squares)
+      const double behind = (1.0 - fmax(static_cast<double>(top_p), 0.0)) * (static_cast<double>(sum) / ratio);
+      middle = static_cast<double>(some) - behind;
+      if (!choose_bin(middle >= 1.0 ? static_cast<u64>(middle) : 1)) return false;
+      width = fmin(4.0 * sqrt(static_cast<double>(weight(bins.edge(s.bin))) * behind), 0.5 * behind);
+      __syncthreads();
+    } else {
+      middle = static_cast<double>(target) / ratio;
+      width = 4.0 * sqrt(middle) + 4.0;
+    }
     from = 0;
     if (middle - width >= 1.0) {
       if (!choose_bin(static_cast<u64>(middle - width))) return false;
       from = s.bin;
       __syncthreads();
     }
-    if (!choose_bin(middle + width >= 1.0 ? static_cast<u64>(middle + width) : 1)) return false;
-    to = s.bin;
+    to = choose_bin(middle + width >= 1.0 ? static_cast<u64>(middle + width) : 1) ? s.bin : kBins - 1;
     return true;
   }
 
   // Of the tokens that `stay` keeps, the last before which fewer than `target` of them lie, or (weights) before which
   // weights of less than top_p of their sum lie.  Its value is in [low, top].
-  __device__ __forceinline__ Border search(bool weights, const Border stay, u64 target, float top_p, float low, Known& known) {
+  __device__ __forceinline__ Border search(bool weights, const Border stay, u64 target, float top_p, float low, u64 sum, Known& known) {
     Bins bins;
     bins.set(low, top);
     u64 before = 0;
@@ -507,10 +655,11 @@ struct Row {
     float lower = low, upper = top;  // the values that are noted
     auto in_range = [&](float x, int i) { return x >= lower && x <= upper && stay.keeps(x, i); };
     known.is = false;
-    bool near = weights && fast && stay.value < low;
+    const bool all = stay.value < low;  // (what does not stay is not among them)
+    bool near = all;
     if (near) {
       int from, to;
-      near = guess(bins, top_p, from, to);
+      near = guess(weights, bins, target, top_p, sum, from, to);
       if (near) {
         lower = fmaxf(low, bins.edge(to + 1));
         if (from > 0) upper = bins.edge(from - 1);
@@ -521,42 +670,44 @@ struct Row {
 #pragma unroll 1
     for (;;) {
       if (whole) {
-        u64 exact = 0, above = 0;
-        noted = 0;
-        each_four([&](const float (&x)[4], int i) {
-          const float largest = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          if (!__any_sync(0xffffffffu, largest >= fmaxf(fminf(lower, lowest), stay.value))) return;
-          if (weights) {
-            u64 w[4];
+        double sums = 0.0;  // of those above what is noted, or of all that stay
+        unsigned counted = 0;  // above what is noted
+        if (lane == 0) s.warp_noted[warp] = 0;
+        __syncwarp();
+        const float least = near ? lower : fmaxf(fminf(lower, lowest), stay.value);
+        each_from(least, [&](const float (&x)[4], int i) {
+          if (weights && (near || !all)) {
+            double w[4];  // (all at once, whether they count or not: their steps wait for one another)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = weight(x[k]);
-            if (!near) {
+            for (int m = 0; m < 4; ++m) w[m] = power(fmaxf(x[m], lowest), top);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = stay.keeps(x[k], i + k) ? w[k] : 0;
+            for (int m = 0; m < 4; ++m) {
+              const bool counts = near ? x[m] > upper : (x[m] >= lowest) & stay.keeps(x[m], i + m);
+              w[m] = counts ? w[m] : 0.0;
             }
-            exact += (w[0] + w[1]) + (w[2] + w[3]);
-            if (__any_sync(0xffffffffu, largest > upper)) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = x[k] > upper ? w[k] : 0;
-              above += (w[0] + w[1]) + (w[2] + w[3]);
-            }
+            sums += (w[0] + w[1]) + (w[2] + w[3]);
           }
-          if (!__any_sync(0xffffffffu, largest >= lower)) return;
+          unsigned mine = 0;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const bool mine = in_range(x[k], i + k);
-            const unsigned all = __ballot_sync(0xffffffffu, mine);
-            const int at = noted + __popc(all & ((1u << lane) - 1));
-            if (mine && at < kSpots) s.spots[warp][at] = static_cast<uint16_t>(i + k - first - begin * kElements);
-            noted += __popc(all);
+          for (int m = 0; m < 4; ++m) {
+            counted += x[m] > upper;
+            mine |= ((x[m] >= lower) & (x[m] <= upper) & (all | stay.keeps(x[m], i + m))) << m;
+          }
+          if (mine != 0) {
+            unsigned at = atomicAdd(&s.warp_noted[warp], static_cast<unsigned>(__popc(mine)));
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              if (((mine >> m) & 1) == 0) continue;
+              if (at < kSpots) s.spots[warp][at] = static_cast<uint16_t>(i + m - first - begin * kElements);
+              ++at;
+            }
           }
         });
-        if (weights) {
-          known.above = tell_total(&s.box.higher[rank], above);
-          known.noted = noted;
-          __syncthreads();
-          tell_total(&s.box.part[rank], exact);
-        }
+        __syncwarp();
+        noted = static_cast<int>(s.warp_noted[warp]);
+        const u64 total_of = tell_total(&s.box.higher[rank], weights ? whole_of(sums) : counted);
+        known.above = near ? total_of : 0;
+        known.noted = noted;
       }
       clear_histogram();
       each_noted(noted, in_range, [&](float x, int) {
@@ -568,9 +719,10 @@ struct Row {
         }
       });
       sync();
-      if (weights && whole) {
-        target = part_of(top_p, total(s.box.part));
-        before = total(s.box.higher);
+      if (whole) {
+        const u64 summed = total(s.box.higher);
+        if (weights) target = part_of(top_p, all ? sum : summed);
+        before = near ? summed : 0;
       }
       merge_bins();
       if ((near && target <= before) || !choose_bin(target - before)) {
@@ -621,7 +773,7 @@ struct Row {
       if (lowest_of == highest_of) {  // equal values: by their places
         const u64 w = weight(lowest_of);
         const u64 some = weights ? (target - before + w - 1) / w : target - before;
-        const Counted what{kEqual, {lowest_of, INT_MAX}, stay};
+        const Counted what{true, {lowest_of, INT_MAX}, stay};
         u64 mine = 0;
         each([&](float x, int i) { mine += measure(what, x, i); });
         return {lowest_of, locate(what, mine, 0.0f, some - 1)};
@@ -640,89 +792,115 @@ struct Row {
     merge_bins();
     if (!choose_bin(k)) return false;
     const int chosen = s.bin;
-    // (of the threads that have one at all; each_four() gave them out)
-    if (largest_of_thread >= bins.low && bins.of(largest_of_thread) <= chosen) {
-#pragma unroll 1
-      for (int four = begin * (kElements / 4) + lane; four < end * (kElements / 4); four += 32) {
-#pragma unroll 1
-        for (int at = 4 * four; at < 4 * four + 4; ++at) {
-          const float x = value(at);
-          if (x >= bins.low && bins.of(x) <= chosen) list(x, first + at);
+    const float least = bins.edge(chosen + 1);  // (surely below)
+    if (__any_sync(0xffffffffu, largest_of_thread >= least)) {
+      each_from(least, [&](const float (&x)[4], int i) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          if (x[m] >= bins.low && bins.of(x[m]) <= chosen) list(x[m], i + m);
         }
-      }
+      });
     }
     return rank_listed(true, k, 0, top_p, border) == kFound;
   }
 };
 
 // `slice`: elements to a block, a multiple of those in sixteen bytes.
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs args, int slice, int unit) {
-  uint4* data = Row<T>::slice_at();
-  constexpr int kElements = kVector / sizeof(T);
+template <typename T, int kBlocks>
+__global__ void __launch_bounds__(kThreads, kBlocks) sample_kernel(const SampleArgs args, int slice, int unit) {
+  constexpr int kElements = kVector / sizeof(T), kMany = Row<T, kBlocks>::kMany;
   cg::cluster_group cluster = cg::this_cluster();
-  Row<T> row;
+  Row<T, kBlocks> row;
   row.rank = static_cast<int>(cluster.block_rank());
   row.size = static_cast<int>(cluster.num_blocks());
   row.warp = threadIdx.x >> 5;
   row.lane = threadIdx.x & 31;
   const int number = blockIdx.x / row.size, lane = row.lane, warp = row.warp;
-  if (threadIdx.x == 0) s.bad = 0;
+  if (threadIdx.x == 0) {
+    s.bad = 0;
+    s.box.first = -1;
+  }
   cluster_arrive();  // (the blocks' shared memory is there)
-#pragma unroll 1
-  for (int i = threadIdx.x; i < kTable; i += kThreads) s.table[i] = __double2uint_rn(exp2(31.0 + i * (1.0 / kTable)));
   wait_for_predecessor();
   release_successor();
   const T* logits = static_cast<const T*>(args.logits) + args.stride * number + static_cast<int64_t>(row.rank) * slice;
-  const int tokens = min(max(args.vocab - row.rank * slice, 0), slice);
   // sixteen bytes at a time from the boundary below; what lies beside the slice is not read
-  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(logits) & (kVector - 1)) / sizeof(T));
-  row.all_chunks = tokens > 0 ? (lead + tokens + kElements - 1) / kElements : 0;
-  row.each_warp = (row.all_chunks + kWarps - 1) / kWarps;
-  row.first = row.rank * slice - lead;
-  row.begin = min(warp * row.each_warp, row.all_chunks);
-  row.end = min(row.begin + row.each_warp, row.all_chunks);
+  row.tokens = min(max(args.vocab - row.rank * slice, 0), slice);
+  row.lead = static_cast<int>((reinterpret_cast<uintptr_t>(logits) & (kVector - 1)) / sizeof(T));
+  row.from = reinterpret_cast<const uint4*>(logits - row.lead);
+  row.vectors = row.tokens > 0 ? (row.lead + row.tokens + kElements - 1) / kElements : 0;
+  row.each_warp = (row.vectors + kWarps - 1) / kWarps;
+  row.first = row.rank * slice - row.lead;
+  row.begin = min(warp * row.each_warp, row.vectors);
+  row.end = min(row.begin + row.each_warp, row.vectors);
   row.unit = unit;
   // (the same in all blocks)
-  row.ratio = fmaxf(1.0f, static_cast<float>((slice / kElements + kWarps) / kWarps * kElements) / (32.0f * kSamples));
-  float mine = -INFINITY;  // the largest
-  bool bad = false;
+  row.ratio = fmaxf(1.0f, static_cast<float>((slice / kElements + kWarps) / kWarps * kElements) / (32.0f * (kSamples / row.size)));
+  const float temperature = args.temperature.of(number), top_p = args.top_p.of(number);
+  const float least = args.min_p.of(number), u = args.uniform[number];
+  const int top_k = args.top_k.of(number);
+  const bool logprobs = args.logprobs != nullptr, some_k = top_k >= 1 && top_k < args.vocab;
+  row.scale = 1.4426950408889634 / static_cast<double>(temperature);
+  // the reference: the largest of the first vectors
+  float reference = -INFINITY;
   {
-    const uint4* from = reinterpret_cast<const uint4*>(logits - lead);
-    constexpr int kAtOnce = 8;
+    constexpr unsigned kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+    uint4 v = make_uint4(kNone, kNone, kNone, kNone);
+    const int c = row.begin + lane;
+    if (c < row.end && row.whole(c)) v = __ldg(row.from + c);
+    if (row.vectors > 0) row.set_edges();
 #pragma unroll 1
-    for (int start = row.begin + lane; start < row.end; start += 32 * kAtOnce) {
-      uint4 v[kAtOnce];
+    for (int i = threadIdx.x; i < kTable; i += kThreads) s.table[i] = exp2(i * (1.0 / kTable));
+    const unsigned words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        const int c = start + 32 * k;
-        if (c < row.end && c * kElements >= lead && (c + 1) * kElements <= lead + tokens) v[k] = __ldcs(from + c);
-      }
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        const int c = start + 32 * k;
-        if (c < row.end && c * kElements >= lead && (c + 1) * kElements <= lead + tokens) data[c] = v[k];
-      }
-    }
-    if (lead > 0 || (lead + tokens) % kElements != 0) {  // the ends
-#pragma unroll 1
-      for (int c = row.begin + lane; c < row.end; c += 32) {
-        if (c * kElements >= lead && (c + 1) * kElements <= lead + tokens) continue;
-        T* some = reinterpret_cast<T*>(data + c);
-#pragma unroll 1
-        for (int i = 0; i < kElements; ++i) {
-          const int at = c * kElements + i - lead;
-          some[i] = at >= 0 && at < tokens ? logits[at] : static_cast<T>(-INFINITY);
-        }
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        reference = fmaxf(reference, __uint_as_float(words[i]));
+      } else {
+        reference = fmaxf(reference, fmaxf(__uint_as_float(words[i] << 16), __uint_as_float(words[i] & 0xffff0000u)));
       }
     }
-    row.each_four([&](const float (&x)[4], int) {
+  }
+  reference = warp_max(reference);
+  if (lane == 0) s.warp_low[warp] = reference;
+  __syncthreads();
+  reference = warp_max(s.warp_low[lane & (kWarps - 1)]);
+  if (!(fabsf(reference) < INFINITY)) reference = 0.0f;
+  // the first time over the row: the largest, sums of weights and of e^(x - reference)
+  float mine = -INFINITY;
+  bool bad = false;
+  double weights = 0.0, sum = 0.0;
+  const bool weighed = temperature > 0.0f && (top_p < 1.0f || !some_k), same = temperature == 1.0f;
+  constexpr double kLog2eOf = 1.4426950408889634;
+  {
+    const float lowest = fmaxf(__double2float_ru(static_cast<double>(reference) - kBelow / row.scale), -FLT_MAX);
+    const float least_of = fmaxf(reference - kBelow * 0.693147f, -FLT_MAX);
+    const bool summed = logprobs && !(weighed && same);
+    const float least_used = fminf(weighed ? lowest : INFINITY, summed ? least_of : INFINITY);
+    __syncthreads();  // (the table, the edges)
+    row.each_many([&](const float (&x)[kMany], int) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        mine = fmaxf(mine, x[k]);
-        bad |= x[k] != x[k];
+      for (int m = 0; m < kMany; ++m) bad |= x[m] != x[m];
+      const float largest = row.largest_of(x);
+      mine = fmaxf(mine, largest);
+      if (!__any_sync(0xffffffffu, largest >= least_used)) return;
+      double w[kMany];
+      if (weighed) {
+#pragma unroll
+        for (int m = 0; m < kMany; ++m) w[m] = row.power(fmaxf(x[m], lowest), reference);
+#pragma unroll
+        for (int m = 0; m < kMany; ++m) w[m] = x[m] >= lowest ? w[m] : 0.0;
+        weights += row.sum_of(w);
+      }
+      if (summed) {
+#pragma unroll
+        for (int m = 0; m < kMany; ++m) w[m] = row.power(fmaxf(x[m], least_of), reference, kLog2eOf);
+#pragma unroll
+        for (int m = 0; m < kMany; ++m) w[m] = x[m] >= least_of ? w[m] : 0.0;
+        sum += row.sum_of(w);
       }
     });
+    if (weighed && same) sum = weights;
   }
   float top = warp_max(mine);
   if (__any_sync(0xffffffffu, bad) && lane == 0) s.bad = 1;
@@ -733,10 +911,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs ar
     row.tell(&s.box.top[row.rank], warp_max(s.warp_top[lane & (kWarps - 1)]));
     row.tell(&s.box.bad[row.rank], s.bad);
   }
-  // (asked for meanwhile)
-  const float temperature = args.temperature.of(number), top_p = args.top_p.of(number);
-  const float least = args.min_p.of(number), u = args.uniform[number];
-  const int top_k = args.top_k.of(number);
   row.sync();
   top = s.box.top[0];
   int any_bad = s.box.bad[0];
@@ -745,7 +919,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs ar
     any_bad |= s.box.bad[r];
   }
   row.top = top;
-  const bool logprobs = args.logprobs != nullptr;
   if (any_bad || !(fabsf(top) < INFINITY)) {  // no distribution
     if (row.rank == 0 && threadIdx.x == 0) {
       args.tokens[number] = -1;
@@ -753,52 +926,56 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs ar
     }
     return;  // (behind a barrier that all blocks have passed; nobody reads a neighbour any more)
   }
-  if (logprobs) {
-    float sum = 0.0f;
-    row.each_four([&](const float (&x)[4], int) {
-      float e[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) e[k] = exp2_approx((x[k] - top) * kLog2e);
-      sum += (e[0] + e[1]) + (e[2] + e[3]);
-    });
-    auto over_warp = [&] {
-#pragma unroll 1
-      for (int step = 16; step > 0; step /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, step);
-    };
-    over_warp();
-    if (lane == 0) s.warp_low[warp] = sum;
-    __syncthreads();
-    if (warp == 0) {
-      sum = lane < kWarps ? s.warp_low[lane] : 0.0f;
-      over_warp();
-      row.tell(&s.box.sum[row.rank], sum);  // (read behind a barrier that is still to come)
-    }
-    __syncthreads();
+  // by the largest now; a block whose own largest lies far above its reference goes over its slice once more
+  const float own = warp_max(s.warp_top[lane & (kWarps - 1)]);
+  row.lowest = top;
+  if (temperature > 0.0f) {
+    // 2^-1.5 of a unit and less is 0
+    const double reach = (unit + 1.5) / row.scale;
+    row.lowest = fmaxf(__double2float_ru(static_cast<double>(top) - reach), -FLT_MAX);
   }
-  typename Row<T>::Counted what{Row<T>::kEqual, {top, INT_MAX}, {-INFINITY, INT_MAX}};  // the first of the largest
-  typename Row<T>::Known known;
+  u64 all_weights = 0;  // of the row
+  if (weighed) {
+    if (own >= reference && static_cast<double>(own) - static_cast<double>(reference) <= kAbove / row.scale) {
+      weights *= exp2((static_cast<double>(reference) - static_cast<double>(top)) * row.scale);
+    } else {
+      weights = 0.0;
+      if (own >= row.lowest) row.each([&](float x, int) { weights += row.weight_of(x); });
+    }
+    row.tell_total(&s.box.part[row.rank], row.whole_of(weights));
+    row.sync();
+    all_weights = row.total(s.box.part);
+  }
+  if (logprobs) {
+    if (own >= reference && static_cast<double>(own) - static_cast<double>(reference) <= kAbove / kLog2eOf) {
+      sum *= exp2((static_cast<double>(reference) - static_cast<double>(top)) * kLog2eOf);
+    } else {
+      sum = 0.0;
+      const float least_of = fmaxf(top - kBelow * 0.693147f, -FLT_MAX);
+      if (own >= least_of) row.each([&](float x, int) { sum += x >= least_of ? row.power(fmaxf(x, least_of), top, kLog2eOf) : 0.0; });
+    }
+    sum = warp_total(sum);
+    if (lane == 0) s.warp_double[warp] = sum;
+    __syncthreads();
+    if (warp == 0) row.tell(&s.box.sum[row.rank], warp_total(lane < kWarps ? s.warp_double[lane] : 0.0));  // (read behind a barrier that is still to come)
+  }
+  typename Row<T, kBlocks>::Counted what{true, {top, INT_MAX}, {-INFINITY, INT_MAX}};  // the first of the largest
+  typename Row<T, kBlocks>::Known known;
   known.is = false;
   if (temperature > 0.0f) {
-    row.scale = 1.4426950408889634 / static_cast<double>(temperature);
-    row.fast_scale = static_cast<float>(row.scale);
-    row.fast = temperature >= 1e-30f && temperature <= 1e30f;
-    // 2^-1.5 of a unit and less is 0 (so shifts in weight() stay below 64)
-    const double reach = (unit + 1.5) * 0.6931471805599453 * static_cast<double>(temperature);
-    row.lowest = fmaxf(__double2float_ru(static_cast<double>(top) - reach), -FLT_MAX);
     Border border{-INFINITY, INT_MAX};
-    const bool some_k = top_k >= 1 && top_k < args.vocab;
     bool done = false;
     if (some_k && top_k <= kFewK) done = row.search_few(mine, top_k, top_p, border);
 #pragma unroll 1
     for (int by_weight = 0; by_weight < 2 && !done; ++by_weight) {
       if (by_weight ? !(top_p < 1.0f) : !some_k) continue;
       float low = border.value;
-      if (by_weight && !some_k && row.fast) {
+      if (by_weight && !some_k) {
         // what lies lower never stays (a hundredth less than that, and nothing for the rounding of weights)
         const double cut = 0.99 * (1.0 - fmax(static_cast<double>(top_p), 0.0)) / args.vocab;
         low = __double2float_rd(static_cast<double>(top) + static_cast<double>(temperature) * log(cut));
       }
-      border = row.search(by_weight != 0, border, top_k, top_p, fmaxf(low, row.lowest), known);
+      border = row.search(by_weight != 0, border, top_k, top_p, fmaxf(low, row.lowest), all_weights, known);
     }
     if (least > 0.0f && temperature < INFINITY) {  // w >= p where x - m >= T ln p
       const double below = least < 1.0f ? static_cast<double>(temperature) * log(static_cast<double>(least)) : 0.0;
@@ -808,32 +985,28 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs ar
         known.is = false;
       }
     }
-    what = {!(border.value > -INFINITY) && row.fast ? Row<T>::kFast : Row<T>::kExact, border, border};
+    what = {false, border, border};
   }
-  int token = -1;
-#pragma unroll 1
-  for (int attempt = 0; attempt < 2 && token < 0; ++attempt) {
-    u64 stays = 0;
-    if (what.measure == Row<T>::kFast) {
-      stays = row.whole_of(row.fast_sum());
-    } else if (known.is) {
-      stays = lane == 0 ? known.above : 0;
-      row.each_noted(known.noted, [](float, int) { return false; }, [&](float x, int i) { stays += row.measure(what, x, i); });
-    } else {
-      row.each_four([&](const float (&x)[4], int i) {
-        if (!__any_sync(0xffffffffu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= what.border.value)) return;
-        u64 w[4];
+  u64 stays = 0;
+  if (!what.equal && weighed && !(what.border.value > -INFINITY)) {
+    stays = row.whole_of(weights);
+  } else if (known.is) {
+    stays = lane == 0 ? known.above : 0;
+    row.each_noted(known.noted, [](float, int) { return false; }, [&](float x, int i) { stays += row.measure(what, x, i); });
+  } else {
+    row.each_from(what.border.value, [&](const float (&x)[4], int i) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = row.measure(what, x[k], i + k);
-        stays += (w[0] + w[1]) + (w[2] + w[3]);
-      });
-    }
-    token = row.locate(what, stays, u, 0);
-    what.measure = Row<T>::kExact;
+      for (int m = 0; m < 4; ++m) {
+        const u64 w = what.equal ? x[m] == top : row.whole_of(row.power(fmaxf(x[m], row.lowest), top));
+        stays += (x[m] >= row.lowest) & what.border.keeps(x[m], i + m) ? w : 0;
+      }
+    });
   }
+  int token = row.locate(what, stays, u, 0);
+  if (static_cast<unsigned>(token) >= static_cast<unsigned>(args.vocab)) token = -1;  // (there is always one)
   if (row.rank == 0 && threadIdx.x == 0) {
     args.tokens[number] = token;
-    if (logprobs) {
+    if (logprobs && token >= 0) {
       double all = 0.0;
       for (int r = 0; r < row.size; ++r) all += s.box.sum[r];
       const float x = static_cast<float>(static_cast<const T*>(args.logits)[args.stride * number + token]);
@@ -844,24 +1017,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs ar
 
 #undef s
 
-size_t shared_bytes(int slice, int size) { return (sizeof(Shared) + 15) / 16 * 16 + static_cast<size_t>(slice) * size + kVector; }
-
-static_assert((sizeof(Shared) + 15) / 16 * 16 + kMostSliceBytes + kVector <= kMaxSharedBytes);
-
-template <typename T>
+template <typename T, int kBlocks>
 cudaError_t launch(const SampleArgs& args, cudaStream_t stream) {
-  // As few blocks to a row as hold it; more where rows are few, so that all SMs read.
-  const int64_t bytes = static_cast<int64_t>(args.vocab) * sizeof(T);
-  const int64_t limit = bytes > static_cast<int64_t>(kSliceBytes) * kMaxCluster ? kMostSliceBytes : kSliceBytes;
-  int size = 1;
-  while (size < kMaxCluster && (bytes > limit * size || (args.rows * size * 2 <= device_sms() && bytes > 8192 * size))) size *= 2;
+  // One block to a row where there are enough; else as many as find room beside each other, but for what clusters leave
+  // empty.
+  const int room = device_sms() * kBlocks * 9 / 10;
   constexpr int kElements = kVector / sizeof(T);
+  int size = 1;
+  while (size < kMaxCluster &&
+         ((args.vocab + size - 1) / size > kMostSlice || (args.rows * size * 2 <= room && args.vocab > 2048 * size))) {
+    size *= 2;
+  }
   const int slice = ((args.vocab + size - 1) / size + kElements - 1) / kElements * kElements;
   int bits = 0;
   while ((1ll << bits) < args.vocab) ++bits;
   const int unit = std::min(kMostUnit, 63 - bits);  // so that the sum of all weights has 64 bits
   static std::atomic<uint64_t> allowed{0};
-  const cudaError_t err = allow_shared_memory_once(sample_kernel<T>, allowed);
+  const cudaError_t err = allow_shared_memory_once(sample_kernel<T, kBlocks>, allowed);
   if (err != cudaSuccess) return err;
   cudaLaunchAttribute attributes[2];
   attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -871,21 +1043,24 @@ cudaError_t launch(const SampleArgs& args, cudaStream_t stream) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(args.rows) * size);
   config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = shared_bytes(slice, sizeof(T));
+  config.dynamicSmemBytes = sizeof(Shared);
   config.stream = stream;
   config.attrs = attributes;
   config.numAttrs = 2;
-  return cudaLaunchKernelEx(&config, sample_kernel<T>, args, slice, unit);
+  return cudaLaunchKernelEx(&config, sample_kernel<T, kBlocks>, args, slice, unit);
 }
 
 }  // namespace
 
 bool sample_supported(int vocab, bool bf16) {
-  return static_cast<int64_t>(vocab) * (bf16 ? 2 : 4) <= static_cast<int64_t>(kMostSliceBytes) * kMaxCluster;
+  return static_cast<int64_t>(vocab) * (bf16 ? 2 : 4) <= kMostRowBytes;
 }
 
 cudaError_t launch_sample(const SampleArgs& args, bool bf16, cudaStream_t stream) {
-  return bf16 ? launch<__nv_bfloat16>(args, stream) : launch<float>(args, stream);
+  // Few rows: one block to an SM, whose threads then have registers enough (64 rows of 131072: 80 us; two blocks, which
+  // spill, 96).  Many: two, which hide each other's waits (256 rows: 68 us; one block to an SM 95).
+  if (args.rows * 10 > device_sms() * 9) return bf16 ? launch<__nv_bfloat16, 2>(args, stream) : launch<float, 2>(args, stream);
+  return bf16 ? launch<__nv_bfloat16, 1>(args, stream) : launch<float, 1>(args, stream);
 }
 
 }  // namespace nmoe
