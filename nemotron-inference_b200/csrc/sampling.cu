@@ -19,12 +19,12 @@
 //   top-k   the k-th largest of the threads' own largest values is no larger than the k-th largest of all: one entry a
 //           thread finds a bound that few more than k tokens reach, and these are ranked
 //   top-p   some thousand of the tokens tell about where the border lies: the pass that sums up the weights above notes
-//           the tokens near it, and the rest goes over these.  (If it lies elsewhere: over all with weights of (1 - p) / n
-//           of the largest's, below which no token of n stays.)
+//           the tokens near it, and the rest goes over these.  (If it lies elsewhere, in one of some hundred rows where
+//           few weights are most of the sum: once more with a wider guess, and then all.)  Counts of many tokens do the same.
 // The sums in order of i come last, of what stays.
 //
-// Measured (B200, FP32): 256 rows of 131072 as they are 68 us, 40 of them for the first pass (two thirds of what copying
-// reaches); 64 rows of as many settings 80 us; one row 31 us; 37 rows of 50001 in BF16, top-k and top-p, 22 us.  Rows that
+// Measured (B200, FP32): 256 rows of 131072 as they are 67 us, 40 of them for the first pass (two thirds of what copying
+// reaches); 64 rows of as many settings 78 to 83 us; one row 31 us; 37 rows of 50001 in BF16, top-k and top-p, 22 us.  Rows that
 // lay in the shared memory of clusters of eight blocks took 145, 102, 33 and 22 us: such clusters left a third of the
 // SMs' room empty, and SMs idle while a row's steps waited.
 #include <cooperative_groups.h>
@@ -50,10 +50,9 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 1024;
 constexpr int kListed = 256;  // tokens ranked one by one
-constexpr int kAside = 160;   // vectors that wait for each_from()
-constexpr int kSpots = 256;   // noted places of a warp
 constexpr int kSamples = 16;  // tokens to a thread that guess() goes by, over the blocks of a row
-constexpr int kFewK = 160;    // top_k that the bound from the threads' largest values is for
+// top_k that the bound from the threads' largest values is for (64 rows, k 50: 39 us, by a guess 49; k 150: 41, 47)
+constexpr int kFewK = 160;
 constexpr int kVector = 16;   // bytes
 constexpr int kMostSlice = 1 << 17;  // tokens to a block (the histogram's words)
 constexpr int kMostRowBytes = 1536 * 1024;
@@ -81,7 +80,10 @@ struct Box {
   int state;  // of a search
 };
 
+template <int kBlocks>
 struct Shared {
+  static constexpr int kSpots = kBlocks == 1 ? 2048 : 1024;  // noted places of a warp
+  static constexpr int kAside = kBlocks == 1 ? 160 : 96;     // vectors that wait for each_from()
   Box box;
   double table[kTable];
   uint4 edges[2];
@@ -171,13 +173,14 @@ struct Bins {
 };
 
 extern __shared__ __align__(16) uint8_t dynamic_shared[];
-#define s (*reinterpret_cast<Shared*>(dynamic_shared))  // (by name: a pointer in a register has no address space)
+#define s (*reinterpret_cast<Shared<kBlocks>*>(dynamic_shared))  // (by name: a pointer in a register has no address space)
 
 template <typename T, int kBlocks>
 struct Row {
   static constexpr int kMany = kBlocks == 1 ? 8 : 4;   // values at once: their steps wait for one another
   static constexpr int kAhead = kBlocks == 1 ? 4 : 2;  // vectors on their way
-  static_assert(32 * (kAhead + 1) <= kAside);
+  static constexpr int kSpots = Shared<kBlocks>::kSpots;
+  static_assert(32 * (kAhead + 1) <= Shared<kBlocks>::kAside);
   static constexpr int kElements = kVector / sizeof(T);
   // This block's slice, in sixteen bytes each: `vectors` of them from an aligned address on, at which `lead` elements
   // of something else come first; `tokens` of its own, the first of them token `first` + `lead`.
@@ -374,16 +377,24 @@ struct Row {
   __device__ u64 whole_of(double w) const { return __double2ull_rn(w * static_cast<double>(1ull << unit)); }
   __device__ __forceinline__ u64 weight(float x) const { return whole_of(weight_of(x)); }
 
-  // visit(x, index) of the noted tokens, or of all for which `in` holds where they were too many to be noted.
+  // visit(x, index) of the noted tokens, or of all from `least` on for which `in` holds where they were too many to be
+  // noted.
   template <typename In, typename Visit>
-  __device__ __forceinline__ void each_noted(int count, In in, Visit visit) const {
-    const bool all = count > kSpots;
-    const int stop = all ? (end - begin) * kElements : count;
+  __device__ __forceinline__ void each_noted(int count, float least, In in, Visit visit) const {
+    if (count > kSpots) {  // (the same for a warp)
+      each_from(least, [&](const float (&x)[4], int i) {
 #pragma unroll 1
-    for (int j = lane; j < stop; j += 32) {
-      const int at = begin * kElements + (all ? j : s.spots[warp][j]);
-      const float x = value(at);
-      if (!all || in(x, first + at)) visit(x, first + at);
+        for (int m = 0; m < 4; ++m) {
+          const float one = m == 0 ? x[0] : m == 1 ? x[1] : m == 2 ? x[2] : x[3];
+          if (in(one, i + m)) visit(one, i + m);
+        }
+      });
+      return;
+    }
+#pragma unroll 1
+    for (int j = lane; j < count; j += 32) {
+      const int at = begin * kElements + s.spots[warp][j];
+      visit(value(at), first + at);
     }
   }
 
@@ -602,7 +613,7 @@ struct Row {
 
   // About where `target` tokens lie, or weights that reach top_p of `sum`, by one in `ratio` of the tokens: the bins of
   // `bins` before which tokens surely stay and behind which none does, most likely; false where these say nothing.
-  __device__ __forceinline__ bool guess(bool weights, const Bins& bins, u64 target, float top_p, u64 sum, int& from, int& to) {
+  __device__ __forceinline__ bool guess(bool weights, const Bins& bins, u64 target, float top_p, u64 sum, int reach, int& from, int& to) {
     clear_histogram();
     for (int k = 0; k < kSamples / size; k += 2) {
       const int at = begin * kElements + lane + 32 * k;
@@ -619,7 +630,7 @@ struct Row {
     }
     sync();
     merge_bins();
-    double middle, width;
+    double middle, above, below;  // how much there may lie between the border and the ends
     if (weights) {
       u64 some = 0;
 #pragma unroll 4
@@ -629,19 +640,21 @@ struct Row {
       const double behind = (1.0 - fmax(static_cast<double>(top_p), 0.0)) * (static_cast<double>(sum) / ratio);
       middle = static_cast<double>(some) - behind;
       if (!choose_bin(middle >= 1.0 ? static_cast<u64>(middle) : 1)) return false;
-      width = fmin(4.0 * sqrt(static_cast<double>(weight(bins.edge(s.bin))) * behind), 0.5 * behind);
+      const double off = sqrt(static_cast<double>(weight(bins.edge(s.bin))) * behind);
+      above = 6.0 * reach * off;  // (weights there are larger)
+      below = fmin(5.0 * reach * off, (reach == 1 ? 0.9 : 1.0) * behind);
       __syncthreads();
     } else {
       middle = static_cast<double>(target) / ratio;
-      width = 4.0 * sqrt(middle) + 4.0;
+      above = below = reach * (5.0 * sqrt(middle) + 4.0);
     }
     from = 0;
-    if (middle - width >= 1.0) {
-      if (!choose_bin(static_cast<u64>(middle - width))) return false;
+    if (middle - above >= 1.0) {
+      if (!choose_bin(static_cast<u64>(middle - above))) return false;
       from = s.bin;
       __syncthreads();
     }
-    to = choose_bin(middle + width >= 1.0 ? static_cast<u64>(middle + width) : 1) ? s.bin : kBins - 1;
+    to = choose_bin(middle + below >= 1.0 ? static_cast<u64>(middle + below) : 1) ? s.bin : kBins - 1;
     return true;
   }
 
@@ -649,40 +662,41 @@ struct Row {
   // weights of less than top_p of their sum lie.  Its value is in [low, top].
   __device__ __forceinline__ Border search(bool weights, const Border stay, u64 target, float top_p, float low, u64 sum, Known& known) {
     Bins bins;
-    bins.set(low, top);
     u64 before = 0;
     int noted = 0;  // of this warp
     float lower = low, upper = top;  // the values that are noted
     auto in_range = [&](float x, int i) { return x >= lower && x <= upper && stay.keeps(x, i); };
     known.is = false;
     const bool all = stay.value < low;  // (what does not stay is not among them)
-    bool near = all;
-    if (near) {
-      int from, to;
-      near = guess(weights, bins, target, top_p, sum, from, to);
-      if (near) {
-        lower = fmaxf(low, bins.edge(to + 1));
-        if (from > 0) upper = bins.edge(from - 1);
-        bins.set(lower, upper);
-      }
-    }
+    float least_of = low, most_of = top;  // the border lies between these
+    int reach = 1;
     bool whole = true;
 #pragma unroll 1
     for (;;) {
       if (whole) {
+        bins.set(low, top);
+        int from, to;
+        const bool guessed = all && reach > 0 && guess(weights, bins, target, top_p, sum, reach, from, to);
+        lower = guessed ? fmaxf(least_of, bins.edge(to + 1)) : least_of;
+        upper = guessed && from > 0 ? fminf(most_of, bins.edge(from - 1)) : most_of;
+        if (!(lower <= upper)) {
+          lower = least_of;
+          upper = most_of;
+        }
+        bins.set(lower, upper);
         double sums = 0.0;  // of those above what is noted, or of all that stay
         unsigned counted = 0;  // above what is noted
         if (lane == 0) s.warp_noted[warp] = 0;
         __syncwarp();
-        const float least = near ? lower : fmaxf(fminf(lower, lowest), stay.value);
+        const float least = all ? lower : fmaxf(fminf(lower, lowest), stay.value);
         each_from(least, [&](const float (&x)[4], int i) {
-          if (weights && (near || !all)) {
+          if (weights) {
             double w[4];  // (all at once, whether they count or not: their steps wait for one another)
 #pragma unroll
             for (int m = 0; m < 4; ++m) w[m] = power(fmaxf(x[m], lowest), top);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-              const bool counts = near ? x[m] > upper : (x[m] >= lowest) & stay.keeps(x[m], i + m);
+              const bool counts = all ? x[m] > upper : (x[m] >= lowest) & stay.keeps(x[m], i + m);
               w[m] = counts ? w[m] : 0.0;
             }
             sums += (w[0] + w[1]) + (w[2] + w[3]);
@@ -706,11 +720,11 @@ struct Row {
         __syncwarp();
         noted = static_cast<int>(s.warp_noted[warp]);
         const u64 total_of = tell_total(&s.box.higher[rank], weights ? whole_of(sums) : counted);
-        known.above = near ? total_of : 0;
+        known.above = all ? total_of : 0;
         known.noted = noted;
       }
       clear_histogram();
-      each_noted(noted, in_range, [&](float x, int) {
+      each_noted(noted, lower, in_range, [&](float x, int) {
         if (!bins.has(x)) return;
         if (weights) {
           count_weight(bins.of(x), weight(x));
@@ -722,15 +736,19 @@ struct Row {
       if (whole) {
         const u64 summed = total(s.box.higher);
         if (weights) target = part_of(top_p, all ? sum : summed);
-        before = near ? summed : 0;
+        before = all ? summed : 0;
       }
       merge_bins();
-      if ((near && target <= before) || !choose_bin(target - before)) {
-        if (!near) return stay;
-        near = false;  // the guess was wrong: all of them
-        lower = low;
-        upper = top;
-        bins.set(lower, upper);
+      if ((all && target <= before) || !choose_bin(target - before)) {
+        if (!all || reach == 0) return stay;
+        // the guess was wrong: a wider one, and then all, on the side where the border is
+        if (target <= before) {
+          least_of = upper;
+        } else {
+          most_of = lower;
+        }
+        reach = reach == 1 ? 4 : 0;
+        whole = true;
         before = 0;
         continue;
       }
@@ -738,7 +756,7 @@ struct Row {
       const int chosen = s.bin;
       before += s.before;
       auto in_bin = [&](float x) { return bins.has(x) && bins.of(x) == chosen; };
-      each_noted(noted, in_range, [&](float x, int i) {
+      each_noted(noted, lower, in_range, [&](float x, int i) {
         if (in_bin(x)) list(x, i);
       });
       Border border;
@@ -746,7 +764,7 @@ struct Row {
       if (rank_listed(!weights, target, before, 1.0f, border) == kFound) return border;
       // too many in the bin: their range
       float lowest_of = INFINITY, highest_of = -INFINITY;
-      each_noted(noted, in_range, [&](float x, int) {
+      each_noted(noted, lower, in_range, [&](float x, int) {
         if (in_bin(x)) {
           lowest_of = fminf(lowest_of, x);
           highest_of = fmaxf(highest_of, x);
@@ -992,7 +1010,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) sample_kernel(const SampleA
     stays = row.whole_of(weights);
   } else if (known.is) {
     stays = lane == 0 ? known.above : 0;
-    row.each_noted(known.noted, [](float, int) { return false; }, [&](float x, int i) { stays += row.measure(what, x, i); });
+    row.each_noted(known.noted, 0.0f, [](float, int) { return false; }, [&](float x, int i) { stays += row.measure(what, x, i); });
   } else {
     row.each_from(what.border.value, [&](const float (&x)[4], int i) {
 #pragma unroll
@@ -1020,12 +1038,13 @@ __global__ void __launch_bounds__(kThreads, kBlocks) sample_kernel(const SampleA
 template <typename T, int kBlocks>
 cudaError_t launch(const SampleArgs& args, cudaStream_t stream) {
   // One block to a row where there are enough; else as many as find room beside each other, but for what clusters leave
-  // empty.
+  // empty, those of eight a quarter (16 rows, top-k: in clusters of eight, some behind the others, 41 us, of four 27).
   const int room = device_sms() * kBlocks * 9 / 10;
   constexpr int kElements = kVector / sizeof(T);
   int size = 1;
   while (size < kMaxCluster &&
-         ((args.vocab + size - 1) / size > kMostSlice || (args.rows * size * 2 <= room && args.vocab > 2048 * size))) {
+         ((args.vocab + size - 1) / size > kMostSlice ||
+          (args.rows * size * 2 <= (size * 2 == 8 ? room * 4 / 5 : room) && args.vocab > 2048 * size))) {
     size *= 2;
   }
   const int slice = ((args.vocab + size - 1) / size + kElements - 1) / kElements * kElements;
@@ -1043,7 +1062,7 @@ cudaError_t launch(const SampleArgs& args, cudaStream_t stream) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(args.rows) * size);
   config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = sizeof(Shared);
+  config.dynamicSmemBytes = sizeof(Shared<kBlocks>);
   config.stream = stream;
   config.attrs = attributes;
   config.numAttrs = 2;
@@ -1058,8 +1077,9 @@ bool sample_supported(int vocab, bool bf16) {
 
 cudaError_t launch_sample(const SampleArgs& args, bool bf16, cudaStream_t stream) {
   // Few rows: one block to an SM, whose threads then have registers enough (64 rows of 131072: 80 us; two blocks, which
-  // spill, 96).  Many: two, which hide each other's waits (256 rows: 68 us; one block to an SM 95).
-  if (args.rows * 10 > device_sms() * 9) return bf16 ? launch<__nv_bfloat16, 2>(args, stream) : launch<float, 2>(args, stream);
+  // spill, 96).  Many, of which an SM has more than one block's: two, which hide each other's waits (128 rows, top-p 106 us,
+  // 96 rows, top-k 55; with one block to an SM 133 and 57; 256 rows as they are 67, 95).
+  if (args.rows * 20 > device_sms() * 9) return bf16 ? launch<__nv_bfloat16, 2>(args, stream) : launch<float, 2>(args, stream);
   return bf16 ? launch<__nv_bfloat16, 1>(args, stream) : launch<float, 1>(args, stream);
 }
 
