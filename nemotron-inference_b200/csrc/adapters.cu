@@ -5,12 +5,15 @@
 // 2 rank (inner + outer) operations, some tens to a byte.  Two launches:
 //   inside   t = x A^T for a tile of rows of one request, the tensor cores taking A as the operand of 128 rows (the
 //            ranks; those behind the rank are whatever lies there and their results are not read) and the rows of x as the
-//            one of 16 or 128, so that a single token costs no more than its own bytes.  The contraction is cut
-//            into parts where tiles are few; each leaves FP32 sums.
+//            other, of 128 too, of which only the rows that there are get read: a tile of 16 was no faster for few rows
+//            and slower from 12 on.  The contraction is cut into parts where tiles are few; each leaves FP32 sums.
 //   outside  out = y + (scale t) B^T, a block to an SM with an even share of all tiles of 128 rows and 128 columns, y and B
-//            on their way tiles ahead.  t, summed up in a fixed order, is two bf16 terms (within 2^-17 of it; as one it would be off by 2^-9, of the size of what y's own rounding
-//            leaves), both multiplied with the same tile of B into one sum; y is added in FP32 and the result rounded
-//            once.  Rows without an adapter are copied.
+//            on their way tiles ahead.  t, summed up in a fixed order, is two bf16 terms (within 2^-17 of it; as one it
+//            would be off by 2^-9, of the size of what y's own rounding leaves), both multiplied with the same tile of B
+//            into one sum; y is added in FP32 and the result rounded once.  Rows without an adapter are copied.
+// Measured (B200, calls one after another): 23 requests of 356 rows, 2688 to 4608, rank 32, 49 us (3.6 TB/s); 64 of 4 rows,
+// 4096 to 2688, rank 64, 26 us (1.5 TB/s: a block's first tiles are on their way for 5 us, in each launch, and a piece
+// begins with t); one row 10.5 us in a graph, 17 called.
 #include <algorithm>
 
 #include "attention.h"
@@ -39,15 +42,15 @@ struct Found {
   RowsTile tile;
 };
 
-// All threads: tile `u` of the entries' tiles of `height` rows.
-__device__ RowsTile find_tile(const AdapterArgs& args, int u, int height, Found* f) {
+// All threads: tile `u` of the entries' tiles of rows.
+__device__ RowsTile find_tile(const AdapterArgs& args, int u, Found* f) {
   const int threads = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int each = (args.count + threads - 1) / threads;
   const int begin = min(static_cast<int>(threadIdx.x) * each, args.count), end = min(begin + each, args.count);
   auto tiles_of = [&](int i, int& from) {
     from = args.offsets[i];
     const int to = args.offsets[i + 1];
-    return from >= 0 && from <= to && to <= args.rows ? (to - from + height - 1) / height : 0;
+    return from >= 0 && from <= to && to <= args.rows ? (to - from + kTile - 1) / kTile : 0;
   };
   if (threadIdx.x == 0) f->tile = {0, 0, -1};
   int mine = 0, from;
@@ -66,8 +69,8 @@ __device__ RowsTile find_tile(const AdapterArgs& args, int u, int height, Found*
     for (int i = begin; i < end; ++i) {
       const int tiles = tiles_of(i, from);
       if (u < at + tiles) {
-        const int skip = (u - at) * height, id = args.ids[i];
-        f->tile = {from + skip, min(args.offsets[i + 1] - from - skip, height),
+        const int skip = (u - at) * kTile, id = args.ids[i];
+        f->tile = {from + skip, min(args.offsets[i + 1] - from - skip, kTile),
                    static_cast<unsigned>(id) < static_cast<unsigned>(args.adapters) ? id : -1};
         break;
       }
@@ -92,7 +95,6 @@ struct InsideControl {
   Found found;
 };
 
-template <int N>
 __global__ void __launch_bounds__(kInsideThreads)
     inside_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const AdapterArgs args,
                   int chunks_each, int stages) {
@@ -101,7 +103,6 @@ __global__ void __launch_bounds__(kInsideThreads)
   uint8_t* ring = raw + sizeof(InsideControl);
   ring += (1024 - (smem_u32(ring) & 1023)) & 1023;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kColumns = N < 32 ? 32 : N;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kMostStages; ++i) {
       mbar_init(&c->full[i], 1);
@@ -111,19 +112,19 @@ __global__ void __launch_bounds__(kInsideThreads)
     fence_barrier_init();
   }
   if (warp == 5) {
-    tmem_alloc(&c->tmem, kColumns);
+    tmem_alloc(&c->tmem, kTile);
     tmem_relinquish();
   }
   tcgen05_fence_before();
   wait_for_predecessor();
-  const RowsTile t = find_tile(args, blockIdx.x, N, &c->found);
+  const RowsTile t = find_tile(args, blockIdx.x, &c->found);
   release_successor();  // (the columns of TMEM are there)
   tcgen05_fence_after();
   if (blockIdx.x == 0 && blockIdx.y == 0) report_entries(args);
   const uint32_t tmem = c->tmem;
   const int chunks = (args.inner + kChunk - 1) / kChunk, from = blockIdx.y * chunks_each;
   const int count = t.rows > 0 && t.adapter >= 0 ? min(chunks_each, chunks - from) : 0;
-  const uint32_t a_bytes = args.rank * 128, stage_bytes = a_bytes + N * 128;
+  const uint32_t a_bytes = args.rank * 128, stage_bytes = a_bytes + kTile * 128;
   const int boxes = (t.rows + 7) / 8;
   if (warp == 4) {
     bool ok = true;
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kInsideThreads)
       }
     }
   } else if (warp == 5) {
-    constexpr uint32_t kDesc = make_idesc_bf16(N, false);
+    constexpr uint32_t kDesc = make_idesc_bf16(kTile, false);
     bool ok = true;
     for (int i = 0; i < count && ok; ++i) {
       const int stage = i % stages;
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kInsideThreads)
   __syncthreads();
   if (warp == 5) {
     tcgen05_fence_after();
-    tmem_dealloc(tmem, kColumns);
+    tmem_dealloc(tmem, kTile);
   }
 }
 
@@ -601,20 +602,19 @@ __global__ void __launch_bounds__(kOutsideThreads, 1)
 
 // How a call is cut.
 struct Plan {
-  int height;       // rows of a tile of the first launch
-  int tiles;        // of these, at most
+  int tiles;        // of rows, at most
   int chunks_each, splits, stages;
   size_t inside_shared;
 
   Plan(int64_t rows, int count, int inner, int rank, int sms) {
-    // A tile of 16 rows holds its sums in fewer columns and less shared memory; one of 128 reads A once for more rows.
-    height = rows <= 16 * static_cast<int64_t>(count) ? 16 : kTile;
-    tiles = static_cast<int>(std::min<int64_t>(rows, rows / height + count));
+    tiles = static_cast<int>(std::min<int64_t>(rows, rows / kTile + count));
+    // Two blocks to an SM, so that one's results go out while the other reads (4096 x 4096, rank 16: 64 entries of 4 rows
+    // 32 us, of 30 rows 38, 23 of 356 50; with four blocks' parts 36, 40, 56, with one 46, - and 60).
     const int chunks = (inner + kChunk - 1) / kChunk;
     splits = std::clamp(2 * sms / tiles, 1, std::min(kMostSplits, std::max(chunks / 3, 1)));
     chunks_each = (chunks + splits - 1) / splits;
     splits = (chunks + chunks_each - 1) / chunks_each;
-    const size_t stage = static_cast<size_t>(rank + height) * 128;
+    const size_t stage = static_cast<size_t>(rank + kTile) * 128;
     stages = static_cast<int>(std::min<size_t>(std::min(kMostStages, chunks_each), 92 * 1024 / stage));
     inside_shared = sizeof(InsideControl) + 1024 + stages * stage + kPanelBytes;  // (128 rows are read of the last A, too)
   }
@@ -637,13 +637,11 @@ cudaError_t launch_adapters(const AdapterArgs& args, cudaStream_t stream) {
       !matrix_tensor_map(args.y, args.rows, args.outer, args.y_stride, 8, &y_few)) {
     return cudaErrorInvalidValue;
   }
-  static std::atomic<uint64_t> allowed[3];
-  cudaError_t err = allow_shared_memory_once(inside_kernel<16>, allowed[0]);
-  if (err == cudaSuccess) err = allow_shared_memory_once(inside_kernel<kTile>, allowed[1]);
-  if (err == cudaSuccess) err = allow_shared_memory_once(outside_kernel, allowed[2]);
+  static std::atomic<uint64_t> allowed[2];
+  cudaError_t err = allow_shared_memory_once(inside_kernel, allowed[0]);
+  if (err == cudaSuccess) err = allow_shared_memory_once(outside_kernel, allowed[1]);
   if (err != cudaSuccess) return err;
-  auto* inside = plan.height == 16 ? inside_kernel<16> : inside_kernel<kTile>;
-  err = launch_kernel(inside, dim3(plan.tiles, plan.splits), kInsideThreads, plan.inside_shared, LaunchStream(stream, true), map_x,
+  err = launch_kernel(inside_kernel, dim3(plan.tiles, plan.splits), kInsideThreads, plan.inside_shared, LaunchStream(stream, true), map_x,
                       map_a, args, plan.chunks_each, plan.stages);
   if (err != cudaSuccess) return err;
   const size_t shared = sizeof(OutsideControl) + 1024 + OutsideLayout(args.rank).total();
