@@ -129,6 +129,39 @@ def test_many_values_close_together(sampling):
         _check(sampling, around_zero, uniform, **setting)
 
 
+def test_many_rows_of_values_close_together(sampling):
+    """One block to a row, and more tokens near the border than it notes."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    logits, uniform = _logits(72, 131072, torch.float32, 17, spread=1.0)
+    close = 1.0 + 1e-3 * torch.rand(logits.shape, generator=g, device="cuda")
+    logits = torch.where(torch.rand(logits.shape, generator=g, device="cuda") < 0.6, close, logits)
+    for setting in (dict(top_p=0.6), dict(top_k=40000), dict(top_k=90000, top_p=0.5)):
+        _check(sampling, logits, uniform, **setting)
+
+
+@pytest.mark.parametrize("rows", [2, 80])
+def test_borders_among_few_heavy_tokens(sampling, rows):
+    """What most of a row's tokens say about the border is wrong: a few others weigh as much as all of them."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    logits, uniform = _logits(rows, 131072, torch.float32, 18, spread=1.0)
+    logits = logits.clamp(max=4.0)
+    heavy = torch.rand((rows, 40), generator=g, device="cuda") * 8.0 + torch.linspace(2.0, 9.0, rows, device="cuda")[:, None]
+    logits.scatter_(1, torch.randint(0, 131072, (rows, 40), generator=g, device="cuda"), heavy)
+    for top_p in (0.3, 0.8, 0.95, 0.99, 0.999):
+        _check(sampling, logits, uniform, top_p=top_p)
+    _check(sampling, logits, uniform, top_k=300, top_p=0.99, temperature=1.4)
+
+
+def test_large_batch(sampling):
+    rows = 150
+    logits, uniform = _logits(rows, 131072, torch.bfloat16, 19)
+    rng = np.random.default_rng(20)
+    vector = lambda values, kind: torch.tensor(rng.choice(values, rows), dtype=kind, device="cuda")  # noqa: E731
+    _check(sampling, logits, uniform, temperature=vector([0.0, 0.5, 1.0, 1.6], torch.float32),
+           top_k=vector([0, 0, 20, 300, 20000], torch.int32), top_p=vector([0.5, 0.95, 0.999, 1.0], torch.float32),
+           min_p=vector([0.0, 0.0, 0.02], torch.float32))
+
+
 def test_masks(sampling):
     logits, uniform = _logits(12, 20000, torch.float32, 9)
     lowest = torch.finfo(torch.float32).min
