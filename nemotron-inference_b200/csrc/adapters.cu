@@ -334,6 +334,7 @@ __device__ bool load_role(const AdapterArgs& args, const CUtensorMap* y_rows, co
         const uint32_t stage = units % layout.stages, y_bar = smem_u32(&c->y_full[stage]), to = y_at + stage * kTileBytes;
         if (!mbar_wait_warp(smem_u32(&c->y_empty[stage]), ((units / layout.stages) & 1) ^ 1)) return false;
         if (elect_one()) {
+          fence_proxy_async_smem();  // (here: in the warps that add up it would wait for their stores to memory)
           mbar_arrive_expect_tx_at(y_bar, bytes);
           for (int half = 0; half < 2; ++half) {
             if (bytes == kTileBytes) {
@@ -513,20 +514,24 @@ __device__ bool sum_role(const AdapterArgs& args, uint8_t* y, uint32_t tmem, con
         if (lane == 0) mbar_arrive(&c->d_empty[buffer]);
         ++adapted;
       }
+      uint4 line[8];
+      if (some) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int r = row0 + k * 4 + (lane >> 3);
+          line[k] = *reinterpret_cast<const uint4*>(tile + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c->y_empty[stage]);
       if (some) {
         const int at = column * kTile + half * 64 + (lane & 7) * 8;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int r = row0 + k * 4 + (lane >> 3);
-          if (r < p.rows && at < args.outer) {
-            *reinterpret_cast<uint4*>(out + r * args.out_stride + at) =
-                *reinterpret_cast<const uint4*>(tile + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-          }
+          if (r < p.rows && at < args.outer) *reinterpret_cast<uint4*>(out + r * args.out_stride + at) = line[k];
         }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c->y_empty[stage]);
     }
   }
   return ok;
