@@ -437,34 +437,60 @@ __device__ bool term_role(const AdapterArgs& args, uint8_t* terms, const Outside
     if (!mbar_wait_warp(smem_u32(&c->t_empty[buffer]), ((records / layout.terms) & 1) ^ 1)) return false;
     const float scale = args.scales[p.adapter];
     const float* inside = args.inside + static_cast<size_t>(p.first) * args.rank;
+    const int all = p.rows * eights;
+    constexpr int kAtOnce = 2, kSplitsAtOnce = 4;  // (their loads wait side by side)
 #pragma unroll 1
-    for (int i = thread; i < p.rows * eights; i += 32 * kTermWarps) {
-      const int row = i / eights, eight = i - row * eights;
-      float v[8];
+    for (int start = thread; start < all; start += kAtOnce * 32 * kTermWarps) {
+      float v[kAtOnce][8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-      if (eight * 8 < args.rank) {
-        const float4* from = reinterpret_cast<const float4*>(inside + static_cast<size_t>(row) * args.rank + eight * 8);
-#pragma unroll 4
-        for (int s = 0; s < splits; ++s) {
-          const float4 lo = __ldcg(from), hi = __ldcg(from + 1);
-          from = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(from) + split);
-          v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
-          v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+      for (int m = 0; m < kAtOnce; ++m) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[m][k] = 0.0f;
+      }
+#pragma unroll 1
+      for (int s = 0; s < splits; s += kSplitsAtOnce) {
+        float4 part[kAtOnce][kSplitsAtOnce][2];
+#pragma unroll
+        for (int m = 0; m < kAtOnce; ++m) {
+          const int i = start + m * 32 * kTermWarps, row = i / eights, eight = i - row * eights;
+          const float4* from = reinterpret_cast<const float4*>(inside + s * split + static_cast<size_t>(row) * args.rank + eight * 8);
+#pragma unroll
+          for (int j = 0; j < kSplitsAtOnce; ++j) {
+            part[m][j][0] = part[m][j][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i < all && eight * 8 < args.rank && s + j < splits) {
+              part[m][j][0] = __ldcg(from);
+              part[m][j][1] = __ldcg(from + 1);
+            }
+            from = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(from) + split);
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < kAtOnce; ++m) {
+#pragma unroll
+          for (int j = 0; j < kSplitsAtOnce; ++j) {
+            const float4 lo = part[m][j][0], hi = part[m][j][1];
+            v[m][0] += lo.x, v[m][1] += lo.y, v[m][2] += lo.z, v[m][3] += lo.w;
+            v[m][4] += hi.x, v[m][5] += hi.y, v[m][6] += hi.z, v[m][7] += hi.w;
+          }
         }
       }
-      uint32_t first[4], second[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float x = v[2 * k] * scale, z = v[2 * k + 1] * scale;
-        first[k] = pack_bf16(x, z);
-        const float x1 = __uint_as_float(first[k] << 16), z1 = __uint_as_float(first[k] & 0xffff0000u);
-        // (nothing is left of what has become infinite)
-        second[k] = pack_bf16(fabsf(x1) < INFINITY ? x - x1 : 0.0f, fabsf(z1) < INFINITY ? z - z1 : 0.0f);
+      for (int m = 0; m < kAtOnce; ++m) {
+        const int i = start + m * 32 * kTermWarps, row = i / eights, eight = i - row * eights;
+        if (i >= all) break;
+        uint32_t first[4], second[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float x = v[m][2 * k] * scale, z = v[m][2 * k + 1] * scale;
+          first[k] = pack_bf16(x, z);
+          const float x1 = __uint_as_float(first[k] << 16), z1 = __uint_as_float(first[k] & 0xffff0000u);
+          // (nothing is left of what has become infinite)
+          second[k] = pack_bf16(fabsf(x1) < INFINITY ? x - x1 : 0.0f, fabsf(z1) < INFINITY ? z - z1 : 0.0f);
+        }
+        uint8_t* to = terms + buffer * layout.t_bytes() + (eight >> 3) * kPanelBytes + row * 128 + (((eight & 7) ^ (row & 7)) << 4);
+        *reinterpret_cast<uint4*>(to) = make_uint4(first[0], first[1], first[2], first[3]);
+        *reinterpret_cast<uint4*>(to + layout.b_bytes()) = make_uint4(second[0], second[1], second[2], second[3]);
       }
-      uint8_t* to = terms + buffer * layout.t_bytes() + (eight >> 3) * kPanelBytes + row * 128 + (((eight & 7) ^ (row & 7)) << 4);
-      *reinterpret_cast<uint4*>(to) = make_uint4(first[0], first[1], first[2], first[3]);
-      *reinterpret_cast<uint4*>(to + layout.b_bytes()) = make_uint4(second[0], second[1], second[2], second[3]);
     }
     fence_proxy_async_smem();
     __syncwarp();
