@@ -11,8 +11,8 @@
 //            on their way tiles ahead.  t, summed up in a fixed order, is two bf16 terms (within 2^-17 of it; as one it
 //            would be off by 2^-9, of the size of what y's own rounding leaves), both multiplied with the same tile of B
 //            into one sum; y is added in FP32 and the result rounded once.  Rows without an adapter are copied.
-// Measured (B200, calls one after another): 23 requests of 356 rows, 2688 to 4608, rank 32, 49 us (3.6 TB/s); 64 of 4 rows,
-// 4096 to 2688, rank 64, 26 us (1.5 TB/s: a block's first tiles are on their way for 5 us, in each launch, and a piece
+// Measured (B200, calls one after another): 23 requests of 356 rows, 2688 to 4608, rank 32, 44 us (4.0 TB/s); 64 of 4 rows,
+// 4096 to 2688, rank 64, 25 us (1.6 TB/s: a block's first tiles are on their way for 5 us, in each launch, and a piece
 // begins with t); one row 10.5 us in a graph, 17 called.
 #include <algorithm>
 
@@ -519,6 +519,12 @@ __device__ bool sum_role(const AdapterArgs& args, uint8_t* y, uint32_t tmem, con
       uint8_t* tile = y + stage * kTileBytes + half * kPanelBytes;
       if (!mbar_wait_warp(smem_u32(&c->y_full[stage]), (units / layout.stages) & 1)) return false;
       if (with) {
+        uint4 own[8];  // (all before the first is written: the compiler does not know that they lie apart)
+        auto at = [&](int k) { return reinterpret_cast<uint4*>(tile + row * 128 + ((k ^ (row & 7)) << 4)); };
+        if (some) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) own[k] = *at(k);
+        }
         if (!mbar_wait_warp(smem_u32(&c->d_full[buffer]), (adapted >> 1) & 1)) return false;
         tcgen05_fence_after();
         if (some) {
@@ -529,10 +535,7 @@ __device__ bool sum_role(const AdapterArgs& args, uint8_t* y, uint32_t tmem, con
             tmem_ld_wait();
             registers_loaded<32>(d);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint4* at = reinterpret_cast<uint4*>(tile + row * 128 + (((k + j) ^ (row & 7)) << 4));
-              *at = add_eight(*at, d + 8 * j);
-            }
+            for (int j = 0; j < 4; ++j) *at(k + j) = add_eight(own[k + j], d + 8 * j);
           }
         }
         tcgen05_fence_before();
