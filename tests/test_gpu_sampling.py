@@ -252,6 +252,47 @@ def test_recorded_and_on_another_stream(sampling):
     _check(sampling, more, numbers, top_p=0.6)
 
 
+def test_more_rows_than_a_grid_dimension_has_blocks(sampling):
+    rows = 70000
+    logits, uniform = _logits(rows, 50, torch.float32, 21)
+    assert torch.equal(sampling.sample(logits, uniform, temperature=0.0).long(), logits.argmax(1))
+    tokens, logprobs = sampling.sample(logits, uniform, temperature=0.8, top_k=20, top_p=0.9, return_logprobs=True)
+    x, u = logits.cpu().numpy(), uniform.cpu().numpy()
+    for i in (0, 1, 65535, 65536, rows - 1):
+        token, logprob = _token(x[i], u[i], temperature=0.8, top_k=20, top_p=0.9)
+        assert tokens[i] == token
+        assert abs(float(logprobs[i]) - logprob) <= 2.0 ** -20 * max(1.0, abs(logprob))
+
+
+def test_two_calls_on_two_streams_and_in_two_graphs(sampling):
+    one, of_one = _logits(40, 70000, torch.float32, 22)
+    two, of_two = _logits(90, 50001, torch.bfloat16, 23)
+    want = sampling.sample(one, of_one, top_p=0.9), sampling.sample(two, of_two, top_k=500, top_p=0.95)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    graphs, outs = [], []
+    for stream, logits, uniform, setting in ((streams[0], one, of_one, dict(top_p=0.9)),
+                                             (streams[1], two, of_two, dict(top_k=500, top_p=0.95))):
+        out = torch.zeros(logits.shape[0], dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            sampling.sample(logits, uniform, out=out, **setting)
+        graphs.append(graph)
+        outs.append(out)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    with torch.cuda.stream(streams[0]):
+        again = sampling.sample(one, of_one, top_p=0.9)
+    with torch.cuda.stream(streams[1]):
+        and_again = sampling.sample(two, of_two, top_k=500, top_p=0.95)
+    torch.cuda.synchronize()
+    for got, expected in zip(outs + [again, and_again], want + want):
+        assert torch.equal(got, expected)
+
+
 def test_refusals(sampling, package):
     logits, uniform = _logits(4, 100, torch.float32, 16)
     for bad in (dict(logits=logits.half()), dict(logits=logits[0]), dict(logits=logits.t()), dict(uniform=uniform[:3]),
