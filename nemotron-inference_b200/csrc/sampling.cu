@@ -12,10 +12,10 @@
 //
 // What bounds it is reading the logits once, and FP64 where all weights are summed up: 16 of a scheduler's cycles for 32
 // tokens, 9 us for a row of 131072 on an SM.  Below that the steps of a row wait for one another: a barrier of a cluster
-// and the sums behind it take 1.5 us each, and a row with top-p has a dozen.  One block or a cluster goes over a row as often as its parameters ask, the
-// first time for the largest and the sum of all weights (by a reference that the first tokens give).  No sort: the
-// border of what stays is found by histograms over the values, whose bin at the border is listed and ranked one by one
-// (or split again while it holds too many; equal values go by their place).
+// and the sums behind it take 1.5 us each, and a row with top-p has a dozen.  One block or a cluster goes over a row as
+// often as its parameters ask, the first time for the largest and the sum of all weights (by a reference that the first
+// tokens give).  No sort: the border of what stays is found by histograms over the values, whose bin at the border is
+// listed and ranked one by one (or split again while it holds too many; equal values go by their place).
 //   top-k   the k-th largest of the threads' own largest values is no larger than the k-th largest of all: one entry a
 //           thread finds a bound that few more than k tokens reach, and these are ranked
 //   top-p   some thousand of the tokens tell about where the border lies: the pass that sums up the weights above notes
