@@ -50,6 +50,8 @@ constexpr float kSumScale = kCodeScale;              // of what is left, as the 
 constexpr float kValueScale = 256.0f * kSumScale;    // and of the products with values
 
 struct Control : WorkControl<S> {
+  // q_empty: by the MMA warp, whose products have read the queries, and by the softmax warps, which have seen q_full (they
+  // may still leave a segment's sums when the next one, of a single tile, has its products with its queries)
   uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_empty, wide_full[kWideSlots], wide_empty[kWideSlots];
   float top[2][S::kRows], other_sum[S::kRows];  // by halves of the tokens
 };
@@ -250,6 +252,7 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, const Q
     const bool present = rows > t * 128;                                      // the tile has rows, ...
     const bool has_rows = rows > t * 128 + (warp & 3) * 32, valid = row < rows;  // ... the warp, the thread
     if (!mbar_wait_warp(smem_u32(&c->q_full), segments & 1)) return false;    // (the factors were there before)
+    if (lane == 0) mbar_arrive(&c->q_empty);
     float factor = 0.0f, shift = 0.0f, sum = 0.0f;
     if (valid) {
       factor = __ldcg(queries.factors + (static_cast<int64_t>(s.kv_head) * args.batch.rows + s.first) * group + s.row0 + row);
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       mbar_init(&c->o_full[i], 1);
       mbar_init(&c->o_empty[i], S::kSoftmaxWarps / 2);
     }
-    mbar_init(&c->q_empty, 1);
+    mbar_init(&c->q_empty, S::kSoftmaxWarps + 1);
     for (int i = 0; i < kWideSlots; ++i) {
       mbar_init(&c->wide_full[i], S::kSoftmaxWarps);
       mbar_init(&c->wide_empty[i], 1);
