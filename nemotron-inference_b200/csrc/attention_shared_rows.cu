@@ -54,6 +54,7 @@ struct Control : WorkControl<S> {
   // may still leave a segment's sums when the next one, of a single tile, has its products with its queries)
   uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_empty, wide_full[kWideSlots], wide_empty[kWideSlots];
   float top[2][S::kRows], other_sum[S::kRows];  // by halves of the tokens
+  int failed[2];                                // a wait of a tile's warps has run out
 };
 
 constexpr size_t kSharedBytes =
@@ -241,18 +242,22 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, const Q
   const uint32_t o_at = tmem + lanes + kSums + t * kHeadDim + half * kHalf;
   const int page_shift = args.cache.page_shift, group = args.heads / args.cache.kv_heads;
   uint32_t no = 0, s_uses = 0, o_uses = 0;
+  // A wait that runs out: the eight warps of a tile meet at barriers that know no limit, so they agree at the next of these
+  // and leave there together.  (The other tile's find out by waits of their own.)
   bool ok = true;
 #pragma unroll 1
   for (uint32_t segments = 0;; ++segments) {
     const uint32_t place = segments % kSegments;
-    if (!mbar_wait_warp(smem_u32(&c->segment_full[place]), (segments / kSegments) & 1)) return false;
-    if (!c->has_segment[place]) return true;
+    ok = mbar_wait_warp(smem_u32(&c->segment_full[place]), (segments / kSegments) & 1);
+    const bool some = ok && c->has_segment[place];
+    ok = ok && (!some || mbar_wait_warp(smem_u32(&c->q_full), segments & 1));  // (the factors were there before)
+    if (tile_any(t, !ok)) return false;
+    if (!some) return true;
+    if (lane == 0) mbar_arrive(&c->q_empty);
     const Segment& s = c->segment[place];
     const int rows = s.rows * group - s.row0;
     const bool present = rows > t * 128;                                      // the tile has rows, ...
     const bool has_rows = rows > t * 128 + (warp & 3) * 32, valid = row < rows;  // ... the warp, the thread
-    if (!mbar_wait_warp(smem_u32(&c->q_full), segments & 1)) return false;    // (the factors were there before)
-    if (lane == 0) mbar_arrive(&c->q_empty);
     float factor = 0.0f, shift = 0.0f, sum = 0.0f;
     if (valid) {
       factor = __ldcg(queries.factors + (static_cast<int64_t>(s.kv_head) * args.batch.rows + s.first) * group + s.row0 + row);
@@ -261,12 +266,17 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, const Q
     for (int j = 0; j < s.tiles; ++j, ++no) {
       const uint32_t slot = no % S::kValueSlots;
       const uint32_t wide_slot = no % kWideSlots;
-      ok = mbar_wait_warp(smem_u32(&c->v_full[slot]), (no / S::kValueSlots) & 1) && ok;
-      ok = mbar_wait_warp(smem_u32(&c->wide_empty[wide_slot]), ((no / kWideSlots) & 1) ^ 1) && ok;
-      widen_values(values + slot * kKeyTileBytes, wide + wide_slot * kWideBytes);
-      if (lane == 0) mbar_arrive(&c->wide_full[wide_slot]);
-      if (present) {
-        ok = mbar_wait_warp(smem_u32(&c->s_full[t]), s_uses & 1) && ok;
+      ok = mbar_wait_warp(smem_u32(&c->v_full[slot]), (no / S::kValueSlots) & 1) &&
+           mbar_wait_warp(smem_u32(&c->wide_empty[wide_slot]), ((no / kWideSlots) & 1) ^ 1);
+      if (ok) {
+        widen_values(values + slot * kKeyTileBytes, wide + wide_slot * kWideBytes);
+        if (lane == 0) mbar_arrive(&c->wide_full[wide_slot]);
+      }
+      if (!present) {
+        if (tile_any(t, !ok)) return false;
+      } else {
+        ok = ok && mbar_wait_warp(smem_u32(&c->s_full[t]), s_uses & 1);
+        if (!ok) *const_cast<volatile int*>(&c->failed[t]) = 1;
         ++s_uses;
         tcgen05_fence_after();
         const bool is_first = j == 0;
@@ -318,7 +328,8 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, const Q
             }
           }
           // (behind this both halves have read the scores: weights may be written over them)
-          if (!tile_any(t, anew || high > kRiseBits)) break;
+          if (!tile_any(t, anew || high > kRiseBits || !ok)) break;
+          if (*const_cast<volatile int*>(&c->failed[t])) return false;
           c->top[half][row] = high;
           tile_sync(t);
           const float top = fmaxf(c->top[0][row], c->top[1][row]);
@@ -359,11 +370,11 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, const Q
       }
     }
     if (present) {
-      ok = mbar_wait_warp(smem_u32(&c->o_full[t]), o_uses & 1) && ok;
+      ok = mbar_wait_warp(smem_u32(&c->o_full[t]), o_uses & 1);
       ++o_uses;
       tcgen05_fence_after();
       if (half) c->other_sum[row] = sum;
-      tile_sync(t);
+      if (tile_any(t, !ok)) return false;
       const int to = valid ? (s.first + (s.row0 + row) / group) * args.heads + s.kv_head * group + (s.row0 + row) % group : -1;
       float* slot = split.slots + slot_floats(S::kRows) * max(s.part, 0);
       float* at = (s.part < 0 ? args.sums + static_cast<size_t>(max(to, 0)) * kHeadDim : slot + row * kHeadDim) + half * kHalf;
@@ -399,7 +410,6 @@ __device__ bool softmax_role(const CachedArgs& args, const Split& split, const Q
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&c->segment_empty[place]);
-    if (!ok) return false;
   }
 }
 
@@ -422,6 +432,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       mbar_init(&c->o_empty[i], S::kSoftmaxWarps / 2);
     }
     mbar_init(&c->q_empty, S::kSoftmaxWarps + 1);
+    c->failed[0] = c->failed[1] = 0;
     for (int i = 0; i < kWideSlots; ++i) {
       mbar_init(&c->wide_full[i], S::kSoftmaxWarps);
       mbar_init(&c->wide_empty[i], 1);
