@@ -54,7 +54,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const JoinArgs
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x;
   // (what these read was there before the first of the three launches)
   const BatchEntry e = part_entry<Part::kOwn>(c, i);
-  if (e.rows == 0) return;
+  if (e.rows == 0) {  // (nor does this launch end ahead of the others where no entry has rows: they may write zeros)
+    wait_for_predecessor();
+    return;
+  }
   bool valid = true;
   if (e.skip > 0) {
     const int g = group_of(c.groups, c.group_count, i, lane);
