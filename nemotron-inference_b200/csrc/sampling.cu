@@ -586,9 +586,23 @@ struct Row {
       const bool mine = own != 0 && sum - own <= target;
       if (mine) atomicMax(&s.bin, static_cast<int>(threadIdx.x));
       __syncthreads();
-      const bool chosen = mine && s.bin == static_cast<int>(threadIdx.x);
+      const bool none = s.bin < 0, chosen = mine && s.bin == static_cast<int>(threadIdx.x);
       __syncthreads();
-      if (chosen) {
+      if (none) {
+        // Each weighs less than half a unit, together they have one: their first, or their last for u of 1 and more.  (Half as
+        // many orders again as `lowest` lies below: the sum of all weights counts those down to kBelow orders.)
+        const float light = fmaxf(fmaf(1.5f, lowest - top, top), -FLT_MAX);
+#pragma unroll 1
+        for (int at = my_from; at < my_to; ++at) {
+          const float x = value(at);
+          if (!(x >= light && what.border.keeps(x, first + at))) continue;
+          if (u >= 1.0f) {
+            atomicMax(&s.bin, first + at);
+          } else {
+            atomicMin(reinterpret_cast<unsigned*>(&s.bin), static_cast<unsigned>(first + at));  // (of -1, the highest)
+          }
+        }
+      } else if (chosen) {
         u64 upto = sum - own;
 #pragma unroll 1
         for (int at = my_from; at < my_to && upto <= target; ++at) {
