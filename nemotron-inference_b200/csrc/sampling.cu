@@ -754,7 +754,10 @@ struct Row {
       }
       merge_bins();
       if ((all && target <= before) || !choose_bin(target - before)) {
-        if (!all || reach == 0) return stay;
+        if (!all || (reach == 0 && !weights)) return stay;  // (all of them)
+        // Known on both sides by now, and the border in neither: the sum of what lies above, rounded once for a thread, and that
+        // of single weights, rounded one by one, have it on different sides of one value.
+        if (reach == 0) return {target <= before ? most_of : least_of, INT_MAX};
         // the guess was wrong: a wider one, and then all, on the side where the border is
         if (target <= before) {
           least_of = upper;

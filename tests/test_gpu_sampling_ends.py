@@ -1,5 +1,5 @@
-"""GPU tests of sampling where rounding decides: random numbers at the ends of rows of very light tokens, and
-log-probabilities.
+"""GPU tests of sampling where rounding decides: random numbers at the ends of rows of very light tokens, borders between
+a sum and the sum of its rounded terms, and log-probabilities.
 
 Tokens are the definition's.  Log-probabilities: x - m and the logarithm are FP64, the sum of e^(x - m) is within 2^-36 of
 itself for its terms, 2^-40 for the order of adding, and what lies below 2^-64 of the largest (2^-64 131072 at most) is left
@@ -7,10 +7,11 @@ out: 2^-35 altogether, and the result is FP32: half a step, 2^-24 of it."""
 import importlib
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_sampling import _logits
+from test_gpu_sampling import _logits, _token
 
 pytestmark = pytest.mark.gpu
 
@@ -42,6 +43,41 @@ def test_ends_of_rows_whose_first_or_last_tokens_weigh_next_to_nothing(sampling,
                         assert bool((tokens == end).all()), (place, u, tokens[:4])
                     else:
                         assert bool((tokens == place).all())
+
+
+def _between_sums():
+    """Logits of three values, and a top_p, for which the tokens that stay - the largest and all of the second value -
+    reach p of the sum, but do not if each one's weight is rounded to 2^-44 of the largest first.  The third value is that of
+    the tokens which the search guesses by."""
+    vocab, unit = 131072, 2.0 ** 44
+    sampled = np.arange(vocab) % 1024 < 64  # (for up to 13 rows: a sixteenth)
+    n_third = int(sampled.sum())
+    n_second = vocab - n_third - 1
+    second = np.float32(-10.0)
+    while not 0.38 < (math.exp(float(second)) * unit) % 1.0 < 0.42:
+        second = np.nextafter(second, np.float32(0))
+    of_second = math.exp(float(second)) * unit
+    above = unit + n_second * of_second
+    gap = n_second * (of_second % 1.0)
+    third = np.float32(-11.5)
+    while True:
+        whole = above + n_third * math.exp(float(third)) * unit
+        top_p = np.float32((above - gap / 2) / whole)
+        if abs(float(top_p) * whole - (above - gap / 2)) < gap / 8:
+            break
+        third = np.nextafter(third, np.float32(0))
+    x = np.where(sampled, third, second).astype(np.float32)
+    x[100] = 0.0  # (not one of the guess's)
+    return x, float(top_p)
+
+
+def test_a_border_between_a_sum_and_that_of_its_rounded_terms(sampling):
+    x, top_p = _between_sums()
+    uniform = np.linspace(0.05, 0.95, 8).astype(np.float32)
+    logits = torch.from_numpy(x)[None].repeat(8, 1).cuda()
+    tokens = sampling.sample(logits, torch.from_numpy(uniform).cuda(), top_p=top_p).tolist()
+    assert all(x[token] > x.min() for token in tokens)
+    assert tokens == [_token(x, u, top_p=top_p)[0] for u in uniform]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
