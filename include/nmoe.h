@@ -637,8 +637,8 @@ NMOE_API nmoe_status nmoe_attention_sync_status(int32_t* error, void* stream);
  * Beside a projection that many requests share, what each one's own adapter adds:
  * out = y + scales[id] (x A[id]^T) B[id]^T for the rows [offsets[i], offsets[i+1]) of
  * entry i with id = ids[i] (device; entries may have the same; -1: none, the rows of y
- * as they are).  x [rows][inner], y and out [rows][outer] bf16, out may be y; `*_stride`
- * elements from row to row, a multiple of 8.  A [adapters][rank][inner],
+ * as they are).  x [rows][inner], y and out [rows][outer] bf16, out may be y, with its
+ * stride; `*_stride` elements from row to row, a multiple of 8.  A [adapters][rank][inner],
  * B [adapters][outer][rank] bf16, scales [adapters] FP32; inner, outer and rank are
  * multiples of 8, rank at most 128.  Sums are FP32, the result is rounded once.  Rows of no entry
  * stay as they are.
@@ -646,7 +646,8 @@ NMOE_API nmoe_status nmoe_attention_sync_status(int32_t* error, void* stream);
  * `workspace`: nmoe_adapters_workspace_bytes() bytes, 256-byte aligned, anything
  * in it, this call's alone until it is done.  `error`: a device word, zero at first,
  * for nmoe_adapters_sync_status: an id that is none (its rows get none) and offsets
- * that do not rise within 0 to `rows` (such an entry's rows stay as they are). */
+ * that do not rise within 0 to `rows` (such an entry's rows stay as they are; where
+ * other entries overlap because of it, the call's results are undefined). */
 typedef struct nmoe_adapters {
   int32_t adapters;
   int32_t rank;

@@ -88,7 +88,7 @@ class AdapterPool:
 
     def add(self, x: torch.Tensor, y: torch.Tensor, ids: torch.Tensor, offsets: torch.Tensor,
             out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """y + scales[id] (x a[id]^T) b[id]^T for the rows of each entry; `out` may be y.  x is [rows, inner],
+        """y + scales[id] (x a[id]^T) b[id]^T for the rows of each entry; `out` may be y itself.  x is [rows, inner],
         y [rows, outer].  Sums are FP32 and the result is rounded once; rows of no entry are as `out` had
         them, undefined without it."""
         device = self.device

@@ -51,6 +51,7 @@ nmoe_status nmoe_adapters_add(const nmoe_adapters* pool, void* stream, const voi
   if (pool->a == nullptr || pool->b == nullptr || pool->scales == nullptr || misaligned(pool->a, 16) ||
       misaligned(pool->b, 16) || misaligned(pool->scales, 4) || !rows_valid(x, x_stride, pool->inner) ||
       !rows_valid(y, y_stride, pool->outer) || !rows_valid(out, out_stride, pool->outer) || error == nullptr ||
+      (out == y && out_stride != y_stride && rows > 1) ||  // (over other rows than its own)
       workspace == nullptr || misaligned(workspace, 256) ||
       workspace_bytes < nmoe::adapter_workspace_bytes(rows, count, pool->inner, pool->rank)) {
     return NMOE_ERR_INVALID_ARGUMENT;
