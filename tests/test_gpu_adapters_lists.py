@@ -68,3 +68,24 @@ def test_results_over_other_rows_are_refused(adapters, package):
         assert info.value.status == 1
     assert pool.add(x, whole[:, :128], ids, offsets, out=whole[:, 128:]).data_ptr() == whole[:, 128:].data_ptr()
     assert pool.sync_status() == 0
+
+
+def test_two_calls_on_two_streams(adapters):
+    """One pool and a word for both, results and workspaces of their own."""
+    pool = _pool(adapters, 5, 16, 1024, 1160)
+    problems = []
+    for seed, counts in ((3, [4] * 60), (9, [300, 1, 129, 0, 40])):
+        x, y = _inputs(pool, sum(counts), seed=seed)
+        offsets = [sum(counts[:i]) for i in range(len(counts) + 1)]
+        problems.append((x, y, _int([i % 5 for i in range(len(counts))]), _int(offsets)))
+    alone = [pool.add(*problem) for problem in problems]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for problem, stream in zip(problems, streams):
+            with torch.cuda.stream(stream):
+                got.append(pool.add(*problem))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, alone))
+    assert pool.sync_status() == 0

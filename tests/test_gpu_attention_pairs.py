@@ -3,13 +3,14 @@
 Tolerances are those of tests/test_gpu_attention_shared.py: its kernel's weights are within 2^-11 of themselves or 2^-25 of
 the largest that its reference allows (2^8), which the bounds there hold with room."""
 import importlib
+import math
 import random
 
 import pytest
 import torch
 
-from test_gpu_attention import _int, _normal, _offsets
-from test_gpu_attention_shared import _attend, _check, _edges, _shared_cache
+from test_gpu_attention import _int, _normal, _offsets, _values
+from test_gpu_attention_shared import _attend, _check, _edges, _expected_shared, _shared_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -115,9 +116,6 @@ def test_powers_of_pages_far_apart(attention, page_tokens, low, high):
 def _check_far(cache, q, sequence, c, got, scale):
     """With powers apart: a weight is relative to the largest of weight times 2^power of its page's values, which is
     what a row's reference goes by; what is off by 2^-20.5 of that is multiplied with codes, of at most 448."""
-    import math
-
-    from test_gpu_attention import _values
     n, p = int(cache.lengths[sequence]), cache.codes.shape[4]
     values = _values(cache, 0, sequence)
     power = torch.exp2(cache.exponents[0, cache.block_table[sequence, :-(-n // p)].long(), 1, 0].double()).repeat_interleave(p)[:n]
@@ -269,3 +267,22 @@ def test_two_graphs_of_one_cache(attention):
             graphs[i].replay()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
     assert cache.sync_status() == 0
+
+
+def test_sequences_in_any_order_wide_rows_and_rows_of_no_entry(attention):
+    """Queries that lie among other columns, entries without rows, entries of no group before and behind, two key heads."""
+    groups = [(600, [30, 40, 50, 60]), (300, [10, 20, 5]), (129, [2, 2])]
+    cache = _shared_cache(attention, groups, [77, 900], 2, 32, seed=15, layers=2)
+    sequences = [10, 2, 0, 3, 1, 6, 4, 5, 7, 8, 9]
+    counts = [3, 4, 0, 5, 6, 4, 0, 3, 1, 1, 3]
+    edges = _int([1, 5, 8, 10])
+    heads, rows = 2 * 36, sum(counts)
+    wide = _normal(16, rows + 5, heads + 8, D).to(torch.bfloat16)
+    q = wide[:, 4:heads + 4]
+    assert -(-(rows + 5) // 3) * 36 > 128 and not q.is_contiguous()
+    out = torch.full((rows + 5, heads, D), 5.0, dtype=torch.bfloat16, device="cuda")
+    got, shared = _attend(cache, 1, q, sequences, counts, edges, out=out)
+    assert got is out and bool((out[rows:] == 5.0).all()) and cache.sync_status() == 0
+    assert shared.tolist() == _expected_shared(cache, sequences, counts, edges.tolist())
+    assert shared.tolist()[0] == 0 and shared.tolist()[1] == 512 and shared.tolist()[5] == 256
+    _check(cache, 1, q, sequences, counts, got)
