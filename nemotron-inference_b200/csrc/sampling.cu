@@ -1061,7 +1061,7 @@ cudaError_t launch(const SampleArgs& args, cudaStream_t stream) {
   int size = 1;
   while (size < kMaxCluster &&
          ((args.vocab + size - 1) / size > kMostSlice ||
-          (args.rows * size * 2 <= (size * 2 == 8 ? room * 4 / 5 : room) && args.vocab > 2048 * size))) {
+          (static_cast<int64_t>(args.rows) * size * 2 <= (size * 2 == 8 ? room * 4 / 5 : room) && args.vocab > 2048 * size))) {
     size *= 2;
   }
   const int slice = ((args.vocab + size - 1) / size + kElements - 1) / kElements * kElements;
@@ -1096,7 +1096,9 @@ cudaError_t launch_sample(const SampleArgs& args, bool bf16, cudaStream_t stream
   // Few rows: one block to an SM, whose threads then have registers enough (64 rows of 131072: 80 us; two blocks, which
   // spill, 96).  Many, of which an SM has more than one block's: two, which hide each other's waits (128 rows, top-p 106 us,
   // 96 rows, top-k 55; with one block to an SM 133 and 57; 256 rows as they are 67, 95).
-  if (args.rows * 20 > device_sms() * 9) return bf16 ? launch<__nv_bfloat16, 2>(args, stream) : launch<float, 2>(args, stream);
+  if (static_cast<int64_t>(args.rows) * 20 > device_sms() * 9) {
+    return bf16 ? launch<__nv_bfloat16, 2>(args, stream) : launch<float, 2>(args, stream);
+  }
   return bf16 ? launch<__nv_bfloat16, 1>(args, stream) : launch<float, 1>(args, stream);
 }
 
