@@ -601,7 +601,8 @@ NMOE_API nmoe_status nmoe_attention_cached(const nmoe_kv_cache* cache, void* str
  * as whole runs of 128 tokens, and 0 where fewer than two members have rows.  It
  * is called once a step, behind nmoe_kv_extend; nmoe_attention_shared then
  * gives the results of nmoe_attention_cached in every layer, reading what is
- * shared once for all rows of a group.
+ * shared once for all rows of a group.  (It is the faster where that saves some
+ * 250 MB of codes in a layer, 256 bytes a token and key head.)
  *
  * `workspace` (256-byte aligned, nmoe_attention_shared_workspace_bytes() bytes,
  * anything in it) is this call's alone until it is done.  A `shared` that is not what

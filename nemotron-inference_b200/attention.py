@@ -345,7 +345,13 @@ class KvCache:
                       groups: torch.Tensor, shared: torch.Tensor, scale: Optional[float] = None,
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """`attend` for a batch in groups, with what `find_shared` found for it: the tokens that a group
-        shares are read once for all of its rows."""
+        shares are read once for all of its rows.  It pays where what is not read again is some 250 MB of
+        codes in a layer or more, 256 bytes a token and key head (64 continuations of 2048 tokens with 8
+        key heads); below, `attend` takes less time.
+
+        Queries are taken as two 8-bit terms, weights as two such (within 2^-8) or, for groups of
+        more than 128 rows of queries to a key head, as binary16 (2^-11; 2^-25 of the largest where
+        that is more); sums are FP32 and results bf16.  Each call allocates some 60 MB meanwhile."""
         stream = self._batch(sequences, offsets)
         self._groups(sequences, groups)
         _require_list(shared, "shared", self.device)

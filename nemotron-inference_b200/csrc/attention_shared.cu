@@ -13,8 +13,14 @@
 // heads in 20 pieces 13 us with its launch; 532 rows 15).
 //
 // Three launches: the groups' shared tokens, the sequences' own ones (the kernels of attention_cached.cuh, which leave
-// sums instead of results), and the join, a warp to a row and head.  The second does not wait for the first: its blocks
-// take the SMs that become free.
+// sums instead of results), and the join, a warp to a row and head.  The second does not wait for the first, but its blocks
+// only find room where one of the first's has left: the call takes about the three's times one after another.
+//
+// So attention_cached.cu's single launch is faster where little is shared.  Both from a recorded graph, caches in memory, 32
+// query heads, 60 tokens of their own, in us (some 6 of each are the graph's): 8 sequences sharing 1024, 8 key heads 22
+// by that, 31 by this; 64 sharing 1024 37, 43; 8 sharing 16384 45, 47; 64 sharing 4096 70, 53; 64 sharing 16384 205, 65; 2
+// key heads: 64 sharing 4096 41, 51; 64 sharing 16384 82, 60.  They are equal at about 250 MB of codes that are
+// not read again.
 #include <algorithm>
 
 #include "attention.h"

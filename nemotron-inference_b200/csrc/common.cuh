@@ -155,9 +155,18 @@ __device__ __forceinline__ uint64_t div2_by_reciprocal(uint64_t x, uint64_t minu
 // Programmatic dependent launch.  The successor on the stream may become resident once every CTA has
 // called release_successor(), so a kernel that allocates TMEM calls it after that (a successor that
 // took the columns first would wait for this kernel, and this kernel for the columns).  Every thread
-// calls wait_for_predecessor() before it touches what other kernels write or read: it returns when
-// the predecessor, and with it all that came before, is complete and visible.  Pointers to such data
-// are not `const __restrict__`, so that no load of theirs moves ahead of it.
+// calls wait_for_predecessor() before it touches what the predecessor writes or reads, and on every
+// way out: it returns when the predecessor, and with it all that came before, is complete and
+// visible, so a kernel that ended without it would let its successor begin ahead of what came
+// before.  Pointers to such data are not `const __restrict__`, so that no load of theirs moves ahead of it.
+//
+// What was complete before the predecessor began its work may be touched ahead of the wait, where
+// every thread of the predecessor waits before it releases (or that holds of the predecessor's own
+// predecessor, and so on up to one launch of the same call): then no block of this kernel runs before that wait has
+// returned everywhere.  The first launch of a call always waits first.  The later launches of attention_shared.cu,
+// attention_shared_rows.cu and adapters.cu read their call's inputs that way, and write rows and
+// parts of the workspace that the launches ahead of them neither write nor read; what these have made is
+// read behind the wait.
 __device__ __forceinline__ void release_successor() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

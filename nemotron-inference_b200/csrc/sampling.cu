@@ -24,7 +24,7 @@
 // The sums in order of i come last, of what stays.
 //
 // Measured (B200, FP32): 256 rows of 131072 as they are 67 us, 40 of them for the first pass (half of what copying
-// reaches); 64 rows of as many settings 78 to 83 us; one row 31 us; 37 rows of 50001 in BF16, top-k and top-p, 22 us.  Rows that
+// reaches); 64 rows of as many settings 80 to 89 us; one row 30 to 33 us; 37 rows of 50001 in BF16, top-k and top-p, 22 us.  Rows that
 // lay in the shared memory of clusters of eight blocks took 145, 102, 33 and 22 us: such clusters left a third of the
 // SMs' room empty, and SMs idle while a row's steps waited.
 #include <cooperative_groups.h>
